@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define WPTV_ABI_VERSION 11
+#define WPTV_ABI_VERSION 12
 
 enum {
   WPTV_OK = 0,
@@ -573,6 +573,97 @@ int wptv_greedy_tree(const void* scores, int64_t scores_stride_b, int64_t scores
  *   nothing, n_tokens -1). */
 int wptv_greedy_tree_best(const int32_t* best, const int64_t* node_tokens, const int32_t* parents, int B, int M,
                           int64_t* path, int64_t* tokens, int32_t* n_tokens, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Beam search: the next beams of every text over its beams and the
+ * vocabulary, and the reordering of the rows' states after it.  No counterpart
+ * in the reference, whose Writer samples each row by itself.
+ *
+ * wptv_beam_step: text i's candidates are its W beams continued by each of V
+ *   tokens, of value totals[i, w] + (x - log sum exp x) over the beam's
+ *   scores x, ranked in 64 bits.  The K largest are the next beams, in order,
+ *   equal values to the lowest w V + v.
+ *   scores   beam w of text i at scores + i*scores_stride_n +
+ *            w*scores_stride_w (elements), V contiguous values of scores_dtype
+ *            (WPTV_F32 or WPTV_BF16)
+ *   totals   [n, W] fp32: each beam's summed log-probability.  A beam whose
+ *            total is not finite, or whose scores hold a NaN or +inf or
+ *            nothing above -inf, has every candidate at -inf
+ *   ended    NULL, or [n, W] bytes: a beam that has ended (not 0) has one
+ *            candidate above -inf, stops[0] at its own total
+ *   stops    n_stops (0 .. 16) token ids in host memory: a beam that writes
+ *            one of them has ended
+ *   new_totals, parents, tokens, new_ended  [n, K] out: the next beams'
+ *            totals (fp32), source beams, tokens (int64) and whether they have
+ *            ended (bytes)
+ *   workspace  wptv_beam_workspace(n, W, V, K) bytes.  W, K <= 64, K <= W V
+ * ------------------------------------------------------------------------- */
+int wptv_beam_workspace(int n, int W, int V, int K, size_t* bytes);
+
+int wptv_beam_step(const void* scores, int64_t scores_stride_n, int64_t scores_stride_w, int scores_dtype,
+                   const float* totals, const unsigned char* ended, const int64_t* stops, int n_stops, int n, int W,
+                   int V, int K, float* new_totals, int64_t* parents, int64_t* tokens, unsigned char* new_ended,
+                   void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* wptv_reorder_rows: beam w of text i takes over the states of beam
+ *   parents[i, w] of the same text, all at once and in place (a beam may be
+ *   taken several times): for each of `count` tables, row n of batch row
+ *   i W + w becomes row n of batch row i W + parents[i, w], for n <
+ *   min(lengths[i W + parents[i, w]], capacity).  A parent outside 0 .. W - 1
+ *   leaves its beam as it is.
+ *   tables, strides_b, strides_n, capacities, row_bytes  host arrays: each
+ *            table's address, its batch rows' and rows' strides in bytes, its
+ *            rows a batch row and a row's contiguous bytes, of any type
+ *   parents  [n, W] int64; lengths  [n W] int64, or NULL: every row
+ *   rows     an upper bound of the lengths (with lengths; rows past it keep
+ *            their values).  W <= 64 */
+int wptv_reorder_rows(void* const* tables, const int64_t* strides_b, const int64_t* strides_n,
+                      const int64_t* capacities, const int64_t* row_bytes, int count, const int64_t* parents,
+                      const int64_t* lengths, int64_t rows, int n, int W, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Eviction: a cache bounded to the rows that have received the most attention.
+ * No counterpart in the reference, whose cache keeps every entry.
+ *
+ * wptv_attention_weights: weights[b, n] += the sum over queries t < counts[b]
+ *   with positions[b, t] >= n and heads h of exp(scale q[b, t, h] . k[b, n] -
+ *   lse[b, t, h]): the softmax weight each table row got from a reading's
+ *   verify attention (lse its log-sum-exp, positions as there).
+ *   counts   NULL (T) or [B] int64: queries counted, the others padding
+ *   start    NULL or [B] int64: rows n >= start[b] begin at zero instead of
+ *            their weight (the reading's own rows: its rows before it)
+ *   weights  row b at weights + b*weights_stride_b, N fp32; rows past the last
+ *            counted position are not touched
+ *   splits, workspace  wptv_attention_weights_workspace: the parts the queries
+ *            are cut into (0 = chosen from B, T, H, N and the GPU) and the
+ *            bytes of their sums, joined in order
+ *   c <= 256 */
+int wptv_attention_weights_workspace(int B, int T, int H, int c, int N, int dtype, int* splits, size_t* bytes);
+
+int wptv_attention_weights(const void* q, const void* k, int64_t k_stride_b, int64_t k_stride_n, int dtype,
+                           const int64_t* positions, const float* lse, const int64_t* counts, const int64_t* start,
+                           int B, int T, int H, int c, int N, float scale, int splits, float* weights,
+                           int64_t weights_stride_b, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* wptv_choose_kept: of the first min(lengths[b], N) rows of each (layer,
+ *   batch row), all when they are at most `keep`; else the first `first`, the
+ *   last `recent`, and the keep - first - recent others of the largest weight
+ *   (equal weights the lowest rows; a NaN counts as the largest).
+ *   weights  row n of (l, b) at weights + l*weights_stride_l +
+ *            b*weights_stride_b + n (fp32)
+ *   kept     [L, B, keep] int64 out: the rows in ascending order, then -1
+ *   counts   [B] int64 out: the rows kept, min(length, keep)
+ * wptv_keep_rows: row j of batch row b of table i becomes its row
+ *   kept[i mod lists, b, j] for j < min(counts[b], keep), in place; the lists
+ *   ascend (as wptv_choose_kept's).  Tables as wptv_reorder_rows; rows from
+ *   counts[b] on keep what they hold. */
+int wptv_choose_kept(const float* weights, int64_t weights_stride_l, int64_t weights_stride_b, const int64_t* lengths,
+                     int L, int B, int N, int keep, int first, int recent, int64_t* kept, int64_t* counts,
+                     hipStream_t stream);
+
+int wptv_keep_rows(void* const* tables, const int64_t* strides_b, const int64_t* strides_n, const int64_t* capacities,
+                   const int64_t* row_bytes, int count, const int64_t* kept, int lists, int keep,
+                   const int64_t* counts, int B, hipStream_t stream);
 
 #ifdef __cplusplus
 }

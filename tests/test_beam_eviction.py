@@ -1,0 +1,143 @@
+"""What the beam and eviction operators refuse, checked on the host before
+anything is launched (no GPU is needed), and their 64-bit definitions on small
+cases done by hand."""
+
+import ctypes
+
+import pytest
+import torch
+
+from oracle import beam as beam_oracle
+from oracle import eviction as eviction_oracle
+from wpt_amd import _lib, kernels, sampling
+
+A = 1 << 20  # an address that is never read: every call here ends on the host
+
+
+def message():
+    return _lib.lib().wptv_last_error().decode()
+
+
+def longs(*values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def beam(n=1, W=2, V=10, K=2, dtype=_lib.WPTV_F32, stops=(), ended=None, n_stops=None, size=1 << 20, scores=A):
+    return _lib.lib().wptv_beam_step(scores, W * V, V, dtype, A, ended, longs(*stops), len(stops) if n_stops is None else
+                                     n_stops, n, W, V, K, A, A, A, A, A, size, None)
+
+
+@pytest.mark.parametrize("status, text, arguments", [
+    (-1, "bad shape", {"n": -1}), (-1, "bad shape", {"W": 0}), (-1, "bad shape", {"V": 0}), (-1, "bad shape", {"K": 0}),
+    (-1, "bad shape", {"K": 21}), (-3, "at most 64", {"W": 65}), (-3, "at most 64", {"W": 64, "K": 65}),
+    (-3, "neither", {"dtype": 7}), (-1, "outside", {"stops": (10,)}), (-1, "outside", {"stops": (1, -1)}),
+    (-1, "0 to 16", {"n_stops": 17}), (-1, "stop token", {"ended": A}), (-1, "workspace", {"size": 8}),
+    (-1, "NULL", {"scores": None}), (-3, "too large", {"n": 1 << 30, "W": 4})])
+def test_beam_step_refuses(status, text, arguments):
+    assert beam(**arguments) == status
+    assert text in message()
+
+
+def test_no_texts_is_no_work():
+    assert beam(n=0) == 0
+
+
+def reorder(base=A, sb=640, sn=64, capacity=10, row=64, count=1, n=1, W=2, parents=A, rows=10):
+    return _lib.lib().wptv_reorder_rows((ctypes.c_void_p * 1)(base), longs(sb), longs(sn), longs(capacity), longs(row), count,
+                                        parents, None, rows, n, W, None)
+
+
+@pytest.mark.parametrize("status, text, arguments", [
+    (-1, "bad shape", {"W": 0}), (-1, "bad shape", {"n": -1}), (-1, "bad shape", {"rows": -1}), (-3, "at most 64", {"W": 65}),
+    (-3, "65535", {"n": 65536}), (-1, "overlap", {"sn": 63}), (-1, "overlap", {"sb": 0}), (-1, "overlap", {"sb": 600}),
+    (-1, "capacity", {"capacity": -1}), (-1, "capacity", {"row": 0}), (-1, "NULL", {"base": None}),
+    (-1, "parents", {"parents": None})])
+def test_reorder_rows_refuses(status, text, arguments):
+    assert reorder(**arguments) == status
+    assert text in message()
+
+
+def keep(base=A, sb=640, sn=64, capacity=10, row=64, count=1, lists=1, kept=A, keep=4, B=2):
+    return _lib.lib().wptv_keep_rows((ctypes.c_void_p * 3)(base, base, base), longs(sb, sb, sb), longs(sn, sn, sn),
+                                     longs(capacity, capacity, capacity), longs(row, row, row), count, kept, lists, keep,
+                                     A, B, None)
+
+
+@pytest.mark.parametrize("status, text, arguments", [
+    (-1, "3 tables for 2", {"count": 3, "lists": 2}), (-1, "for 0 lists", {"lists": 0}), (-1, "B=-1", {"B": -1}),
+    (-3, "65535", {"B": 65536}), (-1, "overlap", {"sb": 639}), (-1, "overlap", {"sn": 32}), (-1, "kept", {"kept": None})])
+def test_keep_rows_refuses(status, text, arguments):
+    assert keep(**arguments) == status
+    assert text in message()
+
+
+@pytest.mark.parametrize("text, arguments", [
+    ("must hold", (0, 0, 0)), ("must hold", (4, 3, 2)), ("must hold", (4, -1, 2)), ("must hold", (4, 1, -1))])
+def test_choose_kept_refuses(text, arguments):
+    assert _lib.lib().wptv_choose_kept(A, 10, 10, A, 1, 1, 10, *arguments, A, A, None) == -1
+    assert text in message()
+
+
+@pytest.mark.parametrize("status, text, arguments", [
+    (-1, "bad shape", {"H": 0}), (-1, "bad shape", {"N": 0}), (-3, "dtype", {"dtype": 3}), (-3, "width", {"c": 257}),
+    (-1, "overlap", {"stride": 100}), (-1, "overlap", {"row": 63}), (-1, "NULL", {"q": None}), (-1, "splits", {"splits": -1})])
+def test_attention_weights_refuse(status, text, arguments):
+    a = dict(q=A, row=64, dtype=_lib.WPTV_BF16, B=2, T=3, H=4, c=64, N=101, splits=1, stride=101) | arguments
+    assert _lib.lib().wptv_attention_weights(a["q"], A, 6464, a["row"], a["dtype"], A, A, None, None, a["B"], a["T"], a["H"],
+                                             a["c"], a["N"], 0.125, a["splits"], A, a["stride"], None, 0, None) == status
+    assert text in message()
+
+
+def test_the_python_entry_points_refuse_what_is_not_theirs():
+    x = torch.zeros(2, 3, 8)
+    with pytest.raises(kernels.KernelUnavailable):
+        sampling.beam_step(x, torch.zeros(2, 3))
+    with pytest.raises(ValueError, match="dimensions"):
+        sampling.beam_step(x[0], torch.zeros(2, 3))
+    with pytest.raises(ValueError, match="bfloat16"):
+        sampling.beam_step(x.half(), torch.zeros(2, 3))
+    with pytest.raises(kernels.KernelUnavailable):
+        kernels.reorder_rows(x, torch.zeros(1, 2, dtype=torch.long))
+    with pytest.raises(ValueError, match="whole numbers"):
+        kernels.reorder_rows(x, torch.zeros(1, 2))
+    with pytest.raises(ValueError, match="texts, beams"):
+        kernels.reorder_rows(x, torch.zeros(2, dtype=torch.long))
+    with pytest.raises(ValueError, match="each table"):
+        kernels.reorder_rows(x[0], torch.zeros(1, 2, dtype=torch.long))
+    with pytest.raises(ValueError, match="no table"):
+        kernels.reorder_rows([], torch.zeros(1, 2, dtype=torch.long))
+    with pytest.raises(kernels.KernelUnavailable):
+        kernels.keep_rows(x, torch.zeros(1, 2, 2, dtype=torch.long), torch.ones(2, dtype=torch.long))
+    with pytest.raises(ValueError, match="layers, B, keep"):
+        kernels.keep_rows(x, torch.zeros(2, 2, dtype=torch.long), torch.ones(2, dtype=torch.long))
+    with pytest.raises(kernels.KernelUnavailable):
+        kernels.choose_kept(x, torch.ones(3, dtype=torch.long), 2, 0, 1)
+    with pytest.raises(ValueError, match="FP32"):
+        kernels.choose_kept(x.double(), torch.ones(3, dtype=torch.long), 2, 0, 1)
+    with pytest.raises(kernels.KernelUnavailable):
+        kernels.add_attention_weights(torch.zeros(1, 1, 2, 8), x[:1], torch.zeros(1, 1, dtype=torch.long),
+                                      torch.zeros(1, 1, 2), 1.0, torch.zeros(1, 3))
+
+
+def test_the_definition_of_the_next_beams():
+    scores = torch.log(torch.tensor([[[0.5, 0.3, 0.2], [0.1, 0.8, 0.1]]]))
+    totals = torch.tensor([[0.0, -0.1]])
+    t, p, v, e = beam_oracle.beam_step(scores, totals, stops=(1,), beams=3)
+    assert p.tolist() == [[1, 0, 0]] and v.tolist() == [[1, 0, 1]] and e.tolist() == [[True, False, True]]
+    assert torch.allclose(t.exp(), torch.tensor([[0.8 * torch.tensor(-0.1).exp().item(), 0.5, 0.3]], dtype=torch.double))
+    # an ended beam stays as it is; equal values to the lowest beam, then token
+    t, p, v, e = beam_oracle.beam_step(torch.zeros(1, 2, 4), torch.tensor([[-1.0, -1.0]]), torch.tensor([[True, False]]),
+                                       stops=(2,), beams=4)
+    assert p.tolist() == [[0, 1, 1, 1]] and v.tolist() == [[2, 0, 1, 2]] and e.tolist() == [[True, False, False, True]]
+
+
+def test_the_definition_of_eviction():
+    weights = torch.tensor([[[9.0, 1.0, 3.0, 2.0, 3.0, 0.0]]])
+    kept, counts = eviction_oracle.choose_kept(weights, torch.tensor([6]), 4, 1, 1)
+    assert kept.tolist() == [[[0, 2, 4, 5]]] and counts.tolist() == [4]
+    table = torch.arange(6.0).view(1, 6, 1)
+    assert eviction_oracle.keep_rows([table], kept, counts)[0].flatten().tolist() == [0, 2, 4, 5, 4, 5]
+    q = torch.ones(1, 2, 1, 1)
+    got = eviction_oracle.attention_weights(q, torch.zeros(1, 3, 1), torch.tensor([[1, 2]]), torch.tensor([[[0.0], [0.0]]]),
+                                            1.0, torch.tensor([[5.0, 5.0, 5.0]]), start=torch.tensor([1]))
+    assert got.tolist() == [[7.0, 2.0, 1.0]]

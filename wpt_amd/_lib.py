@@ -6,13 +6,14 @@ already holds.  A missing or stale library is KernelUnavailable: nothing in
 this package computes the verify step any other way.
 """
 
+import contextlib
 import ctypes
 from pathlib import Path
 
 import torch
 
 LIBRARY = Path(__file__).resolve().parent / "lib" / "libwptv.so"
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 WPTV_F32, WPTV_BF16 = 0, 1
 DTYPES = {torch.float32: WPTV_F32, torch.bfloat16: WPTV_BF16}
@@ -88,6 +89,14 @@ SIGNATURES = {
                              _P, _P, _P, _SZ, _P, _P, _P, _I64, _P, _P, _P],
     "wptv_greedy_tree": [_P, _I64, _I64, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _SZ, _P],
     "wptv_greedy_tree_best": [_P, _P, _P, _I, _I, _P, _P, _P, _P],
+    "wptv_beam_workspace": [_I, _I, _I, _I, ctypes.POINTER(_SZ)],
+    "wptv_beam_step": [_P, _I64, _I64, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _SZ, _P],
+    "wptv_reorder_rows": [_P, _P, _P, _P, _P, _I, _P, _P, _I64, _I, _I, _P],
+    "wptv_attention_weights_workspace": [_I, _I, _I, _I, _I, _I, ctypes.POINTER(_I), ctypes.POINTER(_SZ)],
+    "wptv_attention_weights": [_P, _P, _I64, _I64, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _P, _I64, _P, _SZ,
+                               _P],
+    "wptv_choose_kept": [_P, _I64, _I64, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P],
+    "wptv_keep_rows": [_P, _P, _P, _P, _P, _I, _P, _I, _I, _P, _I, _P],
 }
 
 _handle = None
@@ -146,6 +155,14 @@ def stream(device):
         return torch.cuda.current_stream(device).cuda_stream
     index = device.index
     return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+def on(device):
+    """A context in which device is the current one (nothing to enter where it is)."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(index)
 
 
 _plans = {}  # (entry point, device, part count asked for, its integers) -> (parts, bytes)

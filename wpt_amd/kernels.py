@@ -19,6 +19,8 @@ A bad shape or dtype is ValueError; a device without the library is
 KernelUnavailable, never a fall back to another form.
 """
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -27,7 +29,8 @@ from ._lib import KernelUnavailable, check, ptr
 NAME = "HIP (gfx950)"
 
 __all__ = ["NAME", "KernelUnavailable", "chosen_columns", "exact_attention", "choose_rows", "sparse_attention",
-           "verify_attention", "window_attention", "ring_attention", "tree_attention", "tree_ancestors", "kv_append"]
+           "verify_attention", "window_attention", "ring_attention", "tree_attention", "tree_ancestors", "kv_append",
+           "reorder_rows", "add_attention_weights", "choose_kept", "keep_rows"]
 
 
 def chosen_columns(top_k, window, N):
@@ -359,3 +362,152 @@ def kv_append(table, new, start, counts):
                                     new.stride(0), new.stride(1), ptr(start_), ptr(counts_), B, n, width,
                                     _lib.dtype_code(table.dtype), _lib.stream(table.device)), "kv_append")
     return table
+
+
+# ---- the cache's rows under beam search and eviction -------------------------------
+
+
+def _index(x, shape, name, device):
+    """An int64 tensor of the given shape, contiguous on the device."""
+    if tuple(x.shape) != shape:
+        raise ValueError(f"{name} must be {shape}; got {tuple(x.shape)}")
+    return _long(x, device)
+
+
+def _tables(tables, rows, what):
+    """(device, the library's table arguments: addresses, batch and row strides
+    in bytes, capacities, row bytes, count) of tables (rows, capacity, width)."""
+    tables = list(tables)
+    if not tables:
+        raise ValueError(f"{what}: no table given")
+    device = tables[0].device
+    count = len(tables)
+    for t in tables:
+        if t.dim() != 3 or t.shape[0] != rows or t.shape[2] == 0:
+            raise ValueError(f"{what}: each table must be ({rows}, capacity, width); got {tuple(t.shape)}")
+        if t.device != device or device.type != "cuda":
+            raise KernelUnavailable(f"{what} moves tables on one GPU; got tables on {device} and {t.device}")
+        if t.shape[2] > 1 and t.stride(2) != 1:
+            raise ValueError(f"{what}: each row of a table must be contiguous")
+    sizes = [t.element_size() for t in tables]
+    longs = ctypes.c_int64 * count
+    return device, (
+        (ctypes.c_void_p * count)(*[t.data_ptr() for t in tables]),
+        longs(*[t.stride(0) * s for t, s in zip(tables, sizes)]), longs(*[t.stride(1) * s for t, s in zip(tables, sizes)]),
+        longs(*[t.shape[1] for t in tables]), longs(*[t.shape[2] * s for t, s in zip(tables, sizes)]), count)
+
+
+def reorder_rows(tables, parents, lengths=None, rows=None):
+    """Beam search's reordering of states, in place: in each of tables
+    (n W, capacity, width) (one tensor or several, of any types and widths),
+    batch row i W + w becomes batch row i W + parents[i, w], every beam at
+    once: a beam may be taken several times, and one that nothing takes is
+    gone.  parents (n, W) int64, as sampling.beam_step gives them; one outside
+    0 .. W - 1 leaves its beam as it is.  lengths (n W,): only each source's
+    first lengths rows are taken (None: all); rows: an upper bound of the
+    lengths, where the program knows one.  At most 64 beams a text."""
+    if parents.dim() != 2:
+        raise ValueError(f"parents must be (texts, beams); got {tuple(parents.shape)}")
+    n, W = parents.shape
+    if W == 0:
+        raise ValueError("a text has at least one beam")
+    if parents.is_floating_point() or parents.dtype == torch.bool:
+        raise ValueError(f"parents are whole numbers; got {parents.dtype}")
+    if torch.is_tensor(tables):
+        tables = (tables,)
+    device, arguments = _tables(tables, n * W, "reorder_rows")
+    parents_ = _long(parents, device)
+    lengths_ = None if lengths is None else _index(lengths, (n * W,), "lengths", device)
+    if rows is None:
+        rows = max(arguments[3])
+    with _lib.on(device):
+        check(_lib.lib().wptv_reorder_rows(*arguments, ptr(parents_), ptr(lengths_), int(rows), n, W,
+                                           _lib.stream(device)), "reorder_rows")
+
+
+def add_attention_weights(q, k, positions, lse, scale, weights, *, counts=None, start=None, splits=0):
+    """Adds to weights (B, N) FP32, in place, the softmax weight that each row
+    of the table k (B, N, c) got from a reading's attention: the sum of
+    exp(scale q . k - lse) over the queries q (B, T, H, c) that see the row
+    (positions (B, T), as verify_attention) and their heads, lse (B, T, H) FP32
+    that attention's log-sum-exp.  counts (B,): the queries counted, the
+    others padding or drafts that were taken back (None: all); start (B,):
+    the rows from there on, the reading's own, begin at zero.  Rows past the
+    last counted position are left alone.  splits: parts of the queries (0:
+    the library chooses).  Returns weights."""
+    if k.dim() != 3:
+        raise ValueError(f"k must be (B, N, c); got {tuple(k.shape)}")
+    B, T, H, c, N = _check_inputs(q, k, k, positions)
+    device = q.device
+    if tuple(lse.shape) != (B, T, H) or lse.dtype != torch.float32 or lse.device != device:
+        raise ValueError(f"lse must be FP32 (B={B}, T={T}, H={H}) on {device}; got {lse.dtype} {tuple(lse.shape)}")
+    if tuple(weights.shape) != (B, N) or weights.dtype != torch.float32 or weights.device != device or \
+            (N > 1 and weights.stride(1) != 1):
+        raise ValueError(f"weights must be FP32 (B={B}, N={N}) on {device} with contiguous rows; got {weights.dtype} "
+                         f"{tuple(weights.shape)}")
+    if weights.requires_grad:
+        raise ValueError("weights are a cache's state: they take no gradient")
+    positions_ = _index(positions, (B, T), "positions", device)
+    counts_ = None if counts is None else _index(counts, (B,), "counts", device)
+    start_ = None if start is None else _index(start, (B,), "start", device)
+    q_, lse_ = q.contiguous(), lse.contiguous()
+    dtype = _lib.dtype_code(q.dtype)
+    with _lib.on(device):
+        parts, size = _lib.plan("wptv_attention_weights_workspace", "add_attention_weights", B, T, H, c, N, dtype,
+                                splits=int(splits))
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        check(_lib.lib().wptv_attention_weights(ptr(q_), ptr(k), k.stride(0), k.stride(1), dtype, ptr(positions_),
+                                                ptr(lse_), ptr(counts_), ptr(start_), B, T, H, c, N, float(scale),
+                                                parts, ptr(weights), weights.stride(0), ptr(workspace), size,
+                                                _lib.stream(device)), "add_attention_weights")
+    return weights
+
+
+def choose_kept(weights, lengths, keep, first=4, recent=128):
+    """The rows a cache bounded to `keep` rows keeps: (kept (L, B, keep) int64
+    in ascending order, then -1; counts (B,) = min(lengths, keep)).  Of each
+    layer's and batch row's first lengths[b] rows, all when they are at most
+    keep; else the first `first`, the last `recent`, and of the others those
+    of the largest weights (L, B, N) FP32 (add_attention_weights), equal
+    weights the lowest rows, a NaN the largest weight."""
+    if weights.dim() != 3 or weights.dtype != torch.float32:
+        raise ValueError(f"weights must be FP32 (layers, B, N); got {weights.dtype} {tuple(weights.shape)}")
+    if weights.device.type != "cuda":
+        raise KernelUnavailable(f"the HIP eviction runs on a GPU; the weights are on {weights.device}")
+    L, B, N = weights.shape
+    if N > 1 and weights.stride(2) != 1:
+        weights = weights.contiguous()
+    keep, first, recent = int(keep), int(first), int(recent)
+    if keep <= 0 or first < 0 or recent < 0 or first + recent > keep:
+        raise ValueError(f"keep = {keep} rows must hold the first {first} and the last {recent}")
+    device = weights.device
+    lengths_ = _index(lengths, (B,), "lengths", device)
+    kept = torch.empty(L, B, keep, dtype=torch.long, device=device)
+    counts = torch.empty(B, dtype=torch.long, device=device)
+    with _lib.on(device):
+        check(_lib.lib().wptv_choose_kept(ptr(weights), weights.stride(0), weights.stride(1), ptr(lengths_), L, B, N,
+                                          keep, first, recent, ptr(kept), ptr(counts), _lib.stream(device)),
+              "choose_kept")
+    return kept, counts
+
+
+def keep_rows(tables, kept, counts):
+    """Moves the kept rows of each of tables (B, capacity, width) together, in
+    place: row j becomes row kept[i, b, j] for j < counts[b], i the table's
+    place among tables (modulo kept's layers: several tables a layer in
+    turn).  kept (L, B, keep) int64 ascending, as choose_kept gives it; rows
+    from counts[b] on keep what they hold.  tables: one tensor or several, of
+    any types and widths."""
+    if torch.is_tensor(tables):
+        tables = (tables,)
+    if kept.dim() != 3:
+        raise ValueError(f"kept must be (layers, B, keep); got {tuple(kept.shape)}")
+    L, B, keep = kept.shape
+    device, arguments = _tables(tables, B, "keep_rows")
+    if L == 0 or arguments[5] % L:
+        raise ValueError(f"keep_rows: {arguments[5]} tables for {L} lists of rows")
+    kept_ = _long(kept, device)
+    counts_ = _index(counts, (B,), "counts", device)
+    with _lib.on(device):
+        check(_lib.lib().wptv_keep_rows(*arguments, ptr(kept_), L, keep, ptr(counts_), B, _lib.stream(device)),
+              "keep_rows")

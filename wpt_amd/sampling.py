@@ -16,13 +16,15 @@ the reference's tokens.  `accept` reads a tape drawn up front instead,
 built from what a lazy run drew replays it exactly.
 """
 
+import ctypes
+
 import torch
 
 from . import _lib
 from ._lib import KernelUnavailable, check, ptr
 
 __all__ = ["accept", "accept_in_order", "generator_state", "set_offset", "greedy_chain", "greedy_tree",
-           "greedy_tree_from_argmax", "draws", "written"]
+           "greedy_tree_from_argmax", "draws", "written", "beam_step"]
 
 
 def _on_gpu(*tensors):
@@ -299,3 +301,49 @@ def written(tokens, counts):
                                f"draw from")
         out.append(rows[b][:n])
     return out
+
+
+def beam_step(scores, totals, ended=None, stops=(), beams=None):
+    """Beam search's selection: the next `beams` beams (None: W) of each text
+    over its W beams and the vocabulary, (totals (n, beams) FP32 in falling
+    order, parents (n, beams) int64, tokens (n, beams) int64, ended
+    (n, beams) bool), with no host synchronization.
+
+    scores (n, W, V) FP32 or bf16: the model's scores after each beam's last
+    token; totals (n, W) FP32: each beam's summed log-probability so far (-inf
+    for a place that holds no beam, as all but one at a text's start).  A
+    candidate's value is its beam's total plus the log-softmax of its score,
+    ranked in 64 bits, equal values to the lowest beam, then token.  stops: the
+    token ids that end a beam (at most 16); ended (n, W) bool: such a beam
+    goes on as one candidate, its first stop token at its own total.  A beam
+    whose total is not finite, or whose scores hold a NaN or +inf or nothing
+    above -inf, has every candidate at -inf.  At most 64 beams a text."""
+    scores = _scores(scores)
+    n, W, V = scores.shape
+    device = scores.device
+    _on_gpu(scores)
+    K = W if beams is None else int(beams)
+    if totals.shape != (n, W) or totals.dtype != torch.float32 or totals.device != device:
+        raise ValueError(f"totals must be FP32 (n={n}, W={W}) on {device}; got {totals.dtype} {tuple(totals.shape)}")
+    if ended is not None and (ended.shape != (n, W) or ended.dtype != torch.bool or ended.device != device):
+        raise ValueError(f"ended must be bool (n={n}, W={W}) on {device}; got {ended.dtype} {tuple(ended.shape)}")
+    if K < 1:
+        raise ValueError(f"a text goes on with at least one beam, not {K}")
+    stops = [int(s) for s in stops]
+    if any(not 0 <= s < V for s in stops):
+        raise ValueError(f"stop tokens lie in [0, {V}); got {stops}")
+    new_totals = torch.empty(n, K, dtype=torch.float32, device=device)
+    parents = torch.empty(n, K, dtype=torch.long, device=device)
+    tokens = torch.empty(n, K, dtype=torch.long, device=device)
+    new_ended = torch.empty(n, K, dtype=torch.bool, device=device)
+    totals = totals.contiguous()
+    ended = None if ended is None else ended.contiguous()
+    with _lib.on(device):
+        _, size = _lib.plan("wptv_beam_workspace", "beam_step", n, W, V, K)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        check(_lib.lib().wptv_beam_step(ptr(scores), scores.stride(0), scores.stride(1),
+                                        _lib.dtype_code(scores.dtype), ptr(totals), ptr(ended),
+                                        (ctypes.c_int64 * len(stops))(*stops), len(stops), n, W, V, K,
+                                        ptr(new_totals), ptr(parents), ptr(tokens), ptr(new_ended), ptr(workspace),
+                                        size, _lib.stream(device)), "beam_step")
+    return new_totals, parents, tokens, new_ended
