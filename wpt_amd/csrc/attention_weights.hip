@@ -9,8 +9,13 @@
 // begin at zero: a draft that was taken back leaves nothing behind.  Rows past
 // the last counted position are not touched.
 //
-// No atomics: a wavefront owns its rows and takes the queries in order, so the
-// sums do not depend on the launch.
+// No atomics: a wavefront owns its rows and takes the queries in order, and the
+// parts that many queries are cut into are joined in order, so the sums do not
+// depend on the launch.
+//   attention_weights_mfma     head widths 64 and 128: the products on the
+//                              matrix cores
+//   attention_weights_join     the parts' sums
+//   attention_weights_generic  any other width up to 256, or unaligned rows
 #include "wptv_common.h"
 
 #include <climits>
@@ -22,7 +27,7 @@ constexpr int kKeys = 64;   // table rows of a workgroup of the generic kernel
 constexpr int kGT = 256;
 constexpr int kMaxWidth = 256;
 
-// The counted queries of batch row b, and the last row they see (-1: none).
+// The counted queries of batch row b.
 __device__ __forceinline__ int counted(const int64_t* counts, int b, int T) {
   if (!counts) return T;
   const int64_t n = counts[b];
@@ -70,6 +75,199 @@ __global__ __launch_bounds__(kGT) void attention_weights_generic(
   }
 }
 
+// ---- the matrix-core form ------------------------------------------------------
+
+constexpr int kWaveKeys = 64;    // table rows of a wavefront
+constexpr int kBlockKeys = 256;  // of a workgroup of four
+constexpr int kStage = 1024;     // query heads whose lse and position are staged in LDS at once
+constexpr int kPartRows = 128;   // the fewest query heads of a part
+
+// 16 rows of C values as an operand of the 16-row matrix instructions: lane
+// 16 g + j holds parts of row j.  The products only need both operands to agree
+// on the order of the C values.
+template <typename E, int C>
+struct Rows16;
+
+template <int C>
+struct Rows16<unsigned short, C> {
+  bf16x8 v[C / 32];
+  __device__ __forceinline__ void load(const unsigned short* row, int g) {
+#pragma unroll
+    for (int s = 0; s < C / 32; ++s) v[s] = *reinterpret_cast<const bf16x8*>(row + 32 * s + 8 * g);
+  }
+  static constexpr int kSteps = C / 32;
+  static __device__ __forceinline__ f32x4 step(const Rows16& a, const Rows16& b, int s, f32x4 acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[s], b.v[s], acc, 0, 0, 0);
+  }
+};
+
+template <int C>
+struct Rows16<float, C> {
+  f32x4 v[C / 16];
+  __device__ __forceinline__ void load(const float* row, int g) {
+#pragma unroll
+    for (int s = 0; s < C / 16; ++s) v[s] = *reinterpret_cast<const f32x4*>(row + 16 * s + 4 * g);
+  }
+  static constexpr int kSteps = C / 4;
+  static __device__ __forceinline__ f32x4 step(const Rows16& a, const Rows16& b, int s, f32x4 acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[s / 4][s % 4], b.v[s / 4][s % 4], acc, 0, 0, 0);
+  }
+};
+
+// A wavefront holds 64 table rows as the second operand of four products and
+// streams the query heads, 16 at a time, through the first: a lane ends with
+// four query heads of one row in each, whose exponentials it adds to that row's
+// sum in a register.  Nothing but the sums is written.
+template <typename E, int C>
+__global__ __launch_bounds__(256) void attention_weights_mfma(
+    const E* __restrict__ q, const E* __restrict__ k, int64_t ksb, int64_t ksn, const int64_t* __restrict__ positions,
+    const float* __restrict__ lse, const int64_t* __restrict__ counts, const int64_t* __restrict__ start, int B, int T,
+    int H, int N, float scale_log2, int nkb, int parts, int part_rows, float* __restrict__ weights, int64_t wsb,
+    float* __restrict__ sums) {
+  typedef Rows16<E, C> Op;
+  __shared__ __attribute__((aligned(16))) float l2s[kStage];
+  __shared__ __attribute__((aligned(16))) int seen[kStage];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 15, g = lane >> 4;
+  int kb, b, part;
+  if (parts == 1) {
+    kb = blockIdx.x % nkb;
+    b = blockIdx.x / nkb;
+    part = 0;
+  } else {  // workgroups go to the 8 XCDs in turn: a part's queries are read through one XCD's L2
+    int rest = blockIdx.x / 8;
+    kb = rest % nkb;
+    rest /= nkb;
+    b = rest % B;
+    part = rest / B * 8 + blockIdx.x % 8;
+    if (part >= parts) return;
+  }
+  const int64_t rows_b = (int64_t)b * T * H;
+  const int first = part * part_rows;
+  const int end = min(counted(counts, b, T) * H, first + part_rows);
+  // the rows that the part's queries see end at hi, and each sees those up to lo
+  const int64_t* pos = positions + (int64_t)b * T;
+  int lo = N - 1, hi = -1;
+  if (first < end) {
+    for (int t = first / H + lane; t <= (end - 1) / H; t += 64) {
+      const int64_t p = pos[t];
+      const int c = p < 0 ? -1 : p < N ? (int)p : N - 1;
+      lo = min(lo, c);
+      hi = max(hi, c);
+    }
+    lo = wave_min_i32(lo);
+    hi = wave_max_i32(hi);
+  }
+  const int n0 = kb * kBlockKeys, wn0 = n0 + kWaveKeys * w, n = wn0 + lane;
+  float total = 0.f;
+  if (n0 <= hi) {
+    Op keys[4];
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      keys[u].load(k + (int64_t)b * ksb + (int64_t)min(wn0 + 16 * u + j, N - 1) * ksn, g);
+    const bool whole = wn0 + kWaveKeys - 1 <= lo;
+    for (int s0 = first; s0 < end; s0 += kStage) {
+      const int many = min(kStage, end - s0), blocks = (many + 15) / 16;
+      if (s0 > first) __syncthreads();
+      for (int i = tid; i < 16 * blocks; i += 256) {  // padding query heads: the last one again, at no weight
+        const int r = min(s0 + i, end - 1);
+        const int64_t p = pos[r / H];
+        l2s[i] = i < many ? lse[rows_b + r] * kLog2e : __builtin_inff();
+        seen[i] = i >= many || p < 0 ? -1 : p < N ? (int)p : N - 1;
+      }
+      __syncthreads();
+      if (wn0 > hi) continue;
+      const E* qs = q + (rows_b + s0) * C;
+      for (int m = 0; m < blocks; ++m) {
+        Op query;
+        query.load(qs + (int64_t)min(16 * m + j, many - 1) * C, g);
+        const f32x4 l2 = *reinterpret_cast<const f32x4*>(&l2s[16 * m + 4 * g]);
+        f32x4 acc[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < Op::kSteps; ++s)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) acc[u] = Op::step(query, keys[u], s, acc[u]);
+        // acc[u][i]: query head 16 m + 4 g + i, row wn0 + 16 u + j
+        if (whole) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(acc[u][i], scale_log2, -l2[i]));
+            sum[u] += (e[0] + e[1]) + (e[2] + e[3]);
+          }
+        } else {
+          const i32x4 p = *reinterpret_cast<const i32x4*>(&seen[16 * m + 4 * g]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float x = __builtin_amdgcn_exp2f(fmaf(acc[u][i], scale_log2, -l2[i]));
+              e[i] = wn0 + 16 * u + j <= p[i] ? x : 0.f;  // an unseen row may hold anything
+            }
+            sum[u] += (e[0] + e[1]) + (e[2] + e[3]);
+          }
+        }
+      }
+    }
+    // the four lane groups' sums of the four blocks, block u into lane group u
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[0]), __float_as_uint(sum[1]), false, false);
+    const auto c = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[2]), __float_as_uint(sum[3]), false, false);
+    const float z01 = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const float z23 = __uint_as_float(c[0]) + __uint_as_float(c[1]);
+    const auto d = __builtin_amdgcn_permlane32_swap(__float_as_uint(z01), __float_as_uint(z23), false, false);
+    total = __uint_as_float(d[0]) + __uint_as_float(d[1]);
+  }
+  if (parts > 1) {
+    sums[((int64_t)part * B + b) * nkb * kBlockKeys + n] = total;
+  } else if (n <= hi) {
+    float* out = weights + (int64_t)b * wsb + n;
+    *out = (start && n >= start[b] ? 0.f : *out) + total;
+  }
+}
+
+__global__ __launch_bounds__(256) void attention_weights_join(const float* __restrict__ sums, int parts, int nkb, int B,
+                                                              int T, int N, const int64_t* __restrict__ positions,
+                                                              const int64_t* __restrict__ counts,
+                                                              const int64_t* __restrict__ start,
+                                                              float* __restrict__ weights, int64_t wsb) {
+  __shared__ int most[4];
+  const int b = blockIdx.y, n = blockIdx.x * kBlockKeys + threadIdx.x;
+  const int tn = counted(counts, b, T);
+  int hi = -1;
+  for (int t = threadIdx.x; t < tn; t += 256) {
+    const int64_t p = positions[(int64_t)b * T + t];
+    hi = max(hi, p < 0 ? -1 : p < N ? (int)p : N - 1);
+  }
+  hi = wave_max_i32(hi);
+  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = hi;
+  __syncthreads();
+  hi = max(max(most[0], most[1]), max(most[2], most[3]));
+  if (n > hi) return;
+  float* out = weights + (int64_t)b * wsb + n;
+  const float before = start && n >= start[b] ? 0.f : *out;
+  const int64_t stride = (int64_t)B * nkb * kBlockKeys;
+  const float* s = sums + (int64_t)b * nkb * kBlockKeys + n;
+  float total = 0.f;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) total += s[p * stride];
+  *out = before + total;
+}
+
+// The parts the T H query heads are cut into: enough that B x (blocks of 256
+// rows) x parts workgroups fill the GPU, of at least kPartRows query heads.
+int weight_parts(int B, int T, int H, int N) {
+  const int64_t rows = (int64_t)T * H, units = (int64_t)B * ((N + kBlockKeys - 1) / kBlockKeys);
+  const int64_t fill = (8 * compute_units() + units - 1) / units;
+  return (int)max((int64_t)1, min(fill, rows / kPartRows));
+}
+
+bool matrix_width(int c) { return c == 64 || c == 128; }
+
 }  // namespace
 }  // namespace wptv
 
@@ -83,11 +281,21 @@ extern "C" int wptv_attention_weights_workspace(int B, int T, int H, int c, int 
   if (dtype != WPTV_F32 && dtype != WPTV_BF16) return fail(WPTV_E_UNSUPPORTED, "attention_weights: dtype %d", dtype);
   if (c > kMaxWidth)
     return fail(WPTV_E_UNSUPPORTED, "attention_weights: head width at most %d (got %d)", kMaxWidth, c);
-  if ((int64_t)T * H > INT32_MAX || (int64_t)B * ((N + kKeys - 1) / kKeys) > INT32_MAX)
+  if ((int64_t)T * H > (1 << 29) || (int64_t)B * ((N + kKeys - 1) / kKeys) > INT32_MAX)
     return fail(WPTV_E_UNSUPPORTED, "attention_weights: B=%d T=%d H=%d N=%d is too large", B, T, H, N);
   if (*splits < 0) return fail(WPTV_E_INVALID, "attention_weights: splits = %d", *splits);
-  *splits = 1;
-  *bytes = 0;
+  const int64_t rows = (int64_t)T * H;
+  if (!matrix_width(c) || B == 0 || rows == 0) {
+    *splits = 1;
+  } else if (*splits == 0) {
+    *splits = weight_parts(B, T, H, N);
+  } else {
+    *splits = (int)min((int64_t)*splits, (rows + 15) / 16);  // a part holds at least one block of query heads
+  }
+  const int64_t nkb = (N + kBlockKeys - 1) / kBlockKeys;
+  if ((int64_t)B * nkb * (*splits + 8) > INT32_MAX)
+    return fail(WPTV_E_UNSUPPORTED, "attention_weights: B=%d N=%d in %d parts is too large", B, N, *splits);
+  *bytes = *splits == 1 ? 0 : (size_t)*splits * B * nkb * kBlockKeys * sizeof(float);
   return WPTV_OK;
 }
 
@@ -107,6 +315,28 @@ extern "C" int wptv_attention_weights(const void* q, const void* k, int64_t k_st
                 (long long)k_stride_n, (long long)weights_stride_b);
   if (workspace_bytes < need || (need && !workspace))
     return fail(WPTV_E_INVALID, "attention_weights: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  const int elem = dtype == WPTV_BF16 ? 2 : 4;
+  if (matrix_width(c) && aligned(q, 16) && aligned(k, 16) && k_stride_n * elem % 16 == 0 && k_stride_b * elem % 16 == 0) {
+    const int blocks = (N + kBlockKeys - 1) / kBlockKeys;
+    const int part_rows = (int)(((int64_t)T * H + splits - 1) / splits + 15) / 16 * 16;
+    const int groups = splits == 1 ? 1 : (splits + 7) / 8 * 8;
+    float* sums = static_cast<float*>(workspace);
+#define WPTV_WEIGHTS(E, C)                                                                                            \
+  attention_weights_mfma<E, C><<<B * blocks * groups, 256, 0, stream>>>(                                             \
+      static_cast<const E*>(q), static_cast<const E*>(k), k_stride_b, k_stride_n, positions, lse, counts, start, B, T, \
+      H, N, scale * kLog2e, blocks, splits, part_rows, weights, weights_stride_b, sums)
+    if (dtype == WPTV_BF16) {
+      if (c == 64) WPTV_WEIGHTS(unsigned short, 64); else WPTV_WEIGHTS(unsigned short, 128);
+    } else {
+      if (c == 64) WPTV_WEIGHTS(float, 64); else WPTV_WEIGHTS(float, 128);
+    }
+#undef WPTV_WEIGHTS
+    const int launch = launched("attention_weights_mfma");
+    if (launch != WPTV_OK || splits == 1) return launch;
+    attention_weights_join<<<dim3(blocks, B), 256, 0, stream>>>(sums, splits, blocks, B, T, N, positions, counts, start,
+                                                                weights, weights_stride_b);
+    return launched("attention_weights_join");
+  }
   const int nkb = (N + kKeys - 1) / kKeys;
 #define WPTV_WEIGHTS(E, CMAX)                                                                                        \
   attention_weights_generic<E, CMAX><<<B * nkb, kGT, 0, stream>>>(                                                   \
