@@ -29,6 +29,7 @@ struct Table {
   int64_t stride_b, stride_n;  // bytes
   int capacity;
   int pieces;  // a row's pieces of the launch's unit
+  int list;    // keep_rows: which layer's list of rows
 };
 
 struct Tables {
@@ -60,11 +61,10 @@ struct Unit<1> {
 
 constexpr int kThreads = 256;
 
-// The source beam of beam w of a text: itself where the given one is none of
-// the text's.
-__device__ __forceinline__ int source_beam(const int64_t* parents, int w, int W) {
-  const int64_t p = parents[w];
-  return p >= 0 && p < W ? (int)p : w;
+// p[i] of an input that no kernel of the launch writes: a scalar load where i
+// is uniform.
+__device__ __forceinline__ int64_t const_load(const int64_t* p, int64_t i) {
+  return ((const __attribute__((address_space(4))) int64_t*)(uintptr_t)p)[i];
 }
 
 // W <= WMAX: the beams' pieces of one place in registers.
@@ -73,22 +73,23 @@ __global__ __launch_bounds__(kThreads) void reorder_rows(Tables tables, const in
                                                          const int64_t* __restrict__ lengths, int W) {
   typedef typename Unit<BYTES>::type U;
   const Table& t = tables.t[blockIdx.z];
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t n = at / t.pieces;
-  const int piece = (int)(at % t.pieces);
+  const int text = blockIdx.y;
+  const uint32_t at = blockIdx.x * kThreads + threadIdx.x;  // below 2^31: checked on the host
+  const int n = (int)(at / (uint32_t)t.pieces);
+  const int piece = (int)(at % (uint32_t)t.pieces);
   if (n >= t.capacity) return;
-  const int64_t text = blockIdx.y;
-  const int64_t* p = parents + text * W;
-  unsigned char* place = t.base + text * W * t.stride_b + n * t.stride_n + (int64_t)piece * BYTES;
+  unsigned char* place = t.base + (int64_t)text * W * t.stride_b + n * t.stride_n + (int64_t)piece * BYTES;
   U held[WMAX];
   bool moves[WMAX];
 #pragma unroll
   for (int w = 0; w < WMAX; ++w) {
     moves[w] = false;
     if (w < W) {
-      const int from = source_beam(p, w, W);
-      moves[w] = from != w && (!lengths || n < lengths[text * W + from]);
-      if (moves[w]) held[w] = *reinterpret_cast<const U*>(place + from * t.stride_b);
+      const int64_t from = const_load(parents, (int64_t)text * W + w);  // one that is no beam of the text moves nothing
+      if (from >= 0 && from < W && from != w) {
+        moves[w] = !lengths || n < const_load(lengths, (int64_t)text * W + from);
+        if (moves[w]) held[w] = *reinterpret_cast<const U*>(place + from * t.stride_b);
+      }
     }
   }
 #pragma unroll
@@ -96,31 +97,43 @@ __global__ __launch_bounds__(kThreads) void reorder_rows(Tables tables, const in
     if (w < W && moves[w]) *reinterpret_cast<U*>(place + w * t.stride_b) = held[w];
 }
 
+constexpr int kKeepThreads = 512;
+constexpr int kKeepLoads = 8;  // rows a thread holds at once
+
+// A step holds kKeepLoads rows a thread of the slice, 64 KB a workgroup at the
+// widest unit: its sources' loads are all in flight together, and the step costs
+// one memory round trip however the rows lie.
 template <int BYTES>
-__global__ __launch_bounds__(kThreads) void keep_rows(Tables tables, const int64_t* __restrict__ kept, int first_list,
-                                                      int lists, int B, int keep, const int64_t* __restrict__ counts,
-                                                      int slice_pieces) {
+__global__ __launch_bounds__(kKeepThreads) void keep_rows(Tables tables, const int64_t* __restrict__ kept, int B,
+                                                          int keep, const int64_t* __restrict__ counts,
+                                                          int slice_shift) {
   typedef typename Unit<BYTES>::type U;
   const Table& t = tables.t[blockIdx.z];
   const int b = blockIdx.y;
-  const int piece = blockIdx.x * slice_pieces + threadIdx.x % slice_pieces;
-  const int rows = kThreads / slice_pieces;  // rows a step
-  const int r = threadIdx.x / slice_pieces;
-  int64_t live = counts[b];
-  live = live < keep ? live : keep;
-  const int64_t* list = kept + ((int64_t)((first_list + blockIdx.z) % lists) * B + b) * keep;
+  const int piece = (blockIdx.x << slice_shift) + (threadIdx.x & ((1 << slice_shift) - 1));
+  const int rows = kKeepThreads >> slice_shift;  // rows of one load of the workgroup
+  const int r = threadIdx.x >> slice_shift;
+  const int64_t count = const_load(counts, b);
+  const int live = (int)min(count, (int64_t)min(keep, t.capacity));
+  const int64_t* list = kept + ((int64_t)t.list * B + b) * keep;
   unsigned char* column = t.base + b * t.stride_b + (int64_t)piece * BYTES;
-  for (int64_t j0 = 0; j0 < live; j0 += rows) {
-    const int64_t j = j0 + r;
-    U held;
-    bool moves = false;
-    if (r < rows && piece < t.pieces && j < live && j < t.capacity) {
-      const int64_t from = list[j];
-      moves = from > j && from < t.capacity;
-      if (moves) held = *reinterpret_cast<const U*>(column + from * t.stride_n);
+  const bool inside = piece < t.pieces;
+  for (int j0 = 0; j0 < live; j0 += rows * kKeepLoads) {
+    int64_t from[kKeepLoads];
+    U held[kKeepLoads];
+#pragma unroll
+    for (int i = 0; i < kKeepLoads; ++i) {
+      const int j = j0 + i * rows + r;
+      from[i] = inside && j < live ? list[j] : -1;
+      if (from[i] <= j || from[i] >= t.capacity) from[i] = -1;  // in its place already, or no row
     }
+#pragma unroll
+    for (int i = 0; i < kKeepLoads; ++i)
+      if (from[i] >= 0) held[i] = *reinterpret_cast<const U*>(column + from[i] * t.stride_n);
     __syncthreads();  // every source of the step is read
-    if (moves) *reinterpret_cast<U*>(column + j * t.stride_n) = held;
+#pragma unroll
+    for (int i = 0; i < kKeepLoads; ++i)
+      if (from[i] >= 0) *reinterpret_cast<U*>(column + (j0 + i * rows + r) * t.stride_n) = held[i];
   }
 }
 
@@ -131,8 +144,9 @@ int unit_of(const void* base, int64_t sb, int64_t sn, int64_t row_bytes) {
 }
 
 // Host checks of one table of `rows_b` batch rows.
-int check_table(const char* what, int i, const void* base, int64_t sb, int64_t sn, int64_t capacity, int64_t row_bytes,
+int check_table(const char* what, int i, void* const* bases, int64_t sb, int64_t sn, int64_t capacity, int64_t row_bytes,
                 int64_t rows_b) {
+  const void* base = bases[i];
   if (capacity < 0 || capacity > INT32_MAX || row_bytes <= 0 || row_bytes > INT32_MAX)
     return fail(WPTV_E_INVALID, "%s: table %d has capacity %lld and rows of %lld bytes", what, i, (long long)capacity,
                 (long long)row_bytes);
@@ -142,12 +156,15 @@ int check_table(const char* what, int i, const void* base, int64_t sb, int64_t s
   const bool apart_b = rows_b <= 1 || sb >= row_bytes;
   const bool nested = capacity <= 1 || rows_b <= 1 || sb >= (capacity - 1) * sn + row_bytes ||
                       sn >= (rows_b - 1) * sb + row_bytes;
+  for (int other = 0; other < i; ++other)
+    if (base && bases[other] == base) return fail(WPTV_E_INVALID, "%s: tables %d and %d are the same", what, other, i);
   if (!apart_n || !apart_b || !nested)
     return fail(WPTV_E_INVALID, "%s: the rows of table %d overlap (strides %lld and %lld bytes, rows of %lld)", what, i,
                 (long long)sb, (long long)sn, (long long)row_bytes);
   return WPTV_OK;
 }
 
+// W <= 16, or a unit of at most 4 bytes.
 template <int BYTES>
 int launch_reorder(const Tables& tables, int count, int64_t blocks, int n, const int64_t* parents,
                    const int64_t* lengths, int W, hipStream_t stream) {
@@ -164,11 +181,44 @@ int launch_reorder(const Tables& tables, int count, int64_t blocks, int n, const
 }
 
 template <int BYTES>
-int launch_keep(const Tables& tables, int count, int slices, int slice_pieces, const int64_t* kept, int first_list,
-                int lists, int B, int keep, const int64_t* counts, hipStream_t stream) {
-  keep_rows<BYTES><<<dim3(slices, B, count), kThreads, 0, stream>>>(tables, kept, first_list, lists, B, keep, counts,
-                                                                    slice_pieces);
+int launch_keep(const Tables& tables, int count, int widest, const int64_t* kept, int B, int keep,
+                const int64_t* counts, hipStream_t stream) {
+  // slices of a row, one a workgroup: whole 128-byte lines where the slices fill
+  // the compute units twice, thinner ones where there are few (down to a unit)
+  int shift = 0;
+  while ((BYTES << (shift + 1)) <= 128 && (1 << shift) < widest) ++shift;
+  while (shift > 0 && (int64_t)count * B * ((widest + (1 << shift) - 1) >> shift) < 2 * compute_units()) --shift;
+  const int slices = (widest + (1 << shift) - 1) >> shift;
+  keep_rows<BYTES><<<dim3(slices, B, count), kKeepThreads, 0, stream>>>(tables, kept, B, keep, counts, shift);
   return launched("keep_rows");
+}
+
+// Calls launch(unit, tables, how many, the largest `size` of them) for up to
+// kTables tables of one unit at a time, wider units first.
+template <typename Size, typename Launch>
+int each_launch(void* const* tables, const int64_t* strides_b, const int64_t* strides_n, const int64_t* capacities,
+                const int64_t* row_bytes, int count, int lists, int widest_unit, Size size, Launch launch) {
+  for (int unit = widest_unit; unit >= 1; unit /= 2) {
+    Tables held;
+    int many = 0;
+    int64_t most = 0;
+    for (int i = 0; i <= count; ++i) {
+      if (i < count && capacities[i] > 0 &&
+          min(unit_of(tables[i], strides_b[i], strides_n[i], row_bytes[i]), widest_unit) == unit) {
+        Table& t = held.t[many++];
+        t = Table{static_cast<unsigned char*>(tables[i]), strides_b[i], strides_n[i], (int)capacities[i],
+                  (int)(row_bytes[i] / unit), i % lists};
+        most = max(most, (int64_t)size(t));
+      }
+      if (many == kTables || (i == count && many)) {
+        const int status = launch(unit, held, many, most);
+        if (status != WPTV_OK) return status;
+        many = 0;
+        most = 0;
+      }
+    }
+  }
+  return WPTV_OK;
 }
 
 }  // namespace
@@ -187,49 +237,30 @@ extern "C" int wptv_reorder_rows(void* const* tables, const int64_t* strides_b, 
   if (count && (!tables || !strides_b || !strides_n || !capacities || !row_bytes))
     return fail(WPTV_E_INVALID, "reorder_rows: the tables' addresses and shapes must be given");
   for (int i = 0; i < count; ++i) {
-    const int status = check_table("reorder_rows", i, tables[i], strides_b[i], strides_n[i], capacities[i],
+    const int status = check_table("reorder_rows", i, tables, strides_b[i], strides_n[i], capacities[i],
                                    row_bytes[i], (int64_t)n * W);
     if (status != WPTV_OK) return status;
   }
   if (count == 0 || n == 0 || W == 1) return WPTV_OK;
   if (!parents) return fail(WPTV_E_INVALID, "reorder_rows: parents is NULL");
-  // a launch for up to kTables tables of one unit
-  for (int unit = 16; unit >= 1; unit /= 2) {
-    Tables held;
-    int many = 0;
-    int64_t blocks = 0;
-    for (int i = 0; i <= count; ++i) {
-      if (i < count && capacities[i] > 0) {
-        int u = unit_of(tables[i], strides_b[i], strides_n[i], row_bytes[i]);
-        if (W > 16 && u > 4) u = 4;  // 64 beams' pieces in registers
-        if (u == unit) {
-          const int64_t reach = lengths && rows < capacities[i] ? rows : capacities[i];
-          const int64_t pieces = row_bytes[i] / unit;
-          held.t[many++] = Table{static_cast<unsigned char*>(tables[i]), strides_b[i], strides_n[i], (int)reach,
-                                 (int)pieces};
-          const int64_t need = (reach * pieces + kThreads - 1) / kThreads;
-          if (need > INT32_MAX) return fail(WPTV_E_UNSUPPORTED, "reorder_rows: table %d is too large", i);
-          blocks = blocks > need ? blocks : need;
-        }
-      }
-      if (many == kTables || (i == count && many)) {
-        int status = WPTV_OK;
-        if (blocks) {
-          switch (unit) {
-            case 16: status = launch_reorder<16>(held, many, blocks, n, parents, lengths, W, stream); break;
-            case 8: status = launch_reorder<8>(held, many, blocks, n, parents, lengths, W, stream); break;
-            case 4: status = launch_reorder<4>(held, many, blocks, n, parents, lengths, W, stream); break;
-            case 2: status = launch_reorder<2>(held, many, blocks, n, parents, lengths, W, stream); break;
-            default: status = launch_reorder<1>(held, many, blocks, n, parents, lengths, W, stream); break;
-          }
-        }
-        if (status != WPTV_OK) return status;
-        many = 0;
-        blocks = 0;
-      }
+  const int widest = W > 16 ? 4 : 16;  // 64 beams' pieces are held in registers
+  auto size = [&](Table& t) {
+    if (lengths) t.capacity = (int)min((int64_t)t.capacity, rows);
+    return (int64_t)t.capacity * t.pieces;
+  };
+  auto launch = [&](int unit, const Tables& held, int many, int64_t most) {
+    if (most > INT32_MAX - kThreads) return fail(WPTV_E_UNSUPPORTED, "reorder_rows: a batch row of 2^31 pieces");
+    const int64_t blocks = (most + kThreads - 1) / kThreads;
+    if (blocks == 0) return (int)WPTV_OK;
+    switch (unit) {
+      case 16: return launch_reorder<16>(held, many, blocks, n, parents, lengths, W, stream);
+      case 8: return launch_reorder<8>(held, many, blocks, n, parents, lengths, W, stream);
+      case 4: return launch_reorder<4>(held, many, blocks, n, parents, lengths, W, stream);
+      case 2: return launch_reorder<2>(held, many, blocks, n, parents, lengths, W, stream);
+      default: return launch_reorder<1>(held, many, blocks, n, parents, lengths, W, stream);
     }
-  }
-  return WPTV_OK;
+  };
+  return each_launch(tables, strides_b, strides_n, capacities, row_bytes, count, 1, widest, size, launch);
 }
 
 extern "C" int wptv_keep_rows(void* const* tables, const int64_t* strides_b, const int64_t* strides_n,
@@ -242,28 +273,20 @@ extern "C" int wptv_keep_rows(void* const* tables, const int64_t* strides_b, con
     return fail(WPTV_E_INVALID, "keep_rows: the tables' addresses and shapes must be given");
   for (int i = 0; i < count; ++i) {
     const int status =
-        check_table("keep_rows", i, tables[i], strides_b[i], strides_n[i], capacities[i], row_bytes[i], B);
+        check_table("keep_rows", i, tables, strides_b[i], strides_n[i], capacities[i], row_bytes[i], B);
     if (status != WPTV_OK) return status;
   }
   if (count == 0 || B == 0 || keep == 0) return WPTV_OK;
   if (!kept || !counts) return fail(WPTV_E_INVALID, "keep_rows: kept and counts must be given");
-  for (int i = 0; i < count; ++i) {
-    if (capacities[i] == 0) continue;
-    Tables held;
-    const int unit = unit_of(tables[i], strides_b[i], strides_n[i], row_bytes[i]);
-    const int pieces = (int)(row_bytes[i] / unit);
-    const int slice = pieces < 8 ? pieces : 8;
-    const int slices = (pieces + slice - 1) / slice;
-    held.t[0] = Table{static_cast<unsigned char*>(tables[i]), strides_b[i], strides_n[i], (int)capacities[i], pieces};
-    int status;
+  auto size = [](Table& t) { return t.pieces; };
+  auto launch = [&](int unit, const Tables& held, int many, int64_t most) {
     switch (unit) {
-      case 16: status = launch_keep<16>(held, 1, slices, slice, kept, i, lists, B, keep, counts, stream); break;
-      case 8: status = launch_keep<8>(held, 1, slices, slice, kept, i, lists, B, keep, counts, stream); break;
-      case 4: status = launch_keep<4>(held, 1, slices, slice, kept, i, lists, B, keep, counts, stream); break;
-      case 2: status = launch_keep<2>(held, 1, slices, slice, kept, i, lists, B, keep, counts, stream); break;
-      default: status = launch_keep<1>(held, 1, slices, slice, kept, i, lists, B, keep, counts, stream); break;
+      case 16: return launch_keep<16>(held, many, (int)most, kept, B, keep, counts, stream);
+      case 8: return launch_keep<8>(held, many, (int)most, kept, B, keep, counts, stream);
+      case 4: return launch_keep<4>(held, many, (int)most, kept, B, keep, counts, stream);
+      case 2: return launch_keep<2>(held, many, (int)most, kept, B, keep, counts, stream);
+      default: return launch_keep<1>(held, many, (int)most, kept, B, keep, counts, stream);
     }
-    if (status != WPTV_OK) return status;
-  }
-  return WPTV_OK;
+  };
+  return each_launch(tables, strides_b, strides_n, capacities, row_bytes, count, lists, 16, size, launch);
 }

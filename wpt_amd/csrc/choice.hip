@@ -34,6 +34,7 @@
 //                    byte first; the scores stay in L2), then one pass that
 //                    compacts the chosen rows in row order with wavefront
 //                    ballots
+#include "select_common.h"
 #include "wptv_common.h"
 
 namespace wptv {
@@ -352,27 +353,10 @@ __global__ __launch_bounds__(kST) void choice_select(const float* __restrict__ s
   }
 }
 
-// The sum over the lanes up to and including this one; every lane must be
-// active (DPP: shifts within the rows of 16, then the rows' totals carried on).
-__device__ __forceinline__ int wave_scan_i32(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
-  return x;
-}
-
 // The select for up to 4 V THREADS candidates, one workgroup a query: with
 // nv = ceil(candidates / 4 THREADS) quads each, thread t holds the keys of rows
 // 4 nv t .. 4 nv t + 4 nv - 1 in registers (one memory round trip).  The K-th
-// largest key is found by histograms of 1024 equal bins over the range of keys
-// still open (first smallest to largest): the bin that holds it, then, when
-// that holds at most kCand keys, their ranks among each other by counting, else
-// a histogram of the bin's own range.  A range shrinks 2^9 times a pass at the
-// least, so four passes end it whatever the keys are (equal ones end in a bin
-// of width one); scores take one pass and the ranks.  The chosen rows are
+// largest key is found by histograms and ranks (kth_largest).  The chosen rows are
 // gathered in LDS in row order, after one scan of the threads' counts, and
 // written out in whole lines.  A serial chain of barriers bounds it: about ten,
 // where finding the key two bits at a time took eighteen, with every key compared
@@ -381,14 +365,10 @@ template <int THREADS, int V>
 __global__ __launch_bounds__(THREADS) void choice_select_regs(const float* __restrict__ scores, int64_t ns,
                                                               const int64_t* __restrict__ positions, int N,
                                                               int window, int K, int64_t* __restrict__ chosen) {
-  constexpr int kWaves = THREADS / 64, kBins = 1024, kCand = 256;
-  constexpr int kPerLane = kBins / 64;
+  constexpr int kWaves = THREADS / 64;
   static_assert(4 * V * THREADS < 65536, "packed counts hold 16 bits");
-  static_assert(kBins % THREADS == 0 && kCand <= THREADS, "bins and candidates a thread");
-  __shared__ __attribute__((aligned(16))) int hist[kBins];
-  __shared__ __attribute__((aligned(16))) uint32_t cand[kCand];
-  __shared__ int range[2][kWaves], counts[kWaves], sel[3], ncand;
-  __shared__ uint32_t found;
+  __shared__ SelectShared<THREADS> select;
+  __shared__ int counts[kWaves];
   __shared__ int staged[4 * V * THREADS];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t bt = blockIdx.x;
@@ -420,92 +400,7 @@ __global__ __launch_bounds__(THREADS) void choice_select_regs(const float* __res
         if (4 * v + e < valid) f(4 * v + e, key[4 * v + e]);
     }
   };
-#pragma unroll
-  for (int i = 0; i < kBins / THREADS; ++i) hist[tid + i * THREADS] = 0;
-  if (tid == 0) ncand = 0;
-  int kmin = INT32_MAX, kmax = INT32_MIN;  // as signed, order kept
-  each([&](int, uint32_t x) {
-    const int y = (int)(x ^ 0x80000000u);
-    kmin = min(kmin, y);
-    kmax = max(kmax, y);
-  });
-  kmin = wave_min_i32(kmin);
-  kmax = wave_max_i32(kmax);
-  if (lane == 0) {
-    range[0][w] = kmin;
-    range[1][w] = kmax;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    kmin = min(kmin, range[0][i]);
-    kmax = max(kmax, range[1][i]);
-  }
-  uint32_t lo = (uint32_t)kmin ^ 0x80000000u, hi = (uint32_t)kmax ^ 0x80000000u;
-  int remaining = K;  // the key sought is the remaining-th largest of those in lo .. hi
-  uint32_t tau;
-  for (;;) {
-    const uint32_t span = hi - lo;
-    const int shift = span < kBins ? 0 : 22 - __builtin_clz(span);  // span >> shift < kBins
-    each([&](int, uint32_t x) {
-      if (x >= lo && x <= hi) atomicAdd(&hist[(x - lo) >> shift], 1);
-    });
-    __syncthreads();
-    if (w == 0) {
-      // lane l holds bins top - 15 .. top, top = kBins - 1 - 16 l
-      int cnt[kPerLane], total = 0;
-      const int first = kBins - kPerLane * (lane + 1);
-#pragma unroll
-      for (int e = 0; e < kPerLane; ++e) total += (cnt[e] = hist[first + e]);
-      const int upto = wave_scan_i32(total);
-      if (upto >= remaining && upto - total < remaining) {  // one lane
-        int above = upto - total, bin = first, c = 0;
-#pragma unroll
-        for (int e = kPerLane - 1; e >= 0; --e) {
-          if (c == 0 && above + cnt[e] >= remaining) {
-            bin = first + e;
-            c = cnt[e];
-          }
-          if (c == 0) above += cnt[e];
-        }
-        sel[0] = bin;
-        sel[1] = above;
-        sel[2] = c;
-      }
-    }
-    __syncthreads();
-    const int count = sel[2];
-    remaining -= sel[1];
-    lo += (uint32_t)sel[0] << shift;
-    if (shift == 0) {  // the bin's keys are equal
-      tau = lo;
-      break;
-    }
-    const uint32_t width = (1u << shift) - 1u;
-    if (hi - lo > width) hi = lo + width;
-    if (count <= kCand) {
-      each([&](int, uint32_t x) {
-        if (x >= lo && x <= hi) cand[atomicAdd(&ncand, 1)] = x;
-      });
-      __syncthreads();
-      if (tid < count) {
-        const uint32_t mine = cand[tid];
-        int gt = 0, ge = 0;
-        for (int i = 0; i < count; ++i) {
-          const uint32_t x = cand[i];
-          gt += x > mine ? 1 : 0;
-          ge += x >= mine ? 1 : 0;
-        }
-        if (gt < remaining && ge >= remaining) found = mine;  // the same key from each that writes
-      }
-      __syncthreads();
-      tau = found;
-      break;
-    }
-#pragma unroll
-    for (int i = 0; i < kBins / THREADS; ++i) hist[tid + i * THREADS] = 0;
-    __syncthreads();
-  }
+  const uint32_t tau = kth_largest<THREADS>(each, K, select);
   // rows above tau and equal to it, each in row order: one scan of both counts
   int mine = 0;
   each([&](int, uint32_t x) { mine += x > tau ? 1 : x == tau ? 65536 : 0; });

@@ -5,9 +5,14 @@
 // else the first `first`, the last `recent`, and of the others the
 // keep - first - recent of the largest weight, equal weights the lowest rows
 // first (a NaN counts as the largest weight, -0 as 0), listed in row order.
-// One workgroup a (layer, batch row): a radix select of the smallest weight
-// kept over order-preserving keys, most significant byte first, then one pass
-// that lists the kept rows by wavefront ballots.
+// One workgroup a (layer, batch row):
+//   choose_kept_regs  up to 16384 rows: the weights' keys in registers, the
+//                     smallest one kept by kth_largest, the rows listed after
+//                     one scan of the threads' counts
+//   choose_kept       longer texts: a radix select over the weights in memory,
+//                     most significant byte first, then one pass that lists the
+//                     kept rows by wavefront ballots
+#include "select_common.h"
 #include "wptv_common.h"
 
 #include <climits>
@@ -18,6 +23,73 @@ namespace {
 constexpr int kST = 256;
 
 __device__ __forceinline__ uint32_t weight_key(float f) { return f != f ? ~0u : order_key(f + 0.f); }
+
+// Thread t holds the keys of 4 nv consecutive rows, nv = ceil(candidates / 4
+// THREADS) <= V, so that the kept rows are counted and listed in row order.
+template <int THREADS, int V>
+__global__ __launch_bounds__(THREADS) void choose_kept_regs(const float* __restrict__ weights, int64_t wsl,
+                                                            int64_t wsb, int B, int N,
+                                                            const int64_t* __restrict__ lengths, int keep, int first,
+                                                            int recent, int64_t* __restrict__ kept,
+                                                            int64_t* __restrict__ counts) {
+  constexpr int kWaves = THREADS / 64;
+  static_assert(4 * V * THREADS < 65536, "packed counts hold 16 bits");
+  __shared__ SelectShared<THREADS> select;
+  __shared__ int waves[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int layer = blockIdx.x / B, b = blockIdx.x % B;
+  const int64_t len64 = lengths[b];
+  const int len = len64 < 0 ? 0 : len64 < N ? (int)len64 : N;
+  int64_t* out = kept + (int64_t)blockIdx.x * keep;
+  if (layer == 0 && tid == 0) counts[b] = len < keep ? len : keep;
+  if (len <= keep) {
+    for (int i = tid; i < keep; i += THREADS) out[i] = i < len ? i : -1;
+    return;
+  }
+  const int take = keep - first - recent, candidates = len - first - recent;  // take < candidates
+  for (int i = tid; i < first; i += THREADS) out[i] = i;
+  for (int i = tid; i < recent; i += THREADS) out[keep - recent + i] = len - recent + i;
+  if (take == 0) return;
+  const float* s = weights + layer * wsl + b * wsb + first;
+  const int nv = (candidates + 4 * THREADS - 1) / (4 * THREADS);
+  const int base = tid * 4 * nv, valid = candidates - base;
+  uint32_t key[4 * V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (v >= nv) break;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) key[4 * v + e] = 4 * v + e < valid ? weight_key(s[base + 4 * v + e]) : 0u;
+  }
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (v >= nv) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * v + e < valid) f(4 * v + e, key[4 * v + e]);
+    }
+  };
+  const uint32_t tau = kth_largest<THREADS>(each, take, select);
+  // rows above tau, and the first of those equal to it: one scan of both counts
+  int mine = 0;
+  each([&](int, uint32_t x) { mine += x > tau ? 1 : x == tau ? 65536 : 0; });
+  const int upto = wave_scan_i32(mine);
+  if (lane == 63) waves[w] = upto;
+  __syncthreads();
+  int before = upto - mine, above = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < w) before += waves[i];
+    above += waves[i] & 65535;
+  }
+  const int equal = take - above;  // rows equal to tau that are kept
+  int gt = before & 65535, eq = before >> 16;
+  each([&](int i, uint32_t x) {
+    if (x > tau || (x == tau && eq < equal)) out[first + gt + min(eq, equal)] = first + base + i;
+    gt += x > tau ? 1 : 0;
+    eq += x == tau ? 1 : 0;
+  });
+}
 
 __global__ __launch_bounds__(kST) void choose_kept(const float* __restrict__ weights, int64_t wsl, int64_t wsb, int B,
                                                    int N, const int64_t* __restrict__ lengths, int keep, int first,
@@ -113,7 +185,18 @@ extern "C" int wptv_choose_kept(const float* weights, int64_t weights_stride_l, 
   if (L == 0 || B == 0) return WPTV_OK;
   if ((N && !weights) || !lengths || !kept || !counts)
     return fail(WPTV_E_INVALID, "choose_kept: a required pointer is NULL");
-  choose_kept<<<L * B, kST, 0, stream>>>(weights, weights_stride_l, weights_stride_b, B, N, lengths, keep, first,
-                                         recent, kept, counts);
+#define WPTV_KEPT(THREADS, V)                                                                                    \
+  choose_kept_regs<THREADS, V><<<L * B, THREADS, 0, stream>>>(weights, weights_stride_l, weights_stride_b, B, N, \
+                                                              lengths, keep, first, recent, kept, counts)
+  if (N <= 1024)
+    WPTV_KEPT(256, 1);
+  else if (N <= 4096)
+    WPTV_KEPT(512, 2);
+  else if (N <= 16384)
+    WPTV_KEPT(1024, 4);
+  else
+    choose_kept<<<L * B, kST, 0, stream>>>(weights, weights_stride_l, weights_stride_b, B, N, lengths, keep, first,
+                                           recent, kept, counts);
+#undef WPTV_KEPT
   return launched("choose_kept");
 }
