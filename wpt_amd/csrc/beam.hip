@@ -4,13 +4,18 @@
 // A text's candidates are its W beams continued by each of V tokens, of value
 //   total[w] + (x[w, v] - L[w]),  L[w] = log sum_v exp x[w, v]
 // in 64 bits; the K largest are the next beams, equal values to the lowest
-// w V + v.  The scores need not be normalised nor sorted as a whole: within a
-// beam the value grows with x, so a beam's candidates are its K largest
-// scores, and the next beams are among the W lists of K.  Two launches:
-//   beam_rows   one workgroup a (text, beam): L and the K largest scores, ties
-//               to the lowest token (keys of the score's order and the token)
-//   beam_merge  one wavefront a text: a lane a beam, K times the best head of
-//               the W lists
+// w V + v.  Within a beam the value grows with x, so nothing has to be
+// normalised before it is selected: each score is read once.
+//   beam_parts  a wavefront a part of a beam's scores, all of it in registers:
+//               the part's maximum, its sum of exponentials, and its K largest
+//               scores, ties to the lowest token
+//   beam_merge  a workgroup a text: the parts' sums joined to L in 64 bits, and
+//               the K best of the parts' lists
+// The K largest of a part: the K-th largest of the lanes' maxima bounds them
+// from below, and few scores reach it (in scores without order about K of 4096);
+// those are gathered in LDS, 64 at a time sorted across the lanes and merged
+// into the best so far.  No barrier, and any scores are served: where many reach
+// the bound the part is read again.
 #include "wptv_common.h"
 
 #include <climits>
@@ -18,15 +23,25 @@
 namespace wptv {
 namespace {
 
-constexpr int kMaxBeams = 64;  // beams of a text: a lane each
+constexpr int kMaxBeams = 64;  // beams of a text: a lane each of a sorted list
 constexpr int kMaxStops = 16;
-constexpr int kRowThreads = 256;
+constexpr int kPartWaves = 4;  // wavefronts of a beam_parts workgroup
+constexpr int kGathered = 128; // keys a wavefront gathers: 64 to sort, and what a load adds to them
 constexpr float kNegInf = -__builtin_inff();
 
 struct Stops {
   int n;
   int token[kMaxStops];
 };
+
+// The maximum over the 64 lanes of a wavefront, in every lane (NaNs passed over).
+__device__ __forceinline__ float wave_max_dpp(float x) {
+  x = row16_max(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 
 // A score's place among a beam's: larger scores first, then lower tokens.
 // -0 counts as 0; no key of a token is 0.
@@ -43,124 +58,327 @@ __device__ __forceinline__ double key64_value(uint64_t k) {
   return __longlong_as_double((long long)((k >> 63) ? (k & ~(1ull << 63)) : ~k));
 }
 
-template <typename E>
-__global__ __launch_bounds__(kRowThreads) void beam_rows(const E* __restrict__ scores, int64_t sn, int64_t sw, int W,
-                                                         int V, int K, double* __restrict__ lse,
-                                                         uint64_t* __restrict__ lists) {
-  __shared__ float red[kRowThreads / 64];
-  __shared__ double sums[kRowThreads / 64];
-  __shared__ uint64_t keys[kRowThreads / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.x;
-  const E* x = scores + (row / W) * sn + (row % W) * sw;
-  float m = kNegInf;
-  for (int v = tid; v < V; v += kRowThreads) m = fmaxf(m, load_f32(x + v));
-  m = wave_max(m);
-  if (lane == 0) red[wave] = m;
-  __syncthreads();
-  for (int i = 0; i < kRowThreads / 64; ++i) m = fmaxf(m, red[i]);
-  // NaN, +inf, or nothing above -inf: the sum becomes NaN or 0, and L no number
-  const float at = m == kNegInf ? 0.f : m;
-  double s = 0.;
-  for (int v = tid; v < V; v += kRowThreads) s += (double)expf(load_f32(x + v) - at);
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if (lane == 0) sums[wave] = s;
-  __syncthreads();
-  if (tid == 0) {
-    s = 0.;
-    for (int i = 0; i < kRowThreads / 64; ++i) s += sums[i];
-    lse[row] = (double)at + log(s);
-  }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < K; ++k) {
-    uint64_t best = 0;
-    for (int v = tid; v < V; v += kRowThreads) {
-      const uint64_t key = score_key(load_f32(x + v), v);
-      if (key < last && key > best) best = key;
-    }
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor((unsigned long long)best, o, 64);
-      if (other > best) best = other;
-    }
-    __syncthreads();
-    if (lane == 0) keys[wave] = best;
-    __syncthreads();
-    for (int i = 0; i < kRowThreads / 64; ++i)
-      if (keys[i] > best) best = keys[i];
-    if (tid == 0) lists[row * K + k] = best;  // 0 where the vocabulary holds fewer
-    last = best;
+// ---- sorting across the lanes --------------------------------------------------
+
+// A key of N words, the most significant first; 0 sorts last.
+template <int N>
+struct Key {
+  uint32_t w[N];
+};
+
+template <int N>
+__device__ __forceinline__ bool above(const Key<N>& a, const Key<N>& b) {
+  if constexpr (N == 1) {
+    return a.w[0] > b.w[0];
+  } else {
+    const uint64_t x = ((uint64_t)a.w[0] << 32) | a.w[1], y = ((uint64_t)b.w[0] << 32) | b.w[1];
+    if constexpr (N == 2) return x > y;
+    return x > y || (x == y && a.w[2] > b.w[2]);
   }
 }
 
-__global__ __launch_bounds__(64) void beam_merge(const double* __restrict__ lse, const uint64_t* __restrict__ lists,
-                                                 const float* __restrict__ totals,
-                                                 const unsigned char* __restrict__ ended, Stops stops, int W, int V,
-                                                 int K, float* __restrict__ new_totals, int64_t* __restrict__ parents,
-                                                 int64_t* __restrict__ tokens, unsigned char* __restrict__ new_ended) {
-  const int lane = threadIdx.x;
-  const int64_t row0 = (int64_t)blockIdx.x * W, row = row0 + lane;
-  const bool mine = lane < W;
-  double total = 0., base = 0.;
-  bool over = false, alive = false;
-  if (mine) {
-    total = (double)totals[row];
-    base = lse[row];
-    over = ended && ended[row];
-    alive = isfinite(total) && (over || isfinite(base));
+// x of lane ^ M, without LDS traffic; every lane must be active.
+template <int M>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
+  if constexpr (M >= 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return lane_xor<M - 32>((threadIdx.x & 32) ? r[0] : r[1]);
+  } else if constexpr (M >= 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return lane_xor<M - 16>((threadIdx.x & 16) ? r[0] : r[1]);
+  } else if constexpr (M == 15) {
+    return (uint32_t)dpp_move<kDppMirror>((int)x);
+  } else if constexpr (M == 8) {
+    return (uint32_t)dpp_move<0x128>((int)x);  // row_ror:8
+  } else if constexpr (M == 7) {
+    return (uint32_t)dpp_move<kDppHalfMirror>((int)x);
+  } else if constexpr (M == 4) {
+    return lane_xor<3>((uint32_t)dpp_move<kDppHalfMirror>((int)x));
+  } else if constexpr (M == 3) {
+    return (uint32_t)dpp_move<0x1B>((int)x);  // a quad reversed
+  } else if constexpr (M == 2) {
+    return (uint32_t)dpp_move<kDppXor2>((int)x);
+  } else if constexpr (M == 1) {
+    return (uint32_t)dpp_move<kDppXor1>((int)x);
+  } else {
+    static_assert(M == 0, "a lane exchange of this list");
+    return x;
   }
-  const int stop = stops.n ? stops.token[0] : 0;
-  // The head'th best candidate of this lane's beam: (value, ~(w V + v)), 0 for none.
-  auto candidate = [&](int head, uint64_t& value, uint32_t& order) {
-    value = 0;
-    order = 0;
-    if (!mine || head >= K) return;
-    double f = (double)kNegInf;
-    int64_t v = head;
-    if (alive && over) {
-      if (head == 0) {
-        f = total;
-        v = stop;
-      } else {
-        v = head - 1 + (head - 1 >= stop ? 1 : 0);
+}
+
+// One compare-exchange with lane ^ M: the lanes with bit BIT clear keep the
+// larger key.
+template <int M, int BIT, int N>
+__device__ __forceinline__ void exchange(Key<N>& k) {
+  Key<N> other;
+#pragma unroll
+  for (int i = 0; i < N; ++i) other.w[i] = lane_xor<M>(k.w[i]);
+  const bool mine = above(k, other) == ((threadIdx.x & BIT) == 0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) k.w[i] = mine ? k.w[i] : other.w[i];
+}
+
+template <int BIT, int N>
+__device__ __forceinline__ void merge_down(Key<N>& k) {
+  if constexpr (BIT > 0) {
+    exchange<BIT, BIT>(k);
+    merge_down<BIT / 2>(k);
+  }
+}
+
+template <int SIZE = 2, int N>
+__device__ __forceinline__ void wave_sort(Key<N>& k) {  // falling
+  exchange<SIZE - 1, SIZE / 2>(k);
+  merge_down<SIZE / 4>(k);
+  if constexpr (SIZE < 64) wave_sort<SIZE * 2>(k);
+}
+
+// best = the 64 largest of best and of `reversed`, a falling list read
+// backwards; both falling afterwards.
+template <int N>
+__device__ __forceinline__ void merge_lists(Key<N>& best, const Key<N>& reversed) {
+  if (above(reversed, best)) best = reversed;
+  merge_down<32>(best);
+}
+
+template <int N>
+__device__ __forceinline__ Key<N> backwards(const Key<N>& k) {
+  Key<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.w[i] = lane_xor<63>(k.w[i]);
+  return r;
+}
+
+template <int N>
+__device__ __forceinline__ Key<N> key_of_lane(const Key<N>& k, int lane) {
+  Key<N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.w[i] = __builtin_amdgcn_readlane(k.w[i], lane);
+  return r;
+}
+
+// ---- the parts -------------------------------------------------------------------
+
+// 16 bytes of scores, at any element's address.
+template <typename E>
+struct Scores16;
+template <>
+struct Scores16<float> {
+  typedef float type __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <>
+struct Scores16<unsigned short> {
+  typedef unsigned short type __attribute__((ext_vector_type(8), aligned(2)));
+};
+
+// The lanes before this one in mask.
+__device__ __forceinline__ int below_me(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+struct PartSum {
+  float top, sum;  // the largest score, and the sum of exp(x - top) (of exp x where nothing is above -inf)
+};
+
+template <typename E, int ITEMS>
+__global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restrict__ scores, int64_t sn, int64_t sw,
+                                                              int W, int V, int K, int parts, int64_t waves,
+                                                              PartSum* __restrict__ sums,
+                                                              uint64_t* __restrict__ lists) {
+  typedef typename Scores16<E>::type Vec;
+  constexpr int kVec = 16 / sizeof(E), kLoads = ITEMS / kVec;
+  __shared__ uint64_t gathered[kPartWaves][kGathered];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t wave = (int64_t)blockIdx.x * kPartWaves + w;
+  if (wave >= waves) return;  // no barrier follows
+  const int64_t row = wave / parts;
+  const int v0 = (int)(wave % parts) * 64 * ITEMS + lane * kVec;  // this lane's first token; 64 kVec a load
+  const E* p = scores + (row / W) * sn + (row % W) * sw;
+  float x[ITEMS];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int64_t v = (int64_t)v0 + i * 64 * kVec;
+    if (v + kVec <= V) {
+      const Vec got = *reinterpret_cast<const Vec*>(p + v);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const E one = got[e];
+        x[i * kVec + e] = load_f32(&one);
       }
-    } else if (alive) {
-      const uint64_t key = lists[row * K + head];
-      if (key == 0) return;
-      f = total + ((double)key_value((uint32_t)(key >> 32)) - base);
-      v = (uint32_t)~(uint32_t)key;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) x[i * kVec + e] = v + e < V ? load_f32(p + v + e) : kNegInf;
     }
-    if (v >= V) return;
-    value = order_key64(f);
-    order = ~(uint32_t)(lane * (int64_t)V + v);
+  }
+  float most = kNegInf;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) most = fmaxf(most, x[i]);  // a NaN is passed over here and found in the sum
+  const float top = wave_max_dpp(most);
+  const float at = top == kNegInf ? 0.f : top;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) sum[i % 4] += __builtin_amdgcn_exp2f((x[i] - at) * kLog2e);
+  const float total = wave_sum_dpp((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if (lane == 0) sums[wave] = PartSum{top, total};
+
+  Key<1> maxima{{order_key(most + 0.f)}};
+  wave_sort(maxima);
+  const float bound = key_value(key_of_lane(maxima, K - 1).w[0]);  // K scores at least reach it
+  // the scores that reach the bound, gathered in LDS
+  uint64_t* held = gathered[w];
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(x[i] >= bound);
+    if (mask == 0) continue;
+    const int at = count + below_me(mask);
+    if (x[i] >= bound && at < kGathered) {
+      const int v = v0 + i / kVec * 64 * kVec + i % kVec;
+      held[at] = v < V ? score_key(x[i], v) : 0;
+    }
+    count += __builtin_popcountll(mask);
+  }
+  Key<2> best{{0, 0}}, last{{0, 0}};  // the part's list, and its K-th key
+  auto sort_in = [&](int first, int end) {  // held[first .. end - 1], at most 64
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const uint64_t mine = first + lane < end ? held[first + lane] : 0;
+    Key<2> k{{(uint32_t)(mine >> 32), (uint32_t)mine}};
+    wave_sort(k);
+    merge_lists(best, backwards(k));
+    last = key_of_lane(best, K - 1);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
-  int head = 0;
-  uint64_t value;
-  uint32_t order;
-  candidate(head, value, order);
-  for (int k = 0; k < K; ++k) {
-    uint64_t bv = value;
-    uint32_t bo = order;
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t ov = __shfl_xor((unsigned long long)bv, o, 64);
-      const uint32_t oo = __shfl_xor(bo, o, 64);
-      if (ov > bv || (ov == bv && oo > bo)) {
-        bv = ov;
-        bo = oo;
+  if (count <= kGathered) {
+    for (int first = 0; first < count; first += 64) sort_in(first, count);
+  } else {
+    // many reach it (equal scores, or scores that rise with the lane): the part
+    // again from memory, a load at a time, against the best so far
+    count = 0;
+    for (int i = 0; i < ITEMS; ++i) {
+      const int v = v0 + i / kVec * 64 * kVec + i % kVec;
+      const uint64_t key = v < V ? score_key(load_f32(p + v), v) : 0;
+      const bool in = key > (((uint64_t)last.w[0] << 32) | last.w[1]);
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+      if (mask == 0) continue;
+      if (in) held[count + below_me(mask)] = key;
+      count += __builtin_popcountll(mask);
+      if (count >= 64) {
+        sort_in(0, 64);
+        const uint64_t rest = held[64 + lane];
+        held[lane] = rest;
+        count -= 64;
       }
     }
-    if (mine && value == bv && order == bo) {  // one lane: the orders differ
-      const uint32_t flat = ~bo;
-      const int v = (int)(flat - (uint32_t)lane * (uint32_t)V);
-      const int64_t at = (int64_t)blockIdx.x * K + k;
-      new_totals[at] = (float)key64_value(bv);
-      parents[at] = lane;
-      tokens[at] = v;
-      bool stopped = over;
-      for (int i = 0; i < stops.n; ++i) stopped = stopped || stops.token[i] == v;
-      new_ended[at] = stopped ? 1 : 0;
-      candidate(++head, value, order);
+    if (count > 0) sort_in(0, count);
+  }
+  if (lane < K) lists[wave * K + lane] = ((uint64_t)best.w[0] << 32) | best.w[1];  // 0 where the part holds fewer
+}
+
+// ---- the text's next beams -----------------------------------------------------------
+
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void beam_merge(const PartSum* __restrict__ sums,
+                                                         const uint64_t* __restrict__ lists, int parts,
+                                                         const float* __restrict__ totals,
+                                                         const unsigned char* __restrict__ ended, Stops stops, int W,
+                                                         int V, int K, float* __restrict__ new_totals,
+                                                         int64_t* __restrict__ parents, int64_t* __restrict__ tokens,
+                                                         unsigned char* __restrict__ new_ended) {
+  __shared__ double level[kMaxBeams];  // L
+  __shared__ double from[kMaxBeams];   // the beam's total; -inf where it cannot go on
+  __shared__ Key<3> tops[WAVES][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row0 = (int64_t)blockIdx.x * W;
+  for (int w = wave; w < W; w += WAVES) {
+    const PartSum* part = sums + (row0 + w) * parts;
+    float top = kNegInf;
+    for (int i = lane; i < parts; i += 64) top = fmaxf(top, part[i].top);
+    top = wave_max_dpp(top);
+    const float at = top == kNegInf ? 0.f : top;
+    double sum = 0.;
+    for (int i = lane; i < parts; i += 64) {
+      const PartSum s = part[i];
+      sum += (double)s.sum * exp((double)(s.top == kNegInf ? 0.f : s.top) - (double)at);
+    }
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) {
+      // a NaN or +inf among the scores makes the sum NaN; nothing above -inf leaves top there
+      const double l = (double)at + log(sum), total = (double)totals[row0 + w];
+      const bool over = ended && ended[row0 + w];
+      level[w] = l;
+      from[w] = isfinite(total) && (over || (isfinite(l) && top != kNegInf)) ? total : (double)kNegInf;
     }
   }
+  __syncthreads();
+  const int stop = stops.n ? stops.token[0] : 0;
+  const int many = W * parts;  // the lists; heads first, so that the first batches bound the others
+  Key<3> best{{0, 0, 0}}, last{{0, 0, 0}};
+  bool some = false;
+  for (int64_t c0 = (int64_t)wave * 64; c0 < (int64_t)many * K; c0 += 64 * WAVES) {
+    const int64_t c = c0 + lane;
+    Key<3> k{{0, 0, 0}};
+    if (c < (int64_t)many * K) {
+      const int head = (int)(c / many), list = (int)(c % many), w = list / parts, part = list % parts;
+      const double total = from[w];
+      const bool dead = !(total > (double)kNegInf), over = !dead && ended && ended[row0 + w];
+      double value = (double)kNegInf;
+      int64_t v = V;
+      if (dead || over) {  // one list: the stop token at the beam's total, the others at -inf
+        if (part == 0) {
+          v = head;
+          if (over && head == 0) {
+            value = total;
+            v = stop;
+          } else if (over) {
+            v = head - 1 + (head - 1 >= stop ? 1 : 0);
+          }
+        }
+      } else {
+        const uint64_t key = lists[((row0 + w) * parts + part) * K + head];
+        if (key) {
+          v = (uint32_t)~(uint32_t)key;
+          value = total + ((double)key_value((uint32_t)(key >> 32)) - level[w]);
+        }
+      }
+      if (v < V) {
+        const uint64_t order = order_key64(value);
+        k = Key<3>{{(uint32_t)(order >> 32), (uint32_t)order, ~(uint32_t)(w * (int64_t)V + v)}};
+      }
+    }
+    if (__builtin_amdgcn_ballot_w64(above(k, last)) == 0) continue;
+    wave_sort(k);
+    if (some) {
+      merge_lists(best, backwards(k));
+    } else {
+      best = k;
+    }
+    some = true;
+    last = key_of_lane(best, K - 1);
+  }
+  // the wavefronts' lists, in pairs
+#pragma unroll
+  for (int half = WAVES / 2; half > 0; half /= 2) {
+    if (wave >= half && wave < 2 * half) tops[wave][lane] = best;
+    __syncthreads();
+    if (wave < half) merge_lists(best, tops[wave + half][63 - lane]);
+  }
+  if (wave == 0 && lane < K) {
+    const uint32_t flat = ~best.w[2];
+    const int w = (int)(flat / (uint32_t)V), v = (int)(flat % (uint32_t)V);
+    bool over = ended && ended[row0 + w];
+    for (int i = 0; i < stops.n; ++i) over = over || stops.token[i] == v;
+    const int64_t at = (int64_t)blockIdx.x * K + lane;
+    new_totals[at] = (float)key64_value(((uint64_t)best.w[0] << 32) | best.w[1]);
+    parents[at] = w;
+    tokens[at] = v;
+    new_ended[at] = over ? 1 : 0;
+  }
+}
+
+// Scores a lane of a part: 64 where the parts of 4096 fill the GPU, 16 where
+// they do not, so that few rows are spread over it.
+int part_items(int64_t rows, int V) {
+  return rows * ((V + 4095) / 4096) >= 4 * (int64_t)compute_units() ? 64 : 16;
 }
 
 }  // namespace
@@ -176,7 +394,8 @@ extern "C" int wptv_beam_workspace(int n, int W, int V, int K, size_t* bytes) {
     return fail(WPTV_E_UNSUPPORTED, "beam_workspace: at most %d beams a text (W=%d, K=%d)", kMaxBeams, W, K);
   if ((int64_t)W * V > INT32_MAX || (int64_t)n * W > INT32_MAX)
     return fail(WPTV_E_UNSUPPORTED, "beam_workspace: n=%d W=%d V=%d is too large", n, W, V);
-  *bytes = (size_t)n * W * (sizeof(double) + (size_t)K * sizeof(uint64_t));
+  const int part = 64 * part_items((int64_t)n * W, V);
+  *bytes = (size_t)n * W * ((V + part - 1) / part) * (sizeof(PartSum) + (size_t)K * sizeof(uint64_t));
   return WPTV_OK;
 }
 
@@ -203,17 +422,26 @@ extern "C" int wptv_beam_step(const void* scores, int64_t scores_stride_n, int64
     return fail(WPTV_E_INVALID, "beam_step: a required pointer is NULL");
   if (workspace_bytes < need)
     return fail(WPTV_E_INVALID, "beam_step: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  double* lse = static_cast<double*>(workspace);
-  uint64_t* lists = reinterpret_cast<uint64_t*>(lse + (size_t)n * W);
-  if (scores_dtype == WPTV_F32)
-    beam_rows<float><<<n * W, kRowThreads, 0, stream>>>(static_cast<const float*>(scores), scores_stride_n,
-                                                        scores_stride_w, W, V, K, lse, lists);
-  else
-    beam_rows<unsigned short><<<n * W, kRowThreads, 0, stream>>>(static_cast<const unsigned short*>(scores),
-                                                                 scores_stride_n, scores_stride_w, W, V, K, lse,
-                                                                 lists);
-  const int launch = launched("beam_rows");
+  const int items = part_items((int64_t)n * W, V), parts = (V + 64 * items - 1) / (64 * items);
+  const int64_t waves = (int64_t)n * W * parts, blocks = (waves + kPartWaves - 1) / kPartWaves;
+  PartSum* sums = static_cast<PartSum*>(workspace);
+  uint64_t* lists = reinterpret_cast<uint64_t*>(sums + waves);
+#define WPTV_PARTS(E, ITEMS)                                                                                      \
+  beam_parts<E, ITEMS><<<(unsigned)blocks, 64 * kPartWaves, 0, stream>>>(                                         \
+      static_cast<const E*>(scores), scores_stride_n, scores_stride_w, W, V, K, parts, waves, sums, lists)
+  if (scores_dtype == WPTV_F32) {
+    if (items == 64) WPTV_PARTS(float, 64); else WPTV_PARTS(float, 16);
+  } else {
+    if (items == 64) WPTV_PARTS(unsigned short, 64); else WPTV_PARTS(unsigned short, 16);
+  }
+#undef WPTV_PARTS
+  const int launch = launched("beam_parts");
   if (launch != WPTV_OK) return launch;
-  beam_merge<<<n, 64, 0, stream>>>(lse, lists, totals, ended, s, W, V, K, new_totals, parents, tokens, new_ended);
+  if ((int64_t)W * parts * K <= 1024)
+    beam_merge<4><<<n, 256, 0, stream>>>(sums, lists, parts, totals, ended, s, W, V, K, new_totals, parents, tokens,
+                                         new_ended);
+  else
+    beam_merge<16><<<n, 1024, 0, stream>>>(sums, lists, parts, totals, ended, s, W, V, K, new_totals, parents, tokens,
+                                           new_ended);
   return launched("beam_merge");
 }
