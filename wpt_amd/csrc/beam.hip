@@ -26,7 +26,7 @@ namespace {
 constexpr int kMaxBeams = 64;  // beams of a text: a lane each of a sorted list
 constexpr int kMaxStops = 16;
 constexpr int kPartWaves = 4;  // wavefronts of a beam_parts workgroup
-constexpr int kGathered = 128; // keys a wavefront gathers: 64 to sort, and what a load adds to them
+constexpr int kGathered = 256;  // keys a wavefront gathers
 constexpr float kNegInf = -__builtin_inff();
 
 struct Stops {
@@ -77,6 +77,12 @@ __device__ __forceinline__ bool above(const Key<N>& a, const Key<N>& b) {
   }
 }
 
+// A move within a 16-lane row that every lane takes part in (no old value to keep).
+template <int CTRL>
+__device__ __forceinline__ uint32_t row_move(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true);
+}
+
 // x of lane ^ M, without LDS traffic; every lane must be active.
 template <int M>
 __device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
@@ -87,19 +93,19 @@ __device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
     const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
     return lane_xor<M - 16>((threadIdx.x & 16) ? r[0] : r[1]);
   } else if constexpr (M == 15) {
-    return (uint32_t)dpp_move<kDppMirror>((int)x);
+    return row_move<kDppMirror>(x);
   } else if constexpr (M == 8) {
-    return (uint32_t)dpp_move<0x128>((int)x);  // row_ror:8
+    return row_move<0x128>(x);  // row_ror:8
   } else if constexpr (M == 7) {
-    return (uint32_t)dpp_move<kDppHalfMirror>((int)x);
+    return row_move<kDppHalfMirror>(x);
   } else if constexpr (M == 4) {
-    return lane_xor<3>((uint32_t)dpp_move<kDppHalfMirror>((int)x));
+    return lane_xor<3>(row_move<kDppHalfMirror>(x));
   } else if constexpr (M == 3) {
-    return (uint32_t)dpp_move<0x1B>((int)x);  // a quad reversed
+    return row_move<0x1B>(x);  // a quad reversed
   } else if constexpr (M == 2) {
-    return (uint32_t)dpp_move<kDppXor2>((int)x);
+    return row_move<kDppXor2>(x);
   } else if constexpr (M == 1) {
-    return (uint32_t)dpp_move<kDppXor1>((int)x);
+    return row_move<kDppXor1>(x);
   } else {
     static_assert(M == 0, "a lane exchange of this list");
     return x;
@@ -113,9 +119,14 @@ __device__ __forceinline__ void exchange(Key<N>& k) {
   Key<N> other;
 #pragma unroll
   for (int i = 0; i < N; ++i) other.w[i] = lane_xor<M>(k.w[i]);
-  const bool mine = above(k, other) == ((threadIdx.x & BIT) == 0);
+  const bool larger = (threadIdx.x & BIT) == 0;
+  if constexpr (N == 1) {
+    k.w[0] = larger ? max(k.w[0], other.w[0]) : min(k.w[0], other.w[0]);
+  } else {
+    const bool mine = above(k, other) == larger;
 #pragma unroll
-  for (int i = 0; i < N; ++i) k.w[i] = mine ? k.w[i] : other.w[i];
+    for (int i = 0; i < N; ++i) k.w[i] = mine ? k.w[i] : other.w[i];
+  }
 }
 
 template <int BIT, int N>
@@ -126,11 +137,21 @@ __device__ __forceinline__ void merge_down(Key<N>& k) {
   }
 }
 
-template <int SIZE = 2, int N>
-__device__ __forceinline__ void wave_sort(Key<N>& k) {  // falling
+// Falling order within each LAST lanes.
+template <int LAST = 64, int SIZE = 2, int N>
+__device__ __forceinline__ void wave_sort(Key<N>& k) {
   exchange<SIZE - 1, SIZE / 2>(k);
   merge_down<SIZE / 4>(k);
-  if constexpr (SIZE < 64) wave_sort<SIZE * 2>(k);
+  if constexpr (SIZE < LAST) wave_sort<LAST, SIZE * 2>(k);
+}
+
+// Falling order of keys that only the first `many` lanes hold (the others 0).
+template <int N>
+__device__ __forceinline__ void wave_sort_first(Key<N>& k, int many) {
+  if (many <= 16)
+    wave_sort<16>(k);
+  else
+    wave_sort(k);
 }
 
 // best = the 64 largest of best and of `reversed`, a falling list read
@@ -182,32 +203,49 @@ struct PartSum {
 
 template <typename E, int ITEMS>
 __global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restrict__ scores, int64_t sn, int64_t sw,
-                                                              int W, int V, int K, int parts, int64_t waves,
+                                                              uint32_t W, int V, int K, uint32_t parts, uint32_t waves,
                                                               PartSum* __restrict__ sums,
                                                               uint64_t* __restrict__ lists) {
   typedef typename Scores16<E>::type Vec;
   constexpr int kVec = 16 / sizeof(E), kLoads = ITEMS / kVec;
   __shared__ uint64_t gathered[kPartWaves][kGathered];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t wave = (int64_t)blockIdx.x * kPartWaves + w;
+  const uint32_t wave = blockIdx.x * kPartWaves + w;
   if (wave >= waves) return;  // no barrier follows
-  const int64_t row = wave / parts;
-  const int v0 = (int)(wave % parts) * 64 * ITEMS + lane * kVec;  // this lane's first token; 64 kVec a load
-  const E* p = scores + (row / W) * sn + (row % W) * sw;
+  const uint32_t row = wave / parts, part = wave % parts;
+  const int v0 = (int)part * 64 * ITEMS + lane * kVec;  // this lane's first token; 64 kVec a load
+  const E* p = scores + (int64_t)(row / W) * sn + (int64_t)(row % W) * sw;
+  // a load that would pass the row's end is moved back to it, and the tokens that
+  // another lane holds left out
+  const int last_load = V > kVec ? V - kVec : 0;
+  auto token = [&](int i) { return min(v0 + i / kVec * 64 * kVec, last_load) + i % kVec; };
   float x[ITEMS];
+  if ((part + 1) * 64 * ITEMS <= (uint32_t)V) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int64_t v = (int64_t)v0 + i * 64 * kVec;
-    if (v + kVec <= V) {
-      const Vec got = *reinterpret_cast<const Vec*>(p + v);
+    for (int i = 0; i < kLoads; ++i) {
+      const Vec got = *reinterpret_cast<const Vec*>(p + v0 + i * 64 * kVec);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
         const E one = got[e];
         x[i * kVec + e] = load_f32(&one);
       }
-    } else {
+    }
+  } else {
+    Vec got[kLoads];
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) x[i * kVec + e] = v + e < V ? load_f32(p + v + e) : kNegInf;
+    for (int i = 0; i < kLoads; ++i) {
+      if (V >= kVec) {
+        got[i] = *reinterpret_cast<const Vec*>(p + token(i * kVec));
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) got[i][e] = p[min(e, V - 1)];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int v = token(i);
+      const E one = got[i / kVec][i % kVec];
+      x[i] = v < V && v >= v0 + i / kVec * 64 * kVec ? load_f32(&one) : kNegInf;
     }
   }
   float most = kNegInf;
@@ -221,10 +259,16 @@ __global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restric
   const float total = wave_sum_dpp((sum[0] + sum[1]) + (sum[2] + sum[3]));
   if (lane == 0) sums[wave] = PartSum{top, total};
 
+  if (top == kNegInf) {  // the part's first tokens
+    const int64_t v = (int64_t)part * 64 * ITEMS + lane;
+    if (lane < K) lists[(int64_t)wave * K + lane] = v < V ? score_key(kNegInf, (int)v) : 0;
+    return;
+  }
+  // At least K scores reach the K-th largest of the lanes' maxima.
   Key<1> maxima{{order_key(most + 0.f)}};
   wave_sort(maxima);
-  const float bound = key_value(key_of_lane(maxima, K - 1).w[0]);  // K scores at least reach it
-  // the scores that reach the bound, gathered in LDS
+  const uint32_t kth = key_of_lane(maxima, K - 1).w[0];
+  const float bound = key_value(kth);
   uint64_t* held = gathered[w];
   int count = 0;
 #pragma unroll
@@ -233,33 +277,57 @@ __global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restric
     if (mask == 0) continue;
     const int at = count + below_me(mask);
     if (x[i] >= bound && at < kGathered) {
-      const int v = v0 + i / kVec * 64 * kVec + i % kVec;
-      held[at] = v < V ? score_key(x[i], v) : 0;
+      const int v = token(i);
+      held[at] = v < V && v >= v0 + i / kVec * 64 * kVec ? score_key(x[i], v) : 0;
     }
     count += __builtin_popcountll(mask);
   }
   Key<2> best{{0, 0}}, last{{0, 0}};  // the part's list, and its K-th key
+  bool some = false;
   auto sort_in = [&](int first, int end) {  // held[first .. end - 1], at most 64
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const uint64_t mine = first + lane < end ? held[first + lane] : 0;
     Key<2> k{{(uint32_t)(mine >> 32), (uint32_t)mine}};
-    wave_sort(k);
-    merge_lists(best, backwards(k));
+    wave_sort_first(k, end - first);
+    if (some)
+      merge_lists(best, backwards(k));
+    else
+      best = k;
+    some = true;
     last = key_of_lane(best, K - 1);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
   if (count <= kGathered) {
     for (int first = 0; first < count; first += 64) sort_in(first, count);
   } else {
-    // many reach it (equal scores, or scores that rise with the lane): the part
-    // again from memory, a load at a time, against the best so far
+    // Many scores equal the bound, or one lane holds many large ones.  The part
+    // again from memory: first, of the lanes whose maximum is the bound, each
+    // one's first token with it (the first of these, K less the lanes above the
+    // bound, are enough ties), then every score that is left, against the best
+    // so far.
+    auto each = [&](auto&& f) {  // f(token, score) of this lane, in the order of the tokens
+#pragma unroll 2
+      for (int i = 0; i < kLoads; ++i) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const int v = v0 + i * 64 * kVec + e;
+          f(v, v < V ? load_f32(p + v) : kNegInf);
+        }
+      }
+    };
+    uint32_t first = 0;  // ~token
+    each([&](int v, float f) { first = f == bound ? max(first, ~(uint32_t)v) : first; });
+    Key<1> firsts{{most == bound ? first : 0u}};
+    wave_sort(firsts);
+    const int more = __builtin_popcountll(__builtin_amdgcn_ballot_w64(most > bound));
+    const uint32_t tie = key_of_lane(firsts, K - 1 - more).w[0];
     count = 0;
-    for (int i = 0; i < ITEMS; ++i) {
-      const int v = v0 + i / kVec * 64 * kVec + i % kVec;
-      const uint64_t key = v < V ? score_key(load_f32(p + v), v) : 0;
-      const bool in = key > (((uint64_t)last.w[0] << 32) | last.w[1]);
+    each([&](int v, float f) {
+      const uint64_t key = score_key(f, v);
+      const bool in = v < V && (f > bound || (f == bound && ~(uint32_t)v >= tie)) &&
+                      key > (((uint64_t)last.w[0] << 32) | last.w[1]);
       const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
-      if (mask == 0) continue;
+      if (mask == 0) return;
       if (in) held[count + below_me(mask)] = key;
       count += __builtin_popcountll(mask);
       if (count >= 64) {
@@ -268,10 +336,10 @@ __global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restric
         held[lane] = rest;
         count -= 64;
       }
-    }
+    });
     if (count > 0) sort_in(0, count);
   }
-  if (lane < K) lists[wave * K + lane] = ((uint64_t)best.w[0] << 32) | best.w[1];  // 0 where the part holds fewer
+  if (lane < K) lists[(int64_t)wave * K + lane] = ((uint64_t)best.w[0] << 32) | best.w[1];  // 0 where the part holds fewer
 }
 
 // ---- the text's next beams -----------------------------------------------------------
@@ -378,7 +446,7 @@ __global__ __launch_bounds__(64 * WAVES) void beam_merge(const PartSum* __restri
 // Scores a lane of a part: 64 where the parts of 4096 fill the GPU, 16 where
 // they do not, so that few rows are spread over it.
 int part_items(int64_t rows, int V) {
-  return rows * ((V + 4095) / 4096) >= 4 * (int64_t)compute_units() ? 64 : 16;
+  return rows * (((int64_t)V + 4095) / 4096) >= 4 * (int64_t)compute_units() ? 64 : 16;
 }
 
 }  // namespace
@@ -392,10 +460,12 @@ extern "C" int wptv_beam_workspace(int n, int W, int V, int K, size_t* bytes) {
     return fail(WPTV_E_INVALID, "beam_workspace: bad shape n=%d W=%d V=%d K=%d", n, W, V, K);
   if (W > kMaxBeams || K > kMaxBeams)
     return fail(WPTV_E_UNSUPPORTED, "beam_workspace: at most %d beams a text (W=%d, K=%d)", kMaxBeams, W, K);
-  if ((int64_t)W * V > INT32_MAX || (int64_t)n * W > INT32_MAX)
+  if ((int64_t)W * V > (1 << 30) || (int64_t)n * W > INT32_MAX)
     return fail(WPTV_E_UNSUPPORTED, "beam_workspace: n=%d W=%d V=%d is too large", n, W, V);
   const int part = 64 * part_items((int64_t)n * W, V);
-  *bytes = (size_t)n * W * ((V + part - 1) / part) * (sizeof(PartSum) + (size_t)K * sizeof(uint64_t));
+  if ((int64_t)n * W * (((int64_t)V + part - 1) / part) > INT32_MAX)
+    return fail(WPTV_E_UNSUPPORTED, "beam_workspace: n=%d W=%d V=%d is too large", n, W, V);
+  *bytes = (size_t)n * W * (((int64_t)V + part - 1) / part) * (sizeof(PartSum) + (size_t)K * sizeof(uint64_t));
   return WPTV_OK;
 }
 
@@ -422,7 +492,7 @@ extern "C" int wptv_beam_step(const void* scores, int64_t scores_stride_n, int64
     return fail(WPTV_E_INVALID, "beam_step: a required pointer is NULL");
   if (workspace_bytes < need)
     return fail(WPTV_E_INVALID, "beam_step: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  const int items = part_items((int64_t)n * W, V), parts = (V + 64 * items - 1) / (64 * items);
+  const int items = part_items((int64_t)n * W, V), parts = (int)(((int64_t)V + 64 * items - 1) / (64 * items));
   const int64_t waves = (int64_t)n * W * parts, blocks = (waves + kPartWaves - 1) / kPartWaves;
   PartSum* sums = static_cast<PartSum*>(workspace);
   uint64_t* lists = reinterpret_cast<uint64_t*>(sums + waves);
