@@ -99,6 +99,16 @@ def test_beams_that_cannot_go_on(device):
         check(device, scores.to(torch.bfloat16), totals, ended, stops=(899,), beams=K)
 
 
+@pytest.mark.parametrize("offset", [-30000.0, -900.0, 900.0, 30000.0])
+def test_scores_far_from_zero_with_masked_stretches(device, offset):
+    scores, totals, ended = inputs(2, 3, 13000, torch.float32, seed=6)
+    scores += offset
+    scores[0, :, :9000] = -INF  # whole stretches of the vocabulary
+    scores[1, 1, 4096:8192] = -INF
+    scores[1, 2, 5:] = -INF
+    check(device, scores, totals, ended, stops=(3,), beams=6)
+
+
 def test_ended_beams_of_a_small_vocabulary(device):
     for V, K in ((1, 2), (2, 4), (3, 6)):
         scores, totals, _ = inputs(2, 2, V, torch.float32, seed=V)

@@ -19,6 +19,7 @@
 #include "wptv_common.h"
 
 #include <climits>
+#include <type_traits>
 
 namespace wptv {
 namespace {
@@ -344,6 +345,27 @@ __global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restric
 
 // ---- the text's next beams -----------------------------------------------------------
 
+constexpr int kCandidates = 512;  // that a text gathers
+
+__device__ __forceinline__ double wave_sum_f64(double x) {
+  auto add = [&](auto m) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    const uint64_t o = ((uint64_t)lane_xor<m>((uint32_t)(u >> 32)) << 32) | lane_xor<m>((uint32_t)u);
+    x += __longlong_as_double((long long)o);
+  };
+  add(std::integral_constant<int, 1>());
+  add(std::integral_constant<int, 2>());
+  add(std::integral_constant<int, 4>());
+  add(std::integral_constant<int, 8>());
+  add(std::integral_constant<int, 16>());
+  add(std::integral_constant<int, 32>());
+  return x;
+}
+
+// A text's W parts lists hold W parts K candidates.  The K-th largest of the
+// lists' heads (of the lanes' best heads where there are more than 64), as FP32,
+// bounds the next beams from below: each wavefront finds it for itself, and the
+// few candidates that reach it are gathered in LDS and sorted by the first one.
 template <int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void beam_merge(const PartSum* __restrict__ sums,
                                                          const uint64_t* __restrict__ lists, int parts,
@@ -354,92 +376,123 @@ __global__ __launch_bounds__(64 * WAVES) void beam_merge(const PartSum* __restri
                                                          unsigned char* __restrict__ new_ended) {
   __shared__ double level[kMaxBeams];  // L
   __shared__ double from[kMaxBeams];   // the beam's total; -inf where it cannot go on
-  __shared__ Key<3> tops[WAVES][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ bool over[kMaxBeams];     // ended, and goes on
+  __shared__ Key<3> gathered[kCandidates];
+  __shared__ int count;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row0 = (int64_t)blockIdx.x * W;
+  if (threadIdx.x == 0) count = 0;
   for (int w = wave; w < W; w += WAVES) {
     const PartSum* part = sums + (row0 + w) * parts;
-    float top = kNegInf;
-    for (int i = lane; i < parts; i += 64) top = fmaxf(top, part[i].top);
+    const PartSum mine = lane < parts ? part[lane] : PartSum{kNegInf, 0.f};
+    const double total = (double)totals[row0 + w];
+    const bool end = ended && ended[row0 + w];
+    float top = mine.top;
+    for (int i = lane + 64; i < parts; i += 64) top = fmaxf(top, part[i].top);
     top = wave_max_dpp(top);
-    const float at = top == kNegInf ? 0.f : top;
-    double sum = 0.;
-    for (int i = lane; i < parts; i += 64) {
-      const PartSum s = part[i];
-      sum += (double)s.sum * exp((double)(s.top == kNegInf ? 0.f : s.top) - (double)at);
-    }
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    const double at = top == kNegInf ? 0. : (double)top;
+    // a part with nothing above -inf summed exp x itself: to 0, or NaN with a NaN
+    auto scaled = [&](PartSum s) { return s.top == kNegInf ? (double)s.sum : (double)s.sum * exp((double)s.top - at); };
+    double sum = scaled(mine);
+    for (int i = lane + 64; i < parts; i += 64) sum += scaled(part[i]);
+    sum = wave_sum_f64(sum);
+    const double l = at + log(sum);  // NaN with a NaN or +inf among the scores
     if (lane == 0) {
-      // a NaN or +inf among the scores makes the sum NaN; nothing above -inf leaves top there
-      const double l = (double)at + log(sum), total = (double)totals[row0 + w];
-      const bool over = ended && ended[row0 + w];
+      const bool alive = isfinite(total) && (end || (isfinite(l) && top != kNegInf));
       level[w] = l;
-      from[w] = isfinite(total) && (over || (isfinite(l) && top != kNegInf)) ? total : (double)kNegInf;
+      from[w] = alive ? total : (double)kNegInf;
+      over[w] = alive && end;
     }
   }
   __syncthreads();
   const int stop = stops.n ? stops.token[0] : 0;
-  const int many = W * parts;  // the lists; heads first, so that the first batches bound the others
+  // The head'th candidate of a list: its value, and its token (V: none).  A beam
+  // that has ended or cannot go on has one list: the stop token at the beam's
+  // total, the others at -inf.
+  auto candidate = [&](int list, int head, int& v) {
+    const int w = list / parts, part = list % parts;
+    const double total = from[w];
+    v = V;
+    if (total > (double)kNegInf && !over[w]) {
+      const uint64_t key = lists[((row0 + w) * parts + part) * K + head];
+      if (key == 0) return 0.;
+      v = (int)~(uint32_t)key;
+      return total + ((double)key_value((uint32_t)(key >> 32)) - level[w]);
+    }
+    if (part != 0) return 0.;
+    if (!over[w]) {
+      v = head;
+    } else if (head == 0) {
+      v = stop;
+      return total;
+    } else {
+      v = head - 1 + (head - 1 >= stop ? 1 : 0);
+    }
+    v = min(v, V);
+    return (double)kNegInf;
+  };
+  auto key_of = [&](int list, int v, double value) {
+    const uint64_t order = order_key64(value);
+    return Key<3>{{(uint32_t)(order >> 32), (uint32_t)order, ~(uint32_t)((list / parts) * V + v)}};
+  };
+  const int many = W * parts, all = many * K;
+  Key<1> heads{{0}};
+  for (int list = lane; list < many; list += 64) {
+    int v;
+    const double value = candidate(list, 0, v);
+    if (v < V) heads.w[0] = max(heads.w[0], order_key((float)value + 0.f));
+  }
+  wave_sort(heads);
+  const uint32_t bound = key_of_lane(heads, K - 1).w[0];
+  for (int c0 = wave * 64; c0 < all; c0 += 64 * WAVES) {
+    const int list = (c0 + lane) % many, head = (c0 + lane) / many;
+    int v = V;
+    double value = 0.;
+    if (c0 + lane < all) value = candidate(list, head, v);
+    const bool in = v < V && order_key((float)value + 0.f) >= bound;
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+    if (mask == 0) continue;
+    int first = 0;
+    if (lane == 0) first = atomicAdd(&count, __builtin_popcountll(mask));
+    first = __builtin_amdgcn_readfirstlane(first) + below_me(mask);
+    if (in && first < kCandidates) gathered[first] = key_of(list, v, value);
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  const int found = count;
+  const bool held = found <= kCandidates;  // else every candidate again, against the best so far
+  const int end = held ? found : all;
   Key<3> best{{0, 0, 0}}, last{{0, 0, 0}};
-  bool some = false;
-  for (int64_t c0 = (int64_t)wave * 64; c0 < (int64_t)many * K; c0 += 64 * WAVES) {
-    const int64_t c = c0 + lane;
+  for (int c0 = 0; c0 < end; c0 += 64) {
     Key<3> k{{0, 0, 0}};
-    if (c < (int64_t)many * K) {
-      const int head = (int)(c / many), list = (int)(c % many), w = list / parts, part = list % parts;
-      const double total = from[w];
-      const bool dead = !(total > (double)kNegInf), over = !dead && ended && ended[row0 + w];
-      double value = (double)kNegInf;
-      int64_t v = V;
-      if (dead || over) {  // one list: the stop token at the beam's total, the others at -inf
-        if (part == 0) {
-          v = head;
-          if (over && head == 0) {
-            value = total;
-            v = stop;
-          } else if (over) {
-            v = head - 1 + (head - 1 >= stop ? 1 : 0);
-          }
-        }
+    if (c0 + lane < end) {
+      if (held) {
+        k = gathered[c0 + lane];
       } else {
-        const uint64_t key = lists[((row0 + w) * parts + part) * K + head];
-        if (key) {
-          v = (uint32_t)~(uint32_t)key;
-          value = total + ((double)key_value((uint32_t)(key >> 32)) - level[w]);
-        }
-      }
-      if (v < V) {
-        const uint64_t order = order_key64(value);
-        k = Key<3>{{(uint32_t)(order >> 32), (uint32_t)order, ~(uint32_t)(w * (int64_t)V + v)}};
+        int v;
+        const int list = (c0 + lane) % many;
+        const double value = candidate(list, (c0 + lane) / many, v);
+        if (v < V) k = key_of(list, v, value);
       }
     }
     if (__builtin_amdgcn_ballot_w64(above(k, last)) == 0) continue;
-    wave_sort(k);
-    if (some) {
-      merge_lists(best, backwards(k));
-    } else {
+    wave_sort_first(k, end - c0);
+    if (c0 == 0)
       best = k;
-    }
-    some = true;
+    else
+      merge_lists(best, backwards(k));
     last = key_of_lane(best, K - 1);
   }
-  // the wavefronts' lists, in pairs
-#pragma unroll
-  for (int half = WAVES / 2; half > 0; half /= 2) {
-    if (wave >= half && wave < 2 * half) tops[wave][lane] = best;
-    __syncthreads();
-    if (wave < half) merge_lists(best, tops[wave + half][63 - lane]);
-  }
-  if (wave == 0 && lane < K) {
+  if (lane < K) {
     const uint32_t flat = ~best.w[2];
     const int w = (int)(flat / (uint32_t)V), v = (int)(flat % (uint32_t)V);
-    bool over = ended && ended[row0 + w];
-    for (int i = 0; i < stops.n; ++i) over = over || stops.token[i] == v;
+    bool stopped = ended && ended[row0 + w];
+    for (int i = 0; i < stops.n; ++i) stopped = stopped || stops.token[i] == v;
     const int64_t at = (int64_t)blockIdx.x * K + lane;
     new_totals[at] = (float)key64_value(((uint64_t)best.w[0] << 32) | best.w[1]);
     parents[at] = w;
     tokens[at] = v;
-    new_ended[at] = over ? 1 : 0;
+    new_ended[at] = stopped ? 1 : 0;
   }
 }
 
@@ -460,7 +513,7 @@ extern "C" int wptv_beam_workspace(int n, int W, int V, int K, size_t* bytes) {
     return fail(WPTV_E_INVALID, "beam_workspace: bad shape n=%d W=%d V=%d K=%d", n, W, V, K);
   if (W > kMaxBeams || K > kMaxBeams)
     return fail(WPTV_E_UNSUPPORTED, "beam_workspace: at most %d beams a text (W=%d, K=%d)", kMaxBeams, W, K);
-  if ((int64_t)W * V > (1 << 30) || (int64_t)n * W > INT32_MAX)
+  if ((int64_t)W * V > (1 << 28) || (int64_t)n * W > INT32_MAX)
     return fail(WPTV_E_UNSUPPORTED, "beam_workspace: n=%d W=%d V=%d is too large", n, W, V);
   const int part = 64 * part_items((int64_t)n * W, V);
   if ((int64_t)n * W * (((int64_t)V + part - 1) / part) > INT32_MAX)
@@ -507,8 +560,8 @@ extern "C" int wptv_beam_step(const void* scores, int64_t scores_stride_n, int64
 #undef WPTV_PARTS
   const int launch = launched("beam_parts");
   if (launch != WPTV_OK) return launch;
-  if ((int64_t)W * parts * K <= 1024)
-    beam_merge<4><<<n, 256, 0, stream>>>(sums, lists, parts, totals, ended, s, W, V, K, new_totals, parents, tokens,
+  if ((int64_t)W * parts * K <= 4096)
+    beam_merge<8><<<n, 512, 0, stream>>>(sums, lists, parts, totals, ended, s, W, V, K, new_totals, parents, tokens,
                                          new_ended);
   else
     beam_merge<16><<<n, 1024, 0, stream>>>(sums, lists, parts, totals, ended, s, W, V, K, new_totals, parents, tokens,

@@ -19,7 +19,7 @@ A bad shape or dtype is ValueError; a device without the library is
 KernelUnavailable, never a fall back to another form.
 """
 
-import ctypes
+from array import array
 
 import torch
 
@@ -375,26 +375,34 @@ def _index(x, shape, name, device):
 
 
 def _tables(tables, rows, what):
-    """(device, the library's table arguments: addresses, batch and row strides
-    in bytes, capacities, row bytes, count) of tables (rows, capacity, width)."""
-    tables = list(tables)
-    if not tables:
-        raise ValueError(f"{what}: no table given")
-    device = tables[0].device
-    count = len(tables)
+    """(device, the library's table arguments: the host arrays of addresses,
+    batch and row strides in bytes, capacities and row bytes, then their
+    count; the arrays' owner) of tables (rows, capacity, width)."""
+    device = None
+    addresses, strides_b, strides_n, capacities, row_bytes = [], [], [], [], []
     for t in tables:
-        if t.dim() != 3 or t.shape[0] != rows or t.shape[2] == 0:
-            raise ValueError(f"{what}: each table must be ({rows}, capacity, width); got {tuple(t.shape)}")
-        if t.device != device or device.type != "cuda":
+        shape = t.shape
+        if len(shape) != 3 or shape[0] != rows or shape[2] == 0:
+            raise ValueError(f"{what}: each table must be ({rows}, capacity, width); got {tuple(shape)}")
+        if device is None:
+            device = t.device
+        if t.device != device or not t.is_cuda:
             raise KernelUnavailable(f"{what} moves tables on one GPU; got tables on {device} and {t.device}")
-        if t.shape[2] > 1 and t.stride(2) != 1:
+        stride_b, stride_n, stride_c = t.stride()
+        if stride_c != 1 and shape[2] > 1:
             raise ValueError(f"{what}: each row of a table must be contiguous")
-    sizes = [t.element_size() for t in tables]
-    longs = ctypes.c_int64 * count
-    return device, (
-        (ctypes.c_void_p * count)(*[t.data_ptr() for t in tables]),
-        longs(*[t.stride(0) * s for t, s in zip(tables, sizes)]), longs(*[t.stride(1) * s for t, s in zip(tables, sizes)]),
-        longs(*[t.shape[1] for t in tables]), longs(*[t.shape[2] * s for t, s in zip(tables, sizes)]), count)
+        size = t.element_size()
+        addresses.append(t.data_ptr())
+        strides_b.append(stride_b * size)
+        strides_n.append(stride_n * size)
+        capacities.append(shape[1])
+        row_bytes.append(shape[2] * size)
+    if device is None:
+        raise ValueError(f"{what}: no table given")
+    count = len(addresses)
+    held = array("q", addresses + strides_b + strides_n + capacities + row_bytes)
+    at = held.buffer_info()[0]
+    return device, (at, at + 8 * count, at + 16 * count, at + 24 * count, at + 32 * count, count), held
 
 
 def reorder_rows(tables, parents, lengths=None, rows=None):
@@ -413,13 +421,12 @@ def reorder_rows(tables, parents, lengths=None, rows=None):
         raise ValueError("a text has at least one beam")
     if parents.is_floating_point() or parents.dtype == torch.bool:
         raise ValueError(f"parents are whole numbers; got {parents.dtype}")
-    if torch.is_tensor(tables):
-        tables = (tables,)
-    device, arguments = _tables(tables, n * W, "reorder_rows")
+    tables = (tables,) if torch.is_tensor(tables) else tuple(tables)
+    device, arguments, held = _tables(tables, n * W, "reorder_rows")
     parents_ = _long(parents, device)
     lengths_ = None if lengths is None else _index(lengths, (n * W,), "lengths", device)
     if rows is None:
-        rows = max(arguments[3])
+        rows = max(t.shape[1] for t in tables)
     with _lib.on(device):
         check(_lib.lib().wptv_reorder_rows(*arguments, ptr(parents_), ptr(lengths_), int(rows), n, W,
                                            _lib.stream(device)), "reorder_rows")
@@ -503,7 +510,7 @@ def keep_rows(tables, kept, counts):
     if kept.dim() != 3:
         raise ValueError(f"kept must be (layers, B, keep); got {tuple(kept.shape)}")
     L, B, keep = kept.shape
-    device, arguments = _tables(tables, B, "keep_rows")
+    device, arguments, held = _tables(tables, B, "keep_rows")
     if L == 0 or arguments[5] % L:
         raise ValueError(f"keep_rows: {arguments[5]} tables for {L} lists of rows")
     kept_ = _long(kept, device)
