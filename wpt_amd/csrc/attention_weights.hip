@@ -82,20 +82,16 @@ constexpr int kBlockKeys = 256;  // of a workgroup of four
 constexpr int kStage = 1024;     // query heads whose lse and position are staged in LDS at once
 constexpr int kPartRows = 128;   // the fewest query heads of a part
 
-// 16 rows of C values as an operand of the 16-row matrix instructions: lane
-// 16 g + j holds parts of row j.  The products only need both operands to agree
-// on the order of the C values.
+// 16 rows of C values as an operand of the 16-row matrix instructions, in 16-byte
+// pieces: piece f of lane 16 g + j holds bytes 64 f + 16 g of row j.  The products
+// only need both operands to agree on the order of the C values.
 template <typename E, int C>
 struct Rows16;
 
 template <int C>
 struct Rows16<unsigned short, C> {
-  bf16x8 v[C / 32];
-  __device__ __forceinline__ void load(const unsigned short* row, int g) {
-#pragma unroll
-    for (int s = 0; s < C / 32; ++s) v[s] = *reinterpret_cast<const bf16x8*>(row + 32 * s + 8 * g);
-  }
-  static constexpr int kSteps = C / 32;
+  static constexpr int kPieces = C / 32, kSteps = C / 32;
+  bf16x8 v[kPieces];
   static __device__ __forceinline__ f32x4 step(const Rows16& a, const Rows16& b, int s, f32x4 acc) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[s], b.v[s], acc, 0, 0, 0);
   }
@@ -103,12 +99,8 @@ struct Rows16<unsigned short, C> {
 
 template <int C>
 struct Rows16<float, C> {
-  f32x4 v[C / 16];
-  __device__ __forceinline__ void load(const float* row, int g) {
-#pragma unroll
-    for (int s = 0; s < C / 16; ++s) v[s] = *reinterpret_cast<const f32x4*>(row + 16 * s + 4 * g);
-  }
-  static constexpr int kSteps = C / 4;
+  static constexpr int kPieces = C / 16, kSteps = C / 4;
+  f32x4 v[kPieces];
   static __device__ __forceinline__ f32x4 step(const Rows16& a, const Rows16& b, int s, f32x4 acc) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[s / 4][s % 4], b.v[s / 4][s % 4], acc, 0, 0, 0);
   }
@@ -117,7 +109,10 @@ struct Rows16<float, C> {
 // A wavefront holds 64 table rows as the second operand of four products and
 // streams the query heads, 16 at a time, through the first: a lane ends with
 // four query heads of one row in each, whose exponentials it adds to that row's
-// sum in a register.  Nothing but the sums is written.
+// sum in a register.  Nothing but the sums is written.  The query heads come into
+// LDS by DMA in the order of the operand's registers (1 KiB a piece, read back
+// without a bank conflict), 64 at a time for the four wavefronts, the next ones
+// while these are multiplied.
 template <typename E, int C>
 __global__ __launch_bounds__(256) void attention_weights_mfma(
     const E* __restrict__ q, const E* __restrict__ k, int64_t ksb, int64_t ksn, const int64_t* __restrict__ positions,
@@ -125,6 +120,8 @@ __global__ __launch_bounds__(256) void attention_weights_mfma(
     int H, int N, float scale_log2, int nkb, int parts, int part_rows, float* __restrict__ weights, int64_t wsb,
     float* __restrict__ sums) {
   typedef Rows16<E, C> Op;
+  constexpr int kP = Op::kPieces;
+  __shared__ __attribute__((aligned(16))) unsigned char queries[2][4 * kP * 1024];  // blocks of 16, then pieces
   __shared__ __attribute__((aligned(16))) float l2s[kStage];
   __shared__ __attribute__((aligned(16))) int seen[kStage];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -161,28 +158,54 @@ __global__ __launch_bounds__(256) void attention_weights_mfma(
   const int n0 = kb * kBlockKeys, wn0 = n0 + kWaveKeys * w, n = wn0 + lane;
   float total = 0.f;
   if (n0 <= hi) {
+    // query heads first + r0 .. first + r0 + 63 into a buffer, block w by wavefront w
+    // (past the end: the last one again)
+    auto fetch = [&](int r0, int buffer) {
+      const i32x4 rsrc = buffer_resource(q + (rows_b + first + r0) * C);
+      const int row = min(16 * w + j, end - first - r0 - 1);
+      const uint32_t at = lds_address(&queries[buffer][w * kP * 1024]);
+#pragma unroll
+      for (int f = 0; f < kP; ++f)
+        dma_16B(rsrc, (uint32_t)row * (C * sizeof(E)) + 64 * f + 16 * g, __builtin_amdgcn_readfirstlane(at + 1024 * f));
+    };
+    fetch(0, 0);
     Op keys[4];
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      keys[u].load(k + (int64_t)b * ksb + (int64_t)min(wn0 + 16 * u + j, N - 1) * ksn, g);
-    const bool whole = wn0 + kWaveKeys - 1 <= lo;
-    for (int s0 = first; s0 < end; s0 += kStage) {
-      const int many = min(kStage, end - s0), blocks = (many + 15) / 16;
-      if (s0 > first) __syncthreads();
-      for (int i = tid; i < 16 * blocks; i += 256) {  // padding query heads: the last one again, at no weight
-        const int r = min(s0 + i, end - 1);
-        const int64_t p = pos[r / H];
-        l2s[i] = i < many ? lse[rows_b + r] * kLog2e : __builtin_inff();
-        seen[i] = i >= many || p < 0 ? -1 : p < N ? (int)p : N - 1;
+    for (int u = 0; u < 4; ++u) {
+      const E* row = k + (int64_t)b * ksb + (int64_t)min(wn0 + 16 * u + j, N - 1) * ksn;
+#pragma unroll
+      for (int f = 0; f < kP; ++f)
+        keys[u].v[f] = *reinterpret_cast<const decltype(keys[u].v[f] + 0)*>(reinterpret_cast<const unsigned char*>(row) +
+                                                                            64 * f + 16 * g);
+    }
+    const bool whole = wn0 + kWaveKeys - 1 <= lo, idle = wn0 > hi;
+    const int heads = end - first;
+    for (int r0 = 0; r0 < heads; r0 += 64) {
+      const int buffer = (r0 / 64) & 1;
+      if (r0 % kStage == 0) {  // padding query heads have no weight
+        __syncthreads();
+        for (int i = tid; i < min(kStage, (heads - r0 + 15) / 16 * 16); i += 256) {
+          const int r = min(first + r0 + i, end - 1);
+          const int64_t p = pos[r / H];
+          l2s[i] = r0 + i < heads ? lse[rows_b + r] * kLog2e : __builtin_inff();
+          seen[i] = r0 + i >= heads || p < 0 ? -1 : p < N ? (int)p : N - 1;
+        }
+      }
+      if (r0 + 64 < heads) {
+        fetch(r0 + 64, buffer ^ 1);
+        wait_vmcnt<kP>();  // these 64 have come
+      } else {
+        wait_vmcnt<0>();
       }
       __syncthreads();
-      if (wn0 > hi) continue;
-      const E* qs = q + (rows_b + s0) * C;
+      const int blocks = idle ? 0 : min(4, (heads - r0 + 15) / 16);
       for (int m = 0; m < blocks; ++m) {
         Op query;
-        query.load(qs + (int64_t)min(16 * m + j, many - 1) * C, g);
-        const f32x4 l2 = *reinterpret_cast<const f32x4*>(&l2s[16 * m + 4 * g]);
+#pragma unroll
+        for (int f = 0; f < kP; ++f)
+          query.v[f] = *reinterpret_cast<const decltype(query.v[f] + 0)*>(&queries[buffer][(m * kP + f) * 1024 + lane * 16]);
+        const f32x4 l2 = *reinterpret_cast<const f32x4*>(&l2s[r0 % kStage + 16 * m + 4 * g]);
         f32x4 acc[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -200,7 +223,7 @@ __global__ __launch_bounds__(256) void attention_weights_mfma(
             sum[u] += (e[0] + e[1]) + (e[2] + e[3]);
           }
         } else {
-          const i32x4 p = *reinterpret_cast<const i32x4*>(&seen[16 * m + 4 * g]);
+          const i32x4 p = *reinterpret_cast<const i32x4*>(&seen[r0 % kStage + 16 * m + 4 * g]);
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             float e[4];
@@ -213,6 +236,7 @@ __global__ __launch_bounds__(256) void attention_weights_mfma(
           }
         }
       }
+      __syncthreads();  // the buffer is read
     }
     // the four lane groups' sums of the four blocks, block u into lane group u
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[0]), __float_as_uint(sum[1]), false, false);
