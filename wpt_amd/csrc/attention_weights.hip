@@ -79,7 +79,8 @@ __global__ __launch_bounds__(kGT) void attention_weights_generic(
 
 constexpr int kWaveKeys = 64;    // table rows of a wavefront
 constexpr int kBlockKeys = 256;  // of a workgroup of four
-constexpr int kStage = 1024;     // query heads whose lse and position are staged in LDS at once
+constexpr int kStage = 512;      // query heads whose lse and position are staged in LDS at once
+constexpr float kUnseen = -1.f;  // a part's sum for a row that none of its queries sees (sums are not negative)
 constexpr int kPartRows = 128;   // the fewest query heads of a part
 
 // 16 rows of C values as an operand of the 16-row matrix instructions, in 16-byte
@@ -113,8 +114,10 @@ struct Rows16<float, C> {
 // LDS by DMA in the order of the operand's registers (1 KiB a piece, read back
 // without a bank conflict), 64 at a time for the four wavefronts, the next ones
 // while these are multiplied.
+// At least two wavefronts a SIMD: the compiler then keeps the products out of the
+// accumulation registers, which the exponentials cannot read.
 template <typename E, int C>
-__global__ __launch_bounds__(256) void attention_weights_mfma(
+__global__ __launch_bounds__(256, 2) void attention_weights_mfma(
     const E* __restrict__ q, const E* __restrict__ k, int64_t ksb, int64_t ksn, const int64_t* __restrict__ positions,
     const float* __restrict__ lse, const int64_t* __restrict__ counts, const int64_t* __restrict__ start, int B, int T,
     int H, int N, float scale_log2, int nkb, int parts, int part_rows, float* __restrict__ weights, int64_t wsb,
@@ -152,8 +155,8 @@ __global__ __launch_bounds__(256) void attention_weights_mfma(
       lo = min(lo, c);
       hi = max(hi, c);
     }
-    lo = wave_min_i32(lo);
-    hi = wave_max_i32(hi);
+    lo = __builtin_amdgcn_readfirstlane(wave_min_i32(lo));
+    hi = __builtin_amdgcn_readfirstlane(wave_max_i32(hi));
   }
   const int n0 = kb * kBlockKeys, wn0 = n0 + kWaveKeys * w, n = wn0 + lane;
   float total = 0.f;
@@ -179,6 +182,11 @@ __global__ __launch_bounds__(256) void attention_weights_mfma(
         keys[u].v[f] = *reinterpret_cast<const decltype(keys[u].v[f] + 0)*>(reinterpret_cast<const unsigned char*>(row) +
                                                                             64 * f + 16 * g);
     }
+    // the keys are waited for here: in the loop, the wait would be for the DMA too
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int f = 0; f < kP; ++f) asm volatile("" : "+v"(keys[u].v[f]));
     const bool whole = wn0 + kWaveKeys - 1 <= lo, idle = wn0 > hi;
     const int heads = end - first;
     for (int r0 = 0; r0 < heads; r0 += 64) {
@@ -247,39 +255,41 @@ __global__ __launch_bounds__(256) void attention_weights_mfma(
     total = __uint_as_float(d[0]) + __uint_as_float(d[1]);
   }
   if (parts > 1) {
-    sums[((int64_t)part * B + b) * nkb * kBlockKeys + n] = total;
+    sums[((int64_t)part * B + b) * nkb * kBlockKeys + n] = n <= hi ? total : kUnseen;
   } else if (n <= hi) {
     float* out = weights + (int64_t)b * wsb + n;
     *out = (start && n >= start[b] ? 0.f : *out) + total;
   }
 }
 
+// weights += the parts' sums in order, a fourth of them by each wavefront of a
+// workgroup of 64 rows; rows that no part sees are left alone.
 __global__ __launch_bounds__(256) void attention_weights_join(const float* __restrict__ sums, int parts, int nkb, int B,
-                                                              int T, int N, const int64_t* __restrict__ positions,
-                                                              const int64_t* __restrict__ counts,
-                                                              const int64_t* __restrict__ start,
+                                                              int N, const int64_t* __restrict__ start,
                                                               float* __restrict__ weights, int64_t wsb) {
-  __shared__ int most[4];
-  const int b = blockIdx.y, n = blockIdx.x * kBlockKeys + threadIdx.x;
-  const int tn = counted(counts, b, T);
-  int hi = -1;
-  for (int t = threadIdx.x; t < tn; t += 256) {
-    const int64_t p = positions[(int64_t)b * T + t];
-    hi = max(hi, p < 0 ? -1 : p < N ? (int)p : N - 1);
-  }
-  hi = wave_max_i32(hi);
-  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = hi;
-  __syncthreads();
-  hi = max(max(most[0], most[1]), max(most[2], most[3]));
-  if (n > hi) return;
-  float* out = weights + (int64_t)b * wsb + n;
-  const float before = start && n >= start[b] ? 0.f : *out;
+  __shared__ float shared[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int b = blockIdx.y, n = blockIdx.x * 64 + lane;
   const int64_t stride = (int64_t)B * nkb * kBlockKeys;
+  const int some = (parts + 3) / 4, end = min(parts, (w + 1) * some);
   const float* s = sums + (int64_t)b * nkb * kBlockKeys + n;
-  float total = 0.f;
+  float total = kUnseen;
 #pragma unroll 8
-  for (int p = 0; p < parts; ++p) total += s[p * stride];
-  *out = before + total;
+  for (int p = w * some; p < end; ++p) {
+    const float x = s[p * stride];
+    total = x == kUnseen ? total : total == kUnseen ? x : total + x;
+  }
+  shared[w][lane] = total;
+  __syncthreads();
+  if (w != 0 || n >= N) return;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    const float x = shared[i][lane];
+    total = x == kUnseen ? total : total == kUnseen ? x : total + x;
+  }
+  if (total == kUnseen) return;
+  float* out = weights + (int64_t)b * wsb + n;
+  *out = (start && n >= start[b] ? 0.f : *out) + total;
 }
 
 // The parts the T H query heads are cut into: enough that B x (blocks of 256
@@ -357,8 +367,8 @@ extern "C" int wptv_attention_weights(const void* q, const void* k, int64_t k_st
 #undef WPTV_WEIGHTS
     const int launch = launched("attention_weights_mfma");
     if (launch != WPTV_OK || splits == 1) return launch;
-    attention_weights_join<<<dim3(blocks, B), 256, 0, stream>>>(sums, splits, blocks, B, T, N, positions, counts, start,
-                                                                weights, weights_stride_b);
+    attention_weights_join<<<dim3((N + 63) / 64, B), 256, 0, stream>>>(sums, splits, blocks, B, N, start, weights,
+                                                                       weights_stride_b);
     return launched("attention_weights_join");
   }
   const int nkb = (N + kKeys - 1) / kKeys;
