@@ -81,7 +81,6 @@ constexpr int kWaveKeys = 64;    // table rows of a wavefront
 constexpr int kBlockKeys = 256;  // of a workgroup of four
 constexpr int kStage = 512;      // query heads whose lse and position are staged in LDS at once
 constexpr float kUnseen = -1.f;  // a part's sum for a row that none of its queries sees (sums are not negative)
-constexpr int kPartRows = 128;   // the fewest query heads of a part
 
 // 16 rows of C values as an operand of the 16-row matrix instructions, in 16-byte
 // pieces: piece f of lane 16 g + j holds bytes 64 f + 16 g of row j.  The products
@@ -120,8 +119,8 @@ template <typename E, int C>
 __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
     const E* __restrict__ q, const E* __restrict__ k, int64_t ksb, int64_t ksn, const int64_t* __restrict__ positions,
     const float* __restrict__ lse, const int64_t* __restrict__ counts, const int64_t* __restrict__ start, int B, int T,
-    int H, int N, float scale_log2, int nkb, int parts, int part_rows, float* __restrict__ weights, int64_t wsb,
-    float* __restrict__ sums) {
+    int H, int N, float scale_log2, int nkb, int parts, int part_rows, int by_xcd, float* __restrict__ weights,
+    int64_t wsb, float* __restrict__ sums) {
   typedef Rows16<E, C> Op;
   constexpr int kP = Op::kPieces;
   __shared__ __attribute__((aligned(16))) unsigned char queries[2][4 * kP * 1024];  // blocks of 16, then pieces
@@ -129,43 +128,66 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
   __shared__ __attribute__((aligned(16))) int seen[kStage];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j = lane & 15, g = lane >> 4;
-  int kb, b, part;
-  if (parts == 1) {
-    kb = blockIdx.x % nkb;
-    b = blockIdx.x / nkb;
-    part = 0;
-  } else {  // workgroups go to the 8 XCDs in turn: a part's queries are read through one XCD's L2
-    int rest = blockIdx.x / 8;
-    kb = rest % nkb;
-    rest /= nkb;
-    b = rest % B;
-    part = rest / B * 8 + blockIdx.x % 8;
-    if (part >= parts) return;
+  int kb = blockIdx.x % nkb, chunk = blockIdx.x / nkb;
+  if (by_xcd) {  // workgroups go to the 8 XCDs in turn: the queries of a part are read through one XCD's L2
+    kb = blockIdx.x / 8 % nkb;
+    chunk = blockIdx.x / 8 / nkb * 8 + blockIdx.x % 8;
+    if (chunk >= parts * B) return;
   }
+  const int b = chunk / parts, part = chunk % parts;
   const int64_t rows_b = (int64_t)b * T * H;
   const int first = part * part_rows;
-  const int end = min(counted(counts, b, T) * H, first + part_rows);
-  // the rows that the part's queries see end at hi, and each sees those up to lo
+  // The rows that the part's queries see end at hi, and each sees those up to lo.
   const int64_t* pos = positions + (int64_t)b * T;
-  int lo = N - 1, hi = -1;
-  if (first < end) {
-    for (int t = first / H + lane; t <= (end - 1) / H; t += 64) {
-      const int64_t p = pos[t];
-      const int c = p < 0 ? -1 : p < N ? (int)p : N - 1;
-      lo = min(lo, c);
-      hi = max(hi, c);
-    }
+  auto reach = [&](int64_t p) { return p < 0 ? -1 : p < N ? (int)p : N - 1; };
+  int lo = N - 1, hi = -1, end;
+  {
+    const int t0 = first / H;
+    const int64_t p0 = pos[min(t0 + lane, T - 1)];  // read with the count, not after it
+    end = min(counted(counts, b, T) * H, first + part_rows);
+    const int t1 = (end - 1) / H;
+    if (first < end && t0 + lane <= t1) lo = hi = reach(p0);
+    if (first < end)
+      for (int t = t0 + 64 + lane; t <= t1; t += 64) {
+        const int c = reach(pos[t]);
+        lo = min(lo, c);
+        hi = max(hi, c);
+      }
     lo = __builtin_amdgcn_readfirstlane(wave_min_i32(lo));
     hi = __builtin_amdgcn_readfirstlane(wave_max_i32(hi));
   }
   const int n0 = kb * kBlockKeys, wn0 = n0 + kWaveKeys * w, n = wn0 + lane;
-  float total = 0.f;
+  float total = 0.f, before = 0.f;
   if (n0 <= hi) {
+    const int heads = end - first;
+    // the lse and reach of query heads r0 .. r0 + kStage - 1, from memory and into
+    // LDS; padding query heads have no weight
+    float l2[kStage / 256];
+    int see[kStage / 256];
+    auto read_stage = [&](int r0) {
+#pragma unroll
+      for (int i = 0; i < kStage / 256; ++i) {
+        const int r = min(r0 + tid + 256 * i, heads - 1);
+        l2[i] = lse[rows_b + first + r];
+        see[i] = reach(pos[(first + r) / H]);
+      }
+    };
+    auto write_stage = [&](int r0) {
+#pragma unroll
+      for (int i = 0; i < kStage / 256; ++i) {
+        const bool padding = r0 + tid + 256 * i >= heads;
+        l2s[tid + 256 * i] = padding ? __builtin_inff() : l2[i] * kLog2e;
+        seen[tid + 256 * i] = padding ? -1 : see[i];
+      }
+    };
+    // everything is asked for at once: what is waited for first, first
+    read_stage(0);
+    if (parts == 1 && n <= hi && !(start && n >= start[b])) before = weights[(int64_t)b * wsb + n];
     // query heads first + r0 .. first + r0 + 63 into a buffer, block w by wavefront w
     // (past the end: the last one again)
     auto fetch = [&](int r0, int buffer) {
       const i32x4 rsrc = buffer_resource(q + (rows_b + first + r0) * C);
-      const int row = min(16 * w + j, end - first - r0 - 1);
+      const int row = min(16 * w + j, heads - r0 - 1);
       const uint32_t at = lds_address(&queries[buffer][w * kP * 1024]);
 #pragma unroll
       for (int f = 0; f < kP; ++f)
@@ -182,23 +204,18 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
         keys[u].v[f] = *reinterpret_cast<const decltype(keys[u].v[f] + 0)*>(reinterpret_cast<const unsigned char*>(row) +
                                                                             64 * f + 16 * g);
     }
+    write_stage(0);
     // the keys are waited for here: in the loop, the wait would be for the DMA too
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int f = 0; f < kP; ++f) asm volatile("" : "+v"(keys[u].v[f]));
     const bool whole = wn0 + kWaveKeys - 1 <= lo, idle = wn0 > hi;
-    const int heads = end - first;
     for (int r0 = 0; r0 < heads; r0 += 64) {
       const int buffer = (r0 / 64) & 1;
-      if (r0 % kStage == 0) {  // padding query heads have no weight
-        __syncthreads();
-        for (int i = tid; i < min(kStage, (heads - r0 + 15) / 16 * 16); i += 256) {
-          const int r = min(first + r0 + i, end - 1);
-          const int64_t p = pos[r / H];
-          l2s[i] = r0 + i < heads ? lse[rows_b + r] * kLog2e : __builtin_inff();
-          seen[i] = r0 + i >= heads || p < 0 ? -1 : p < N ? (int)p : N - 1;
-        }
+      if (r0 > 0 && r0 % kStage == 0) {  // the last barrier is behind the reads of the stage before
+        read_stage(r0);
+        write_stage(r0);
       }
       if (r0 + 64 < heads) {
         fetch(r0 + 64, buffer ^ 1);
@@ -258,7 +275,7 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
     sums[((int64_t)part * B + b) * nkb * kBlockKeys + n] = n <= hi ? total : kUnseen;
   } else if (n <= hi) {
     float* out = weights + (int64_t)b * wsb + n;
-    *out = (start && n >= start[b] ? 0.f : *out) + total;
+    *out = before + total;
   }
 }
 
@@ -292,12 +309,19 @@ __global__ __launch_bounds__(256) void attention_weights_join(const float* __res
   *out = (start && n >= start[b] ? 0.f : *out) + total;
 }
 
-// The parts the T H query heads are cut into: enough that B x (blocks of 256
-// rows) x parts workgroups fill the GPU, of at least kPartRows query heads.
+// The parts the T H query heads are cut into.  A workgroup a compute unit where
+// parts of 32 query heads give them; above that, parts of about 512 query heads
+// balance what a causal prompt leaves of them, up to 16 workgroups a compute unit
+// (the parts' sums have to be joined).  Measured, us, by parts: two prompts of 4096
+// tokens 121 [32], 73 [64], 67 [128], 71 [192]; a chunk of 1024 tokens over 4096 rows
+// 38 [16], 26 [32], 32 [96], 39 [192]; one of 64 over 8192 34 [1], 14 [4], 11 [8],
+// 14 [32]; a prompt of 512 36 [8], 11.2 [64], 10.4 [128], 12.9 [192]; 9 queries of 32
+// heads over 1000 rows 12.8 [1], 9.0 [4], 8.0 [12].
 int weight_parts(int B, int T, int H, int N) {
   const int64_t rows = (int64_t)T * H, units = (int64_t)B * ((N + kBlockKeys - 1) / kBlockKeys);
-  const int64_t fill = (8 * compute_units() + units - 1) / units;
-  return (int)max((int64_t)1, min(fill, rows / kPartRows));
+  const int64_t cus = compute_units();
+  const int64_t parts = max(min(cus / units, rows / 32), min(rows / 512, 16 * cus / units));
+  return (int)max((int64_t)1, parts);
 }
 
 bool matrix_width(int c) { return c == 64 || c == 128; }
@@ -327,7 +351,7 @@ extern "C" int wptv_attention_weights_workspace(int B, int T, int H, int c, int 
     *splits = (int)min((int64_t)*splits, (rows + 15) / 16);  // a part holds at least one block of query heads
   }
   const int64_t nkb = (N + kBlockKeys - 1) / kBlockKeys;
-  if ((int64_t)B * nkb * (*splits + 8) > INT32_MAX)
+  if ((int64_t)B * nkb * *splits + nkb * 8 > INT32_MAX)
     return fail(WPTV_E_UNSUPPORTED, "attention_weights: B=%d N=%d in %d parts is too large", B, N, *splits);
   *bytes = *splits == 1 ? 0 : (size_t)*splits * B * nkb * kBlockKeys * sizeof(float);
   return WPTV_OK;
@@ -353,12 +377,14 @@ extern "C" int wptv_attention_weights(const void* q, const void* k, int64_t k_st
   if (matrix_width(c) && aligned(q, 16) && aligned(k, 16) && k_stride_n * elem % 16 == 0 && k_stride_b * elem % 16 == 0) {
     const int blocks = (N + kBlockKeys - 1) / kBlockKeys;
     const int part_rows = (int)(((int64_t)T * H + splits - 1) / splits + 15) / 16 * 16;
-    const int groups = splits == 1 ? 1 : (splits + 7) / 8 * 8;
+    const int chunks = splits * B;
+    const int by_xcd = splits > 1 && (chunks % 8 == 0 || chunks >= 64);  // as many chunks an XCD, nearly
+    const int groups = by_xcd ? (chunks + 7) / 8 * 8 : chunks;
     float* sums = static_cast<float*>(workspace);
 #define WPTV_WEIGHTS(E, C)                                                                                            \
-  attention_weights_mfma<E, C><<<B * blocks * groups, 256, 0, stream>>>(                                             \
+  attention_weights_mfma<E, C><<<blocks * groups, 256, 0, stream>>>  (                                             \
       static_cast<const E*>(q), static_cast<const E*>(k), k_stride_b, k_stride_n, positions, lse, counts, start, B, T, \
-      H, N, scale * kLog2e, blocks, splits, part_rows, weights, weights_stride_b, sums)
+      H, N, scale * kLog2e, blocks, splits, part_rows, by_xcd, weights, weights_stride_b, sums)
     if (dtype == WPTV_BF16) {
       if (c == 64) WPTV_WEIGHTS(unsigned short, 64); else WPTV_WEIGHTS(unsigned short, 128);
     } else {

@@ -74,27 +74,31 @@ __global__ __launch_bounds__(kThreads) void reorder_rows(Tables tables, const in
   typedef typename Unit<BYTES>::type U;
   const Table& t = tables.t[blockIdx.z];
   const int text = blockIdx.y;
+  // lane w: beam w's source, and how many of its rows beam w takes (none where
+  // it stays as it is, or the source is no beam of the text)
+  const int lane = threadIdx.x & 63;
+  int source = 0, taken = 0;
+  if (lane < W) {
+    const int64_t p = parents[(int64_t)text * W + lane];
+    if (p >= 0 && p < W && p != lane) {
+      source = (int)p;
+      taken = t.capacity;
+      if (lengths) taken = (int)min(max(lengths[(int64_t)text * W + p], (int64_t)0), (int64_t)t.capacity);
+    }
+  }
   const uint32_t at = blockIdx.x * kThreads + threadIdx.x;  // below 2^31: checked on the host
   const int n = (int)(at / (uint32_t)t.pieces);
   const int piece = (int)(at % (uint32_t)t.pieces);
-  if (n >= t.capacity) return;
   unsigned char* place = t.base + (int64_t)text * W * t.stride_b + n * t.stride_n + (int64_t)piece * BYTES;
   U held[WMAX];
-  bool moves[WMAX];
 #pragma unroll
   for (int w = 0; w < WMAX; ++w) {
-    moves[w] = false;
-    if (w < W) {
-      const int64_t from = const_load(parents, (int64_t)text * W + w);  // one that is no beam of the text moves nothing
-      if (from >= 0 && from < W && from != w) {
-        moves[w] = !lengths || n < const_load(lengths, (int64_t)text * W + from);
-        if (moves[w]) held[w] = *reinterpret_cast<const U*>(place + from * t.stride_b);
-      }
-    }
+    const int from = __builtin_amdgcn_readlane(source, w), end = __builtin_amdgcn_readlane(taken, w);
+    if (n < end) held[w] = *reinterpret_cast<const U*>(place + from * t.stride_b);
   }
 #pragma unroll
   for (int w = 0; w < WMAX; ++w)
-    if (w < W && moves[w]) *reinterpret_cast<U*>(place + w * t.stride_b) = held[w];
+    if (n < __builtin_amdgcn_readlane(taken, w)) *reinterpret_cast<U*>(place + w * t.stride_b) = held[w];
 }
 
 constexpr int kKeepThreads = 512;
@@ -183,11 +187,14 @@ int launch_reorder(const Tables& tables, int count, int64_t blocks, int n, const
 template <int BYTES>
 int launch_keep(const Tables& tables, int count, int widest, const int64_t* kept, int B, int keep,
                 const int64_t* counts, hipStream_t stream) {
-  // slices of a row, one a workgroup: whole 128-byte lines where the slices fill
-  // the compute units twice, thinner ones where there are few (down to a unit)
+  // Slices of a row, one a workgroup: whole 128-byte lines, thinner where there
+  // would be hardly any workgroup.  Measured, us, 24 layers, rows of 512 bytes, slices
+  // of 32, 64, 128 and 256 bytes: 16 texts from 4096 to 2048 rows 231, 151, 115, 111; one
+  // text 25, 16, 14, 23; 32 texts, a quarter of them over 1024 rows, 90, 51, 38, 43; one
+  // layer of one text of 16000 rows 29, 35, 51, 100.
   int shift = 0;
   while ((BYTES << (shift + 1)) <= 128 && (1 << shift) < widest) ++shift;
-  while (shift > 0 && (int64_t)count * B * ((widest + (1 << shift) - 1) >> shift) < 2 * compute_units()) --shift;
+  while (shift > 0 && (int64_t)count * B * ((widest + (1 << shift) - 1) >> shift) < 16) --shift;
   const int slices = (widest + (1 << shift) - 1) >> shift;
   keep_rows<BYTES><<<dim3(slices, B, count), kKeepThreads, 0, stream>>>(tables, kept, B, keep, counts, shift);
   return launched("keep_rows");
