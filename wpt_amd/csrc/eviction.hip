@@ -9,9 +9,8 @@
 //   choose_kept_regs  up to 16384 rows: the weights' keys in registers, the
 //                     smallest one kept by kth_largest, the rows listed after
 //                     one scan of the threads' counts
-//   choose_kept       longer texts: a radix select over the weights in memory,
-//                     most significant byte first, then one pass that lists the
-//                     kept rows by wavefront ballots
+//   choose_kept_long  longer texts: the same over the weights in memory, each
+//                     wavefront listing a stretch of the rows by ballots
 #include "select_common.h"
 #include "wptv_common.h"
 
@@ -19,8 +18,6 @@
 
 namespace wptv {
 namespace {
-
-constexpr int kST = 256;
 
 __device__ __forceinline__ uint32_t weight_key(float f) { return f != f ? ~0u : order_key(f + 0.f); }
 
@@ -91,82 +88,86 @@ __global__ __launch_bounds__(THREADS) void choose_kept_regs(const float* __restr
   });
 }
 
-__global__ __launch_bounds__(kST) void choose_kept(const float* __restrict__ weights, int64_t wsl, int64_t wsb, int B,
-                                                   int N, const int64_t* __restrict__ lengths, int keep, int first,
-                                                   int recent, int64_t* __restrict__ kept,
-                                                   int64_t* __restrict__ counts) {
-  __shared__ int hist[256];
-  __shared__ int sel[2];
-  __shared__ int wcount[2][kST / 64];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+constexpr int kLongThreads = 1024, kLongWaves = kLongThreads / 64;
+constexpr int kLongLoads = 8;  // rows a thread asks for at once
+
+__global__ __launch_bounds__(kLongThreads) void choose_kept_long(const float* __restrict__ weights, int64_t wsl,
+                                                                 int64_t wsb, int B, int N,
+                                                                 const int64_t* __restrict__ lengths, int keep,
+                                                                 int first, int recent, int64_t* __restrict__ kept,
+                                                                 int64_t* __restrict__ counts) {
+  __shared__ SelectShared<kLongThreads> select;
+  __shared__ int above[kLongWaves], equals[kLongWaves];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int layer = blockIdx.x / B, b = blockIdx.x % B;
-  int64_t len64 = lengths[b];
+  const int64_t len64 = lengths[b];
   const int len = len64 < 0 ? 0 : len64 < N ? (int)len64 : N;
   int64_t* out = kept + (int64_t)blockIdx.x * keep;
   if (layer == 0 && tid == 0) counts[b] = len < keep ? len : keep;
   if (len <= keep) {
-    for (int i = tid; i < keep; i += kST) out[i] = i < len ? i : -1;
+    for (int i = tid; i < keep; i += kLongThreads) out[i] = i < len ? i : -1;
     return;
   }
-  const float* s = weights + layer * wsl + b * wsb;
-  const int end = len - recent;          // candidates: rows first .. end - 1
-  const int take = keep - first - recent;  // fewer than the candidates
-  uint32_t tau = ~0u;
-  int need_eq = 0;
-  if (take > 0) {
-    uint32_t prefix = 0, mask = 0;
-    int remaining = take;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      hist[tid] = 0;
-      __syncthreads();
-      for (int n = first + tid; n < end; n += kST) {
-        const uint32_t u = weight_key(s[n]);
-        if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int above = 0, digit = 255;
-        while (above + hist[digit] < remaining) above += hist[digit--];
-        sel[0] = digit;
-        sel[1] = remaining - above;
-      }
-      __syncthreads();
-      prefix |= (uint32_t)sel[0] << shift;
-      mask |= 255u << shift;
-      remaining = sel[1];
+  const int take = keep - first - recent, candidates = len - first - recent;  // take < candidates
+  for (int i = tid; i < first; i += kLongThreads) out[i] = i;
+  for (int i = tid; i < recent; i += kLongThreads) out[keep - recent + i] = len - recent + i;
+  if (take == 0) return;
+  const float* s = weights + layer * wsl + b * wsb + first;
+  // f(row, key) of rows begin + step i, several asked for at once
+  auto rows = [&](int begin, int end, int step, auto&& f) {
+    for (int n = begin; n < end; n += kLongLoads * step) {
+      float x[kLongLoads];
+#pragma unroll
+      for (int i = 0; i < kLongLoads; ++i) x[i] = n + i * step < end ? s[n + i * step] : 0.f;
+#pragma unroll
+      for (int i = 0; i < kLongLoads; ++i)
+        if (n + i * step < end) f(n + i * step, weight_key(x[i]));
     }
-    tau = prefix;
-    need_eq = remaining;
+  };
+  auto each = [&](auto&& f) { rows(tid, candidates, kLongThreads, f); };
+  const uint32_t tau = kth_largest<kLongThreads>(each, take, select);
+  // each wavefront counts, then lists, a stretch of consecutive rows
+  const int stretch = ((candidates + kLongWaves - 1) / kLongWaves + 63) / 64 * 64;
+  const int begin = min(w * stretch, candidates), end = min(begin + stretch, candidates);
+  int gt = 0, eq = 0;
+  rows(begin + lane, end, 64, [&](int, uint32_t x) {
+    gt += x > tau ? 1 : 0;
+    eq += x == tau ? 1 : 0;
+  });
+  gt = (int)wave_sum_u32(gt);
+  eq = (int)wave_sum_u32(eq);
+  if (lane == 0) {
+    above[w] = gt;
+    equals[w] = eq;
   }
-  // one pass in row order: rows equal to the smallest kept weight are counted
-  // so that the first need_eq of them are kept
-  const uint64_t below = (1ull << lane) - 1ull;
-  int base = 0, base_eq = 0;
-  for (int start = 0; start < len; start += kST) {
-    const int n = start + tid;
-    const bool candidate = n >= first && n < end;
-    const uint32_t u = candidate ? weight_key(s[n]) : 0u;
-    const bool eq = candidate && take > 0 && u == tau;
-    const uint64_t be = __builtin_amdgcn_ballot_w64(eq);
-    if (lane == 0) wcount[0][w] = __builtin_popcountll(be);
-    __syncthreads();
-    int pe = base_eq;
-    for (int i = 0; i < w; ++i) pe += wcount[0][i];
-    pe += __builtin_popcountll(be & below);
-    const bool in = n < len && (!candidate || (take > 0 && (u > tau || (eq && pe < need_eq))));
-    const uint64_t bi = __builtin_amdgcn_ballot_w64(in);
-    if (lane == 0) wcount[1][w] = __builtin_popcountll(bi);
-    __syncthreads();
-    int p = base;
-    for (int i = 0; i < w; ++i) p += wcount[1][i];
-    p += __builtin_popcountll(bi & below);
-    if (in) out[p] = n;
-    for (int i = 0; i < kST / 64; ++i) {
-      base_eq += wcount[0][i];
-      base += wcount[1][i];
+  __syncthreads();
+  int all = 0;
+  gt = eq = 0;
+  for (int i = 0; i < kLongWaves; ++i) {
+    all += above[i];
+    if (i < w) {
+      gt += above[i];
+      eq += equals[i];
     }
-    __syncthreads();
+  }
+  const int equal = take - all;  // rows equal to tau that are kept, the first ones
+  const uint64_t below = (1ull << lane) - 1ull;
+  for (int n0 = begin; n0 < end; n0 += kLongLoads * 64) {
+    float x[kLongLoads];
+#pragma unroll
+    for (int i = 0; i < kLongLoads; ++i) x[i] = n0 + 64 * i + lane < end ? s[n0 + 64 * i + lane] : 0.f;
+#pragma unroll
+    for (int i = 0; i < kLongLoads; ++i) {
+      const int n = n0 + 64 * i + lane;
+      const uint32_t u = weight_key(x[i]);
+      const uint64_t more = __builtin_amdgcn_ballot_w64(n < end && u > tau);
+      const uint64_t same = __builtin_amdgcn_ballot_w64(n < end && u == tau);
+      const int e = eq + __builtin_popcountll(same & below);
+      if (n < end && (u > tau || (u == tau && e < equal)))
+        out[first + gt + __builtin_popcountll(more & below) + min(e, equal)] = first + n;
+      gt += __builtin_popcountll(more);
+      eq += __builtin_popcountll(same);
+    }
   }
 }
 
@@ -195,8 +196,8 @@ extern "C" int wptv_choose_kept(const float* weights, int64_t weights_stride_l, 
   else if (N <= 16384)
     WPTV_KEPT(1024, 4);
   else
-    choose_kept<<<L * B, kST, 0, stream>>>(weights, weights_stride_l, weights_stride_b, B, N, lengths, keep, first,
-                                           recent, kept, counts);
+    choose_kept_long<<<L * B, kLongThreads, 0, stream>>>(weights, weights_stride_l, weights_stride_b, B, N, lengths,
+                                                         keep, first, recent, kept, counts);
 #undef WPTV_KEPT
   return launched("choose_kept");
 }
