@@ -23,6 +23,16 @@ table in place up to each query's position.  Undo restores the lengths from
 before the undoable reading plus kept; the entries past a row's length are
 never read, and are written again when the row reaches them.
 
+A beam search's rows take over each other's states with reorder, in place.  A
+weighted cache also keeps the attention weight that each exact layer's rows have
+received (`weights`, FP32 (exact layers, B, capacity)): the decoder adds each
+reading's, an undoable one's when its kept tokens are known.  evict then brings
+every row down to its first, its last and its heaviest entries, moved together
+in place: from then on token p is no longer at row p of the exact layers' tables
+(whose attention has no use for the position), and `evicted` counts each row's
+entries taken out, so that the window layers' rings still place token
+lengths + evicted.
+
 The lengths stay on the device; `bound` is a host-side upper bound of every
 row's length (raised by each reading's width, never lowered by undo) so that
 growing the tables needs no host synchronization.  The tables grow to
@@ -32,7 +42,7 @@ step is captured with the capacity reserved beforehand.
 
 import torch
 
-from . import _lib
+from . import _lib, kernels
 from ._lib import check, ptr
 
 
@@ -49,9 +59,11 @@ def _lengths(lengths, before, counts, undo):
 class Cache:
     """rings: the layers whose table is a ring of ring_rows rows (window
     layers); bare: the layers with no table (sparse layers); every other
-    layer's table grows with the text."""
+    layer's table grows with the text.  weighted: the growing tables' rows
+    carry the attention weight they have received, and may be evicted."""
 
-    def __init__(self, rows, layers, width, dtype, device, capacity=256, rings=(), ring_rows=256, bare=()):
+    def __init__(self, rows, layers, width, dtype, device, capacity=256, rings=(), ring_rows=256, bare=(),
+                 weighted=False):
         if ring_rows <= 0 or ring_rows & (ring_rows - 1):
             raise ValueError(f"a ring holds a power of 2 of rows, not {ring_rows}")
         self.lengths = torch.zeros(rows, dtype=torch.long, device=device)
@@ -63,6 +75,18 @@ class Cache:
         self.pending = False
         self.bound = 0
         self.routes = None
+        self.weights = self.evicted = None
+        self._read = []  # a weighted cache's undoable reading: (weights' row, layer, q, positions, lse, scale, counts)
+        if weighted:
+            if not self.growing:
+                raise ValueError("a weighted cache has at least one table that grows with the text")
+            self.weights = torch.zeros(len(self.growing), rows, capacity, dtype=torch.float32, device=device)
+            self.evicted = torch.zeros_like(self.lengths)
+
+    @property
+    def growing(self):
+        """The layers whose table grows with the text."""
+        return [i for i, t in enumerate(self.tables) if t is not None and i not in self.rings]
 
     @property
     def rows(self):
@@ -90,6 +114,14 @@ class Cache:
         self.tables = [t if t is None or i in self.rings else torch.cat([t, t.new_zeros(t.shape[0], grown - t.shape[1],
                                                                            t.shape[2])], 1)
                        for i, t in enumerate(self.tables)]
+        if self.weights is not None:
+            self.weights = torch.cat([self.weights, self.weights.new_zeros(*self.weights.shape[:2],
+                                                                           grown - self.weights.shape[2])], 2)
+
+    def starts(self):
+        """The position of each row's next token in its text: its length, and
+        the entries evicted before."""
+        return self.lengths if self.evicted is None else self.lengths + self.evicted
 
     def tail(self, layer, steps):
         """A window layer's carried tail (B, steps, width): the entries of the
@@ -101,7 +133,7 @@ class Cache:
         R = ring.shape[1]
         if steps > R:
             raise ValueError(f"the ring holds {R} rows, fewer than {steps}")
-        positions = self.lengths[:, None] - steps + torch.arange(steps, device=ring.device)
+        positions = self.starts()[:, None] - steps + torch.arange(steps, device=ring.device)
         rows = ring.gather(1, (positions % R)[..., None].expand(-1, -1, ring.shape[2]))
         return rows.masked_fill((positions < 0)[..., None], 0)
 
@@ -117,7 +149,11 @@ class Cache:
         """Back to the lengths before the last undoable reading, plus kept."""
         if not self.pending:
             raise ValueError("no undoable extend to undo")
+        if self.weights is not None and not self._read:
+            raise ValueError("the weights of the reading to undo are not here: a captured undoable reading of a weighted "
+                             "cache is captured together with its undo")
         _lengths(self.lengths, self.before, kept, undo=True)
+        self.settle(kept)
         self.pending = False
 
     def undo_on_device(self):
@@ -126,8 +162,32 @@ class Cache:
         reading counts as undone from here on."""
         if not self.pending:
             raise ValueError("no undoable extend to undo")
+        if self.weights is not None:
+            raise ValueError("a weighted cache adds the kept tokens' weights in undo()")
         self.pending = False
         return self.lengths, self.before
+
+    def weigh(self, layer, q, positions, lse, scale, counts, undoable):
+        """Adds the weights that a growing layer's rows got from a reading of
+        counts tokens (q (B, T, H, c) at positions, lse the attention's); an
+        undoable reading's when undo tells how many tokens were kept."""
+        reading = (self.growing.index(layer), layer, q, positions, lse, scale, counts)
+        if undoable:
+            self._read.append(reading)
+        else:
+            self._add(reading, counts, self.lengths)
+
+    def _add(self, reading, counts, start):
+        at, layer, q, positions, lse, scale, _ = reading
+        kernels.add_attention_weights(q, self.tables[layer][..., :q.shape[-1]], positions, lse, scale, self.weights[at],
+                                      counts=counts, start=start)
+
+    def settle(self, kept=None):
+        """Adds the weights of an undoable reading of which kept tokens stay
+        (None: all of them, when another reading follows it)."""
+        for reading in self._read:
+            self._add(reading, reading[-1] if kept is None else kept, self.before)
+        self._read = []
 
     def select(self, index):
         """A new cache of the rows index names (a row may come several times),
@@ -141,4 +201,43 @@ class Cache:
         copy.tables = [None if t is None else t[index] for t in self.tables]
         copy.rings = self.rings
         copy.pending, copy.bound, copy.routes = False, self.bound, None
+        copy.weights = None if self.weights is None else self.weights[:, index]
+        copy.evicted = None if self.evicted is None else self.evicted[index]
+        copy._read = []
         return copy
+
+    def reorder(self, parents):
+        """Beam search's step: row i W + w takes over row i W + parents[i, w], for
+        parents (texts, W) int64 and every row at once, in place (select copies
+        into a new cache): only what the sources hold is moved."""
+        if self.pending:
+            raise ValueError("an undoable extend is pending: undo it before moving rows")
+        if parents.dim() != 2 or parents.shape[0] * parents.shape[1] != self.rows:
+            raise ValueError(f"parents must be (texts, beams) of the cache's {self.rows} rows; got {tuple(parents.shape)}")
+        tables = [self.tables[i] for i in self.growing]
+        if self.weights is not None:
+            tables += [w[..., None] for w in self.weights]
+        if tables:  # (a graph is replayed on longer texts than it was captured on)
+            bound = None if torch.cuda.is_current_stream_capturing() else self.bound
+            kernels.reorder_rows(tables, parents, self.lengths, rows=bound)
+        if self.rings:
+            kernels.reorder_rows([self.tables[i] for i in sorted(self.rings)], parents, self.starts())
+        states = [self.lengths] if self.evicted is None else [self.lengths, self.evicted]
+        kernels.reorder_rows([x.view(-1, 1, 1) for x in states], parents)
+
+    def evict(self, keep, first=4, recent=128):
+        """Brings every row of a weighted cache down to at most keep entries a
+        layer: its first `first`, its last `recent`, and the others that have
+        received the most attention weight, in their order, in place.  Returns
+        the rows kept, (exact layers, B, keep) int64, -1 past a row's count."""
+        if self.weights is None:
+            raise ValueError("only a weighted cache evicts: it keeps the attention weight its rows have received")
+        if self.pending:
+            raise ValueError("an undoable extend is pending: undo it before evicting rows")
+        kept, counts = kernels.choose_kept(self.weights, self.lengths, keep, first, recent)
+        kernels.keep_rows([self.tables[i] for i in self.growing], kept, counts)
+        kernels.keep_rows([w[..., None] for w in self.weights], kept, counts)
+        self.evicted += self.lengths - counts
+        self.lengths.copy_(counts)
+        self.bound = min(self.bound, int(keep))
+        return kept

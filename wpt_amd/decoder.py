@@ -27,6 +27,10 @@ On the GPU:
                     each row's own length (no host sync)
     norms, SwiGLU   wptv_add_rms_norm (residual add + RMSNorm), wptv_swiglu
     the lengths     wptv_cache_lengths after the reading and after an undo
+    a weighted cache wptv_attention_weights after each exact layer's attention
+                    (an undoable reading's after its undo); evict chooses and
+                    moves the kept rows (wptv_choose_kept, wptv_keep_rows), and
+                    reorder the rows of a beam search (wptv_reorder_rows)
     verify attention wptv_verify_attention, reading only the rows the query
                     positions reach in the cache's table
     projections     the matrix products of the dtype on MFMA: at up to 320
@@ -201,16 +205,17 @@ class MQADecoder:
     def parameters(self):
         return iter(self.w.values())
 
-    def new_cache(self, rows, routes=False, capacity=256, widest=129):
+    def new_cache(self, rows, routes=False, capacity=256, widest=129, weighted=False):
         """An empty cache of `rows` rows (the reference's WPT.new_cache); its
         window layers' rings hold readings of up to `widest` tokens (wider
-        ones are read in pieces)."""
+        ones are read in pieces).  weighted: it keeps the attention weight that
+        the exact layers' rows receive, so that evict can bound it."""
         if routes:
             raise NotImplementedError("this decoder has no routed experts to record")
         c = self.config.head_dim
         ring = 1 << max(0, (self.config.window - 1 + widest - 1).bit_length())
         return Cache(rows, self.config.layers, 2 * c, self.dtype, self.device, capacity, self.config.windows, ring,
-                     self.config.sparse)
+                     self.config.sparse, weighted)
 
     def widest(self, cache):
         """The most tokens one reading of the cache takes (its rings' size)."""
@@ -236,7 +241,7 @@ class MQADecoder:
         """Whether layer i's attention block reads its input x in the fm layout."""
         return fm and i < self.config.layers and self.config.kind(i) == EXACT
 
-    def _layer(self, i, h, x, cache, positions, counts, next_norm, handoff, xf=None):
+    def _layer(self, i, h, x, cache, positions, counts, next_norm, handoff, xf=None, places=None, undoable=False):
         """One layer on the residual stream h (B, T, D), x = RMSNorm(h) with the
         layer's attention norm; leaves h updated and x = RMSNorm(h) with
         next_norm (the next layer's attention norm, or the final norm).
@@ -244,18 +249,21 @@ class MQADecoder:
         the handoff for the next layer.  xf: a flat fm operand of the rows
         when the reading runs the fm products: the norms write x there
         instead of into x when the product that reads it is an fm one (an
-        exact layer's q/k/v, every feed-forward block)."""
+        exact layer's q/k/v, every feed-forward block).  places: the tokens'
+        starts and positions in their texts, where a cache has evicted rows
+        (None: those in its tables); undoable: as extend's, for a weighted
+        cache."""
         w = self.w
         B, T, _ = h.shape
         kind = self.config.kind(i)
         fm = xf is not None
         x_in = xf if self._attn_input_fm(i, fm) else x
         if kind == WINDOW:
-            self._window_attention(i, h, x_in, cache, positions, counts, xf)
+            self._window_attention(i, h, x_in, cache, positions, counts, xf, places)
         elif kind == SPARSE:
             self._sparse_attention(i, h, x_in, positions, handoff, xf)
         else:
-            handoff = self._exact_attention(i, h, x_in, cache, positions, counts, xf)
+            handoff = self._exact_attention(i, h, x_in, cache, positions, counts, xf, undoable)
         if fm:
             act = layers.linear_fm_swiglu(xf, B * T, self.fm[f"layers.{i}.gate_up_tiles"], any_rows=True)
             nxt = self._attn_input_fm(i + 1, fm)
@@ -307,16 +315,17 @@ class MQADecoder:
         else:
             layers.add_rms_norm(h, F.linear(o.reshape(B, T, H * c), out), self.w[f"layers.{i}.ffn_norm"], x)
 
-    def _window_attention(self, i, h, x, cache, positions, counts, xf=None):
+    def _window_attention(self, i, h, x, cache, positions, counts, xf=None, places=None):
         """A window layer's attention block: h += out(o * sigmoid(gate(x))),
         x = RMSNorm(h) with the feed-forward norm."""
         w, cfg = self.w, self.config
         B, T, _ = h.shape
         H, c = cfg.heads, cfg.head_dim
         ring = cache.tables[i]
+        start, positions = (cache.lengths, positions) if places is None else places
         proj = self._linear(x, w[f"layers.{i}.qkvg"])  # (B, T, (2H + 2) c): q, k, v, gate
-        q = layers.window_qkv_post(proj, w[f"layers.{i}.q_norm"], w[f"layers.{i}.k_norm"], ring, cache.lengths,
-                                   counts, H, cfg.rope_dims, cfg.rope_base)
+        q = layers.window_qkv_post(proj, w[f"layers.{i}.q_norm"], w[f"layers.{i}.k_norm"], ring, start, counts, H,
+                                   cfg.rope_dims, cfg.rope_base)
         o = kernels.ring_attention(q, ring, positions, c ** -0.5, cfg.window, w[f"layers.{i}.sink"],
                                    gate=proj[..., (H + 2) * c:])
         self._attention_out(i, h, x, o, xf)
@@ -334,7 +343,7 @@ class MQADecoder:
                                      gate=proj[..., H * c:])
         self._attention_out(i, h, x, o, xf)
 
-    def _exact_attention(self, i, h, x, cache, positions, counts, xf=None):
+    def _exact_attention(self, i, h, x, cache, positions, counts, xf=None, undoable=False):
         """An exact layer's attention block: h += out(o), x = RMSNorm(h) with
         the feed-forward norm.  Returns (keys, values, chosen), the sparse
         layers' handoff (chosen None when no sparse layer follows).  xf
@@ -362,10 +371,14 @@ class MQADecoder:
                                 H)
         keys, values = table[..., :c], table[..., c:]
         chosen = None
-        if cfg.chooses(i):  # the top_k rows outside the window by the largest max_h log-softmax weight
+        weighted = cache.weights is not None
+        if weighted or cfg.chooses(i):
             o, lse = kernels.verify_attention(q, keys, values, positions, c ** -0.5, lse=True, from_positions=True,
                                               out_fm=fm, captured=True)
-            chosen = kernels.choose_rows(q, keys, positions, lse, c ** -0.5, cfg.top_k, cfg.window)
+            if cfg.chooses(i):  # the top_k rows outside the window by the largest max_h log-softmax weight
+                chosen = kernels.choose_rows(q, keys, positions, lse, c ** -0.5, cfg.top_k, cfg.window)
+            if weighted:
+                cache.weigh(i, q, positions, lse, c ** -0.5, counts, undoable)
         else:
             o = kernels.verify_attention(q, keys, values, positions, c ** -0.5, from_positions=True, out_fm=fm,
                                          captured=True)  # a decoder's steady steps are graphs
@@ -411,6 +424,7 @@ class MQADecoder:
                                    features=features, logits=logits)
                 pieces.append(part)
             return tuple(torch.cat([p[i] for p in pieces], 1) for i in range(len(pieces[0])))
+        cache.settle()
         cache.reserve(cache.bound + T)
         D = self.config.d_model
         h = torch.empty(B, T, D, dtype=self.dtype, device=self.device)
@@ -422,6 +436,9 @@ class MQADecoder:
         # the embedding, the first norm and each token's position in one pass
         layers.embed_rms_norm(ids.contiguous(), self.w["embedding"], self.w["layers.0.attn_norm"], h,
                               xf if first_fm else x, cache.lengths, positions, fm=first_fm)
+        places = None
+        if cache.evicted is not None and cache.rings:  # the rings hold tokens by their place in the text
+            places = cache.starts(), positions + cache.evicted[:, None]
         found = {}
         handoff = None
         for i in range(self.config.layers):
@@ -429,7 +446,7 @@ class MQADecoder:
                 found[i] = h.float()
             last = i + 1 == self.config.layers
             next_norm = self.w["final_norm"] if last else self.w[f"layers.{i + 1}.attn_norm"]
-            handoff = self._layer(i, h, x, cache, positions, counts_, next_norm, handoff, xf)
+            handoff = self._layer(i, h, x, cache, positions, counts_, next_norm, handoff, xf, places, undoable)
         if self.config.layers in features:
             found[self.config.layers] = h.float()
         head = self.w["head"]
@@ -455,6 +472,27 @@ class MQADecoder:
         if not (torch.is_tensor(kept) and kept.dtype in (torch.int64, torch.int32)):
             kept = torch.as_tensor(kept, dtype=torch.long)
         cache.undo(kept.to(self.device))
+
+    @torch.no_grad()
+    def reorder(self, cache, parents):
+        """Beam search's reordering: row i W + w of the cache takes over row
+        i W + parents[i, w] (parents (texts, W) int64, sampling.beam_step's), in
+        place."""
+        cache.reorder(parents.to(self.device))
+
+    @torch.no_grad()
+    def evict(self, cache, keep, first=4, recent=None):
+        """Brings a weighted cache's rows down to at most keep entries an exact
+        layer (Cache.evict): the first, the last `recent` (None: the window, or
+        as many of it as keep holds) and those that received the most attention.
+        The sparse layers read an exact layer's last `window` rows: recent must
+        hold them."""
+        if recent is None:
+            recent = min(self.config.window, int(keep) - int(first))
+        if self.config.sparse and recent < self.config.window:
+            raise ValueError(f"the sparse layers read the last {self.config.window} tokens: recent = {recent} does not "
+                             "hold them")
+        return cache.evict(keep, first, recent)
 
     @torch.no_grad()
     def __call__(self, ids):

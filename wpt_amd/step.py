@@ -81,7 +81,8 @@ class VerifyStep:
         # the pick's kernel also takes back the rejected drafts (the model's
         # undo, which for this cache is its lengths alone), makes the drawn
         # token each row's next pending token and grows the running counts
-        if isinstance(self.cache, Cache) and type(self.model).undo is MQADecoder.undo:
+        # (a weighted cache's undo also adds the kept tokens' attention weights)
+        if isinstance(self.cache, Cache) and self.cache.weights is None and type(self.model).undo is MQADecoder.undo:
             lengths, before = self.cache.undo_on_device()
             commit = (lengths, before, self.feeds, self.failed, self.written)
         else:
