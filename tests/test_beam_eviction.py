@@ -42,28 +42,35 @@ def test_no_texts_is_no_work():
     assert beam(n=0) == 0
 
 
-def reorder(base=A, sb=640, sn=64, capacity=10, row=64, count=1, n=1, W=2, parents=A, rows=10):
+def reorder(base=A, sb=640, sn=64, capacity=10, row=64, count=1, n=1, W=2, parents=2 * A, lengths=None, rows=10):
     return _lib.lib().wptv_reorder_rows((ctypes.c_void_p * 1)(base), longs(sb), longs(sn), longs(capacity), longs(row), count,
-                                        parents, None, rows, n, W, None)
+                                        parents, lengths, rows, n, W, None)
 
 
 @pytest.mark.parametrize("status, text, arguments", [
     (-1, "bad shape", {"W": 0}), (-1, "bad shape", {"n": -1}), (-1, "bad shape", {"rows": -1}), (-3, "at most 64", {"W": 65}),
     (-3, "65535", {"n": 65536}), (-1, "overlap", {"sn": 63}), (-1, "overlap", {"sb": 0}), (-1, "overlap", {"sb": 600}),
     (-1, "capacity", {"capacity": -1}), (-1, "capacity", {"row": 0}), (-1, "NULL", {"base": None}),
-    (-1, "parents", {"parents": None})])
+    (-1, "parents", {"parents": None}), (-1, "list of rows", {"parents": A}), (-1, "list of rows", {"lengths": A})])
 def test_reorder_rows_refuses(status, text, arguments):
     assert reorder(**arguments) == status
     assert text in message()
 
 
-def keep(base=A, sb=640, sn=64, capacity=10, row=64, count=1, lists=1, kept=A, keep=4, B=2):
-    return _lib.lib().wptv_keep_rows((ctypes.c_void_p * 3)(base, base, base), longs(sb, sb, sb), longs(sn, sn, sn),
+def test_a_table_given_twice_is_refused():
+    two = [(ctypes.c_void_p * 2)(A, A), longs(640, 640), longs(64, 64), longs(10, 10), longs(64, 64), 2]
+    assert _lib.lib().wptv_reorder_rows(*two, 2 * A, None, 10, 1, 2, None) == -1 and "the same" in message()
+    assert _lib.lib().wptv_keep_rows(*two, 2 * A, 1, 4, 3 * A, 1, None) == -1 and "the same" in message()
+
+
+def keep(base=A, sb=640, sn=64, capacity=10, row=64, count=1, lists=1, kept=2 * A, keep=4, B=2):
+    return _lib.lib().wptv_keep_rows((ctypes.c_void_p * 3)(base, 4 * A, 5 * A), longs(sb, sb, sb), longs(sn, sn, sn),
                                      longs(capacity, capacity, capacity), longs(row, row, row), count, kept, lists, keep,
-                                     A, B, None)
+                                     3 * A, B, None)
 
 
 @pytest.mark.parametrize("status, text, arguments", [
+    (-1, "list of rows", {"base": 2 * A}), (-1, "list of rows", {"base": 3 * A}),
     (-1, "3 tables for 2", {"count": 3, "lists": 2}), (-1, "for 0 lists", {"lists": 0}), (-1, "B=-1", {"B": -1}),
     (-3, "65535", {"B": 65536}), (-1, "overlap", {"sb": 639}), (-1, "overlap", {"sn": 32}), (-1, "kept", {"kept": None})])
 def test_keep_rows_refuses(status, text, arguments):
@@ -78,7 +85,15 @@ def test_choose_kept_refuses(text, arguments):
     assert text in message()
 
 
+def test_choose_kept_takes_at_least_one_layer_and_texts_that_fit_its_counts():
+    assert _lib.lib().wptv_choose_kept(A, 10, 10, A, 0, 1, 10, 4, 1, 1, A, A, None) == -1 and "bad shape" in message()
+    assert _lib.lib().wptv_choose_kept(A, 10, 10, A, 1, 1, (1 << 30) + 1, 4, 1, 1, A, A, None) == -3
+    assert "too large" in message()
+    assert _lib.lib().wptv_choose_kept(A, 10, 10, A, 1, 0, 10, 4, 1, 1, A, A, None) == 0
+
+
 @pytest.mark.parametrize("status, text, arguments", [
+    (-3, "too large", {"N": (1 << 30) + 1}), (-3, "too large", {"T": 1 << 29, "H": 2}),
     (-1, "bad shape", {"H": 0}), (-1, "bad shape", {"N": 0}), (-3, "dtype", {"dtype": 3}), (-3, "width", {"c": 257}),
     (-1, "overlap", {"stride": 100}), (-1, "overlap", {"row": 63}), (-1, "NULL", {"q": None}), (-1, "splits", {"splits": -1})])
 def test_attention_weights_refuse(status, text, arguments):

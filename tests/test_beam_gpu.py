@@ -128,6 +128,19 @@ def test_strided_scores_and_totals(device):
     assert torch.equal(got[1], expected[1]) and torch.equal(got[2], expected[2])
 
 
+def test_scores_past_4_gb(device):
+    n, W, V = 1100, 16, 131072  # 4.6 GB of bf16: the last texts lie past 2^31 elements
+    scores = torch.empty(n, W, V, dtype=torch.bfloat16, device=device)
+    for first in range(0, n, 100):
+        scores[first:first + 100].normal_(std=3)
+    totals = -20 * torch.rand(n, W, device=device)
+    got = [x[[0, -1]].cpu() for x in sampling.beam_step(scores, totals)]
+    expected = oracle.beam_step(scores[[0, -1]].cpu(), totals[[0, -1]].cpu())
+    for a, b in zip(got[1:], expected[1:]):
+        assert torch.equal(a, b)
+    totals_close(got[0], expected[0], V)
+
+
 def test_no_texts(device):
     got = sampling.beam_step(torch.empty(0, 3, 10, device=device), torch.empty(0, 3, device=device))
     assert [tuple(x.shape) for x in got] == [(0, 3)] * 4

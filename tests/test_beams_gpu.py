@@ -236,6 +236,11 @@ def test_what_the_beam_writer_refuses(device):
             BeamWriter(model, *arguments)
     with pytest.raises(ValueError, match="keep"):
         BeamWriter(model, [[1]], 2, keep=3, first=4)
+    with pytest.raises(ValueError, match="sparse layers"):
+        BeamWriter(decoder(device, MIXED), [[1]], 2, keep=17, first=2)
+    for prompts, stops in (([[1, 512]], ()), ([[-1]], ()), ([[1]], (512,))):
+        with pytest.raises(IndexError):
+            BeamWriter(model, prompts, 2, stops=stops)
 
 
 def test_a_captured_beam_step(device):

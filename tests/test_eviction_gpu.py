@@ -240,6 +240,19 @@ def test_tables_that_are_views_move_in_place(device):
                        oracle.keep_rows([rows_first.transpose(0, 1)], kept.cpu(), counts.cpu())[0])
 
 
+def test_kept_rows_past_4_gb(device):
+    B, N, width, keep = 3, 500, 512, 200
+    kept, counts = choose(device, torch.rand(1, B, N, generator=torch.Generator().manual_seed(3)), torch.tensor([N] * B),
+                          keep, 1, 5)
+    stride = 2_200_000_000
+    whole = torch.empty(2 * stride + N * width, dtype=torch.uint8, device=device)
+    table = whole.as_strided((B, N, width), (stride, width, 1))
+    small = torch.randint(0, 100, (B, N, width), generator=torch.Generator().manual_seed(4)).to(torch.uint8)
+    table.copy_(small)
+    kernels.keep_rows(table, kept, counts)
+    assert torch.equal(table.cpu(), oracle.keep_rows([small], kept.cpu(), counts.cpu())[0])
+
+
 def test_lists_that_name_no_row_move_nothing_out_of_range(device):
     table = torch.arange(20.0).view(1, 10, 2)
     kept = torch.tensor([[[0, 3, -1, 99, 7, 8]]])

@@ -157,12 +157,13 @@ def stream(device):
     return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on(device):
     """A context in which device is the current one (nothing to enter where it is)."""
     index = device.index
-    if index is None or index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(index)
+    return _HERE if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 _plans = {}  # (entry point, device, part count asked for, its integers) -> (parts, bytes)

@@ -34,10 +34,11 @@ class BeamWriter:
             raise ValueError("beam search writes for at least one prompt, each of at least one token")
         if not 1 <= beams <= 64:
             raise ValueError(f"a text is written by 1 to 64 beams; got {beams}")
-        if keep is not None and (first < 0 or keep < first + max(1, recent or 0)):
-            raise ValueError(f"keep = {keep} entries must hold the first {first} and the last {recent or 1}")
+        vocab = model.config.vocab
+        if any(not 0 <= t < vocab for p in prompts for t in p) or any(not 0 <= t < vocab for t in stops):
+            raise IndexError(f"token ids must lie in [0, {vocab})")
         self.model, self.beams, self.stops = model, int(beams), tuple(int(s) for s in stops)
-        self.keep, self.first, self.recent = keep, first, recent
+        self.bounds = None if keep is None else model.evict_rows(keep, first, recent)
         self.device = next(model.parameters()).device
         n = len(prompts)
         self.cache = model.new_cache(n, weighted=keep is not None)
@@ -60,8 +61,8 @@ class BeamWriter:
         self._steps = []  # (parents, tokens) of each step
 
     def _evict(self):
-        if self.keep is not None and self.cache.bound > self.keep + self.keep // 8:
-            self.model.evict(self.cache, self.keep, self.first, self.recent)
+        if self.bounds is not None and self.cache.bound > self.bounds[0] + self.bounds[0] // 8:
+            self.model.evict(self.cache, *self.bounds)
 
     @torch.no_grad()
     def step(self):

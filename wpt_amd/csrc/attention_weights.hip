@@ -339,7 +339,7 @@ extern "C" int wptv_attention_weights_workspace(int B, int T, int H, int c, int 
   if (dtype != WPTV_F32 && dtype != WPTV_BF16) return fail(WPTV_E_UNSUPPORTED, "attention_weights: dtype %d", dtype);
   if (c > kMaxWidth)
     return fail(WPTV_E_UNSUPPORTED, "attention_weights: head width at most %d (got %d)", kMaxWidth, c);
-  if ((int64_t)T * H > (1 << 29) || (int64_t)B * ((N + kKeys - 1) / kKeys) > INT32_MAX)
+  if (N > (1 << 30) || (int64_t)T * H > (1 << 29) || (int64_t)B * ((N + kKeys - 1) / kKeys) > INT32_MAX)
     return fail(WPTV_E_UNSUPPORTED, "attention_weights: B=%d T=%d H=%d N=%d is too large", B, T, H, N);
   if (*splits < 0) return fail(WPTV_E_INVALID, "attention_weights: splits = %d", *splits);
   const int64_t rows = (int64_t)T * H;

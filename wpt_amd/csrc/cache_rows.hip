@@ -17,6 +17,7 @@
 #include "wptv_common.h"
 
 #include <climits>
+#include <initializer_list>
 
 namespace wptv {
 namespace {
@@ -170,7 +171,7 @@ int unit_of(const void* base, int64_t sb, int64_t sn, int64_t row_bytes) {
 
 // Host checks of one table of `rows_b` batch rows.
 int check_table(const char* what, int i, void* const* bases, int64_t sb, int64_t sn, int64_t capacity, int64_t row_bytes,
-                int64_t rows_b) {
+                int64_t rows_b, const void* list, const void* lengths) {
   const void* base = bases[i];
   if (capacity < 0 || capacity > INT32_MAX || row_bytes <= 0 || row_bytes > INT32_MAX)
     return fail(WPTV_E_INVALID, "%s: table %d has capacity %lld and rows of %lld bytes", what, i, (long long)capacity,
@@ -183,6 +184,8 @@ int check_table(const char* what, int i, void* const* bases, int64_t sb, int64_t
                       sn >= (rows_b - 1) * sb + row_bytes;
   for (int other = 0; other < i; ++other)
     if (base && bases[other] == base) return fail(WPTV_E_INVALID, "%s: tables %d and %d are the same", what, other, i);
+  for (const void* read : {list, lengths})  // what the launch reads while it moves the rows
+    if (base && read == base) return fail(WPTV_E_INVALID, "%s: table %d is also read as a list of rows", what, i);
   if (!apart_n || !apart_b || !nested)
     return fail(WPTV_E_INVALID, "%s: the rows of table %d overlap (strides %lld and %lld bytes, rows of %lld)", what, i,
                 (long long)sb, (long long)sn, (long long)row_bytes);
@@ -266,7 +269,7 @@ extern "C" int wptv_reorder_rows(void* const* tables, const int64_t* strides_b, 
     return fail(WPTV_E_INVALID, "reorder_rows: the tables' addresses and shapes must be given");
   for (int i = 0; i < count; ++i) {
     const int status = check_table("reorder_rows", i, tables, strides_b[i], strides_n[i], capacities[i],
-                                   row_bytes[i], (int64_t)n * W);
+                                   row_bytes[i], (int64_t)n * W, parents, lengths);
     if (status != WPTV_OK) return status;
   }
   if (count == 0 || n == 0 || W == 1) return WPTV_OK;
@@ -301,7 +304,7 @@ extern "C" int wptv_keep_rows(void* const* tables, const int64_t* strides_b, con
     return fail(WPTV_E_INVALID, "keep_rows: the tables' addresses and shapes must be given");
   for (int i = 0; i < count; ++i) {
     const int status =
-        check_table("keep_rows", i, tables, strides_b[i], strides_n[i], capacities[i], row_bytes[i], B);
+        check_table("keep_rows", i, tables, strides_b[i], strides_n[i], capacities[i], row_bytes[i], B, kept, counts);
     if (status != WPTV_OK) return status;
   }
   if (count == 0 || B == 0 || keep == 0) return WPTV_OK;

@@ -179,12 +179,12 @@ using namespace wptv;
 extern "C" int wptv_choose_kept(const float* weights, int64_t weights_stride_l, int64_t weights_stride_b,
                                 const int64_t* lengths, int L, int B, int N, int keep, int first, int recent,
                                 int64_t* kept, int64_t* counts, hipStream_t stream) {
-  if (L < 0 || B < 0 || N < 0) return fail(WPTV_E_INVALID, "choose_kept: bad shape L=%d B=%d N=%d", L, B, N);
+  if (L <= 0 || B < 0 || N < 0) return fail(WPTV_E_INVALID, "choose_kept: bad shape L=%d B=%d N=%d", L, B, N);
   if (first < 0 || recent < 0 || keep <= 0 || (int64_t)first + recent > keep)
     return fail(WPTV_E_INVALID, "choose_kept: keep=%d rows must hold the first %d and the last %d", keep, first, recent);
   if ((int64_t)L * B > INT32_MAX || N > (1 << 30))
     return fail(WPTV_E_UNSUPPORTED, "choose_kept: L=%d B=%d N=%d is too large", L, B, N);
-  if (L == 0 || B == 0) return WPTV_OK;
+  if (B == 0) return WPTV_OK;
   if ((N && !weights) || !lengths || !kept || !counts)
     return fail(WPTV_E_INVALID, "choose_kept: a required pointer is NULL");
 #define WPTV_KEPT(THREADS, V)                                                                                    \

@@ -487,12 +487,18 @@ class MQADecoder:
         as many of it as keep holds) and those that received the most attention.
         The sparse layers read an exact layer's last `window` rows: recent must
         hold them."""
-        if recent is None:
-            recent = min(self.config.window, int(keep) - int(first))
+        return cache.evict(*self.evict_rows(keep, first, recent))
+
+    def evict_rows(self, keep, first=4, recent=None):
+        """evict's (keep, first, recent), checked."""
+        keep, first = int(keep), int(first)
+        recent = min(self.config.window, keep - first) if recent is None else int(recent)
+        if keep <= 0 or first < 0 or recent < 0 or first + recent > keep:
+            raise ValueError(f"keep = {keep} entries must hold the first {first} and the last {recent}")
         if self.config.sparse and recent < self.config.window:
             raise ValueError(f"the sparse layers read the last {self.config.window} tokens: recent = {recent} does not "
                              "hold them")
-        return cache.evict(keep, first, recent)
+        return keep, first, recent
 
     @torch.no_grad()
     def __call__(self, ids):

@@ -369,9 +369,9 @@ def kv_append(table, new, start, counts):
 
 def _index(x, shape, name, device):
     """An int64 tensor of the given shape, contiguous on the device."""
-    if tuple(x.shape) != shape:
+    if x.shape != shape:
         raise ValueError(f"{name} must be {shape}; got {tuple(x.shape)}")
-    return _long(x, device)
+    return x if x.dtype is torch.long and x.device == device and x.is_contiguous() else _long(x, device)
 
 
 def _tables(tables, rows, what):
@@ -442,13 +442,21 @@ def add_attention_weights(q, k, positions, lse, scale, weights, *, counts=None, 
     the rows from there on, the reading's own, begin at zero.  Rows past the
     last counted position are left alone.  splits: parts of the queries (0:
     the library chooses).  Returns weights."""
-    if k.dim() != 3:
-        raise ValueError(f"k must be (B, N, c); got {tuple(k.shape)}")
-    B, T, H, c, N = _check_inputs(q, k, k, positions)
-    device = q.device
-    if tuple(lse.shape) != (B, T, H) or lse.dtype != torch.float32 or lse.device != device:
+    if q.dim() != 4 or k.dim() != 3:
+        raise ValueError(f"q must be (B, T, H, c) and k (B, N, c); got {tuple(q.shape)}, {tuple(k.shape)}")
+    B, T, H, c = q.shape
+    N = k.shape[1]
+    device, dtype = q.device, _lib.dtype_code(q.dtype)
+    if k.shape != (B, N, c) or k.dtype != q.dtype or N == 0:
+        raise ValueError(f"k must be (B={B}, N > 0, c={c}) in q's {q.dtype}; got {k.dtype} {tuple(k.shape)}")
+    if not q.is_cuda or k.device != device:
+        raise KernelUnavailable(f"the HIP attention weights are added up on one GPU; q is on {device}, k on {k.device}")
+    k_stride_b, k_stride_n, k_stride_c = k.stride()
+    if k_stride_c != 1 and c > 1:
+        raise ValueError("each row of k must be contiguous")
+    if lse.shape != (B, T, H) or lse.dtype != torch.float32 or lse.device != device:
         raise ValueError(f"lse must be FP32 (B={B}, T={T}, H={H}) on {device}; got {lse.dtype} {tuple(lse.shape)}")
-    if tuple(weights.shape) != (B, N) or weights.dtype != torch.float32 or weights.device != device or \
+    if weights.shape != (B, N) or weights.dtype != torch.float32 or weights.device != device or \
             (N > 1 and weights.stride(1) != 1):
         raise ValueError(f"weights must be FP32 (B={B}, N={N}) on {device} with contiguous rows; got {weights.dtype} "
                          f"{tuple(weights.shape)}")
@@ -458,12 +466,11 @@ def add_attention_weights(q, k, positions, lse, scale, weights, *, counts=None, 
     counts_ = None if counts is None else _index(counts, (B,), "counts", device)
     start_ = None if start is None else _index(start, (B,), "start", device)
     q_, lse_ = q.contiguous(), lse.contiguous()
-    dtype = _lib.dtype_code(q.dtype)
     with _lib.on(device):
         parts, size = _lib.plan("wptv_attention_weights_workspace", "add_attention_weights", B, T, H, c, N, dtype,
                                 splits=int(splits))
         workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        check(_lib.lib().wptv_attention_weights(ptr(q_), ptr(k), k.stride(0), k.stride(1), dtype, ptr(positions_),
+        check(_lib.lib().wptv_attention_weights(ptr(q_), ptr(k), k_stride_b, k_stride_n, dtype, ptr(positions_),
                                                 ptr(lse_), ptr(counts_), ptr(start_), B, T, H, c, N, float(scale),
                                                 parts, ptr(weights), weights.stride(0), ptr(workspace), size,
                                                 _lib.stream(device)), "add_attention_weights")
