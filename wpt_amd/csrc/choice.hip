@@ -400,7 +400,7 @@ __global__ __launch_bounds__(THREADS) void choice_select_regs(const float* __res
         if (4 * v + e < valid) f(4 * v + e, key[4 * v + e]);
     }
   };
-  const uint32_t tau = kth_largest<THREADS>(each, K, select);
+  const uint32_t tau = kth_largest<THREADS, false>(each, K, select);
   // rows above tau and equal to it, each in row order: one scan of both counts
   int mine = 0;
   each([&](int, uint32_t x) { mine += x > tau ? 1 : x == tau ? 65536 : 0; });

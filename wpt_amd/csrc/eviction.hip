@@ -66,7 +66,7 @@ __global__ __launch_bounds__(THREADS) void choose_kept_regs(const float* __restr
         if (4 * v + e < valid) f(4 * v + e, key[4 * v + e]);
     }
   };
-  const uint32_t tau = kth_largest<THREADS>(each, take, select);
+  const uint32_t tau = kth_largest<THREADS, true>(each, take, select);
   // rows above tau, and the first of those equal to it: one scan of both counts
   int mine = 0;
   each([&](int, uint32_t x) { mine += x > tau ? 1 : x == tau ? 65536 : 0; });
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(kLongThreads) void choose_kept_long(const float* __
     }
   };
   auto each = [&](auto&& f) { rows(tid, candidates, kLongThreads, f); };
-  const uint32_t tau = kth_largest<kLongThreads>(each, take, select);
+  const uint32_t tau = kth_largest<kLongThreads, true>(each, take, select);
   // each wavefront counts, then lists, a stretch of consecutive rows
   const int stretch = ((candidates + kLongWaves - 1) / kLongWaves + 63) / 64 * 64;
   const int begin = min(w * stretch, candidates), end = min(begin + stretch, candidates);

@@ -4,8 +4,6 @@
 
 #include "wptv_common.h"
 
-#include <type_traits>
-
 namespace wptv {
 namespace {
 
@@ -28,18 +26,22 @@ struct SelectShared {
   __attribute__((aligned(16))) int hist[kSelectBins];
   __attribute__((aligned(16))) uint32_t cand[kSelectCand];
   int range[2][THREADS / 64], sel[3], ncand;
+  uint32_t found;
 };
 
 // The `remaining`-th largest key, the same in every thread, of those that
 // each(f) calls f(item, key) with in each thread (at least `remaining` in all).
 // Histograms of 1024 equal bins over the range of keys still open (first smallest
 // to largest): the bin that holds it, then, when that holds at most kSelectCand
-// keys, a search of its bits by ballots, else a histogram of the bin's own range.
-// A range shrinks 2^9 times a pass at the least, so four passes end it whatever
-// the keys are (equal ones end in a bin of width one); scores take one pass and
-// the search.  (Ranking the bin's keys by counting, a chain of up to 256 LDS reads,
-// took 384 selections of 3964 weights from 11 to 16 us.)
-template <int THREADS, typename Each>
+// keys, the one among them, else a histogram of the bin's own range.  A range
+// shrinks 2^9 times a pass at the least, so four passes end it whatever the keys
+// are (equal ones end in a bin of width one); scores take one pass.
+//
+// Among the bin's keys: BY_BITS, a search of its bits by ballots, else their ranks
+// by counting, a loop as long as the bin is full.  Weights fill it (384 selections
+// of 3964 weights 16 us by counting, 13.6 by bits), scores do not (160 selections
+// among 3972 half a microsecond longer by bits).
+template <int THREADS, bool BY_BITS, typename Each>
 __device__ __forceinline__ uint32_t kth_largest(Each&& each, int remaining, SelectShared<THREADS>& shared) {
   constexpr int kWaves = THREADS / 64, kBins = kSelectBins, kCand = kSelectCand;
   constexpr int kPerLane = kBins / 64;
@@ -104,9 +106,9 @@ __device__ __forceinline__ uint32_t kth_largest(Each&& each, int remaining, Sele
       }
     }
     __syncthreads();
-    const int count = __builtin_amdgcn_readfirstlane(sel[2]);
-    remaining -= __builtin_amdgcn_readfirstlane(sel[1]);
-    lo += (uint32_t)__builtin_amdgcn_readfirstlane(sel[0]) << shift;
+    const int count = sel[2];
+    remaining -= sel[1];
+    lo += (uint32_t)sel[0] << shift;
     if (shift == 0) {  // the bin's keys are equal
       tau = lo;
       break;
@@ -118,25 +120,35 @@ __device__ __forceinline__ uint32_t kth_largest(Each&& each, int remaining, Sele
         if (x >= lo && x <= hi) cand[atomicAdd(&ncand, 1)] = x;
       });
       __syncthreads();
-      // every wavefront for itself: the largest offset into the bin that `remaining`
-      // of its keys reach, a bit at a time
-      uint32_t offset[kCand / 64], reached = 0;
+      if constexpr (BY_BITS) {
+        // every wavefront for itself: the largest offset into the bin that
+        // `remaining` of its keys reach, a bit at a time
+        uint32_t offset[kCand / 64], reached = 0;
 #pragma unroll
-      for (int i = 0; i < kCand / 64; ++i) offset[i] = lane + 64 * i < count ? cand[lane + 64 * i] - lo : 0u;
-      auto search = [&](auto groups) {
+        for (int i = 0; i < kCand / 64; ++i) offset[i] = lane + 64 * i < count ? cand[lane + 64 * i] - lo : 0u;
         for (int bit = shift - 1; bit >= 0; --bit) {
           const uint32_t trial = reached | (1u << bit);
           int many = 0;
 #pragma unroll
-          for (int i = 0; i < groups; ++i) many += __builtin_popcountll(__builtin_amdgcn_ballot_w64(offset[i] >= trial));
+          for (int i = 0; i < kCand / 64; ++i)
+            many += __builtin_popcountll(__builtin_amdgcn_ballot_w64(offset[i] >= trial));
           if (many >= remaining) reached = trial;
         }
-      };
-      if (count <= 64)
-        search(std::integral_constant<int, 1>());
-      else
-        search(std::integral_constant<int, kCand / 64>());
-      tau = lo + reached;
+        tau = lo + reached;
+      } else {
+        if (tid < count) {
+          const uint32_t mine = cand[tid];
+          int gt = 0, ge = 0;
+          for (int i = 0; i < count; ++i) {
+            const uint32_t x = cand[i];
+            gt += x > mine ? 1 : 0;
+            ge += x >= mine ? 1 : 0;
+          }
+          if (gt < remaining && ge >= remaining) shared.found = mine;  // the same key from each that writes
+        }
+        __syncthreads();
+        tau = shared.found;
+      }
       break;
     }
 #pragma unroll
