@@ -17,6 +17,10 @@ Modules, each citing the reference lines it follows:
                (lazily drawn from a torch generator, or read from a tape),
                greedy chain and tree verification, the prefix scheduler:
                wpt_inference/__init__.py
+    beam       beam search's selection by sorting every candidate, and the
+               reordering of rows (no counterpart in the reference)
+    eviction   the attention weight that cached rows receive, the rows a
+               bounded cache keeps and their move (no counterpart)
     decoder    the build's generic MQA decoder (random-init weights, exact
                and window layers) behind the reference's model protocol
                new_cache / extend / undo
@@ -40,6 +44,7 @@ tests/test_scheduling.py):
                the model's distribution (total variation < 0.05 over 4000
                rows); the scheduler's known answers (test_sampling.py:230-238)
                and a brute force over widths
+    beam, eviction  cases done by hand (tests/test_beam_eviction.py)
 The exact token stream the reference's Writer draws from a seed through its
 lazy generator order (its own tests assert only "same seed, same tokens") is
 pinned by golden streams of the reference's Writer itself

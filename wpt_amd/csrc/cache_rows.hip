@@ -14,6 +14,10 @@
 //                 below it: step by step, the sources of a step are read
 //                 before the barrier and its rows written after it, and no
 //                 later step reads what this one writes
+// Bound by HBM: a copy of 1 GiB runs at 5.15 TB/s, read and written.  24 tables of 8
+// texts of 4 beams, three of them moved, 1125 rows of 512 bytes on average: 117 us, 4.7
+// TB/s (8 and 16 beams 5.4 and 5.2); 24 tables of 16 texts, 2048 rows kept: 115 us, 4.4
+// TB/s, the rows left out breaking its reads up.
 #include "wptv_common.h"
 
 #include <climits>

@@ -11,6 +11,8 @@
 //                     one scan of the threads' counts
 //   choose_kept_long  longer texts: the same over the weights in memory, each
 //                     wavefront listing a stretch of the rows by ballots
+// A serial chain of barriers bounds them, not the bytes: 24 layers of 16 texts of up
+// to 4096 rows 13.8 us, one text of each 9.6, of 40000 rows 42.
 #include "select_common.h"
 #include "wptv_common.h"
 
