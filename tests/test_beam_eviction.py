@@ -31,7 +31,7 @@ def beam(n=1, W=2, V=10, K=2, dtype=_lib.WPTV_F32, stops=(), ended=None, n_stops
     (-1, "bad shape", {"n": -1}), (-1, "bad shape", {"W": 0}), (-1, "bad shape", {"V": 0}), (-1, "bad shape", {"K": 0}),
     (-1, "bad shape", {"K": 21}), (-3, "at most 64", {"W": 65}), (-3, "at most 64", {"W": 64, "K": 65}),
     (-3, "neither", {"dtype": 7}), (-1, "outside", {"stops": (10,)}), (-1, "outside", {"stops": (1, -1)}),
-    (-1, "0 to 16", {"n_stops": 17}), (-1, "stop token", {"ended": A}), (-1, "workspace", {"size": 8}),
+    (-1, "0 to 16", {"n_stops": 17}), (-1, "stop token", {"ended": A}), (-1, "workspace", {"V": 100000, "size": 8}),
     (-1, "NULL", {"scores": None}), (-3, "too large", {"n": 1 << 30, "W": 4})])
 def test_beam_step_refuses(status, text, arguments):
     assert beam(**arguments) == status

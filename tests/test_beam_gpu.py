@@ -51,7 +51,8 @@ def inputs(n, W, V, dtype, seed):
 @pytest.mark.parametrize("n, W, V, K", [
     (1, 1, 1, 1), (1, 1, 5, 5), (2, 3, 7, 8), (1, 2, 40, 64), (1, 4, 8192, 4), (3, 8, 32768, 8), (2, 16, 50257, 16),
     (1, 64, 300, 64), (4, 5, 1001, 5), (1, 1, 131073, 32), (1, 64, 4099, 64), (40, 3, 4095, 3), (2, 1, 32768, 64),
-    (300, 2, 1024, 2), (1, 7, 4097, 1)])
+    (300, 2, 1024, 2), (1, 7, 4097, 1), (256, 2, 2049, 2), (257, 2, 2049, 2), (3, 8, 4096, 8),
+    (3, 8, 4097, 8), (5, 9, 100, 9), (1, 1, 32768, 64), (2, 8, 17, 64), (2, 16, 2000, 16)])
 def test_the_next_beams_are_those_of_the_sorted_candidates(device, n, W, V, K, dtype):
     print(f"beam_step n={n} W={W} V={V} K={K} {dtype}", flush=True)
     scores, totals, ended = inputs(n, W, V, dtype, seed=n + W + V)

@@ -11,6 +11,7 @@
 //               scores, ties to the lowest token
 //   beam_merge  a workgroup a text: the parts' sums joined to L in 64 bits, and
 //               the K best of the parts' lists
+//   beam_text   both, for a text whose parts fit one workgroup
 // The K largest of a part: the K-th largest of the lanes' maxima bounds them
 // from below, and few scores reach it (in scores without order about K of 4096);
 // those are gathered in LDS, 64 at a time sorted across the lanes and merged
@@ -19,8 +20,8 @@
 //
 // 64 texts of 5 beams over 50257 FP32 scores: 16.5 us and 5.9 (64 MB at 3.9 TB/s; the
 // loads of all parts are in flight at once and their arithmetic follows); 32 texts of
-// 8 beams over 32768 bf16 scores: 7.3 and 6.6; one text of 4 beams over 8192: 3.6 and
-// 4.8, two dependent launches' latency.
+// 8 beams over 32768 bf16 scores: 7.3 and 6.6; one text of 4 beams over 8192: 9.0 in one
+// launch, the latency of its steps.
 #include "wptv_common.h"
 
 #include <climits>
@@ -207,26 +208,21 @@ struct PartSum {
   float top, sum;  // the largest score, and the sum of exp(x - top) (of exp x where nothing is above -inf)
 };
 
+// The sum and the list (K keys, 0 where it holds fewer) of part `part` of the V
+// scores at p, by one wavefront.  held: kGathered keys of LDS.
 template <typename E, int ITEMS>
-__global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restrict__ scores, int64_t sn, int64_t sw,
-                                                              uint32_t W, int V, int K, uint32_t parts, uint32_t waves,
-                                                              PartSum* __restrict__ sums,
-                                                              uint64_t* __restrict__ lists) {
+__device__ __forceinline__ void part_list(const E* p, int V, int part, int K, uint64_t* held, PartSum* result,
+                                          uint64_t* list) {
   typedef typename Scores16<E>::type Vec;
   constexpr int kVec = 16 / sizeof(E), kLoads = ITEMS / kVec;
-  __shared__ uint64_t gathered[kPartWaves][kGathered];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t wave = blockIdx.x * kPartWaves + w;
-  if (wave >= waves) return;  // no barrier follows
-  const uint32_t row = wave / parts, part = wave % parts;
-  const int v0 = (int)part * 64 * ITEMS + lane * kVec;  // this lane's first token; 64 kVec a load
-  const E* p = scores + (int64_t)(row / W) * sn + (int64_t)(row % W) * sw;
+  const int lane = threadIdx.x & 63;
+  const int v0 = part * 64 * ITEMS + lane * kVec;  // this lane's first token; 64 kVec a load
   // a load that would pass the row's end is moved back to it, and the tokens that
   // another lane holds left out
   const int last_load = V > kVec ? V - kVec : 0;
   auto token = [&](int i) { return min(v0 + i / kVec * 64 * kVec, last_load) + i % kVec; };
   float x[ITEMS];
-  if ((part + 1) * 64 * ITEMS <= (uint32_t)V) {
+  if ((part + 1) * 64 * ITEMS <= V) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const Vec got = *reinterpret_cast<const Vec*>(p + v0 + i * 64 * kVec);
@@ -263,11 +259,11 @@ __global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restric
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) sum[i % 4] += __builtin_amdgcn_exp2f((x[i] - at) * kLog2e);
   const float total = wave_sum_dpp((sum[0] + sum[1]) + (sum[2] + sum[3]));
-  if (lane == 0) sums[wave] = PartSum{top, total};
+  if (lane == 0) *result = PartSum{top, total};
 
   if (top == kNegInf) {  // the part's first tokens
-    const int64_t v = (int64_t)part * 64 * ITEMS + lane;
-    if (lane < K) lists[(int64_t)wave * K + lane] = v < V ? score_key(kNegInf, (int)v) : 0;
+    const int v = part * 64 * ITEMS + lane;
+    if (lane < K) list[lane] = v < V ? score_key(kNegInf, v) : 0;
     return;
   }
   // At least K scores reach the K-th largest of the lanes' maxima.
@@ -275,7 +271,6 @@ __global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restric
   wave_sort(maxima);
   const uint32_t kth = key_of_lane(maxima, K - 1).w[0];
   const float bound = key_value(kth);
-  uint64_t* held = gathered[w];
   int count = 0;
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
@@ -345,7 +340,21 @@ __global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restric
     });
     if (count > 0) sort_in(0, count);
   }
-  if (lane < K) lists[(int64_t)wave * K + lane] = ((uint64_t)best.w[0] << 32) | best.w[1];  // 0 where the part holds fewer
+  if (lane < K) list[lane] = ((uint64_t)best.w[0] << 32) | best.w[1];
+}
+
+template <typename E, int ITEMS>
+__global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restrict__ scores, int64_t sn, int64_t sw,
+                                                              uint32_t W, int V, int K, uint32_t parts,
+                                                              uint32_t waves, PartSum* __restrict__ sums,
+                                                              uint64_t* __restrict__ lists) {
+  __shared__ uint64_t gathered[kPartWaves][kGathered];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t wave = blockIdx.x * kPartWaves + w;
+  if (wave >= waves) return;
+  const uint32_t row = wave / parts, part = wave % parts;
+  part_list<E, ITEMS>(scores + (int64_t)(row / W) * sn + (int64_t)(row % W) * sw, V, (int)part, K, gathered[w],
+                      sums + wave, lists + (int64_t)wave * K);
 }
 
 // ---- the text's next beams -----------------------------------------------------------
@@ -367,31 +376,30 @@ __device__ __forceinline__ double wave_sum_f64(double x) {
   return x;
 }
 
-// A text's W parts lists hold W parts K candidates.  The K-th largest of the
-// lists' heads (of the lanes' best heads where there are more than 64), as FP32,
-// bounds the next beams from below: each wavefront finds it for itself, and the
-// few candidates that reach it are gathered in LDS and sorted by the first one.
+// A text's W parts lists hold W parts K candidates.  The K-th largest of 64 of them,
+// the lists' heads and what follows them (of the lanes' best heads where there are
+// more lists), as FP32, bounds the next beams from below: each wavefront finds it for
+// itself, and the few candidates that reach it are gathered in LDS and sorted by the
+// first one.
+//   sums, lists  the text's, [W, parts] and [W, parts, K]
+//   totals, ended and the outputs  the text's rows
 template <int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void beam_merge(const PartSum* __restrict__ sums,
-                                                         const uint64_t* __restrict__ lists, int parts,
-                                                         const float* __restrict__ totals,
-                                                         const unsigned char* __restrict__ ended, Stops stops, int W,
-                                                         int V, int K, float* __restrict__ new_totals,
-                                                         int64_t* __restrict__ parents, int64_t* __restrict__ tokens,
-                                                         unsigned char* __restrict__ new_ended) {
+__device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* lists, int parts, const float* totals,
+                                           const unsigned char* ended, const Stops& stops, int W, int V, int K,
+                                           float* new_totals, int64_t* parents, int64_t* tokens,
+                                           unsigned char* new_ended) {
   __shared__ double level[kMaxBeams];  // L
   __shared__ double from[kMaxBeams];   // the beam's total; -inf where it cannot go on
   __shared__ bool over[kMaxBeams];     // ended, and goes on
   __shared__ Key<3> gathered[kCandidates];
   __shared__ int count;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t row0 = (int64_t)blockIdx.x * W;
   if (threadIdx.x == 0) count = 0;
   for (int w = wave; w < W; w += WAVES) {
-    const PartSum* part = sums + (row0 + w) * parts;
+    const PartSum* part = sums + w * parts;
     const PartSum mine = lane < parts ? part[lane] : PartSum{kNegInf, 0.f};
-    const double total = (double)totals[row0 + w];
-    const bool end = ended && ended[row0 + w];
+    const double total = (double)totals[w];
+    const bool end = ended && ended[w];
     float top = mine.top;
     for (int i = lane + 64; i < parts; i += 64) top = fmaxf(top, part[i].top);
     top = wave_max_dpp(top);
@@ -419,7 +427,7 @@ __global__ __launch_bounds__(64 * WAVES) void beam_merge(const PartSum* __restri
     const double total = from[w];
     v = V;
     if (total > (double)kNegInf && !over[w]) {
-      const uint64_t key = lists[((row0 + w) * parts + part) * K + head];
+      const uint64_t key = lists[(w * parts + part) * K + head];
       if (key == 0) return 0.;
       v = (int)~(uint32_t)key;
       return total + ((double)key_value((uint32_t)(key >> 32)) - level[w]);
@@ -442,9 +450,9 @@ __global__ __launch_bounds__(64 * WAVES) void beam_merge(const PartSum* __restri
   };
   const int many = W * parts, all = many * K;
   Key<1> heads{{0}};
-  for (int list = lane; list < many; list += 64) {
+  for (int c = lane; c < max(many, min(all, 64)); c += 64) {
     int v;
-    const double value = candidate(list, 0, v);
+    const double value = candidate(c % many, c / many, v);
     if (v < V) heads.w[0] = max(heads.w[0], order_key((float)value + 0.f));
   }
   wave_sort(heads);
@@ -491,14 +499,65 @@ __global__ __launch_bounds__(64 * WAVES) void beam_merge(const PartSum* __restri
   if (lane < K) {
     const uint32_t flat = ~best.w[2];
     const int w = (int)(flat / (uint32_t)V), v = (int)(flat % (uint32_t)V);
-    bool stopped = ended && ended[row0 + w];
+    bool stopped = ended && ended[w];
     for (int i = 0; i < stops.n; ++i) stopped = stopped || stops.token[i] == v;
-    const int64_t at = (int64_t)blockIdx.x * K + lane;
-    new_totals[at] = (float)key64_value(((uint64_t)best.w[0] << 32) | best.w[1]);
-    parents[at] = w;
-    tokens[at] = v;
-    new_ended[at] = stopped ? 1 : 0;
+    new_totals[lane] = (float)key64_value(((uint64_t)best.w[0] << 32) | best.w[1]);
+    parents[lane] = w;
+    tokens[lane] = v;
+    new_ended[lane] = stopped ? 1 : 0;
   }
+}
+
+// The arguments of text i: its rows of each array.
+struct Beams {
+  const float* totals;
+  const unsigned char* ended;
+  float* new_totals;
+  int64_t *parents, *tokens;
+  unsigned char* new_ended;
+};
+
+template <int WAVES>
+__device__ __forceinline__ void next_beams_of(int64_t i, const PartSum* sums, const uint64_t* lists, int parts,
+                                              const Beams& a, const Stops& stops, int W, int V, int K) {
+  next_beams<WAVES>(sums, lists, parts, a.totals + i * W, a.ended ? a.ended + i * W : nullptr, stops, W, V, K,
+                    a.new_totals + i * K, a.parents + i * K, a.tokens + i * K, a.new_ended + i * K);
+}
+
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void beam_merge(const PartSum* __restrict__ sums,
+                                                         const uint64_t* __restrict__ lists, int parts, Beams a,
+                                                         Stops stops, int W, int V, int K) {
+  const int64_t i = blockIdx.x, first = i * W * parts;
+  next_beams_of<WAVES>(i, sums + first, lists + first * K, parts, a, stops, W, V, K);
+}
+
+// A text of few scores in one launch: a wavefront a part, the lists in LDS.
+constexpr int kTextWaves = 16, kTextItems = 32;
+
+template <typename E>
+__global__ __launch_bounds__(64 * kTextWaves) void beam_text(const E* __restrict__ scores, int64_t sn, int64_t sw,
+                                                             Beams a, Stops stops, int W, int V, int K, int parts) {
+  __shared__ uint64_t gathered[kTextWaves][kGathered];
+  __shared__ uint64_t lists[kTextWaves * kMaxBeams];
+  __shared__ PartSum sums[kTextWaves];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (w < W * parts)
+    part_list<E, kTextItems>(scores + (int64_t)blockIdx.x * sn + (int64_t)(w / parts) * sw, V, w % parts, K,
+                             gathered[w], sums + w, lists + w * K);
+  __syncthreads();
+  next_beams_of<kTextWaves>(blockIdx.x, sums, lists, parts, a, stops, W, V, K);
+}
+
+
+// The parts of a beam in beam_text, or 0 where the text takes two launches: where a
+// workgroup's wavefronts do not hold its parts, or the texts outnumber the compute
+// units.  Measured, us, in a graph and from a program, one launch and two: one text of
+// 4 beams over 8192 scores 9.0, 8.3 and 13.9, 17.7; 200 texts 9.8, 11.5 and 13.5, 17.4;
+// 8 beams over 4000 11.0, 9.8 and 13.8, 18.1; 16 over 2000 13.8, 12.3 and 13.7, 17.6.
+int text_parts(int n, int W, int V) {
+  const int64_t parts = ((int64_t)V + 64 * kTextItems - 1) / (64 * kTextItems);
+  return W * parts <= kTextWaves && n <= compute_units() ? (int)parts : 0;
 }
 
 // Scores a lane of a part: 64 where the parts of 4096 fill the GPU, 16 where
@@ -520,6 +579,10 @@ extern "C" int wptv_beam_workspace(int n, int W, int V, int K, size_t* bytes) {
     return fail(WPTV_E_UNSUPPORTED, "beam_workspace: at most %d beams a text (W=%d, K=%d)", kMaxBeams, W, K);
   if ((int64_t)W * V > (1 << 28) || (int64_t)n * W > INT32_MAX)
     return fail(WPTV_E_UNSUPPORTED, "beam_workspace: n=%d W=%d V=%d is too large", n, W, V);
+  if (text_parts(n, W, V)) {
+    *bytes = 0;
+    return WPTV_OK;
+  }
   const int part = 64 * part_items((int64_t)n * W, V);
   if ((int64_t)n * W * (((int64_t)V + part - 1) / part) > INT32_MAX)
     return fail(WPTV_E_UNSUPPORTED, "beam_workspace: n=%d W=%d V=%d is too large", n, W, V);
@@ -546,10 +609,20 @@ extern "C" int wptv_beam_step(const void* scores, int64_t scores_stride_n, int64
     s.token[i] = (int)stops[i];
   }
   if (n == 0) return WPTV_OK;
-  if (!scores || !totals || !new_totals || !parents || !tokens || !new_ended || !workspace)
+  if (!scores || !totals || !new_totals || !parents || !tokens || !new_ended || (need && !workspace))
     return fail(WPTV_E_INVALID, "beam_step: a required pointer is NULL");
   if (workspace_bytes < need)
     return fail(WPTV_E_INVALID, "beam_step: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  const Beams beams{totals, ended, new_totals, parents, tokens, new_ended};
+  if (const int parts = text_parts(n, W, V)) {
+    if (scores_dtype == WPTV_F32)
+      beam_text<<<n, 64 * kTextWaves, 0, stream>>>(static_cast<const float*>(scores), scores_stride_n, scores_stride_w,
+                                                   beams, s, W, V, K, parts);
+    else
+      beam_text<<<n, 64 * kTextWaves, 0, stream>>>(static_cast<const unsigned short*>(scores), scores_stride_n,
+                                                   scores_stride_w, beams, s, W, V, K, parts);
+    return launched("beam_text");
+  }
   const int items = part_items((int64_t)n * W, V), parts = (int)(((int64_t)V + 64 * items - 1) / (64 * items));
   const int64_t waves = (int64_t)n * W * parts, blocks = (waves + kPartWaves - 1) / kPartWaves;
   PartSum* sums = static_cast<PartSum*>(workspace);
@@ -566,10 +639,8 @@ extern "C" int wptv_beam_step(const void* scores, int64_t scores_stride_n, int64
   const int launch = launched("beam_parts");
   if (launch != WPTV_OK) return launch;
   if ((int64_t)W * parts * K <= 4096)
-    beam_merge<8><<<n, 512, 0, stream>>>(sums, lists, parts, totals, ended, s, W, V, K, new_totals, parents, tokens,
-                                         new_ended);
+    beam_merge<8><<<n, 512, 0, stream>>>(sums, lists, parts, beams, s, W, V, K);
   else
-    beam_merge<16><<<n, 1024, 0, stream>>>(sums, lists, parts, totals, ended, s, W, V, K, new_totals, parents, tokens,
-                                           new_ended);
+    beam_merge<16><<<n, 1024, 0, stream>>>(sums, lists, parts, beams, s, W, V, K);
   return launched("beam_merge");
 }

@@ -340,7 +340,7 @@ def beam_step(scores, totals, ended=None, stops=(), beams=None):
     ended = None if ended is None else ended.contiguous()
     with _lib.on(device):
         _, size = _lib.plan("wptv_beam_workspace", "beam_step", n, W, V, K)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         check(_lib.lib().wptv_beam_step(ptr(scores), scores.stride(0), scores.stride(1),
                                         _lib.dtype_code(scores.dtype), ptr(totals), ptr(ended),
                                         (ctypes.c_int64 * len(stops))(*stops), len(stops), n, W, V, K,
