@@ -378,15 +378,15 @@ def _tables(tables, rows, what):
     """(device, the library's table arguments: the host arrays of addresses,
     batch and row strides in bytes, capacities and row bytes, then their
     count; the arrays' owner) of tables (rows, capacity, width)."""
-    device = None
+    device = index = None
     addresses, strides_b, strides_n, capacities, row_bytes = [], [], [], [], []
     for t in tables:
         shape = t.shape
         if len(shape) != 3 or shape[0] != rows or shape[2] == 0:
             raise ValueError(f"{what}: each table must be ({rows}, capacity, width); got {tuple(shape)}")
         if device is None:
-            device = t.device
-        if t.device != device or not t.is_cuda:
+            device, index = t.device, t.get_device()
+        if index < 0 or t.get_device() != index:
             raise KernelUnavailable(f"{what} moves tables on one GPU; got tables on {device} and {t.device}")
         stride_b, stride_n, stride_c = t.stride()
         if stride_c != 1 and shape[2] > 1:
