@@ -180,6 +180,11 @@ def test_verify_steps_on_a_weighted_cache(device):
             for _ in range(5):
                 step.run()
         torch.cuda.synchronize()
+        copy = cache.select([1, 0])  # a cache whose host bound the replays have not raised
+        model.reorder(cache, torch.tensor([[1, 0]]))
+        assert torch.equal(cache.lengths, copy.lengths)
+        for b, n in enumerate(cache.lengths.tolist()):
+            assert all(torch.equal(x[b, :n], y[b, :n]) for x, y in zip(cache.tables, copy.tables))
         caches.append(cache)
         assert torch.allclose(cache.weights.sum(-1), 4.0 * cache.lengths.float().expand(3, 2), rtol=1e-2)
     assert torch.equal(caches[0].lengths, caches[1].lengths)
@@ -211,6 +216,15 @@ def test_the_beams_written_are_those_of_a_plain_search(device, config, beams, st
         assert [x for _, x in found] == pytest.approx(totals, abs=1e-3)
 
 
+def test_a_search_of_ended_beams_stops(device):
+    model = decoder(device)
+    writer = BeamWriter(model, [[1, 2], [3]], 3, stops=iter((7,)))
+    writer.ended.fill_(True)
+    writer.totals.copy_(torch.tensor([[-1.0, -2.0, -float("inf")], [-1.0, -1.5, -3.0]]))
+    assert [[t for t, _ in beams] for beams in writer.write(50)] == [[[], []], [[], [], []]]
+    assert not writer._steps
+
+
 def test_beam_search_on_a_bounded_cache(device):
     model = decoder(device, MIXED, torch.bfloat16)
     prompts = [tokens(n, seed=n).tolist() for n in (90, 3, 41)]
@@ -236,6 +250,8 @@ def test_what_the_beam_writer_refuses(device):
             BeamWriter(model, *arguments)
     with pytest.raises(ValueError, match="keep"):
         BeamWriter(model, [[1]], 2, keep=3, first=4)
+    with pytest.raises(ValueError, match="16 tokens"):
+        BeamWriter(model, [[1]], 2, stops=range(17))
     with pytest.raises(ValueError, match="sparse layers"):
         BeamWriter(decoder(device, MIXED), [[1]], 2, keep=17, first=2)
     for prompts, stops in (([[1, 512]], ()), ([[-1]], ()), ([[1]], (512,))):

@@ -34,10 +34,13 @@ class BeamWriter:
             raise ValueError("beam search writes for at least one prompt, each of at least one token")
         if not 1 <= beams <= 64:
             raise ValueError(f"a text is written by 1 to 64 beams; got {beams}")
+        stops = tuple(int(s) for s in stops)
+        if len(stops) > 16:
+            raise ValueError(f"a beam ends at one of at most 16 tokens; got {len(stops)}")
         vocab = model.config.vocab
         if any(not 0 <= t < vocab for p in prompts for t in p) or any(not 0 <= t < vocab for t in stops):
             raise IndexError(f"token ids must lie in [0, {vocab})")
-        self.model, self.beams, self.stops = model, int(beams), tuple(int(s) for s in stops)
+        self.model, self.beams, self.stops = model, int(beams), stops
         self.bounds = None if keep is None else model.evict_rows(keep, first, recent)
         self.device = next(model.parameters()).device
         n = len(prompts)
@@ -80,7 +83,7 @@ class BeamWriter:
         """Up to limit more tokens a beam, fewer when every beam has ended:
         texts()."""
         for i in range(limit):
-            if self.stops and i % CHECK == 0 and bool(self.ended.all()):
+            if self.stops and i % CHECK == 0 and bool((self.ended | (self.totals == float("-inf"))).all()):
                 break
             self.step()
         return self.texts()

@@ -217,9 +217,8 @@ class Cache:
         tables = [self.tables[i] for i in self.growing]
         if self.weights is not None:
             tables += [w[..., None] for w in self.weights]
-        if tables:  # (a graph is replayed on longer texts than it was captured on)
-            bound = None if torch.cuda.is_current_stream_capturing() else self.bound
-            kernels.reorder_rows(tables, parents, self.lengths, rows=bound)
+        if tables:  # not bounded by `bound`: replays of a captured reading do not raise it
+            kernels.reorder_rows(tables, parents, self.lengths)
         if self.rings:
             kernels.reorder_rows([self.tables[i] for i in sorted(self.rings)], parents, self.starts())
         states = [self.lengths] if self.evicted is None else [self.lengths, self.evicted]

@@ -209,7 +209,8 @@ class MQADecoder:
         """An empty cache of `rows` rows (the reference's WPT.new_cache); its
         window layers' rings hold readings of up to `widest` tokens (wider
         ones are read in pieces).  weighted: it keeps the attention weight that
-        the exact layers' rows receive, so that evict can bound it."""
+        the exact layers' rows receive (from those layers' own queries), so
+        that evict can bound it."""
         if routes:
             raise NotImplementedError("this decoder has no routed experts to record")
         c = self.config.head_dim
