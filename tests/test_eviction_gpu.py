@@ -68,7 +68,7 @@ def check(device, q, table, positions, lse, weights, counts=None, start=None, sp
 @pytest.mark.parametrize("B, T, H, c, N", [
     (1, 1, 1, 64, 1), (1, 1, 16, 128, 300), (3, 5, 16, 128, 517), (2, 7, 4, 64, 1029), (2, 3, 12, 128, 65),
     (1, 9, 32, 64, 255), (2, 1, 8, 64, 64), (1, 70, 16, 128, 70), (2, 130, 8, 64, 200), (1, 64, 16, 64, 1000),
-    (2, 4, 3, 96, 130), (1, 2, 5, 33, 77), (1, 3, 2, 256, 100), (2, 33, 128, 64, 40), (1, 2, 200, 16, 30)])
+    (2, 4, 3, 96, 130), (1, 2, 5, 33, 77), (5, 20, 16, 64, 129), (3, 21, 16, 128, 257), (70, 1, 4, 64, 4000), (1, 3, 2, 256, 100), (2, 33, 128, 64, 40), (1, 2, 200, 16, 30)])
 def test_the_weights_of_a_reading(device, B, T, H, c, N, dtype):
     print(f"attention weights B={B} T={T} H={H} c={c} N={N} {dtype}", flush=True)
     q, table, positions, lse, start = reading(B, T, H, c, N, dtype, seed=B + T + H + N)

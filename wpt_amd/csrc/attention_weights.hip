@@ -21,8 +21,8 @@
 // cycles and its vector unit 96 (an exponential at a quarter of the rate, the scaling
 // and the sum): a prompt is bound by the latter.  Two prompts of 4096 tokens, 16 heads:
 // 64 us and 4 for the join, 1.06 PFLOP/s of the products alone.  Few queries are bound
-// by the keys: 32 texts of 4100 rows, 5 queries, 12.5 us for 27 MB, of which the chain
-// positions, keys, products, write takes 5 whatever is read.
+// by the keys: 32 texts of 4100 rows, 5 queries, 11.4 us for 27 MB, of which the chain
+// positions, keys, products, write takes 4 whatever is read.
 #include "wptv_common.h"
 
 #include <climits>
@@ -84,8 +84,7 @@ __global__ __launch_bounds__(kGT) void attention_weights_generic(
 
 // ---- the matrix-core form ------------------------------------------------------
 
-constexpr int kWaveKeys = 64;    // table rows of a wavefront
-constexpr int kBlockKeys = 256;  // of a workgroup of four
+constexpr int kBlockKeys = 256;  // table rows of a workgroup of four wavefronts of 64
 constexpr int kStage = 512;      // query heads whose lse and position are staged in LDS at once
 constexpr float kUnseen = -1.f;  // a part's sum for a row that none of its queries sees (sums are not negative)
 
@@ -122,14 +121,15 @@ struct Rows16<float, C> {
 // while these are multiplied.
 // At least two wavefronts a SIMD: the compiler then keeps the products out of the
 // accumulation registers, which the exponentials cannot read.
-template <typename E, int C>
+template <typename E, int C, int U>
 __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
     const E* __restrict__ q, const E* __restrict__ k, int64_t ksb, int64_t ksn, const int64_t* __restrict__ positions,
     const float* __restrict__ lse, const int64_t* __restrict__ counts, const int64_t* __restrict__ start, int B, int T,
     int H, int N, float scale_log2, int nkb, int parts, int part_rows, int by_xcd, float* __restrict__ weights,
-    int64_t wsb, float* __restrict__ sums) {
+    int64_t wsb, float* __restrict__ sums, int64_t sums_stride) {
   typedef Rows16<E, C> Op;
-  constexpr int kP = Op::kPieces;
+  static_assert(U == 2 || U == 4, "blocks of 16 rows a wavefront holds");
+  constexpr int kP = Op::kPieces, kWaveKeys = 16 * U;
   __shared__ __attribute__((aligned(16))) unsigned char queries[2][4 * kP * 1024];  // blocks of 16, then pieces
   __shared__ __attribute__((aligned(16))) float l2s[kStage];
   __shared__ __attribute__((aligned(16))) int seen[kStage];
@@ -163,7 +163,8 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
     lo = __builtin_amdgcn_readfirstlane(wave_min_i32(lo));
     hi = __builtin_amdgcn_readfirstlane(wave_max_i32(hi));
   }
-  const int n0 = kb * kBlockKeys, wn0 = n0 + kWaveKeys * w, n = wn0 + lane;
+  const int n0 = kb * 4 * kWaveKeys, wn0 = n0 + kWaveKeys * w, n = wn0 + lane;
+  const bool mine = lane < kWaveKeys;  // lane l ends with row wn0 + l's sum
   float total = 0.f, before = 0.f;
   if (n0 <= hi) {
     const int heads = end - first;
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
     };
     // everything is asked for at once: what is waited for first, first
     read_stage(0);
-    if (parts == 1 && n <= hi && !(start && n >= start[b])) before = weights[(int64_t)b * wsb + n];
+    if (parts == 1 && mine && n <= hi && !(start && n >= start[b])) before = weights[(int64_t)b * wsb + n];
     // query heads first + r0 .. first + r0 + 63 into a buffer, block w by wavefront w
     // (past the end: the last one again)
     auto fetch = [&](int r0, int buffer) {
@@ -201,10 +202,11 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
         dma_16B(rsrc, (uint32_t)row * (C * sizeof(E)) + 64 * f + 16 * g, __builtin_amdgcn_readfirstlane(at + 1024 * f));
     };
     fetch(0, 0);
-    Op keys[4];
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    Op keys[U];
+    float sum[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
+      sum[u] = 0.f;
       const E* row = k + (int64_t)b * ksb + (int64_t)min(wn0 + 16 * u + j, N - 1) * ksn;
 #pragma unroll
       for (int f = 0; f < kP; ++f)
@@ -214,7 +216,7 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
     write_stage(0);
     // the keys are waited for here: in the loop, the wait would be for the DMA too
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int f = 0; f < kP; ++f) asm volatile("" : "+v"(keys[u].v[f]));
     const bool whole = wn0 + kWaveKeys - 1 <= lo, idle = wn0 > hi;
@@ -238,17 +240,17 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
         for (int f = 0; f < kP; ++f)
           query.v[f] = *reinterpret_cast<const decltype(query.v[f] + 0)*>(&queries[buffer][(m * kP + f) * 1024 + lane * 16]);
         const f32x4 l2 = *reinterpret_cast<const f32x4*>(&l2s[r0 % kStage + 16 * m + 4 * g]);
-        f32x4 acc[4];
+        f32x4 acc[U];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < U; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < Op::kSteps; ++s)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) acc[u] = Op::step(query, keys[u], s, acc[u]);
+          for (int u = 0; u < U; ++u) acc[u] = Op::step(query, keys[u], s, acc[u]);
         // acc[u][i]: query head 16 m + 4 g + i, row wn0 + 16 u + j
         if (whole) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
+          for (int u = 0; u < U; ++u) {
             float e[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(acc[u][i], scale_log2, -l2[i]));
@@ -257,7 +259,7 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
         } else {
           const i32x4 p = *reinterpret_cast<const i32x4*>(&seen[r0 % kStage + 16 * m + 4 * g]);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
+          for (int u = 0; u < U; ++u) {
             float e[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -270,16 +272,21 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
       }
       __syncthreads();  // the buffer is read
     }
-    // the four lane groups' sums of the four blocks, block u into lane group u
+    // the four lane groups' sums of each block, block u into lane group u (two blocks:
+    // into the first two groups)
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[0]), __float_as_uint(sum[1]), false, false);
-    const auto c = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[2]), __float_as_uint(sum[3]), false, false);
     const float z01 = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const float z23 = __uint_as_float(c[0]) + __uint_as_float(c[1]);
+    float z23 = z01;
+    if constexpr (U == 4) {
+      const auto c = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[2]), __float_as_uint(sum[3]), false, false);
+      z23 = __uint_as_float(c[0]) + __uint_as_float(c[1]);
+    }
     const auto d = __builtin_amdgcn_permlane32_swap(__float_as_uint(z01), __float_as_uint(z23), false, false);
     total = __uint_as_float(d[0]) + __uint_as_float(d[1]);
   }
+  if (!mine) return;
   if (parts > 1) {
-    sums[((int64_t)part * B + b) * nkb * kBlockKeys + n] = n <= hi ? total : kUnseen;
+    sums[((int64_t)part * B + b) * sums_stride + n] = n <= hi ? total : kUnseen;
   } else if (n <= hi) {
     float* out = weights + (int64_t)b * wsb + n;
     *out = before + total;
@@ -288,15 +295,15 @@ __global__ __launch_bounds__(256, 2) void attention_weights_mfma(
 
 // weights += the parts' sums in order, a fourth of them by each wavefront of a
 // workgroup of 64 rows; rows that no part sees are left alone.
-__global__ __launch_bounds__(256) void attention_weights_join(const float* __restrict__ sums, int parts, int nkb, int B,
-                                                              int N, const int64_t* __restrict__ start,
+__global__ __launch_bounds__(256) void attention_weights_join(const float* __restrict__ sums, int parts, int64_t sums_stride,
+                                                              int B, int N, const int64_t* __restrict__ start,
                                                               float* __restrict__ weights, int64_t wsb) {
   __shared__ float shared[4][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int b = blockIdx.y, n = blockIdx.x * 64 + lane;
-  const int64_t stride = (int64_t)B * nkb * kBlockKeys;
+  const int64_t stride = B * sums_stride;
   const int some = (parts + 3) / 4, end = min(parts, (w + 1) * some);
-  const float* s = sums + (int64_t)b * nkb * kBlockKeys + n;
+  const float* s = sums + b * sums_stride + n;
   float total = kUnseen;
 #pragma unroll 8
   for (int p = w * some; p < end; ++p) {
@@ -323,15 +330,29 @@ __global__ __launch_bounds__(256) void attention_weights_join(const float* __res
 // tokens 121 [32], 73 [64], 67 [128], 71 [192]; a chunk of 1024 tokens over 4096 rows
 // 38 [16], 26 [32], 32 [96], 39 [192]; one of 64 over 8192 34 [1], 14 [4], 11 [8],
 // 14 [32]; a prompt of 512 36 [8], 11.2 [64], 10.4 [128], 12.9 [192]; 9 queries of 32
-// heads over 1000 rows 12.8 [1], 9.0 [4], 8.0 [12].
+// heads over 1000 rows 9.1 [1], 9.0 [4], 8.1 [12].
 int weight_parts(int B, int T, int H, int N) {
   const int64_t rows = (int64_t)T * H, units = (int64_t)B * ((N + kBlockKeys - 1) / kBlockKeys);
   const int64_t cus = compute_units();
   const int64_t parts = max(min(cus / units, rows / 32), min(rows / 512, 16 * cus / units));
+  // few query heads in few parts: the join costs more than it gives (80 over 2000 rows
+  // of 16 texts 5.9 [1], 8.6 [2]; 256 over 16000 of two 8.9 [1], 10.6 [2])
+  if (rows < 256 || (rows <= 512 && parts < 4)) return 1;
   return (int)max((int64_t)1, parts);
 }
 
 bool matrix_width(int c) { return c == 64 || c == 128; }
+
+// Blocks of 16 rows a wavefront holds: four, so that a query head read from LDS meets
+// 64 rows; two where the queries are few and the workgroups of four do not fill the
+// compute units four times, so that twice as many share the chain's latency.
+// Measured, us, two and four: 32 texts of 4100 rows, 5 queries of 16 heads, 11.4, 12.6;
+// 8 texts 5.9, 7.4; one token over 4096 rows 4.2, 5.1; 6 texts of 3001 FP32 rows, 7
+// queries of 4 heads, 5.6, 7.3; 64 texts of 4100, one query, 14.3, 13.4.
+int wave_blocks(int B, int64_t heads, int N, int parts) {
+  const int64_t units = (int64_t)B * ((N + kBlockKeys - 1) / kBlockKeys);
+  return parts == 1 && heads <= 320 && units <= 4 * (int64_t)compute_units() ? 2 : 4;
+}
 
 }  // namespace
 }  // namespace wptv
@@ -382,25 +403,29 @@ extern "C" int wptv_attention_weights(const void* q, const void* k, int64_t k_st
     return fail(WPTV_E_INVALID, "attention_weights: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   const int elem = dtype == WPTV_BF16 ? 2 : 4;
   if (matrix_width(c) && aligned(q, 16) && aligned(k, 16) && k_stride_n * elem % 16 == 0 && k_stride_b * elem % 16 == 0) {
-    const int blocks = (N + kBlockKeys - 1) / kBlockKeys;
+    const int held = wave_blocks(B, (int64_t)T * H, N, splits);
+    const int blocks = (N + 64 * held - 1) / (64 * held);
+    const int64_t sums_stride = (int64_t)((N + kBlockKeys - 1) / kBlockKeys) * kBlockKeys;
     const int part_rows = (int)(((int64_t)T * H + splits - 1) / splits + 15) / 16 * 16;
     const int chunks = splits * B;
     const int by_xcd = splits > 1 && (chunks % 8 == 0 || chunks >= 64);  // as many chunks an XCD, nearly
     const int groups = by_xcd ? (chunks + 7) / 8 * 8 : chunks;
     float* sums = static_cast<float*>(workspace);
-#define WPTV_WEIGHTS(E, C)                                                                                            \
-  attention_weights_mfma<E, C><<<blocks * groups, 256, 0, stream>>>  (                                             \
+#define WPTV_WEIGHTS(E, C, U)                                                                                         \
+  attention_weights_mfma<E, C, U><<<blocks * groups, 256, 0, stream>>>(                                              \
       static_cast<const E*>(q), static_cast<const E*>(k), k_stride_b, k_stride_n, positions, lse, counts, start, B, T, \
-      H, N, scale * kLog2e, blocks, splits, part_rows, by_xcd, weights, weights_stride_b, sums)
+      H, N, scale * kLog2e, blocks, splits, part_rows, by_xcd, weights, weights_stride_b, sums, sums_stride)
+#define WPTV_WEIGHTS_U(E, C) (held == 2 ? WPTV_WEIGHTS(E, C, 2) : WPTV_WEIGHTS(E, C, 4))
     if (dtype == WPTV_BF16) {
-      if (c == 64) WPTV_WEIGHTS(unsigned short, 64); else WPTV_WEIGHTS(unsigned short, 128);
+      if (c == 64) WPTV_WEIGHTS_U(unsigned short, 64); else WPTV_WEIGHTS_U(unsigned short, 128);
     } else {
-      if (c == 64) WPTV_WEIGHTS(float, 64); else WPTV_WEIGHTS(float, 128);
+      if (c == 64) WPTV_WEIGHTS_U(float, 64); else WPTV_WEIGHTS_U(float, 128);
     }
+#undef WPTV_WEIGHTS_U
 #undef WPTV_WEIGHTS
     const int launch = launched("attention_weights_mfma");
     if (launch != WPTV_OK || splits == 1) return launch;
-    attention_weights_join<<<dim3((N + 63) / 64, B), 256, 0, stream>>>(sums, splits, blocks, B, N, start, weights,
+    attention_weights_join<<<dim3((N + 63) / 64, B), 256, 0, stream>>>(sums, splits, sums_stride, B, N, start, weights,
                                                                        weights_stride_b);
     return launched("attention_weights_join");
   }
