@@ -655,7 +655,8 @@ int wptv_attention_weights(const void* q, const void* k, int64_t k_stride_b, int
  *   counts   [B] int64 out: the rows kept, min(length, keep)
  * wptv_keep_rows: row j of batch row b of table i becomes its row
  *   kept[i mod lists, b, j] for j < min(counts[b], keep), in place; the lists
- *   ascend (as wptv_choose_kept's).  Tables as wptv_reorder_rows; rows from
+ *   do not fall (wptv_choose_kept's ascend; a row below its place, or past the
+ *   capacity, moves nothing).  Tables as wptv_reorder_rows; rows from
  *   counts[b] on keep what they hold. */
 int wptv_choose_kept(const float* weights, int64_t weights_stride_l, int64_t weights_stride_b, const int64_t* lengths,
                      int L, int B, int N, int keep, int first, int recent, int64_t* kept, int64_t* counts,

@@ -263,6 +263,42 @@ def test_lists_that_name_no_row_move_nothing_out_of_range(device):
     assert torch.equal(moved.cpu(), expected)
 
 
+def test_a_list_that_names_a_row_twice(device):
+    table = torch.randint(0, 100, (1, 3000, 8), generator=torch.Generator().manual_seed(1)).float()
+    rows = torch.sort(torch.randint(0, 3000, (1, 1, 1400), generator=torch.Generator().manual_seed(2))).values
+    rows = torch.maximum(rows, torch.arange(1400))  # not below their places
+    moved = table.to(device)
+    kernels.keep_rows(moved, rows.to(device), torch.tensor([1400], device=device))
+    assert torch.equal(moved.cpu(), oracle.keep_rows([table], rows, torch.tensor([1400]))[0])
+
+
+def test_two_streams_at_once(device):
+    B, T, H, c, N, keep = 2, 40, 16, 64, 600, 200
+    sets, streams = [], [torch.cuda.Stream(device) for _ in range(2)]
+    for seed in range(2):
+        q, table, positions, lse, start = (x.to(device) for x in reading(B, T, H, c, N, torch.bfloat16, seed=seed))
+        sets.append((q, table, positions, lse, start, torch.rand(1, B, N, device=device)))
+
+    def step(q, table, positions, lse, start, weights):
+        table, weights = table.clone(), weights.clone()
+        kernels.add_attention_weights(q, table[..., :c], positions, lse, c ** -0.5, weights[0], start=start)
+        kept, counts = kernels.choose_kept(weights, positions[:, -1] + 1, keep, 2, 16)
+        kernels.keep_rows(table, kept, counts)
+        return weights, kept, table
+
+    expected = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(step(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, expected[i]))
+
+
 def test_in_a_graph_on_another_stream(device):
     L, B, T, H, c, N, keep = 2, 2, 3, 16, 128, 200, 64
     q, table, positions, lse, start = reading(B, T, H, c, N, torch.bfloat16, seed=8)

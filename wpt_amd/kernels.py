@@ -407,8 +407,8 @@ def _tables(tables, rows, what):
 
 def reorder_rows(tables, parents, lengths=None, rows=None):
     """Beam search's reordering of states, in place: in each of tables
-    (n W, capacity, width) (one tensor or several, of any types and widths),
-    batch row i W + w becomes batch row i W + parents[i, w], every beam at
+    (n W, capacity, width) (one tensor or several, of any types and widths,
+    none overlapping another), batch row i W + w becomes batch row i W + parents[i, w], every beam at
     once: a beam may be taken several times, and one that nothing takes is
     gone.  parents (n, W) int64, as sampling.beam_step gives them; one outside
     0 .. W - 1 leaves its beam as it is.  lengths (n W,): only each source's
