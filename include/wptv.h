@@ -582,7 +582,8 @@ int wptv_greedy_tree_best(const int32_t* best, const int64_t* node_tokens, const
  * wptv_beam_step: text i's candidates are its W beams continued by each of V
  *   tokens, of value totals[i, w] + (x - log sum exp x) over the beam's
  *   scores x, ranked in 64 bits.  The K largest are the next beams, in order,
- *   equal values to the lowest w V + v.
+ *   equal values to the lowest w V + v.  (log sum exp x is added up in FP32
+ *   parts, and again in 64 bits where those do not tell two candidates apart.)
  *   scores   beam w of text i at scores + i*scores_stride_n +
  *            w*scores_stride_w (elements), V contiguous values of scores_dtype
  *            (WPTV_F32 or WPTV_BF16)
@@ -594,8 +595,8 @@ int wptv_greedy_tree_best(const int32_t* best, const int64_t* node_tokens, const
  *   stops    n_stops (0 .. 16) token ids in host memory: a beam that writes
  *            one of them has ended
  *   new_totals, parents, tokens, new_ended  [n, K] out: the next beams'
- *            totals (fp32), source beams, tokens (int64) and whether they have
- *            ended (bytes)
+ *            totals (fp32: off by the rounding and at most (3 ln V + 33) 2^-24),
+ *            source beams, tokens (int64) and whether they have ended (bytes)
  *   workspace  wptv_beam_workspace(n, W, V, K) bytes.  W, K <= 64, K <= W V
  * ------------------------------------------------------------------------- */
 int wptv_beam_workspace(int n, int W, int V, int K, size_t* bytes);

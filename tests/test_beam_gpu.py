@@ -249,3 +249,43 @@ def test_on_another_stream_and_in_a_graph(device):
         if i == 0:
             for a, b in zip(got, list(side) + [after]):
                 assert torch.equal(a, b)
+
+
+# ---- values close to each other ----------------------------------------------------
+
+
+def close_beams(n, W, V, dtype, seed):
+    """Texts whose beams' best candidates are equal but for the rounding of the
+    totals to FP32, some 1e-8 to 1e-7: the totals level the beams out."""
+    g = torch.Generator().manual_seed(seed)
+    scores = (3 * torch.randn(n, W, V, generator=g)).to(dtype)
+    best = torch.log_softmax(scores.double(), -1).amax(-1)
+    totals = (-2.5 - best).float()
+    gaps = (totals.double() + best).sort(-1).values.diff(dim=-1)
+    # far from 64 bits' own steps, and closer than FP32 sums tell apart
+    assert float(gaps[gaps > 0].min()) > 1e-13 and float(gaps.max()) < 1e-6
+    return scores, totals
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n, W, V, K", [
+    (48, 2, 4000, 1), (48, 2, 4000, 2), (48, 5, 1500, 3), (300, 2, 4000, 2), (600, 2, 4000, 1), (600, 2, 4000, 2),
+    (40, 4, 33001, 4), (3, 16, 20000, 7), (2, 64, 5000, 64)])
+def test_beams_closer_than_fp32_sums_tell_apart(device, n, W, V, K, dtype):
+    print(f"beam_step close beams n={n} W={W} V={V} K={K} {dtype}", flush=True)
+    scores, totals = close_beams(n, W, V, dtype, seed=n + K)
+    check(device, scores, totals, beams=K)
+    ended = torch.zeros(n, W, dtype=torch.bool)
+    ended[:, 0] = True  # an ended beam's own total beside the others' values
+    totals[:, 0] = -2.5
+    check(device, scores, totals, ended, stops=(5,), beams=K)
+
+
+def test_the_beams_of_a_text_do_not_depend_on_the_batch(device):
+    scores, totals = close_beams(600, 2, 4000, torch.float32, seed=4)  # other parts of a beam at each size
+    scores, totals = scores.to(device), totals.to(device)
+    whole = sampling.beam_step(scores, totals)
+    for n in (1, 64, 300):
+        got = sampling.beam_step(scores[:n], totals[:n])
+        for a, b in zip(got[1:], whole[1:]):
+            assert torch.equal(a, b[:n])

@@ -9,8 +9,9 @@
 //   beam_parts  a wavefront a part of a beam's scores, all of it in registers:
 //               the part's maximum, its sum of exponentials, and its K largest
 //               scores, ties to the lowest token
-//   beam_merge  a workgroup a text: the parts' sums joined to L in 64 bits, and
-//               the K best of the parts' lists
+//   beam_merge  a workgroup a text: the parts' FP32 sums joined to L, and the K
+//               best of the parts' lists; where two beams' candidates are closer
+//               than those sums tell apart, L again in 64 bits from the scores
 //   beam_text   both, for a text whose parts fit one workgroup
 // The K largest of a part: the K-th largest of the lanes' maxima bounds them
 // from below, and few scores reach it (in scores without order about K of 4096);
@@ -25,6 +26,7 @@
 #include "wptv_common.h"
 
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 namespace wptv {
@@ -175,6 +177,11 @@ __device__ __forceinline__ Key<N> backwards(const Key<N>& k) {
 #pragma unroll
   for (int i = 0; i < N; ++i) r.w[i] = lane_xor<63>(k.w[i]);
   return r;
+}
+
+// x of lane + 1 (the last lane's: no use).
+__device__ __forceinline__ uint32_t next_lane(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x130, 0xf, 0xf, false);  // wave_shl:1
 }
 
 template <int N>
@@ -376,25 +383,58 @@ __device__ __forceinline__ double wave_sum_f64(double x) {
   return x;
 }
 
+// L of each beam that goes on, in 64 bits: the scores again, by the whole workgroup.
+template <int WAVES, typename E>
+__device__ __forceinline__ void exact_levels(const E* scores, int64_t sw, int W, int V, const double* from,
+                                             const bool* over, const float* tops, double* level) {
+  __shared__ double partial[WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int w = 0; w < W; ++w) {
+    if (!(from[w] > (double)kNegInf) || over[w]) continue;  // uniform
+    const E* x = scores + w * sw;
+    const double top = (double)tops[w];
+    double sum = 0.;
+#pragma unroll 4
+    for (int v = threadIdx.x; v < V; v += 64 * WAVES) sum += exp((double)load_f32(x + v) - top);
+    sum = wave_sum_f64(sum);
+    if (lane == 0) partial[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < WAVES; ++i) sum += partial[i];
+      level[w] = top + log(sum);
+    }
+    __syncthreads();
+  }
+}
+
 // A text's W parts lists hold W parts K candidates.  The K-th largest of 64 of them,
 // the lists' heads and what follows them (of the lanes' best heads where there are
 // more lists), as FP32, bounds the next beams from below: each wavefront finds it for
 // itself, and the few candidates that reach it are gathered in LDS and sorted by the
-// first one.
+// first one.  Values formed with the FP32 sums' L are off by at most `slack`; where a
+// candidate of another beam comes that close to one that is taken, which of them is
+// larger (and which is the K-th) is decided with L in 64 bits.  Within a beam L is the
+// same and the order right as it is.  Of texts of 5 to 16 beams fewer than one in a
+// thousand goes that way; a batch of 64 of 5 beams over 50257 scores with one of them
+// takes 182 us in place of 22 (one workgroup's exponentials in 64 bits).
 //   sums, lists  the text's, [W, parts] and [W, parts, K]
+//   scores, sw   its first beam's scores, and the beams' stride
 //   totals, ended and the outputs  the text's rows
-template <int WAVES>
-__device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* lists, int parts, const float* totals,
-                                           const unsigned char* ended, const Stops& stops, int W, int V, int K,
-                                           float* new_totals, int64_t* parents, int64_t* tokens,
-                                           unsigned char* new_ended) {
+template <int WAVES, typename E>
+__device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* lists, int parts, const E* scores,
+                                           int64_t sw, float slack, const float* totals, const unsigned char* ended,
+                                           const Stops& stops, int W, int V, int K, float* new_totals,
+                                           int64_t* parents, int64_t* tokens, unsigned char* new_ended) {
   __shared__ double level[kMaxBeams];  // L
   __shared__ double from[kMaxBeams];   // the beam's total; -inf where it cannot go on
+  __shared__ float tops[kMaxBeams];    // its largest score
   __shared__ bool over[kMaxBeams];     // ended, and goes on
   __shared__ Key<3> gathered[kCandidates];
-  __shared__ int count;
+  __shared__ int count, again;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (threadIdx.x == 0) count = 0;
+  float highest = lane < W ? totals[lane] : 0.f;  // the largest total above 0
+  highest = highest > 0.f && highest < __builtin_inff() ? highest : 0.f;
   for (int w = wave; w < W; w += WAVES) {
     const PartSum* part = sums + w * parts;
     const PartSum mine = lane < parts ? part[lane] : PartSum{kNegInf, 0.f};
@@ -414,9 +454,11 @@ __device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* 
       const bool alive = isfinite(total) && (end || (isfinite(l) && top != kNegInf));
       level[w] = l;
       from[w] = alive ? total : (double)kNegInf;
+      tops[w] = top;
       over[w] = alive && end;
     }
   }
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(highest > 0.f) != 0, 0)) highest = wave_max_dpp(highest);
   __syncthreads();
   const int stop = stops.n ? stops.token[0] : 0;
   // The head'th candidate of a list: its value, and its token (V: none).  A beam
@@ -448,64 +490,113 @@ __device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* 
     const uint64_t order = order_key64(value);
     return Key<3>{{(uint32_t)(order >> 32), (uint32_t)order, ~(uint32_t)((list / parts) * V + v)}};
   };
+  auto value_of = [](Key<3> k) { return key64_value(((uint64_t)k.w[0] << 32) | k.w[1]); };
+  auto beam_of = [&](const Key<3>& k) { return (int)(~k.w[2] / (uint32_t)V); };
   const int many = W * parts, all = many * K;
-  Key<1> heads{{0}};
-  for (int c = lane; c < max(many, min(all, 64)); c += 64) {
-    int v;
-    const double value = candidate(c % many, c / many, v);
-    if (v < V) heads.w[0] = max(heads.w[0], order_key((float)value + 0.f));
-  }
-  wave_sort(heads);
-  const uint32_t bound = key_of_lane(heads, K - 1).w[0];
-  for (int c0 = wave * 64; c0 < all; c0 += 64 * WAVES) {
-    const int list = (c0 + lane) % many, head = (c0 + lane) / many;
-    int v = V;
-    double value = 0.;
-    if (c0 + lane < all) value = candidate(list, head, v);
-    const bool in = v < V && order_key((float)value + 0.f) >= bound;
-    const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
-    if (mask == 0) continue;
-    int first = 0;
-    if (lane == 0) first = atomicAdd(&count, __builtin_popcountll(mask));
-    first = __builtin_amdgcn_readfirstlane(first) + below_me(mask);
-    if (in && first < kCandidates) gathered[first] = key_of(list, v, value);
-  }
-  __syncthreads();
-  if (wave != 0) return;
-  const int found = count;
-  const bool held = found <= kCandidates;  // else every candidate again, against the best so far
-  const int end = held ? found : all;
-  Key<3> best{{0, 0, 0}}, last{{0, 0, 0}};
-  for (int c0 = 0; c0 < end; c0 += 64) {
-    Key<3> k{{0, 0, 0}};
-    if (c0 + lane < end) {
-      if (held) {
-        k = gathered[c0 + lane];
-      } else {
-        int v;
-        const int list = (c0 + lane) % many;
-        const double value = candidate(list, (c0 + lane) / many, v);
-        if (v < V) k = key_of(list, v, value);
-      }
+  // Selects the next beams with L as it stands (exact: in 64 bits) and writes them;
+  // returns true, with nothing written, where L does not decide them.
+  auto select = [&](auto exact_) {
+    constexpr bool exact = decltype(exact_)::value;
+    // How far apart the values of two beams' candidates are told apart: the errors of
+    // both L, and some steps in 64 bits of the largest number in their sums (a value
+    // itself where the totals are none above 0).  In FP32 the values' rounding beside.
+    const float apart = exact ? 0.f : 2.f * slack + 0x1p-47f * highest;
+    auto margin = [&](double value) { return fma(0x1p-48, fabs(value), (double)apart); };
+    auto margin32 = [&](float value) { return fmaf(0x1p-22f, fabsf(value), apart); };
+    Key<1> heads{{0}};
+    for (int c = lane; c < max(many, min(all, 64)); c += 64) {
+      int v;
+      const double value = candidate(c % many, c / many, v);
+      if (v < V) heads.w[0] = max(heads.w[0], order_key((float)value + 0.f));
     }
-    if (__builtin_amdgcn_ballot_w64(above(k, last)) == 0) continue;
-    wave_sort_first(k, end - c0);
-    if (c0 == 0)
-      best = k;
-    else
-      merge_lists(best, backwards(k));
-    last = key_of_lane(best, K - 1);
-  }
-  if (lane < K) {
-    const uint32_t flat = ~best.w[2];
-    const int w = (int)(flat / (uint32_t)V), v = (int)(flat % (uint32_t)V);
-    bool stopped = ended && ended[w];
-    for (int i = 0; i < stops.n; ++i) stopped = stopped || stops.token[i] == v;
-    new_totals[lane] = (float)key64_value(((uint64_t)best.w[0] << 32) | best.w[1]);
-    parents[lane] = w;
-    tokens[lane] = v;
-    new_ended[lane] = stopped ? 1 : 0;
-  }
+    wave_sort(heads);
+    const uint32_t kth = key_of_lane(heads, K - 1).w[0];
+    // the K-th value is not below kth but for its rounding; what is close to it counts too
+    const float bound = kth ? key_value(kth) : kNegInf, low = bound - margin32(bound);
+    for (int c0 = wave * 64; c0 < all; c0 += 64 * WAVES) {
+      const int list = (c0 + lane) % many, head = (c0 + lane) / many;
+      int v = V;
+      double value = 0.;
+      if (c0 + lane < all) value = candidate(list, head, v);
+      const bool in = v < V && (float)value >= low;
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
+      if (mask == 0) continue;
+      int first = 0;
+      if (lane == 0) first = atomicAdd(&count, __builtin_popcountll(mask));
+      first = __builtin_amdgcn_readfirstlane(first) + below_me(mask);
+      if (in && first < kCandidates) gathered[first] = key_of(list, v, value);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      const int found = count;
+      const bool held = found <= kCandidates;  // else every candidate again, against the best so far
+      const int end = held ? found : all;
+      auto key_at = [&](int c) {
+        if (c >= end) return Key<3>{{0, 0, 0}};
+        if (held) return gathered[c];
+        int v;
+        const int list = c % many;
+        const double value = candidate(list, c / many, v);
+        return v < V ? key_of(list, v, value) : Key<3>{{0, 0, 0}};
+      };
+      Key<3> best{{0, 0, 0}}, last{{0, 0, 0}};
+      for (int c0 = 0; c0 < end; c0 += 64) {
+        Key<3> k = key_at(c0 + lane);
+        if (__builtin_amdgcn_ballot_w64(above(k, last)) == 0) continue;
+        wave_sort_first(k, end - c0);
+        if (c0 == 0)
+          best = k;
+        else
+          merge_lists(best, backwards(k));
+        last = key_of_lane(best, K - 1);
+      }
+      // Neighbours of two beams that are close, among the K and beyond (all of them
+      // where at most 64 were gathered): hardly ever any.
+      const int parent = beam_of(best), next_parent = (int)next_lane((uint32_t)parent);
+      const double value = value_of(best);
+      const float total = (float)value;
+      const float drop = total - __uint_as_float(next_lane(__float_as_uint(total)));
+      bool close = lane + 1 < min(end, 64) && parent != next_parent && drop <= margin32(total);
+      bool repeat = false;
+      if (__builtin_expect(!exact && (__builtin_amdgcn_ballot_w64(close) != 0 || end > 64), 0)) {
+        // In 64 bits: both among the K, or one at the K-th value?  Values of ended beams
+        // are exact, and those at -inf equal.
+        const double next = value_of({{next_lane(best.w[0]), next_lane(best.w[1]), 0}});
+        close = close && lane < K - 1 && value - next <= margin(value) && !(over[parent] && over[next_parent]);
+        const double least = value_of(last);
+        const int owner = beam_of(last);
+        if (least > (double)kNegInf)
+          for (int c0 = 0; c0 < end; c0 += 64) {
+            const Key<3> k = key_at(c0 + lane);
+            if ((k.w[0] | k.w[1] | k.w[2]) != 0 && above(last, k) && least - value_of(k) <= margin(least)) {
+              const int beam = beam_of(k);
+              close = close || (beam != owner && !(over[beam] && over[owner]));
+            }
+          }
+        repeat = __builtin_amdgcn_ballot_w64(close) != 0;
+      }
+      if (exact || __builtin_expect(!repeat, 1)) {
+        if (lane < K) {
+          const int v = (int)(~best.w[2] % (uint32_t)V);
+          bool stopped = ended && ended[parent];
+          for (int i = 0; i < stops.n; ++i) stopped = stopped || stops.token[i] == v;
+          new_totals[lane] = total;
+          parents[lane] = parent;
+          tokens[lane] = v;
+          new_ended[lane] = stopped ? 1 : 0;
+        }
+      }
+      if (!exact && lane == 0) again = repeat;
+    }
+    if (exact) return false;
+    __syncthreads();
+    return __builtin_expect(again, 0) != 0;
+  };
+  if (!select(std::false_type())) return;
+  exact_levels<WAVES>(scores, sw, W, V, from, over, tops, level);
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  select(std::true_type());
 }
 
 // The arguments of text i: its rows of each array.
@@ -517,19 +608,22 @@ struct Beams {
   unsigned char* new_ended;
 };
 
-template <int WAVES>
+template <int WAVES, typename E>
 __device__ __forceinline__ void next_beams_of(int64_t i, const PartSum* sums, const uint64_t* lists, int parts,
-                                              const Beams& a, const Stops& stops, int W, int V, int K) {
-  next_beams<WAVES>(sums, lists, parts, a.totals + i * W, a.ended ? a.ended + i * W : nullptr, stops, W, V, K,
-                    a.new_totals + i * K, a.parents + i * K, a.tokens + i * K, a.new_ended + i * K);
+                                              const E* scores, int64_t sn, int64_t sw, float slack, const Beams& a,
+                                              const Stops& stops, int W, int V, int K) {
+  next_beams<WAVES>(sums, lists, parts, scores + i * sn, sw, slack, a.totals + i * W,
+                    a.ended ? a.ended + i * W : nullptr, stops, W, V, K, a.new_totals + i * K, a.parents + i * K,
+                    a.tokens + i * K, a.new_ended + i * K);
 }
 
-template <int WAVES>
+template <int WAVES, typename E>
 __global__ __launch_bounds__(64 * WAVES) void beam_merge(const PartSum* __restrict__ sums,
-                                                         const uint64_t* __restrict__ lists, int parts, Beams a,
-                                                         Stops stops, int W, int V, int K) {
+                                                         const uint64_t* __restrict__ lists, int W, int V, int K,
+                                                         int parts, const E* __restrict__ scores, int64_t sn,
+                                                         int64_t sw, float slack, Beams a, Stops stops) {
   const int64_t i = blockIdx.x, first = i * W * parts;
-  next_beams_of<WAVES>(i, sums + first, lists + first * K, parts, a, stops, W, V, K);
+  next_beams_of<WAVES>(i, sums + first, lists + first * K, parts, scores, sn, sw, slack, a, stops, W, V, K);
 }
 
 // A text of few scores in one launch: a wavefront a part, the lists in LDS.
@@ -537,7 +631,8 @@ constexpr int kTextWaves = 16, kTextItems = 32;
 
 template <typename E>
 __global__ __launch_bounds__(64 * kTextWaves) void beam_text(const E* __restrict__ scores, int64_t sn, int64_t sw,
-                                                             Beams a, Stops stops, int W, int V, int K, int parts) {
+                                                             int W, int V, int K, int parts, float slack, Beams a,
+                                                             Stops stops) {
   __shared__ uint64_t gathered[kTextWaves][kGathered];
   __shared__ uint64_t lists[kTextWaves * kMaxBeams];
   __shared__ PartSum sums[kTextWaves];
@@ -546,9 +641,8 @@ __global__ __launch_bounds__(64 * kTextWaves) void beam_text(const E* __restrict
     part_list<E, kTextItems>(scores + (int64_t)blockIdx.x * sn + (int64_t)(w / parts) * sw, V, w % parts, K,
                              gathered[w], sums + w, lists + w * K);
   __syncthreads();
-  next_beams_of<kTextWaves>(blockIdx.x, sums, lists, parts, a, stops, W, V, K);
+  next_beams_of<kTextWaves>(blockIdx.x, sums, lists, parts, scores, sn, sw, slack, a, stops, W, V, K);
 }
-
 
 // The parts of a beam in beam_text, or 0 where the text takes two launches: where a
 // workgroup's wavefronts do not hold its parts, or the texts outnumber the compute
@@ -559,6 +653,13 @@ int text_parts(int n, int W, int V) {
   const int64_t parts = ((int64_t)V + 64 * kTextItems - 1) / (64 * kTextItems);
   return W * parts <= kTextWaves && n <= compute_units() ? (int)parts : 0;
 }
+
+// What the FP32 sums may put a beam's L = log S off by.  A term exp(x - top): the
+// argument's rounding, log2 e's and their product's, at most 2.3 2^-24 |x - top|, whose
+// mean over the terms is at most log V (their entropy less log S); the exponential, one
+// step, 2 2^-24; and a part's 24 additions in turn (at most 18 of a lane's, 6 across
+// the lanes), 2^-24 each of terms of one sign.  The parts are joined in 64 bits.
+float level_slack(int V) { return (float)((3. * std::log((double)V) + 33.) * 0x1p-24); }
 
 // Scores a lane of a part: 64 where the parts of 4096 fill the GPU, 16 where
 // they do not, so that few rows are spread over it.
@@ -614,13 +715,14 @@ extern "C" int wptv_beam_step(const void* scores, int64_t scores_stride_n, int64
   if (workspace_bytes < need)
     return fail(WPTV_E_INVALID, "beam_step: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   const Beams beams{totals, ended, new_totals, parents, tokens, new_ended};
+  const float slack = level_slack(V);
   if (const int parts = text_parts(n, W, V)) {
     if (scores_dtype == WPTV_F32)
       beam_text<<<n, 64 * kTextWaves, 0, stream>>>(static_cast<const float*>(scores), scores_stride_n, scores_stride_w,
-                                                   beams, s, W, V, K, parts);
+                                                   W, V, K, parts, slack, beams, s);
     else
       beam_text<<<n, 64 * kTextWaves, 0, stream>>>(static_cast<const unsigned short*>(scores), scores_stride_n,
-                                                   scores_stride_w, beams, s, W, V, K, parts);
+                                                   scores_stride_w, W, V, K, parts, slack, beams, s);
     return launched("beam_text");
   }
   const int items = part_items((int64_t)n * W, V), parts = (int)(((int64_t)V + 64 * items - 1) / (64 * items));
@@ -638,9 +740,15 @@ extern "C" int wptv_beam_step(const void* scores, int64_t scores_stride_n, int64
 #undef WPTV_PARTS
   const int launch = launched("beam_parts");
   if (launch != WPTV_OK) return launch;
-  if ((int64_t)W * parts * K <= 4096)
-    beam_merge<8><<<n, 512, 0, stream>>>(sums, lists, parts, beams, s, W, V, K);
-  else
-    beam_merge<16><<<n, 1024, 0, stream>>>(sums, lists, parts, beams, s, W, V, K);
+#define WPTV_MERGE(WAVES, E)                                                                                       \
+  beam_merge<WAVES, E><<<n, 64 * WAVES, 0, stream>>>(sums, lists, W, V, K, parts, static_cast<const E*>(scores),   \
+                                                     scores_stride_n, scores_stride_w, slack, beams, s)
+  const bool few = (int64_t)W * parts * K <= 4096;
+  if (scores_dtype == WPTV_F32) {
+    if (few) WPTV_MERGE(8, float); else WPTV_MERGE(16, float);
+  } else {
+    if (few) WPTV_MERGE(8, unsigned short); else WPTV_MERGE(16, unsigned short);
+  }
+#undef WPTV_MERGE
   return launched("beam_merge");
 }

@@ -313,7 +313,9 @@ def beam_step(scores, totals, ended=None, stops=(), beams=None):
     token; totals (n, W) FP32: each beam's summed log-probability so far (-inf
     for a place that holds no beam, as all but one at a text's start).  A
     candidate's value is its beam's total plus the log-softmax of its score,
-    ranked in 64 bits, equal values to the lowest beam, then token.  stops: the
+    ranked in 64 bits, equal values to the lowest beam, then token (whatever the
+    batch; the totals themselves are off by their rounding and at most
+    (3 ln V + 33) 2^-24, FP32 sums of exponentials).  stops: the
     token ids that end a beam (at most 16); ended (n, W) bool: such a beam
     goes on as one candidate, its first stop token at its own total.  A beam
     whose total is not finite, or whose scores hold a NaN or +inf or nothing
