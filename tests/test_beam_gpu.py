@@ -289,3 +289,28 @@ def test_the_beams_of_a_text_do_not_depend_on_the_batch(device):
         got = sampling.beam_step(scores[:n], totals[:n])
         for a, b in zip(got[1:], whole[1:]):
             assert torch.equal(a, b[:n])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n, V", [(2, 40), (2, 700), (2, 33000), (400, 4100)])
+@pytest.mark.parametrize("kind", ["rising", "falling", "mixed", "signs", "far total"])
+def test_scores_apart_whose_values_are_equal(device, kind, n, V, dtype):
+    """Scores so small, or totals so large, that 64 bits hold the values of many
+    of a beam's scores as one: equal values fall to the lowest tokens."""
+    W = 3
+    g = torch.Generator().manual_seed(V)
+    ramp = torch.arange(V, dtype=torch.float32) * 1e-20
+    shuffled = ramp[torch.randperm(V, generator=g)]
+    scores = {"rising": ramp, "falling": -ramp, "signs": torch.where(torch.rand(V, generator=g) < 0.5, shuffled, -shuffled),
+              "mixed": torch.where(torch.rand(V, generator=g) < 4 / V, torch.rand(V, generator=g) + 1, shuffled),
+              "far total": 1e-3 * torch.randn(V, generator=g)}[kind].expand(n, W, V).contiguous().to(dtype)
+    totals = torch.tensor([-1.0, -2.5, -3.0] if kind != "far total" else [-1e30, -1.5e30, -1e30]).expand(n, W).contiguous()
+    totals[0] = totals[0].flip(0)
+    totals[1, 1] = totals[1, 0]
+    some = slice(0, 3)  # of the larger batch, as many as plain loops read in time
+    for K in (1, 3, 15, 64):
+        print(f"beam_step {kind} n={n} V={V} K={K} {dtype}", flush=True)
+        got = [x.cpu()[some] for x in sampling.beam_step(scores.to(device), totals.to(device), beams=K)]
+        expected = oracle.beam_step(scores[some], totals[some], beams=K)
+        assert torch.equal(got[1], expected[1]) and torch.equal(got[2], expected[2])
+        totals_close(got[0], expected[0], V)

@@ -4,7 +4,7 @@
 // A text's candidates are its W beams continued by each of V tokens, of value
 //   total[w] + (x[w, v] - L[w]),  L[w] = log sum_v exp x[w, v]
 // in 64 bits; the K largest are the next beams, equal values to the lowest
-// w V + v.  Within a beam the value grows with x, so nothing has to be
+// w V + v.  Within a beam the value does not fall with x, so nothing has to be
 // normalised before it is selected: each score is read once.
 //   beam_parts  a wavefront a part of a beam's scores, all of it in registers:
 //               the part's maximum, its sum of exponentials, and its K largest
@@ -366,8 +366,6 @@ __global__ __launch_bounds__(64 * kPartWaves) void beam_parts(const E* __restric
 
 // ---- the text's next beams -----------------------------------------------------------
 
-constexpr int kCandidates = 512;  // that a text gathers
-
 __device__ __forceinline__ double wave_sum_f64(double x) {
   auto add = [&](auto m) {
     const uint64_t u = (uint64_t)__double_as_longlong(x);
@@ -414,9 +412,12 @@ __device__ __forceinline__ void exact_levels(const E* scores, int64_t sw, int W,
 // first one.  Values formed with the FP32 sums' L are off by at most `slack`; where a
 // candidate of another beam comes that close to one that is taken, which of them is
 // larger (and which is the K-th) is decided with L in 64 bits.  Within a beam L is the
-// same and the order right as it is.  Of texts of 5 to 16 beams fewer than one in a
-// thousand goes that way; a batch of 64 of 5 beams over 50257 scores with one of them
-// takes 182 us in place of 22 (one workgroup's exponentials in 64 bits).
+// same and the order right as it is, but for scores whose values 64 bits hold as one
+// (scores below 1e-7, totals of 1e9): where all of a list may be taken and its last
+// value is also that of the next lower score, every candidate is ranked by its value.
+// Of texts of 5 to 16 beams fewer than one in a thousand is decided in 64 bits; a batch
+// of 64 of 5 beams over 50257 scores with one of them takes 182 us in place of 22 (one
+// workgroup's exponentials in 64 bits).
 //   sums, lists  the text's, [W, parts] and [W, parts, K]
 //   scores, sw   its first beam's scores, and the beams' stride
 //   totals, ended and the outputs  the text's rows
@@ -429,10 +430,11 @@ __device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* 
   __shared__ double from[kMaxBeams];   // the beam's total; -inf where it cannot go on
   __shared__ float tops[kMaxBeams];    // its largest score
   __shared__ bool over[kMaxBeams];     // ended, and goes on
+  constexpr int kCandidates = 64 * WAVES;  // that a text gathers
   __shared__ Key<3> gathered[kCandidates];
-  __shared__ int count, again;
+  __shared__ int count, again, crowded;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (threadIdx.x == 0) count = 0;
+  if (threadIdx.x == 0) count = crowded = 0;
   float highest = lane < W ? totals[lane] : 0.f;  // the largest total above 0
   highest = highest > 0.f && highest < __builtin_inff() ? highest : 0.f;
   for (int w = wave; w < W; w += WAVES) {
@@ -461,18 +463,21 @@ __device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* 
   if (__builtin_expect(__builtin_amdgcn_ballot_w64(highest > 0.f) != 0, 0)) highest = wave_max_dpp(highest);
   __syncthreads();
   const int stop = stops.n ? stops.token[0] : 0;
-  // The head'th candidate of a list: its value, and its token (V: none).  A beam
+  // The head'th candidate of a list: its value, its token (V: none) and its score's
+  // order key (0: not by a score).  A beam
   // that has ended or cannot go on has one list: the stop token at the beam's
   // total, the others at -inf.
-  auto candidate = [&](int list, int head, int& v) {
+  auto candidate = [&](int list, int head, int& v, uint32_t& order) {
     const int w = list / parts, part = list % parts;
     const double total = from[w];
     v = V;
+    order = 0;
     if (total > (double)kNegInf && !over[w]) {
       const uint64_t key = lists[(w * parts + part) * K + head];
       if (key == 0) return 0.;
       v = (int)~(uint32_t)key;
-      return total + ((double)key_value((uint32_t)(key >> 32)) - level[w]);
+      order = (uint32_t)(key >> 32);
+      return total + ((double)key_value(order) - level[w]);
     }
     if (part != 0) return 0.;
     if (!over[w]) {
@@ -486,15 +491,44 @@ __device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* 
     v = min(v, V);
     return (double)kNegInf;
   };
-  auto key_of = [&](int list, int v, double value) {
+  auto key_of = [&](uint32_t flat, double value) {
     const uint64_t order = order_key64(value);
-    return Key<3>{{(uint32_t)(order >> 32), (uint32_t)order, ~(uint32_t)((list / parts) * V + v)}};
+    return Key<3>{{(uint32_t)(order >> 32), (uint32_t)order, ~flat}};
   };
+  auto flat_of = [&](int list, int v) { return (uint32_t)((list / parts) * V + v); };
   auto value_of = [](Key<3> k) { return key64_value(((uint64_t)k.w[0] << 32) | k.w[1]); };
   auto beam_of = [&](const Key<3>& k) { return (int)(~k.w[2] / (uint32_t)V); };
   const int many = W * parts, all = many * K;
-  // Selects the next beams with L as it stands (exact: in 64 bits) and writes them;
-  // returns true, with nothing written, where L does not decide them.
+  // wave 0: writes the text's rows
+  auto write = [&](const Key<3>& best, int parent, float total) {
+    if (lane >= K) return;
+    const int v = (int)(~best.w[2] % (uint32_t)V);
+    bool stopped = ended && ended[parent];
+    for (int i = 0; i < stops.n; ++i) stopped = stopped || stops.token[i] == v;
+    new_totals[lane] = total;
+    parents[lane] = parent;
+    tokens[lane] = v;
+    new_ended[lane] = stopped ? 1 : 0;
+  };
+  // The largest of the keys key_at(c), c < end, by wave 0: the K first lanes' (all of
+  // them in order where there are at most 64), and the K-th.
+  auto largest = [&](int end, Key<3>& best, Key<3>& last, auto&& key_at) {
+    best = last = Key<3>{{0, 0, 0}};
+    for (int c0 = 0; c0 < end; c0 += 64) {
+      Key<3> k = key_at(c0 + lane);
+      if (__builtin_amdgcn_ballot_w64(above(k, last)) == 0) continue;
+      wave_sort_first(k, end - c0);
+      if (c0 == 0)
+        best = k;
+      else
+        merge_lists(best, backwards(k));
+      last = key_of_lane(best, K - 1);
+    }
+  };
+  // Selects the next beams with L as it stands (exact: in 64 bits) from the lists and
+  // writes them; with nothing written returns kLevels where L does not decide them,
+  // kScan where the lists may not hold them.
+  constexpr int kLevels = 1, kScan = 2;
   auto select = [&](auto exact_) {
     constexpr bool exact = decltype(exact_)::value;
     // How far apart the values of two beams' candidates are told apart: the errors of
@@ -506,7 +540,8 @@ __device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* 
     Key<1> heads{{0}};
     for (int c = lane; c < max(many, min(all, 64)); c += 64) {
       int v;
-      const double value = candidate(c % many, c / many, v);
+      uint32_t order;
+      const double value = candidate(c % many, c / many, v, order);
       if (v < V) heads.w[0] = max(heads.w[0], order_key((float)value + 0.f));
     }
     wave_sort(heads);
@@ -516,15 +551,22 @@ __device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* 
     for (int c0 = wave * 64; c0 < all; c0 += 64 * WAVES) {
       const int list = (c0 + lane) % many, head = (c0 + lane) / many;
       int v = V;
+      uint32_t order = 0;
       double value = 0.;
-      if (c0 + lane < all) value = candidate(list, head, v);
+      if (c0 + lane < all) value = candidate(list, head, v, order);
       const bool in = v < V && (float)value >= low;
       const uint64_t mask = __builtin_amdgcn_ballot_w64(in);
       if (mask == 0) continue;
       int first = 0;
       if (lane == 0) first = atomicAdd(&count, __builtin_popcountll(mask));
       first = __builtin_amdgcn_readfirstlane(first) + below_me(mask);
-      if (in && first < kCandidates) gathered[first] = key_of(list, v, value);
+      if (in && first < kCandidates) gathered[first] = key_of(flat_of(list, v), value);
+      if (__builtin_expect(in && head == K - 1 && order != 0, 0)) {
+        // A whole list may be taken.  What it leaves out has no larger value, but an
+        // equal one, and a lower token, where 64 bits hold a lower score's as the same.
+        const double total = from[list / parts], below = total + ((double)key_value(order - 1) - level[list / parts]);
+        if (value - below <= 0x1p-49 * (fabs(value) + fabs(total))) crowded = 1;
+      }
     }
     __syncthreads();
     if (wave == 0) {
@@ -535,21 +577,13 @@ __device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* 
         if (c >= end) return Key<3>{{0, 0, 0}};
         if (held) return gathered[c];
         int v;
+        uint32_t order;
         const int list = c % many;
-        const double value = candidate(list, c / many, v);
-        return v < V ? key_of(list, v, value) : Key<3>{{0, 0, 0}};
+        const double value = candidate(list, c / many, v, order);
+        return v < V ? key_of(flat_of(list, v), value) : Key<3>{{0, 0, 0}};
       };
-      Key<3> best{{0, 0, 0}}, last{{0, 0, 0}};
-      for (int c0 = 0; c0 < end; c0 += 64) {
-        Key<3> k = key_at(c0 + lane);
-        if (__builtin_amdgcn_ballot_w64(above(k, last)) == 0) continue;
-        wave_sort_first(k, end - c0);
-        if (c0 == 0)
-          best = k;
-        else
-          merge_lists(best, backwards(k));
-        last = key_of_lane(best, K - 1);
-      }
+      Key<3> best, last;
+      largest(end, best, last, key_at);
       // Neighbours of two beams that are close, among the K and beyond (all of them
       // where at most 64 were gathered): hardly ever any.
       const int parent = beam_of(best), next_parent = (int)next_lane((uint32_t)parent);
@@ -575,28 +609,45 @@ __device__ __forceinline__ void next_beams(const PartSum* sums, const uint64_t* 
           }
         repeat = __builtin_amdgcn_ballot_w64(close) != 0;
       }
-      if (exact || __builtin_expect(!repeat, 1)) {
-        if (lane < K) {
-          const int v = (int)(~best.w[2] % (uint32_t)V);
-          bool stopped = ended && ended[parent];
-          for (int i = 0; i < stops.n; ++i) stopped = stopped || stops.token[i] == v;
-          new_totals[lane] = total;
-          parents[lane] = parent;
-          tokens[lane] = v;
-          new_ended[lane] = stopped ? 1 : 0;
-        }
-      }
-      if (!exact && lane == 0) again = repeat;
+      const int next = __builtin_expect(crowded, 0) ? kScan : repeat ? kLevels : 0;
+      if (__builtin_expect(next == 0, 1)) write(best, parent, total);
+      if (lane == 0) again = next;
     }
-    if (exact) return false;
     __syncthreads();
-    return __builtin_expect(again, 0) != 0;
+    return __builtin_expect(again, 0);
   };
-  if (!select(std::false_type())) return;
+  const int next = select(std::false_type());
+  if (next == 0) return;
   exact_levels<WAVES>(scores, sw, W, V, from, over, tops, level);
-  if (threadIdx.x == 0) count = 0;
+  if (next == kLevels) {
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    if (select(std::true_type()) == 0) return;
+  }
+  // Every candidate, by its value: each wavefront's K largest, then the largest of these.
+  const uint32_t flats = (uint32_t)W * V;
+  Key<3> best{{0, 0, 0}}, last{{0, 0, 0}};
+  for (uint32_t f0 = wave * 64; f0 < flats; f0 += 64 * WAVES) {
+    Key<3> k{{0, 0, 0}};
+    if (f0 + lane < flats) {
+      const int w = (int)((f0 + lane) / (uint32_t)V), v = (int)((f0 + lane) % (uint32_t)V);
+      double value = (double)kNegInf;
+      if (over[w])
+        value = v == stop ? from[w] : value;
+      else if (from[w] > (double)kNegInf)
+        value = from[w] + ((double)load_f32(scores + w * sw + v) - level[w]);
+      k = key_of(f0 + lane, value);
+    }
+    if (__builtin_amdgcn_ballot_w64(above(k, last)) == 0) continue;
+    wave_sort(k);
+    merge_lists(best, backwards(k));
+    last = key_of_lane(best, K - 1);
+  }
+  gathered[threadIdx.x] = best;
   __syncthreads();
-  select(std::true_type());
+  if (wave != 0) return;
+  largest(kCandidates, best, last, [&](int c) { return gathered[c]; });
+  write(best, beam_of(best), (float)value_of(best));
 }
 
 // The arguments of text i: its rows of each array.
