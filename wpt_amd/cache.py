@@ -77,6 +77,7 @@ class Cache:
         self.routes = None
         self.weights = self.evicted = None
         self._read = []  # a weighted cache's undoable reading: (weights' row, layer, q, positions, lse, scale, counts)
+        self._captured = False  # whether that reading was made under stream capture
         if weighted:
             if not self.growing:
                 raise ValueError("a weighted cache has at least one table that grows with the text")
@@ -152,6 +153,7 @@ class Cache:
         if self.weights is not None and not self._read:
             raise ValueError("the weights of the reading to undo are not here: a captured undoable reading of a weighted "
                              "cache is captured together with its undo")
+        self._together()
         _lengths(self.lengths, self.before, kept, undo=True)
         self.settle(kept)
         self.pending = False
@@ -173,6 +175,7 @@ class Cache:
         undoable reading's when undo tells how many tokens were kept."""
         reading = (self.growing.index(layer), layer, q, positions, lse, scale, counts)
         if undoable:
+            self._captured = torch.cuda.is_current_stream_capturing()
             self._read.append(reading)
         else:
             self._add(reading, counts, self.lengths)
@@ -182,9 +185,19 @@ class Cache:
         kernels.add_attention_weights(q, self.tables[layer][..., :q.shape[-1]], positions, lse, scale, self.weights[at],
                                       counts=counts, start=start)
 
+    def _together(self):
+        """Refuses to add an undoable reading's weights in a capture that it was
+        not made in, where every replay would add them again, or a captured
+        reading's outside its capture, where they were never computed."""
+        if self._read and self._captured != torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured undoable reading of a weighted cache is captured together with its undo"
+                               if self._captured else
+                               "an undoable reading of this weighted cache is pending: undo it before capturing a step")
+
     def settle(self, kept=None):
         """Adds the weights of an undoable reading of which kept tokens stay
         (None: all of them, when another reading follows it)."""
+        self._together()
         for reading in self._read:
             self._add(reading, reading[-1] if kept is None else kept, self.before)
         self._read = []
@@ -203,7 +216,7 @@ class Cache:
         copy.pending, copy.bound, copy.routes = False, self.bound, None
         copy.weights = None if self.weights is None else self.weights[:, index]
         copy.evicted = None if self.evicted is None else self.evicted[index]
-        copy._read = []
+        copy._read, copy._captured = [], False
         return copy
 
     def reorder(self, parents):
