@@ -97,3 +97,16 @@ def test_a_captured_reading_is_not_added_outside_its_capture(host):
     with pytest.raises(RuntimeError, match="captured together"):
         read(cache, 2, 1, undoable=False)
     assert not host.added
+
+
+def test_a_reading_that_failed_half_way_leaves_nothing_to_add(host):
+    cache = weighted()
+    read(cache, 1, 3, undoable=False)
+    counts = torch.tensor([2, 2])
+    cache.weigh(0, torch.full((2, 2, 1, 4), 9.0), None, None, 1.0, counts, True)  # an error before the next layer
+    read(cache, 2, 1, undoable=False)
+    assert [x[0] for x in host.added] == [1, 1, 2, 2]
+    cache.weigh(0, torch.full((2, 2, 1, 4), 9.0), None, None, 1.0, counts, True)
+    read(cache, 3, 2, undoable=True)
+    cache.undo(torch.tensor([1, 1]))
+    assert [x[0] for x in host.added[4:]] == [3, 3]

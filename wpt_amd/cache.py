@@ -196,7 +196,11 @@ class Cache:
 
     def settle(self, kept=None):
         """Adds the weights of an undoable reading of which kept tokens stay
-        (None: all of them, when another reading follows it)."""
+        (None: all of them, when another reading follows it).  What a reading
+        that failed before its end has left is dropped: the lengths before it
+        are not in `before`, and none of its tokens is in the cache."""
+        if not self.pending:
+            self._read = []
         self._together()
         for reading in self._read:
             self._add(reading, reading[-1] if kept is None else kept, self.before)
