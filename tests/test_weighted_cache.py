@@ -110,3 +110,9 @@ def test_a_reading_that_failed_half_way_leaves_nothing_to_add(host):
     read(cache, 3, 2, undoable=True)
     cache.undo(torch.tensor([1, 1]))
     assert [x[0] for x in host.added[4:]] == [3, 3]
+    read(cache, 4, 2, undoable=True)
+    cache.settle()  # the next reading begins: the one before is whole
+    cache.weigh(0, torch.full((2, 2, 1, 4), 9.0), None, None, 1.0, counts, True)
+    with pytest.raises(ValueError, match="not here"):
+        cache.undo(torch.tensor([1, 1]))
+    assert [x[0] for x in host.added[6:]] == [4, 4]

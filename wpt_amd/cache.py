@@ -78,6 +78,7 @@ class Cache:
         self.weights = self.evicted = None
         self._read = []  # a weighted cache's undoable reading: (weights' row, layer, q, positions, lse, scale, counts)
         self._captured = False  # whether that reading was made under stream capture
+        self._reading = []  # the same of a reading that has not finished
         if weighted:
             if not self.growing:
                 raise ValueError("a weighted cache has at least one table that grows with the text")
@@ -145,6 +146,8 @@ class Cache:
         _lengths(self.lengths, self.before if undoable else None, counts, undo=False)
         self.pending = bool(undoable)
         self.bound += width
+        self._read, self._reading = self._reading, []
+        self._captured = bool(self._read) and torch.cuda.is_current_stream_capturing()
 
     def undo(self, kept):
         """Back to the lengths before the last undoable reading, plus kept."""
@@ -175,8 +178,7 @@ class Cache:
         undoable reading's when undo tells how many tokens were kept."""
         reading = (self.growing.index(layer), layer, q, positions, lse, scale, counts)
         if undoable:
-            self._captured = torch.cuda.is_current_stream_capturing()
-            self._read.append(reading)
+            self._reading.append(reading)
         else:
             self._add(reading, counts, self.lengths)
 
@@ -197,11 +199,10 @@ class Cache:
     def settle(self, kept=None):
         """Adds the weights of an undoable reading of which kept tokens stay
         (None: all of them, when another reading follows it).  What a reading
-        that failed before its end has left is dropped: the lengths before it
-        are not in `before`, and none of its tokens is in the cache."""
-        if not self.pending:
-            self._read = []
+        that failed before its end has left is dropped: none of its tokens is in
+        the cache."""
         self._together()
+        self._reading = []
         for reading in self._read:
             self._add(reading, reading[-1] if kept is None else kept, self.before)
         self._read = []
@@ -220,7 +221,7 @@ class Cache:
         copy.pending, copy.bound, copy.routes = False, self.bound, None
         copy.weights = None if self.weights is None else self.weights[:, index]
         copy.evicted = None if self.evicted is None else self.evicted[index]
-        copy._read, copy._captured = [], False
+        copy._read, copy._captured, copy._reading = [], False, []
         return copy
 
     def reorder(self, parents):
