@@ -156,3 +156,11 @@ def test_the_definition_of_eviction():
     got = eviction_oracle.attention_weights(q, torch.zeros(1, 3, 1), torch.tensor([[1, 2]]), torch.tensor([[[0.0], [0.0]]]),
                                             1.0, torch.tensor([[5.0, 5.0, 5.0]]), start=torch.tensor([1]))
     assert got.tolist() == [[7.0, 2.0, 1.0]]
+
+
+def test_tables_that_take_a_gradient_are_refused():
+    x = torch.zeros(2, 3, 8, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        kernels.reorder_rows([torch.zeros(2, 3, 8, requires_grad=True)], torch.zeros(1, 2, dtype=torch.long))
+    with pytest.raises(ValueError, match="gradient"):
+        kernels.keep_rows(x, torch.zeros(1, 2, 2, dtype=torch.long), torch.ones(2, dtype=torch.long))

@@ -384,6 +384,8 @@ def _tables(tables, rows, what):
         shape = t.shape
         if len(shape) != 3 or shape[0] != rows or shape[2] == 0:
             raise ValueError(f"{what}: each table must be ({rows}, capacity, width); got {tuple(shape)}")
+        if t.requires_grad:
+            raise ValueError(f"{what}: a table is a cache's state, moved in place: it takes no gradient")
         if device is None:
             device, index = t.device, t.get_device()
         if index < 0 or t.get_device() != index:
