@@ -614,7 +614,9 @@ int wptv_beam_step(const void* scores, int64_t scores_stride_n, int64_t scores_s
  *   leaves its beam as it is.
  *   tables, strides_b, strides_n, capacities, row_bytes  host arrays: each
  *            table's address, its batch rows' and rows' strides in bytes, its
- *            rows a batch row and a row's contiguous bytes, of any type
+ *            rows a batch row and a row's contiguous bytes, of any type.  Tables
+ *            that overlap each other or the lists are refused (of tables whose
+ *            ranges of addresses meet, those whose strides differ)
  *   parents  [n, W] int64; lengths  [n W] int64, or NULL: every row
  *   rows     an upper bound of the lengths (with lengths; rows past it keep
  *            their values).  W <= 64 */

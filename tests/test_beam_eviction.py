@@ -164,3 +164,81 @@ def test_tables_that_take_a_gradient_are_refused():
         kernels.reorder_rows([torch.zeros(2, 3, 8, requires_grad=True)], torch.zeros(1, 2, dtype=torch.long))
     with pytest.raises(ValueError, match="gradient"):
         kernels.keep_rows(x, torch.zeros(1, 2, 2, dtype=torch.long), torch.ones(2, dtype=torch.long))
+
+
+def two_tables(first, second, parents=1 << 40, n=1, W=2):
+    """(status of reorder_rows, of keep_rows) of two tables (address, batch stride, row stride, capacity, row bytes)."""
+    arrays = [(ctypes.c_void_p * 2)(first[0], second[0])] + [longs(a, b) for a, b in zip(first[1:], second[1:])] + [2]
+    # a part of the moves that launches nothing: one beam a text, lists of no rows
+    return (_lib.lib().wptv_reorder_rows(*arrays, parents, None, 10, n * W, 1, None),
+            _lib.lib().wptv_keep_rows(*arrays, parents, 1, 0, 1 << 41, n * W, None))
+
+
+@pytest.mark.parametrize("overlap, first, second", [
+    (True, (A, 640, 64, 10, 64), (A + 63, 640, 64, 10, 64)), (True, (A, 640, 64, 10, 64), (A + 640, 640, 64, 10, 64)),
+    (False, (A, 640, 64, 10, 64), (A + 1280, 640, 64, 10, 64)),
+    (True, (A, 640, 64, 10, 64), (A + 1279, 640, 64, 10, 64)),
+    # the two halves of each row, and one byte more
+    (False, (A, 640, 64, 10, 32), (A + 32, 640, 64, 10, 32)), (True, (A, 640, 64, 10, 33), (A + 32, 640, 64, 10, 32)),
+    (False, (A + 32, 640, 64, 10, 32), (A, 640, 64, 10, 32)), (True, (A + 32, 640, 64, 10, 32), (A, 640, 64, 10, 33)),
+    # the halves again, the second a row further: its first row beside the other's second
+    (False, (A, 1000, 64, 10, 32), (A + 96, 1000, 64, 10, 32)), (True, (A, 1000, 64, 10, 32), (A + 90, 1000, 64, 10, 32)),
+    # in each batch row's block one table behind the other, of other rows
+    (False, (A, 1000, 64, 10, 64), (A + 640, 1000, 36, 10, 36)), (True, (A, 1000, 64, 10, 64), (A + 620, 1000, 36, 10, 36)),
+    # the end of one batch row's block and the start of the next one's
+    (True, (A, 1000, 64, 10, 64), (A + 650, 1000, 36, 10, 36)), (False, (A, 1010, 64, 10, 64), (A + 650, 1010, 36, 10, 36)),
+    # token rows outermost
+    (False, (A, 64, 128, 10, 32), (A + 32, 64, 128, 10, 32)), (True, (A, 64, 128, 10, 32), (A + 31, 64, 128, 10, 32)),
+    (True, (A, 64, 128, 10, 32), (A + 32, 1280, 128, 10, 32)),  # one nested each way: not told apart
+    # a table of one row, and an empty one
+    (False, (A, 640, 64, 10, 60), (A + 60, 640, 1, 1, 4)), (True, (A, 640, 64, 10, 60), (A + 59, 640, 1, 1, 4)),
+    (False, (A, 640, 64, 10, 64), (A, 640, 64, 0, 64)), (False, (A, 640, 64, 0, 64), (A, 640, 64, 10, 64))])
+def test_tables_that_overlap_are_refused(overlap, first, second):
+    for status in two_tables(first, second):
+        assert status == (-1 if overlap else 0), message()
+    if overlap:
+        assert "overlap" in message()
+
+
+def test_lists_within_a_table_are_refused():
+    # lists of 16 bytes: in a row, between two rows, behind the last
+    for at, status in ((A + 8, -1), (A + 40, 0), (A + 50, -1), (A + 616, 0), (A + 1280, 0), (A - 8, -1), (A - 16, 0)):
+        assert reorder(row=32, parents=at, W=2, n=1) == status if status else True
+        assert reorder(row=32, parents=at, W=1, n=2) == status, (at - A, message())
+    assert reorder(lengths=A + 700) == -1 and "list of rows" in message()
+    assert keep(kept=A + 100, keep=0) == 0 and keep(kept=A + 100) == -1 and "list of rows" in message()
+
+
+def test_overlapping_tables_by_their_bytes():
+    """Random small tables against the sets of their bytes: every overlap is
+    refused, and where the strides are the same nothing else."""
+    import random
+    rng = random.Random(0)
+
+    def places(table, rows_b):
+        base, sb, sn, capacity, row = table
+        rows = [base + b * sb + n * sn for b in range(rows_b) for n in range(capacity)]
+        got = {x + i for x in rows for i in range(row)}
+        return got if len(got) == len(rows) * row else None
+
+    seen = [0, 0]
+    for _ in range(4000):
+        rows_b, row, capacity = rng.randint(1, 3), rng.randint(1, 5), rng.randint(0, 4)
+        sn = rng.randint(row, 12)
+        sb = rng.choice([sn * capacity + rng.randint(0, 30), rng.randint(1, 40)])
+        first = (A, sb, sn, capacity, row)
+        same = rng.random() < 0.7
+        second = (A + rng.randint(-150, 150), sb if same else rng.randint(1, 80), sn if same else rng.randint(1, 12),
+                  rng.randint(0, 4), rng.randint(1, 5))
+        a, b = places(first, rows_b), places(second, rows_b)
+        nested = [t[3] <= 1 or rows_b <= 1 or t[1] >= (t[3] - 1) * t[2] + t[4] or t[2] >= (rows_b - 1) * t[1] + t[4]
+                  for t in (first, second)]
+        if a is None or b is None or not all(nested):
+            continue
+        for status in two_tables(first, second, n=1, W=rows_b):
+            if a & b:
+                assert status == -1, (first, second, rows_b)
+            elif same:
+                assert status == 0, (first, second, rows_b, message())
+            seen[bool(a & b)] += 1
+    assert min(seen) > 500

@@ -175,26 +175,121 @@ int unit_of(const void* base, int64_t sb, int64_t sn, int64_t row_bytes) {
   return (int)(bits & ~(bits - 1));
 }
 
-// Host checks of one table of `rows_b` batch rows.
-int check_table(const char* what, int i, void* const* bases, int64_t sb, int64_t sn, int64_t capacity, int64_t row_bytes,
-                int64_t rows_b, const void* list, const void* lengths) {
-  const void* base = bases[i];
-  if (capacity < 0 || capacity > INT32_MAX || row_bytes <= 0 || row_bytes > INT32_MAX)
-    return fail(WPTV_E_INVALID, "%s: table %d has capacity %lld and rows of %lld bytes", what, i, (long long)capacity,
-                (long long)row_bytes);
-  if (capacity > 0 && rows_b > 0 && !base) return fail(WPTV_E_INVALID, "%s: table %d is NULL", what, i);
-  // rows apart within a batch row and batch rows apart, in either nesting: a place written twice would race
-  const bool apart_n = capacity <= 1 || sn >= row_bytes;
-  const bool apart_b = rows_b <= 1 || sb >= row_bytes;
-  const bool nested = capacity <= 1 || rows_b <= 1 || sb >= (capacity - 1) * sn + row_bytes ||
-                      sn >= (rows_b - 1) * sb + row_bytes;
-  for (int other = 0; other < i; ++other)
-    if (base && bases[other] == base) return fail(WPTV_E_INVALID, "%s: tables %d and %d are the same", what, other, i);
-  for (const void* read : {list, lengths})  // what the launch reads while it moves the rows
-    if (base && read == base) return fail(WPTV_E_INVALID, "%s: table %d is also read as a list of rows", what, i);
-  if (!apart_n || !apart_b || !nested)
-    return fail(WPTV_E_INVALID, "%s: the rows of table %d overlap (strides %lld and %lld bytes, rows of %lld)", what, i,
-                (long long)sb, (long long)sn, (long long)row_bytes);
+// A table's bytes: `count` blocks `stride` apart, of blocks, of `bytes` bytes; batch rows
+// outermost ([0]), or token rows where those are.
+struct Extent {
+  uint64_t base;
+  int64_t stride[2], count[2], bytes;
+
+  __int128 size(int level) const {
+    __int128 n = bytes;
+    for (int i = level; i < 2; ++i) n += (__int128)(count[i] - 1) * stride[i];
+    return n;
+  }
+};
+
+// Whether a byte is both in a and in b, whose base lies d bytes behind a's: blocks m
+// strides apart meet where what is in them does.  Tables of other strides whose ranges
+// meet are not told apart, and taken to.
+bool meet(const Extent& a, const Extent& b, __int128 d, int level = 0) {
+  if (d >= a.size(level) || d + b.size(level) <= 0) return false;
+  if (level == 2) return true;
+  const bool one = a.count[level] == 1, other = b.count[level] == 1;
+  if (!one && !other && a.stride[level] != b.stride[level]) return true;
+  if (one && other) return meet(a, b, d, level + 1);
+  const __int128 s = one ? b.stride[level] : a.stride[level];
+  const __int128 in_a = a.size(level + 1), in_b = b.size(level + 1);
+  const __int128 least = -(a.count[level] - 1), most = b.count[level] - 1;
+  // -in_b < d + m s < in_a
+  __int128 m = (-in_b - d) / s - 1, end = (in_a - d) / s + 1;
+  m = m > least ? m : least;
+  end = end < most ? end : most;
+  if (end - m > 256) return true;
+  for (; m <= end; ++m)
+    if (meet(a, b, d + m * s, level + 1)) return true;
+  return false;
+}
+
+// rows_first: token rows outermost.
+Extent extent(const void* base, int64_t sb, int64_t sn, int64_t capacity, int64_t row_bytes, int64_t rows_b,
+              bool rows_first) {
+  Extent e{reinterpret_cast<uint64_t>(base), {sb, sn}, {rows_b, capacity}, row_bytes};
+  if (rows_first) {
+    e.stride[0] = sn, e.stride[1] = sb;
+    e.count[0] = capacity, e.count[1] = rows_b;
+  }
+  return e;
+}
+
+// What a launch reads while it moves the rows.
+struct List {
+  const void* base;
+  int64_t bytes;
+};
+
+constexpr int kRanges = 256;  // tables whose range of addresses is kept for the tables after them
+
+// Host checks of `count` tables of `rows_b` batch rows: a place written twice, or read
+// as a list, would race.
+int check_tables(const char* what, void* const* bases, const int64_t* strides_b, const int64_t* strides_n,
+                 const int64_t* capacities, const int64_t* row_bytes, int count, int64_t rows_b,
+                 std::initializer_list<List> lists) {
+  uint64_t from[kRanges], to[kRanges];
+  auto extent_of = [&](int i, bool rows_first) {
+    return extent(bases[i], strides_b[i], strides_n[i], capacities[i], row_bytes[i], rows_b, rows_first);
+  };
+  // batch rows (or token rows) may stand outermost: their blocks hold those of the others
+  auto nests = [&](int i, bool rows_first) {
+    return capacities[i] <= 1 || rows_b <= 1 ||
+           (rows_first ? strides_n[i] >= strides_b[i] : strides_b[i] >= strides_n[i]);
+  };
+  auto range = [&](int i, uint64_t& begin, uint64_t& end) {
+    begin = reinterpret_cast<uint64_t>(bases[i]);
+    end = begin;
+    if (capacities[i] > 0 && rows_b > 0) end += (uint64_t)extent_of(i, false).size(0);
+  };
+  for (int i = 0; i < count; ++i) {
+    const void* base = bases[i];
+    const int64_t sb = strides_b[i], sn = strides_n[i], capacity = capacities[i], bytes = row_bytes[i];
+    if (capacity < 0 || capacity > INT32_MAX || bytes <= 0 || bytes > INT32_MAX)
+      return fail(WPTV_E_INVALID, "%s: table %d has capacity %lld and rows of %lld bytes", what, i, (long long)capacity,
+                  (long long)bytes);
+    if (capacity > 0 && rows_b > 0 && !base) return fail(WPTV_E_INVALID, "%s: table %d is NULL", what, i);
+    if (capacity == 0 || rows_b == 0) {  // no bytes
+      if (i < kRanges) from[i] = to[i] = 0;
+      continue;
+    }
+    // rows apart within a batch row and batch rows apart, in either nesting
+    const bool apart_n = capacity <= 1 || sn >= bytes;
+    const bool apart_b = rows_b <= 1 || sb >= bytes;
+    const bool nested = capacity <= 1 || rows_b <= 1 || sb >= (__int128)(capacity - 1) * sn + bytes ||
+                        sn >= (__int128)(rows_b - 1) * sb + bytes;
+    if (!apart_n || !apart_b || !nested)
+      return fail(WPTV_E_INVALID, "%s: the rows of table %d overlap (strides %lld and %lld bytes, rows of %lld)", what, i,
+                  (long long)sb, (long long)sn, (long long)bytes);
+    uint64_t begin, end;
+    range(i, begin, end);
+    if (i < kRanges) from[i] = begin, to[i] = end;
+    for (int other = 0; other < i; ++other) {
+      uint64_t first, last;
+      if (other < kRanges)
+        first = from[other], last = to[other];
+      else
+        range(other, first, last);
+      if (begin >= last || first >= end || first == last) continue;
+      const bool rows_first = !(nests(i, false) && nests(other, false));
+      const Extent a = extent_of(other, rows_first), b = extent_of(i, rows_first);
+      if ((rows_first && !(nests(i, true) && nests(other, true))) || meet(a, b, (__int128)b.base - a.base))
+        return fail(WPTV_E_INVALID, "%s: tables %d and %d are the same, or overlap", what, other, i);
+    }
+    for (const List& list : lists) {
+      const uint64_t at = reinterpret_cast<uint64_t>(list.base);
+      if (!list.base || list.bytes <= 0 || begin >= at + (uint64_t)list.bytes || at >= end) continue;
+      const Extent a = extent_of(i, !nests(i, false)), b = extent(list.base, 0, 0, 1, list.bytes, 1, false);
+      if (meet(a, b, (__int128)b.base - a.base))
+        return fail(WPTV_E_INVALID, "%s: table %d is also read as a list of rows", what, i);
+    }
+  }
   return WPTV_OK;
 }
 
@@ -273,11 +368,10 @@ extern "C" int wptv_reorder_rows(void* const* tables, const int64_t* strides_b, 
   if (n > 65535) return fail(WPTV_E_UNSUPPORTED, "reorder_rows: at most 65535 texts (got %d)", n);
   if (count && (!tables || !strides_b || !strides_n || !capacities || !row_bytes))
     return fail(WPTV_E_INVALID, "reorder_rows: the tables' addresses and shapes must be given");
-  for (int i = 0; i < count; ++i) {
-    const int status = check_table("reorder_rows", i, tables, strides_b[i], strides_n[i], capacities[i],
-                                   row_bytes[i], (int64_t)n * W, parents, lengths);
-    if (status != WPTV_OK) return status;
-  }
+  const int64_t listed = (int64_t)n * W * sizeof(int64_t);
+  const int status = check_tables("reorder_rows", tables, strides_b, strides_n, capacities, row_bytes, count,
+                                  (int64_t)n * W, {{parents, listed}, {lengths, listed}});
+  if (status != WPTV_OK) return status;
   if (count == 0 || n == 0 || W == 1) return WPTV_OK;
   if (!parents) return fail(WPTV_E_INVALID, "reorder_rows: parents is NULL");
   const int widest = W > 16 ? 4 : 16;  // 64 beams' pieces are held in registers
@@ -308,11 +402,11 @@ extern "C" int wptv_keep_rows(void* const* tables, const int64_t* strides_b, con
   if (B > 65535) return fail(WPTV_E_UNSUPPORTED, "keep_rows: at most 65535 batch rows (got %d)", B);
   if (count && (!tables || !strides_b || !strides_n || !capacities || !row_bytes))
     return fail(WPTV_E_INVALID, "keep_rows: the tables' addresses and shapes must be given");
-  for (int i = 0; i < count; ++i) {
-    const int status =
-        check_table("keep_rows", i, tables, strides_b[i], strides_n[i], capacities[i], row_bytes[i], B, kept, counts);
-    if (status != WPTV_OK) return status;
-  }
+  if ((__int128)lists * B * keep > INT64_MAX / 8) return fail(WPTV_E_INVALID, "keep_rows: lists of 2^60 rows");
+  const int status = check_tables("keep_rows", tables, strides_b, strides_n, capacities, row_bytes, count, B,
+                                  {{kept, (int64_t)lists * B * keep * (int64_t)sizeof(int64_t)},
+                                   {counts, B * (int64_t)sizeof(int64_t)}});
+  if (status != WPTV_OK) return status;
   if (count == 0 || B == 0 || keep == 0) return WPTV_OK;
   if (!kept || !counts) return fail(WPTV_E_INVALID, "keep_rows: kept and counts must be given");
   auto size = [](Table& t) { return t.pieces; };

@@ -513,7 +513,7 @@ def keep_rows(tables, kept, counts):
     place among tables (modulo kept's layers: several tables a layer in
     turn).  kept (L, B, keep) int64 ascending, as choose_kept gives it; rows
     from counts[b] on keep what they hold.  tables: one tensor or several, of
-    any types and widths."""
+    any types and widths, none overlapping another or the lists."""
     if torch.is_tensor(tables):
         tables = (tables,)
     if kept.dim() != 3:
