@@ -303,3 +303,10 @@ def test_a_captured_beam_step(device):
         results.append([totals.clone(), last.clone(), cache.lengths.clone(), cache.weights[..., :11].clone()])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+def test_the_cache_itself_knows_what_the_sparse_layers_read(device):
+    cache = decoder(device, MIXED).new_cache(1, weighted=True)
+    with pytest.raises(ValueError, match="sparse layers read the last 16"):
+        cache.evict(30, 2, 15)
+    decoder(device).new_cache(1, weighted=True).evict(30, 2, 0)  # no sparse layers

@@ -116,3 +116,10 @@ def test_a_reading_that_failed_half_way_leaves_nothing_to_add(host):
     with pytest.raises(ValueError, match="not here"):
         cache.undo(torch.tensor([1, 1]))
     assert [x[0] for x in host.added[6:]] == [4, 4]
+
+
+def test_the_rows_that_sparse_layers_read_are_not_evicted(host):
+    cache = Cache(2, 2, 8, torch.float32, "cpu", capacity=16, bare=(1,), weighted=True, recent=16)
+    for held in (cache, cache.select([1, 0])):
+        with pytest.raises(ValueError, match="sparse layers read the last 16"):
+            held.evict(20, 2, 15)

@@ -60,10 +60,11 @@ class Cache:
     """rings: the layers whose table is a ring of ring_rows rows (window
     layers); bare: the layers with no table (sparse layers); every other
     layer's table grows with the text.  weighted: the growing tables' rows
-    carry the attention weight they have received, and may be evicted."""
+    carry the attention weight they have received, and may be evicted, but for
+    the last `recent` (what the sparse layers read of them by position)."""
 
     def __init__(self, rows, layers, width, dtype, device, capacity=256, rings=(), ring_rows=256, bare=(),
-                 weighted=False):
+                 weighted=False, recent=0):
         if ring_rows <= 0 or ring_rows & (ring_rows - 1):
             raise ValueError(f"a ring holds a power of 2 of rows, not {ring_rows}")
         self.lengths = torch.zeros(rows, dtype=torch.long, device=device)
@@ -76,6 +77,7 @@ class Cache:
         self.bound = 0
         self.routes = None
         self.weights = self.evicted = None
+        self.recent = recent
         self._read = []  # a weighted cache's undoable reading: (weights' row, layer, q, positions, lse, scale, counts)
         self._captured = False  # whether that reading was made under stream capture
         self._reading = []  # the same of a reading that has not finished
@@ -217,7 +219,7 @@ class Cache:
         copy.lengths = self.lengths[index]
         copy.before = torch.zeros_like(copy.lengths)
         copy.tables = [None if t is None else t[index] for t in self.tables]
-        copy.rings = self.rings
+        copy.rings, copy.recent = self.rings, self.recent
         copy.pending, copy.bound, copy.routes = False, self.bound, None
         copy.weights = None if self.weights is None else self.weights[:, index]
         copy.evicted = None if self.evicted is None else self.evicted[index]
@@ -251,6 +253,8 @@ class Cache:
             raise ValueError("only a weighted cache evicts: it keeps the attention weight its rows have received")
         if self.pending:
             raise ValueError("an undoable extend is pending: undo it before evicting rows")
+        if recent < self.recent:
+            raise ValueError(f"the sparse layers read the last {self.recent} tokens: recent = {recent} does not hold them")
         kept, counts = kernels.choose_kept(self.weights, self.lengths, keep, first, recent)
         kernels.keep_rows([self.tables[i] for i in self.growing], kept, counts)
         kernels.keep_rows([w[..., None] for w in self.weights], kept, counts)

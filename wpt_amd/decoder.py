@@ -216,7 +216,7 @@ class MQADecoder:
         c = self.config.head_dim
         ring = 1 << max(0, (self.config.window - 1 + widest - 1).bit_length())
         return Cache(rows, self.config.layers, 2 * c, self.dtype, self.device, capacity, self.config.windows, ring,
-                     self.config.sparse, weighted)
+                     self.config.sparse, weighted, self.config.window if self.config.sparse else 0)
 
     def widest(self, cache):
         """The most tokens one reading of the cache takes (its rings' size)."""
