@@ -242,3 +242,12 @@ def test_overlapping_tables_by_their_bytes():
                 assert status == 0, (first, second, rows_b, message())
             seen[bool(a & b)] += 1
     assert min(seen) > 500
+
+
+def test_more_texts_than_the_join_s_grid_holds_are_not_cut_in_parts():
+    size = ctypes.c_size_t(0)
+    for B, asked, given in ((65535, 2, 2), (65536, 2, 1), (65536, 0, 1)):
+        parts = ctypes.c_int(asked)
+        assert _lib.lib().wptv_attention_weights_workspace(B, 2, 16, 64, 64, _lib.WPTV_BF16, ctypes.byref(parts),
+                                                           ctypes.byref(size)) == 0
+        assert parts.value == given and (size.value == 0) == (given == 1)

@@ -371,7 +371,7 @@ extern "C" int wptv_attention_weights_workspace(int B, int T, int H, int c, int 
     return fail(WPTV_E_UNSUPPORTED, "attention_weights: B=%d T=%d H=%d N=%d is too large", B, T, H, N);
   if (*splits < 0) return fail(WPTV_E_INVALID, "attention_weights: splits = %d", *splits);
   const int64_t rows = (int64_t)T * H;
-  if (!matrix_width(c) || B == 0 || rows == 0) {
+  if (!matrix_width(c) || B == 0 || rows == 0 || B > 65535) {  // (the join's grid has B rows)
     *splits = 1;
   } else if (*splits == 0) {
     *splits = weight_parts(B, T, H, N);
