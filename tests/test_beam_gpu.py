@@ -314,3 +314,15 @@ def test_scores_apart_whose_values_are_equal(device, kind, n, V, dtype):
         expected = oracle.beam_step(scores[some], totals[some], beams=K)
         assert torch.equal(got[1], expected[1]) and torch.equal(got[2], expected[2])
         totals_close(got[0], expected[0], V)
+
+
+def test_batch_rows_past_4_gb(device):
+    W, N, width = 3, 300, 512
+    stride = 2_200_000_000  # the last batch row starts past 2^32 bytes
+    whole = torch.empty(2 * stride + N * width, dtype=torch.uint8, device=device)
+    table = whole.as_strided((W, N, width), (stride, width, 1))
+    small = fill((W, N, width), torch.uint8, 5)
+    table.copy_(small)
+    lengths = torch.tensor([300, 120, 250])
+    kernels.reorder_rows(table, torch.tensor([[2, 0, 1]], device=device), lengths.to(device))
+    assert torch.equal(table.cpu(), oracle.reorder_rows([small], torch.tensor([[2, 0, 1]]), lengths)[0])

@@ -310,3 +310,63 @@ def test_the_cache_itself_knows_what_the_sparse_layers_read(device):
     with pytest.raises(ValueError, match="sparse layers read the last 16"):
         cache.evict(30, 2, 15)
     decoder(device).new_cache(1, weighted=True).evict(30, 2, 0)  # no sparse layers
+
+
+def test_evictions_in_a_captured_step(device):
+    model = decoder(device, MIXED, torch.bfloat16)
+    prompt = tokens(3, 30, seed=1)
+    cache = model.new_cache(3, capacity=64, widest=16, weighted=True)
+    model.extend(prompt, cache, torch.tensor([30, 22, 9]))
+    last = tokens(3, 2, seed=2).to(device)
+    state = [t for t in cache.tables if t is not None] + [cache.weights, cache.lengths, cache.evicted]
+    start, bound = [x.clone() for x in state], cache.bound
+
+    def step():
+        scores = model.extend(last, cache)[0]
+        kept = model.evict(cache, 24, 2, 16)
+        last.copy_(scores.argmax(-1))
+        return kept
+
+    def reset():
+        for x, y in zip(state, start):
+            x.copy_(y)
+        last.copy_(tokens(3, 2, seed=2))
+        cache.bound = bound
+
+    stream = torch.cuda.Stream(device)
+    stream.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream(device).wait_stream(stream)
+    reset()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    runs = [[], []]
+    for run, replayed in zip(runs, (True, False)):
+        reset()
+        for _ in range(5):
+            torch.cuda.synchronize()
+            kept = step() if not replayed else (graph.replay(), captured)[1]
+            torch.cuda.synchronize()
+            run.append([kept.clone(), last.clone(), cache.lengths.clone(), cache.evicted.clone()])
+        run.append([t[:, :24].clone() for t in state[:-3]] + [cache.weights[..., :20].clone()])
+    for a, b in zip(*runs):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert cache.lengths.tolist() == [24, 24, 19] and cache.evicted.tolist() == [16, 8, 0]
+
+
+def test_prompts_of_several_chunks_on_a_bounded_cache(device):
+    # the exact layer's attention adds nothing to the stream: evictions while the prompts are read change nothing
+    config = DecoderConfig(layers=3, d_model=256, heads=4, head_dim=64, ffn=256, vocab=512, kinds=(WINDOW, EXACT, WINDOW),
+                           window=16)
+    model = decoder(device, config, std=0.12, silent=(1,))
+    prompts = [tokens(n, seed=n).tolist() for n in (2300, 1100, 40)]
+    plain = BeamWriter(model, prompts, 3).write(6)
+    writer = BeamWriter(model, prompts, 3, keep=200, first=4, recent=50)
+    got = writer.write(6)
+    assert [[t for t, _ in beams] for beams in got] == [[t for t, _ in beams] for beams in plain]
+    for a, b in zip(got, plain):
+        assert [x for _, x in a] == pytest.approx([x for _, x in b], abs=1e-3)
+    assert int(writer.cache.lengths.max()) <= 225
+    assert writer.cache.starts().tolist() == [len(p) - 1 + 6 for p in prompts for _ in range(3)]

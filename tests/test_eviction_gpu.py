@@ -343,3 +343,36 @@ def test_in_a_graph_on_another_stream(device):
         if i == 0:
             for a, b in zip(got, side):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("B, splits", [(13, 5), (11, 7), (67, 2)])
+def test_parts_that_do_not_divide_over_the_xcds(device, B, splits):
+    """64 chunks of a batch row and a part or more, and no multiple of 8."""
+    assert B * splits >= 64 and B * splits % 8
+    q, table, positions, lse, start = reading(B, 20, 16, 64, 300, torch.bfloat16, seed=B)
+    weights = torch.rand(B, 300, generator=torch.Generator().manual_seed(B))
+    check(device, q, table, positions, lse, weights, start=start, splits=splits)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("c", [64, 128, 96])
+def test_the_weights_to_their_last_bits(device, dtype, c):
+    """Queries and keys of -1, 0 and 1 and a scale of 2^-4: the products are
+    exact, so what is left of a term exp(s - lse) are, in steps of 2^-24, the
+    rounding of log2 e (0.22) on |s|, with its product's (1.22) on |lse|, that of
+    the difference on |s - lse|, the exponential's 2; and the sum's R additions of
+    terms of one sign, no more than R / 4 + 8 in turn in any form, and the last."""
+    B, T, H, N = 3, 5, 16, 420
+    g = torch.Generator().manual_seed(c)
+    q, k = (torch.randint(-1, 2, shape, generator=g).to(dtype) for shape in ((B, T, H, c), (B, N, c)))
+    positions = torch.tensor([N - T, 200, 17])[:, None] + torch.arange(T)
+    lse = oracle.log_sum_exp(q, k, positions, 2.0 ** -4).float()
+    old = torch.zeros(B, N)
+    expected = oracle.attention_weights(q, k, positions, lse, 2.0 ** -4, old)
+    held = old.to(device)
+    kernels.add_attention_weights(q.to(device), k.to(device), positions.to(device), lse.to(device), 2.0 ** -4, held)
+    s = float((torch.matmul(q.float().reshape(B, T * H, c), k.float().transpose(1, 2)) * 2.0 ** -4).abs().max())
+    high = float(lse.abs().max())
+    steps = 0.22 * s + 1.22 * high + (s + high) + 2 + T * H / 4 + 8 + 1
+    assert steps < 64
+    assert bool(((held.cpu().double() - expected).abs() <= expected * steps * 2.0 ** -24).all())

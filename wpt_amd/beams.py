@@ -9,7 +9,9 @@ How a step runs here, with no host synchronization:
     reorder    the cache's rows take over their parents' states in place
                (MQADecoder.reorder)
     evict      with `keep`, a weighted cache is brought back to keep entries an
-               exact layer whenever it holds an eighth more (MQADecoder.evict)
+               exact layer whenever it may hold an eighth more (MQADecoder.evict):
+               the host knows the longest row's bound, so that a text is evicted
+               from when the longest beside it is
 Each beam's text is read back along its parents when it is asked for.
 """
 
