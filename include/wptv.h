@@ -631,7 +631,8 @@ int wptv_reorder_rows(void* const* tables, const int64_t* strides_b, const int64
  * wptv_attention_weights: weights[b, n] += the sum over queries t < counts[b]
  *   with positions[b, t] >= n and heads h of exp(scale q[b, t, h] . k[b, n] -
  *   lse[b, t, h]): the softmax weight each table row got from a reading's
- *   verify attention (lse its log-sum-exp, positions as there).
+ *   verify attention (lse its log-sum-exp, positions as there), in FP32: a term
+ *   is off by a few 2^-24 (1 + |lse| + |scale q . k|) of itself.
  *   counts   NULL (T) or [B] int64: queries counted, the others padding
  *   start    NULL or [B] int64: rows n >= start[b] begin at zero instead of
  *            their weight (the reading's own rows: its rows before it)

@@ -17,10 +17,16 @@
 //   attention_weights_join     the parts' sums
 //   attention_weights_generic  any other width up to 256, or unaligned rows
 //
+// A term's exponent is formed in FP32 from lse log2 e and scale log2 e, each rounded: a
+// weight is off by a few steps of 2^-24 times |lse| + |scale q . k|.
+//
 // Per 16 query heads x 16 rows at head width 128, a SIMD's matrix cores take 64
-// cycles and its vector unit 96 (an exponential at a quarter of the rate, the scaling
-// and the sum): a prompt is bound by the latter.  Two prompts of 4096 tokens, 16 heads:
-// 64 us and 4 for the join, 1.06 PFLOP/s of the products alone.  Few queries are bound
+// cycles and its vector unit about 110 (16.6 instructions, of them four exponentials at
+// a quarter of the rate).  Two prompts of 4096 tokens, 16 heads: 62 us and 4 for the
+// join, 1.1 PFLOP/s of the products alone; by the counters the matrix cores are busy 25 %
+// of that time and the vector units 40 %, with two wavefronts a SIMD on average: neither
+// is full, a wavefront's products and exponentials follow each other, and the parts of a
+// causal prompt end at different times.  Few queries are bound
 // by the keys: 32 texts of 4100 rows, 5 queries, 11.4 us for 27 MB, of which the chain
 // positions, keys, products, write takes 4 whatever is read.
 #include "wptv_common.h"

@@ -19,9 +19,9 @@
 // into the best so far.  No barrier, and any scores are served: where many reach
 // the bound the part is read again.
 //
-// 64 texts of 5 beams over 50257 FP32 scores: 16.5 us and 5.9 (64 MB at 3.9 TB/s; the
+// 64 texts of 5 beams over 50257 FP32 scores: 16.4 us and 6.2 (64 MB at 3.9 TB/s; the
 // loads of all parts are in flight at once and their arithmetic follows); 32 texts of
-// 8 beams over 32768 bf16 scores: 7.3 and 6.6; one text of 4 beams over 8192: 9.0 in one
+// 8 beams over 32768 bf16 scores: 7.1 and 7.0; one text of 4 beams over 8192: 9.1 in one
 // launch, the latency of its steps.
 #include "wptv_common.h"
 
@@ -700,6 +700,8 @@ __global__ __launch_bounds__(64 * kTextWaves) void beam_text(const E* __restrict
 // units.  Measured, us, in a graph and from a program, one launch and two: one text of
 // 4 beams over 8192 scores 9.0, 8.3 and 13.9, 17.7; 200 texts 9.8, 11.5 and 13.5, 17.4;
 // 8 beams over 4000 11.0, 9.8 and 13.8, 18.1; 16 over 2000 13.8, 12.3 and 13.7, 17.6.
+// The rule goes by a program's calls, whose host time it saves; in a graph a few texts
+// are 0.7 to 1.5 us slower by it.
 int text_parts(int n, int W, int V) {
   const int64_t parts = ((int64_t)V + 64 * kTextItems - 1) / (64 * kTextItems);
   return W * parts <= kTextWaves && n <= compute_units() ? (int)parts : 0;

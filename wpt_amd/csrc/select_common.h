@@ -1,5 +1,6 @@
-// The K-th largest of a workgroup's 32-bit keys, held in its threads' registers:
-// what the choice of rows (choice.hip) and the eviction (eviction.hip) select by.
+// The K-th largest of a workgroup's 32-bit keys, held in its threads' registers or read
+// again for each pass (long texts): what the choice of rows (choice.hip) and the eviction
+// (eviction.hip) select by.
 #pragma once
 
 #include "wptv_common.h"

@@ -442,8 +442,9 @@ def add_attention_weights(q, k, positions, lse, scale, weights, *, counts=None, 
     that attention's log-sum-exp.  counts (B,): the queries counted, the
     others padding or drafts that were taken back (None: all); start (B,):
     the rows from there on, the reading's own, begin at zero.  Rows past the
-    last counted position are left alone.  splits: parts of the queries (0:
-    the library chooses).  Returns weights."""
+    last counted position are left alone.  The terms and their sums are FP32:
+    a term is off by a few 2^-24 (1 + |lse| + |scale q . k|) of itself.  splits:
+    parts of the queries (0: the library chooses).  Returns weights."""
     if q.dim() != 4 or k.dim() != 3:
         raise ValueError(f"q must be (B, T, H, c) and k (B, N, c); got {tuple(q.shape)}, {tuple(k.shape)}")
     B, T, H, c = q.shape
