@@ -326,3 +326,18 @@ def test_batch_rows_past_4_gb(device):
     lengths = torch.tensor([300, 120, 250])
     kernels.reorder_rows(table, torch.tensor([[2, 0, 1]], device=device), lengths.to(device))
     assert torch.equal(table.cpu(), oracle.reorder_rows([small], torch.tensor([[2, 0, 1]]), lengths)[0])
+
+
+@pytest.mark.parametrize("n, W, V, K", [(3, 4, 3000, 16), (300, 8, 7, 9), (300, 3, 9001, 12), (2, 16, 30001, 64)])
+def test_beams_of_the_same_scores_in_another_order(device, n, W, V, K):
+    """Their log-sum-exp is one number, whatever the order of its terms: with
+    equal totals equal scores fall to the lowest beam and token."""
+    print(f"beam_step permuted beams n={n} W={W} V={V} K={K}", flush=True)
+    g = torch.Generator().manual_seed(V)
+    scores = torch.empty(n, W, V)
+    for i in range(n):
+        row = 2 * torch.randn(V, generator=g)
+        scores[i] = torch.stack([row[torch.randperm(V, generator=g)] for _ in range(W)])
+    got = [x.cpu() for x in sampling.beam_step(scores.to(device), torch.full((n, W), -2.5, device=device), beams=K)]
+    order = scores.view(n, W * V).sort(dim=-1, descending=True, stable=True).indices[:, :K]
+    assert torch.equal(got[1], order // V) and torch.equal(got[2], order % V)
