@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define WPTV_ABI_VERSION 12
+#define WPTV_ABI_VERSION 13
 
 enum {
   WPTV_OK = 0,
@@ -573,6 +573,80 @@ int wptv_greedy_tree(const void* scores, int64_t scores_stride_b, int64_t scores
  *   nothing, n_tokens -1). */
 int wptv_greedy_tree_best(const int32_t* best, const int64_t* node_tokens, const int32_t* parents, int B, int M,
                           int64_t* path, int64_t* tokens, int32_t* n_tokens, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * A mixture of experts: the router's choice and the experts' products, for the
+ * few rows of a verify step (any number is taken).  The reference's experts
+ * (packages/wpt-model/src/wpt_model/experts.py) stand in the feed-forward
+ * block's place; the form here is a linear router and SwiGLU experts.
+ *
+ * wptv_route: for row m = (b, t) of x [B, T, D] the k experts e of the largest
+ *   l_e + bias_e, l = x[m] . router[e] formed and ranked in 64 bits, largest
+ *   first, equal values the lowest expert (a NaN counts as the largest); gates =
+ *   the softmax of the chosen experts' l (without the bias), rounded to FP32.
+ *   router [E, D] fp32; bias NULL or [E] fp32 (-inf takes an expert out: one at
+ *   -inf is never chosen).  counts NULL or [B] int64: rows t >= counts[b] are
+ *   padding.  chosen [B, T, k] int32, gates [B, T, k] fp32; where no expert is
+ *   chosen (padding, fewer than k above -inf) chosen is -1 and the gate 0.  A
+ *   NaN or +inf among a row's chosen l makes its gates NaN.
+ *   D a multiple of 8, E <= 512, k <= 16; rows contiguous and 16-byte aligned.
+ * ------------------------------------------------------------------------- */
+int wptv_route(const void* x, int dtype, const float* router, const float* bias, const int64_t* counts, int B, int T,
+               int D, int E, int k, int32_t* chosen, float* gates, hipStream_t stream);
+
+/* wptv_experts_packed, wptv_pack_experts: the experts' weights in the order the
+ *   products read them, laid out once: gate_up [E, 2F, D] (each expert's F gate
+ *   rows, then its F up rows) and down [E, D, F], row-major in dtype, into
+ *   buffers of E times the bytes wptv_experts_packed gives an expert.
+ * wptv_experts: y[m] = the sum over j of gates[m, j] down_e (silu(gate_e x[m])
+ *   * (up_e x[m])), e = chosen[m, j]; a choice outside 0 .. E - 1 adds nothing.
+ *   FP32 sums; silu(g) u is rounded once to dtype between the products.  x
+ *   [rows, D]; the result in one of two forms, the other pointer NULL:
+ *   parts    [k, rows, D] fp32: choice j's gated term in parts[j], for a
+ *            consumer that sums them (wptv_add_rms_norm_parts, k <= 8)
+ *   y        [rows, D] in dtype, their sum in order, rounded once
+ *   workspace  wptv_experts_workspace bytes (parts_out: the parts are the
+ *            output)
+ * wptv_mixture: wptv_route, then wptv_experts on its choice (chosen and gates
+ *   are outputs). */
+int wptv_experts_packed(int D, int F, int dtype, size_t* gate_up_bytes, size_t* down_bytes);
+
+int wptv_pack_experts(const void* gate_up, const void* down, int E, int D, int F, int dtype, void* gate_up_packed,
+                      void* down_packed, hipStream_t stream);
+
+int wptv_experts_workspace(int rows, int D, int F, int k, int dtype, int parts_out, size_t* bytes);
+
+int wptv_experts(const void* x, int dtype, const void* gate_up_packed, const void* down_packed, const int32_t* chosen,
+                 const float* gates, int rows, int D, int E, int k, int F, float* parts, void* y, void* workspace,
+                 size_t workspace_bytes, hipStream_t stream);
+
+int wptv_mixture(const void* x, int dtype, const float* router, const float* bias, const int64_t* counts, int B, int T,
+                 int D, int E, int k, int F, const void* gate_up_packed, const void* down_packed, int32_t* chosen,
+                 float* gates, float* parts, void* y, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * wptv_log_probs: what the model gave to tokens that were written: for row m of
+ *   scores (V values of scores_dtype, row (b, t) at scores + b*scores_stride_b +
+ *   t*scores_stride_t elements) and z = scores / temperature
+ *   logprobs [B, T] fp32 = z[token] - log sum exp z, token = tokens[b, t] (int64,
+ *            contiguous); 0 for a token outside 0 .. V - 1 (the -1 past a row's
+ *            written tokens)
+ *   entropy  [B, T] fp32: that of softmax(z)
+ *   ids      [B, T, top] int64: the tokens of the largest scores, largest first,
+ *            equal scores the lowest token (a NaN counts as the largest, -0 as 0)
+ *   best     [B, T, top] fp32: their log-probabilities
+ *   A row that holds a NaN or +inf, or nothing above -inf, has no distribution:
+ *   its log-probabilities and its entropy are NaN.  -inf scores have
+ *   log-probability -inf.  top <= 64, top <= V; V <= 2^24; temperature positive
+ *   and finite.  The reference's Writer returns tokens alone.
+ *   workspace  wptv_log_probs_workspace(B, T, V, top) bytes
+ * ------------------------------------------------------------------------- */
+int wptv_log_probs_workspace(int B, int T, int V, int top, size_t* bytes);
+
+int wptv_log_probs(const void* scores, int64_t scores_stride_b, int64_t scores_stride_t, int scores_dtype,
+                   const int64_t* tokens, float temperature, int B, int T, int V, int top, float* logprobs,
+                   float* entropy, int64_t* ids, float* best, void* workspace, size_t workspace_bytes,
+                   hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
  * Beam search: the next beams of every text over its beams and the

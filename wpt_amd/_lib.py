@@ -13,7 +13,7 @@ from pathlib import Path
 import torch
 
 LIBRARY = Path(__file__).resolve().parent / "lib" / "libwptv.so"
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 WPTV_F32, WPTV_BF16 = 0, 1
 DTYPES = {torch.float32: WPTV_F32, torch.bfloat16: WPTV_BF16}
@@ -89,6 +89,14 @@ SIGNATURES = {
                              _P, _P, _P, _SZ, _P, _P, _P, _I64, _P, _P, _P],
     "wptv_greedy_tree": [_P, _I64, _I64, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _SZ, _P],
     "wptv_greedy_tree_best": [_P, _P, _P, _I, _I, _P, _P, _P, _P],
+    "wptv_route": [_P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P],
+    "wptv_experts_packed": [_I, _I, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
+    "wptv_pack_experts": [_P, _P, _I, _I, _I, _I, _P, _P, _P],
+    "wptv_experts_workspace": [_I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)],
+    "wptv_experts": [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _SZ, _P],
+    "wptv_mixture": [_P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+    "wptv_log_probs_workspace": [_I, _I, _I, _I, ctypes.POINTER(_SZ)],
+    "wptv_log_probs": [_P, _I64, _I64, _I, _P, _F, _I, _I, _I, _I, _P, _P, _P, _P, _P, _SZ, _P],
     "wptv_beam_workspace": [_I, _I, _I, _I, ctypes.POINTER(_SZ)],
     "wptv_beam_step": [_P, _I64, _I64, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _SZ, _P],
     "wptv_reorder_rows": [_P, _P, _P, _P, _P, _I, _P, _P, _I64, _I, _I, _P],

@@ -22,9 +22,10 @@ import torch
 
 from . import _lib
 from ._lib import KernelUnavailable, check, ptr
+from .kernels import _forward_only
 
 __all__ = ["accept", "accept_in_order", "generator_state", "set_offset", "greedy_chain", "greedy_tree",
-           "greedy_tree_from_argmax", "draws", "written", "beam_step"]
+           "greedy_tree_from_argmax", "draws", "written", "beam_step", "log_probs"]
 
 
 def _on_gpu(*tensors):
@@ -349,3 +350,41 @@ def beam_step(scores, totals, ended=None, stops=(), beams=None):
                                         ptr(new_totals), ptr(parents), ptr(tokens), ptr(new_ended), ptr(workspace),
                                         size, _lib.stream(device)), "beam_step")
     return new_totals, parents, tokens, new_ended
+
+
+def log_probs(scores, tokens, top=0, temperature=1.0):
+    """What the model gave to written tokens: (logprobs (B, T) FP32, entropy
+    (B, T) FP32, ids (B, T, top) int64, best (B, T, top) FP32).
+
+    scores (B, T, V) FP32 or bf16: the model's scores at each place; tokens
+    (B, T) int64: the token written there.  logprobs: the tokens' log-softmax of
+    scores / temperature, 0 for a token outside 0 .. V - 1 (the -1 past a row's
+    written tokens); entropy: that of the distribution; ids, best: the tokens
+    of the `top` largest scores (at most 64), largest first, equal scores the
+    lowest token (a NaN counts as the largest), and their log-probabilities.  A
+    place whose scores hold a NaN or +inf, or nothing above -inf, has no
+    distribution: its log-probabilities and its entropy are NaN."""
+    scores_ = _scores(scores)
+    B, T, V = scores_.shape
+    device = scores_.device
+    _on_gpu(scores_)
+    top, temperature = int(top), float(temperature)
+    if tokens.shape != (B, T) or tokens.dtype != torch.int64 or tokens.device != device:
+        raise ValueError(f"tokens must be int64 (B={B}, T={T}) on {device}; got {tokens.dtype} {tuple(tokens.shape)}")
+    if not 0 <= top <= V:
+        raise ValueError(f"the top {top} of {V} tokens")
+    if not 0 < temperature < float("inf"):
+        raise ValueError(f"the temperature must be positive and finite; got {temperature}")
+    tokens = tokens.contiguous()
+    logprobs = torch.empty(B, T, dtype=torch.float32, device=device)
+    entropy = torch.empty(B, T, dtype=torch.float32, device=device)
+    ids = torch.empty(B, T, top, dtype=torch.long, device=device)
+    best = torch.empty(B, T, top, dtype=torch.float32, device=device)
+    with _lib.on(device):
+        _, size = _lib.plan("wptv_log_probs_workspace", "log_probs", B, T, V, top)
+        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        check(_lib.lib().wptv_log_probs(ptr(scores_), scores_.stride(0), scores_.stride(1),
+                                        _lib.dtype_code(scores_.dtype), ptr(tokens), temperature, B, T, V, top,
+                                        ptr(logprobs), ptr(entropy), ptr(ids), ptr(best), ptr(workspace), size,
+                                        _lib.stream(device)), "log_probs")
+    return _forward_only(logprobs, scores), _forward_only(entropy, scores), ids, _forward_only(best, scores)
