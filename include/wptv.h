@@ -590,9 +590,13 @@ int wptv_greedy_tree_best(const int32_t* best, const int64_t* node_tokens, const
  *   chosen (padding, fewer than k above -inf) chosen is -1 and the gate 0.  A
  *   NaN or +inf among a row's chosen l makes its gates NaN.
  *   D a multiple of 8, E <= 512, k <= 16; rows contiguous and 16-byte aligned.
+ *   workspace  wptv_route_workspace(B T, D, E) bytes
  * ------------------------------------------------------------------------- */
+int wptv_route_workspace(int rows, int D, int E, size_t* bytes);
+
 int wptv_route(const void* x, int dtype, const float* router, const float* bias, const int64_t* counts, int B, int T,
-               int D, int E, int k, int32_t* chosen, float* gates, hipStream_t stream);
+               int D, int E, int k, int32_t* chosen, float* gates, void* workspace, size_t workspace_bytes,
+               hipStream_t stream);
 
 /* wptv_experts_packed, wptv_pack_experts: the experts' weights in the order the
  *   products read them, laid out once: gate_up [E, 2F, D] (each expert's F gate
@@ -608,7 +612,7 @@ int wptv_route(const void* x, int dtype, const float* router, const float* bias,
  *   workspace  wptv_experts_workspace bytes (parts_out: the parts are the
  *            output)
  * wptv_mixture: wptv_route, then wptv_experts on its choice (chosen and gates
- *   are outputs). */
+ *   are outputs); workspace wptv_mixture_workspace bytes. */
 int wptv_experts_packed(int D, int F, int dtype, size_t* gate_up_bytes, size_t* down_bytes);
 
 int wptv_pack_experts(const void* gate_up, const void* down, int E, int D, int F, int dtype, void* gate_up_packed,
@@ -619,6 +623,8 @@ int wptv_experts_workspace(int rows, int D, int F, int k, int dtype, int parts_o
 int wptv_experts(const void* x, int dtype, const void* gate_up_packed, const void* down_packed, const int32_t* chosen,
                  const float* gates, int rows, int D, int E, int k, int F, float* parts, void* y, void* workspace,
                  size_t workspace_bytes, hipStream_t stream);
+
+int wptv_mixture_workspace(int rows, int D, int E, int F, int k, int dtype, int parts_out, size_t* bytes);
 
 int wptv_mixture(const void* x, int dtype, const float* router, const float* bias, const int64_t* counts, int B, int T,
                  int D, int E, int k, int F, const void* gate_up_packed, const void* down_packed, int32_t* chosen,

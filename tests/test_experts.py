@@ -83,16 +83,19 @@ def test_weights_of_shapes_without_a_kernel_are_refused(arguments, status):
     (1, 1, 64, 513, 2, 1, -3), (1, 1, 64, 40, 17, 1, -3), (1, 1, 64, 4, 2, 5, -3), (4097, 4097, 64, 4, 2, 1, -3)])
 def test_routes_of_shapes_without_a_kernel_are_refused(B, T, D, E, k, dtype, status):
     library = _lib.lib()
-    assert library.wptv_route(16, dtype, 16, None, None, B, T, D, E, k, 16, 16, None) == status
+    assert library.wptv_route(16, dtype, 16, None, None, B, T, D, E, k, 16, 16, 16, 1 << 40, None) == status
     assert library.wptv_mixture(16, dtype, 16, None, None, B, T, D, E, k, 64, 16, 16, 16, 16, None, 16, 16, 1 << 40,
                                 None) == status
 
 
 def test_null_and_misaligned_pointers_and_small_workspaces_are_refused():
     library = _lib.lib()
-    assert library.wptv_route(None, 1, 16, None, None, 1, 1, 64, 4, 2, 16, 16, None) == -1
-    assert library.wptv_route(8, 1, 16, None, None, 1, 1, 64, 4, 2, 16, 16, None) == -1
+    assert library.wptv_route(None, 1, 16, None, None, 1, 1, 64, 4, 2, 16, 16, 16, 0, None) == -1
+    assert library.wptv_route(8, 1, 16, None, None, 1, 1, 64, 4, 2, 16, 16, 16, 0, None) == -1
     assert b"16-byte" in library.wptv_last_error()
+    assert library.wptv_route(16, 1, 16, None, None, 1, 1, 2048, 64, 2, 16, 16, 16, 63, None) == -1
+    assert library.wptv_route(16, 1, 16, None, None, 1, 1, 2048, 64, 2, 16, 16, None, 1 << 40, None) == -1
+    assert b"workspace" in library.wptv_last_error()
 
     def products(parts=None, y=16, workspace=16, size=1 << 30, x=16, F=64, rows=3):
         return library.wptv_experts(x, 1, 16, 16, 16, 16, rows, 64, 4, 2, F, parts, y, workspace, size, None)

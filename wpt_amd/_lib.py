@@ -89,11 +89,13 @@ SIGNATURES = {
                              _P, _P, _P, _SZ, _P, _P, _P, _I64, _P, _P, _P],
     "wptv_greedy_tree": [_P, _I64, _I64, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _SZ, _P],
     "wptv_greedy_tree_best": [_P, _P, _P, _I, _I, _P, _P, _P, _P],
-    "wptv_route": [_P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P],
+    "wptv_route_workspace": [_I, _I, _I, ctypes.POINTER(_SZ)],
+    "wptv_route": [_P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _SZ, _P],
     "wptv_experts_packed": [_I, _I, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)],
     "wptv_pack_experts": [_P, _P, _I, _I, _I, _I, _P, _P, _P],
     "wptv_experts_workspace": [_I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)],
     "wptv_experts": [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _SZ, _P],
+    "wptv_mixture_workspace": [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)],
     "wptv_mixture": [_P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
     "wptv_log_probs_workspace": [_I, _I, _I, _I, ctypes.POINTER(_SZ)],
     "wptv_log_probs": [_P, _I64, _I64, _I, _P, _F, _I, _I, _I, _I, _P, _P, _P, _P, _P, _SZ, _P],

@@ -106,207 +106,367 @@ __device__ __forceinline__ uint64_t order_key64(double f) {
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-constexpr int kRouteThreads = 512, kMaxExperts = 512, kMaxChosen = 16;
+constexpr int kMaxExperts = 512, kMaxChosen = 16;
 
-// A workgroup TM tokens: its wavefronts share out the experts, the lanes the width;
-// the products of two FP32 values are exact in 64 bits, and so is the order of the
-// logits but for the sums' own rounding.  An expert's place is the count of those
-// before it.
-template <typename T, int TM>
-__global__ __launch_bounds__(kRouteThreads) void route(const T* __restrict__ x, const float* __restrict__ router,
-                                                       const float* __restrict__ bias,
-                                                       const int64_t* __restrict__ counts, int rows, int per_row, int D,
-                                                       int E, int k, int* __restrict__ chosen,
-                                                       float* __restrict__ gates) {
-  constexpr int kWaves = kRouteThreads / 64, kTokenThreads = kRouteThreads / TM;
-  __shared__ double logit[TM][kMaxExperts];
-  __shared__ uint64_t key[TM][kMaxExperts];
-  __shared__ int place[TM][kMaxChosen];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int m0 = blockIdx.x * TM;
-  const T* xr[TM];
-#pragma unroll
-  for (int t = 0; t < TM; ++t) xr[t] = x + (int64_t)min(m0 + t, rows - 1) * D;
-  for (int e = wv; e < E; e += kWaves) {
-    const float* w = router + (int64_t)e * D;
-    double sum[TM];
-#pragma unroll
-    for (int t = 0; t < TM; ++t) sum[t] = 0.;
-    for (int d = 4 * lane; d < D; d += 256) {
-      const float4 a = *reinterpret_cast<const float4*>(w + d);
-#pragma unroll
-      for (int t = 0; t < TM; ++t) {
-        float b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = load_f32<T>(xr[t] + d + i);
-        sum[t] = fma((double)a.x, (double)b[0], sum[t]);
-        sum[t] = fma((double)a.y, (double)b[1], sum[t]);
-        sum[t] = fma((double)a.z, (double)b[2], sum[t]);
-        sum[t] = fma((double)a.w, (double)b[3], sum[t]);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < TM; ++t) {
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) sum[t] += __shfl_xor(sum[t], o, 64);
-      if (lane == 0) {
-        logit[t][e] = sum[t];
-        key[t][e] = order_key64(bias ? sum[t] + (double)bias[e] : sum[t]);
-      }
-    }
-  }
-  const int t = threadIdx.x / kTokenThreads, tt = threadIdx.x % kTokenThreads, m = m0 + t;
-  if (tt < k) place[t][tt] = -1;
-  __syncthreads();
-  const bool read = m < rows && (!counts || m % per_row < counts[m / per_row]);
+// The places of a token's experts (the count of those before each), by the
+// `threads` threads tid, tid + threads, ... of its own; place holds -1 before.
+__device__ __forceinline__ void place_experts(const uint64_t* key, int tid, int threads, int E, int k, int* place) {
   const uint64_t none = order_key64(-__builtin_inf());
-  if (read)
-    for (int e = tt; e < E; e += kTokenThreads) {
-      const uint64_t mine = key[t][e];
-      int before = 0;
-      for (int i = 0; i < E; ++i) {
-        const uint64_t other = key[t][i];
-        before += other > mine || (other == mine && i < e) ? 1 : 0;
-      }
-      if (before < k && mine != none) place[t][before] = e;
+  for (int e = tid; e < E; e += threads) {
+    const uint64_t mine = key[e];
+    int before = 0;
+    for (int i = 0; i < E; ++i) {
+      const uint64_t other = key[i];
+      before += other > mine || (other == mine && i < e) ? 1 : 0;
     }
-  __syncthreads();
-  if (m < rows && tt < k) {
-    double high = -__builtin_inf(), total = 0.;
-    bool nan = false;
-    for (int i = 0; i < k; ++i)
-      if (place[t][i] >= 0) {
-        const double l = logit[t][place[t][i]];
-        nan |= l != l;
-        high = fmax(high, l);
-      }
-    for (int i = 0; i < k; ++i)
-      if (place[t][i] >= 0) total += exp(logit[t][place[t][i]] - high);
-    const int e = place[t][tt];
-    chosen[(int64_t)m * k + tt] = e;
-    gates[(int64_t)m * k + tt] =
-        e < 0 ? 0.f : nan ? __builtin_nanf("") : (float)(exp(logit[t][e] - high) / total);
+    if (before < k && mine != none) place[before] = e;
   }
 }
 
+// Choice i of a token and its gate, the softmax of the chosen logits in 64 bits.
+__device__ __forceinline__ void store_choice(const double* logit, const int* place, int i, int k, int* chosen,
+                                             float* gates) {
+  double high = -__builtin_inf(), total = 0.;
+  bool nan = false;
+  for (int c = 0; c < k; ++c)
+    if (place[c] >= 0) {
+      const double l = logit[place[c]];
+      nan |= l != l;
+      high = fmax(high, l);
+    }
+  for (int c = 0; c < k; ++c)
+    if (place[c] >= 0) total += exp(logit[place[c]] - high);
+  const int e = place[i];
+  *chosen = e;
+  *gates = e < 0 ? 0.f : nan ? __builtin_nanf("") : (float)(exp(logit[e] - high) / total);
+}
+
+template <typename T>
+__device__ __forceinline__ void load_four(const T* p, float* to) {
+  typedef T four __attribute__((ext_vector_type(4)));
+  const four v = *reinterpret_cast<const four*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const T x = v[i];
+    to[i] = load_f32<T>(&x);
+  }
+}
+
+// A narrow router in one launch: a workgroup a token, its wavefronts share out the
+// experts, the lanes the width.
+template <typename T>
+__global__ __launch_bounds__(256) void route_token(const T* __restrict__ x, const float* __restrict__ router,
+                                                   const float* __restrict__ bias, const int64_t* __restrict__ counts,
+                                                   int per_row, int D, int E, int k, int* __restrict__ chosen,
+                                                   float* __restrict__ gates) {
+  __shared__ double logit[kMaxExperts];
+  __shared__ uint64_t key[kMaxExperts];
+  __shared__ int place[kMaxChosen];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t m = blockIdx.x;
+  const T* row = x + m * D;
+  for (int e = tid >> 6; e < E; e += 4) {
+    double sum = 0.;
+    for (int d = 4 * lane; d < D; d += 256) {
+      const float4 w = *reinterpret_cast<const float4*>(router + (int64_t)e * D + d);
+      float b[4];
+      load_four<T>(row + d, b);
+      sum = fma((double)w.x, (double)b[0], sum);
+      sum = fma((double)w.y, (double)b[1], sum);
+      sum = fma((double)w.z, (double)b[2], sum);
+      sum = fma((double)w.w, (double)b[3], sum);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) {
+      logit[e] = sum;
+      key[e] = order_key64(bias ? sum + (double)bias[e] : sum);
+    }
+  }
+  if (tid < k) place[tid] = -1;
+  __syncthreads();
+  if (!counts || m % per_row < counts[m / per_row]) place_experts(key, tid, 256, E, k, place);
+  __syncthreads();
+  if (tid < k) store_choice(logit, place, tid, k, chosen + m * k + tid, gates + m * k + tid);
+}
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+constexpr int kAhead = 4;  // steps whose loads a wavefront waits for together
+
+// The logits of a wider one on the 64-bit matrix instruction (16 experts by 16
+// tokens by 4 columns; the product of two FP32 values is exact): grid (E / 16,
+// rows / 16, splits), workgroup z's four wavefronts taking the 16-column steps
+// 4 z + wv, 4 z + wv + 4 splits, ...; sums[z] [rows, E] in 64 bits.  A lane's four
+// columns are the steps' four instructions.
+template <typename T>
+__global__ __launch_bounds__(256) void route_logits(const T* __restrict__ x, const float* __restrict__ router, int rows,
+                                                    int D, int E, double* __restrict__ sums) {
+  __shared__ double red[4][256];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, j = lane & 15, g = lane >> 4;
+  const int e0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+  const float* w = router + (int64_t)min(e0 + j, E - 1) * D;
+  const T* row = x + (int64_t)min(m0 + j, rows - 1) * D;
+  f64x4 acc = {0., 0., 0., 0.};
+  const int steps = (D + 15) / 16, stride = 4 * (int)gridDim.z;
+  for (int first = 4 * (int)blockIdx.z + __builtin_amdgcn_readfirstlane(wv); first < steps; first += kAhead * stride) {
+    float a[kAhead][4], b[kAhead][4];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {  // all asked for at once; past the width zeros
+      const int d = 16 * (first + u * stride) + 4 * g;
+      const bool inside = d < D;
+      load_four<float>(w + (inside ? d : 0), a[u]);
+      load_four<T>(row + (inside ? d : 0), b[u]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        a[u][i] = inside ? a[u][i] : 0.f;
+        b[u][i] = inside ? b[u][i] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (first + u * stride < steps)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)a[u][i], (double)b[u][i], acc, 0, 0, 0);
+  }
+  // register i of lane (j, g): expert 4 i + g, token j
+#pragma unroll
+  for (int i = 0; i < 4; ++i) red[wv][j * 16 + 4 * i + g] = acc[i];
+  __syncthreads();
+  const int m = m0 + (tid >> 4), e = e0 + (tid & 15);
+  if (m < rows && e < E)
+    sums[((int64_t)blockIdx.z * rows + m) * E + e] = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+}
+
+// A wavefront a token.
+__global__ __launch_bounds__(256) void route_choose(const double* __restrict__ sums, const float* __restrict__ bias,
+                                                    const int64_t* __restrict__ counts, int rows, int per_row, int E,
+                                                    int splits, int k, int* __restrict__ chosen,
+                                                    float* __restrict__ gates) {
+  __shared__ double logits[4][kMaxExperts];
+  __shared__ uint64_t keys[4][kMaxExperts];
+  __shared__ int places[4][kMaxChosen];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, m = blockIdx.x * 4 + wv;
+  double* logit = logits[wv];
+  const bool read = m < rows && (!counts || m % per_row < counts[m / per_row]);
+  if (lane < k) places[wv][lane] = -1;
+  if (read)
+    for (int e = lane; e < E; e += 64) {
+      double sum = 0.;
+      for (int z = 0; z < splits; ++z) sum += sums[((int64_t)z * rows + m) * E + e];
+      logit[e] = sum;
+      keys[wv][e] = order_key64(bias ? sum + (double)bias[e] : sum);
+    }
+  __syncthreads();
+  if (read) place_experts(keys[wv], lane, 64, E, k, places[wv]);
+  __syncthreads();
+  if (m < rows && lane < k)
+    store_choice(logit, places[wv], lane, k, chosen + (int64_t)m * k + lane, gates + (int64_t)m * k + lane);
+}
+
+// The router's form: one launch where a token's workgroup reads little, else the
+// parts the width is cut into (the tiles of 16 by 16 cover the compute units twice).
+int route_splits(int64_t rows, int D, int E) {
+  if ((int64_t)E * D <= 16384) return 0;
+  const int64_t tiles = (rows + 15) / 16 * ((E + 15) / 16);
+  const int64_t want = 512 / tiles, most = (D + 63) / 64;
+  const int64_t splits = want < 1 ? 1 : want < most ? want : most;
+  return (int)(splits < 32 ? splits : 32);
+}
+
 // ---- the experts' products ---------------------------------------------------
+
+// A buffer of up to 2 GiB, read 16 bytes a lane at a lane's offset and a uniform
+// one, both unsigned bytes; past the end a load gives zeros, and kOutside is past
+// every end.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+constexpr unsigned kOutside = 0x80000000u;
+constexpr int64_t kBufferBytes = 0x7fffff00;
+
+__device__ __forceinline__ Buffer buffer(const void* base, unsigned bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+
+__device__ __forceinline__ u32x4 load16(Buffer from, unsigned lane_offset, unsigned offset) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset, offset, 0));
+}
+
+// Weights: read once, no cache line kept for them.
+__device__ __forceinline__ u32x4 load16_once(Buffer from, unsigned lane_offset, unsigned offset) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset, offset, 2));
+}
 
 constexpr int kRange = 4096;  // pairs whose expert is looked up at a time
 
 enum Product { kGateUp = 0, kDown = 1 };
 
-// The pairs of the range [r0, r0 + kRange) that expert e takes, in their order:
-// wavefront w lists those of its quarter in list[w].  Returns their count.
-// e == E: the pairs of no expert.
-__device__ __forceinline__ int list_pairs(const int* __restrict__ chosen, int64_t r0, int64_t pairs, int e, int E,
-                                          int (*list)[kRange / 4], int* listed) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  int n = 0;
-  const uint64_t below = (1ull << lane) - 1ull;
-  for (int i = 0; i < kRange / 4; i += 64) {
-    const int64_t p = r0 + wv * (kRange / 4) + i + lane;
-    if (r0 + wv * (kRange / 4) + i >= pairs) break;
-    bool mine = false;
-    if (p < pairs) {
-      const int c = chosen[p];
-      mine = c == e || (e == E && (unsigned)c >= (unsigned)E);
-    }
-    const uint64_t found = __builtin_amdgcn_ballot_w64(mine);
-    if (mine) list[wv][n + __builtin_popcountll(found & below)] = (int)(p - r0);
-    n += __builtin_popcountll(found);
-  }
-  if (lane == 0) listed[wv] = n;
-  __syncthreads();
-  return listed[0] + listed[1] + listed[2] + listed[3];
-}
+// The pairs of a range [r0, r0 + kRange) that one expert takes, in their order,
+// listed by a workgroup of WAVES wavefronts, a stretch of the range each.
+template <int WAVES>
+struct PairList {
+  static constexpr int kTurns = kRange / WAVES / 64;
+  uint16_t list[kRange];
+  int listed[WAVES];
 
-// The i-th listed pair of the range.
-__device__ __forceinline__ int listed_pair(int i, const int (*list)[kRange / 4], const int* listed) {
+  // A thread's choices of a range (loaded ahead of other loads, whose arrival the
+  // list then does not wait for).
+  struct Choices {
+    int c[kTurns];
+  };
+
+  static __device__ __forceinline__ int turns(int here) { return (here + 64 * WAVES - 1) / (64 * WAVES); }
+
+  static __device__ __forceinline__ void load(Choices& choices, const int* __restrict__ chosen, int r0, int pairs) {
+    // the stretches follow the pairs' count, in whole wavefronts, so that a few pairs are listed by all at once
+    const int here = min(pairs - r0, kRange), many = turns(here);
+    const int at = (threadIdx.x >> 6) * many * 64 + (threadIdx.x & 63);
 #pragma unroll
-  for (int w = 0; w < 3; ++w) {
-    if (i < listed[w]) return list[w][i];
-    i -= listed[w];
+    for (int i = 0; i < kTurns; ++i)
+      if (i < many) choices.c[i] = chosen[r0 + min(at + 64 * i, here - 1)];
   }
-  return list[3][i];
+
+  // Lists expert e's pairs, counted from r0 (e == E: those of no expert), and
+  // returns their count.  Ends with a barrier.
+  __device__ __forceinline__ int fill(const Choices& choices, int r0, int pairs, int e, int E) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const uint64_t below = (1ull << lane) - 1ull;
+    const int here = min(pairs - r0, kRange), many = turns(here), begin = wv * many * 64;
+    auto mine = [&](int i) {
+      const int c = choices.c[i];
+      return begin + 64 * i + lane < here && (c == e || (e == E && (unsigned)c >= (unsigned)E));
+    };
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
+      if (i < many) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine(i)));
+    if (lane == 0) listed[wv] = n;
+    __syncthreads();
+    int total = 0, at = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      at += w < wv ? listed[w] : 0;
+      total += listed[w];
+    }
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i)
+      if (i < many) {
+        const uint64_t found = __builtin_amdgcn_ballot_w64(mine(i));
+        if (mine(i)) list[at + __builtin_popcountll(found & below)] = (uint16_t)(begin + 64 * i + lane);
+        at += __builtin_popcountll(found);
+      }
+    __syncthreads();
+    return total;
+  }
+
+  __device__ __forceinline__ int at(int i) const { return list[i]; }
+};
+
+// The parts' rows that no expert of the range writes, cleared by workgroups of
+// their own, the grid's first `groups` (at least one) of each column.
+template <int WAVES>
+__device__ __forceinline__ void clear_rows(const PairList<WAVES>& pairs, int n, int r0, int group, int groups, int first, int last, int D,
+                                           int64_t total, int k, float* __restrict__ parts) {
+  const int lane = threadIdx.x & 63;
+  for (int i = group * WAVES + (threadIdx.x >> 6); i < n; i += groups * WAVES) {  // a wavefront a row
+    const int p = r0 + pairs.at(i);
+    float* to = parts + ((p % k) * total + p / k) * D;
+    for (int d = first + 4 * lane; d < min(D, last); d += 256) *reinterpret_cast<f32x4*>(to + d) = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 }
 
-// grid (row-block pairs / (4 / KW), experts or pairs): a workgroup's four
-// wavefronts take 4 / KW row-block pairs of one expert's matrix, KW of them the
-// k-steps of one pair in turn (their sums joined in LDS, in order), over tiles of
-// 16 NT of the expert's tokens.  The weights are the A operand, the tokens the B
-// operand, both straight from memory into registers, kDepth k-steps ahead.
-//   kGateUp   x [rows, D] -> act [pairs, Fp]: silu(g) u of the FP32 sums, rounded
-//             once to T, which the down product takes
-//   kDown     act -> parts [k, rows, D]: gates[p] times the product, FP32
+// What the two products store.  The gate scales silu(g) u before its one rounding,
+// which is a relative one: the down product's sums are then the gated terms.
+template <typename T, int PRODUCT>
+__device__ __forceinline__ void store_block(f32x4 a, f32x4 b, int p, int block, int g, const ExpertShape& shape,
+                                            int64_t total, int k, const float* __restrict__ gates,
+                                            void* __restrict__ out) {
+  if constexpr (PRODUCT == kGateUp) {
+    const float gate = gates[p];
+    T* to = static_cast<T*>(out) + (int64_t)p * shape.Fp + 16 * block + 4 * g;
+    union {
+      T element[4];
+      unsigned int word[sizeof(T)];
+    } v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.element[i] = from_f32<T>(a[i] / (1.f + expf(-a[i])) * b[i] * gate);
+    typedef unsigned int words __attribute__((ext_vector_type(sizeof(T))));
+    *reinterpret_cast<words*>(to) = *reinterpret_cast<const words*>(v.word);
+  } else {
+    float* to = static_cast<float*>(out) + ((p % k) * total + p / k) * shape.D + 32 * block + 4 * g;
+    const int left = shape.D - 32 * block - 4 * g;
+    if (left > 0) *reinterpret_cast<f32x4*>(to) = a;
+    if (left > 16) *reinterpret_cast<f32x4*>(to + 16) = b;
+  }
+}
+
+// grid (row-block pairs, experts or pairs): a workgroup's four wavefronts share
+// out the k-steps of one row-block pair of one expert's matrix (their sums joined
+// in LDS, in order), over tiles of 16 NT of the expert's tokens.  The weights are
+// the A operand, the tokens the B operand, both straight from memory into
+// registers, kDepth k-steps ahead.
+//   kGateUp   x [rows, D] -> act [pairs, Fp]: gates[p] silu(g) u of the FP32 sums,
+//             rounded once to T, which the down product takes
+//   kDown     act -> parts [k, rows, D] FP32
 // BY_PAIR (fewer pairs than experts): workgroup y serves the expert of pair y,
 // if that is the expert's first.
-template <typename T, int PRODUCT, int NT, int KW, bool BY_PAIR>
-__global__ __launch_bounds__(256) void expert_product(const T* __restrict__ in, const u32x4* __restrict__ weights,
+template <typename T, int PRODUCT, int NT, bool BY_PAIR>
+__global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, const u32x4* __restrict__ weights,
                                                       const int* __restrict__ chosen, const float* __restrict__ gates,
-                                                      ExpertShape shape, int64_t rows, int E, int k,
-                                                      void* __restrict__ out) {
+                                                      ExpertShape shape, int rows, int64_t total, int E, int k,
+                                                      int clears, void* __restrict__ out) {
   using O = Operand<T>;
   constexpr int kDepth = NT == 1 ? 8 : 4;
-  __shared__ int list[4][kRange / 4];
-  __shared__ int listed[4];
-  __shared__ float red[KW == 1 ? 1 : 4 * NT * 2 * 4 * 64];
+  __shared__ PairList<4> list;
+  __shared__ float red[4 * NT * 2 * 4 * 64];
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t pairs = rows * k;
-  int e = blockIdx.y;
+  const int pairs = rows * k;
+  int e = BY_PAIR ? blockIdx.y : (int)blockIdx.y < clears ? E : blockIdx.y - clears;
   if constexpr (BY_PAIR) {
     const int at = e;
     e = chosen[at];
     for (int p = lane; p - lane < at; p += 64)
       if (__builtin_amdgcn_ballot_w64(p < at && chosen[p] == e)) return;
+    e = __builtin_amdgcn_readfirstlane(e);
     if ((unsigned)e >= (unsigned)E) e = E;  // no expert: several of them clear the same rows
   }
-  const int pairs_of_blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
   const int KS = PRODUCT == kGateUp ? shape.KSx : shape.KSf;
-  const int K = PRODUCT == kGateUp ? shape.D : shape.Fp;
-  const int block = blockIdx.x * (4 / KW) + wv / KW, part = wv % KW;
-  const bool live = block < pairs_of_blocks;
-  const int steps = live ? (KS - part + KW - 1) / KW : 0;
-  const u32x4* w0 = weights + (((int64_t)e * pairs_of_blocks + block) * 2 * KS + part) * 64 + lane;
-  const u32x4* w1 = w0 + (int64_t)KS * 64;
+  const unsigned width = (PRODUCT == kGateUp ? shape.D : shape.Fp) * sizeof(T);
+  const int block = blockIdx.x, blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
+  const int steps = (KS - wv + 3) / 4;
+  const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + block) * 2 * KS * 64, 2u * KS * 1024);
+  const Buffer x = buffer(in, (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width));
 
-  for (int64_t r0 = 0; r0 < pairs; r0 += kRange) {
-    const int n = list_pairs(chosen, r0, pairs, e, E, list, listed);
-    if (e == E) {  // rows that no expert takes
-      if constexpr (PRODUCT == kDown)
-        for (int i = 0; i < n; ++i) {
-          const int64_t p = r0 + listed_pair(i, list, listed);
-          float* to = static_cast<float*>(out) + ((p % k) * rows + p / k) * shape.D;
-          for (int d = blockIdx.x * (4 / KW) * 32 + threadIdx.x; d < min(shape.D, (int)(blockIdx.x + 1) * (4 / KW) * 32);
-               d += 256)
-            to[d] = 0.f;
-        }
+  for (int r0 = 0; r0 < pairs; r0 += kRange) {
+    PairList<4>::Choices choices;
+    list.load(choices, chosen, r0, pairs);
+    const int n = list.fill(choices, r0, pairs, e, E);
+    if (e == E) {
+      if (PRODUCT == kDown && clears > 0)
+        clear_rows(list, n, r0, BY_PAIR ? 0 : blockIdx.y, BY_PAIR ? 1 : clears, 32 * block, 32 * block + 32, shape.D, total, k, static_cast<float*>(out));
       __syncthreads();
       continue;
     }
     for (int first = 0; first < n; first += 16 * NT) {
-      int64_t pair[NT];
-      const T* row[NT];
+      int pair[NT];
+      unsigned row[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         // columns past the last token repeat it; nothing of them is stored
-        pair[t] = r0 + listed_pair(min(first + 16 * t + j, n - 1), list, listed);
-        row[t] = PRODUCT == kGateUp ? in + pair[t] / k * shape.D : in + pair[t] * shape.Fp;
+        pair[t] = r0 + list.at(min(first + 16 * t + j, n - 1));
+        row[t] = (PRODUCT == kGateUp ? pair[t] / k : pair[t]) * width + 16 * g;
       }
       f32x4 acc[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
       u32x4 wb[kDepth][2], xb[kDepth][NT];
       auto load = [&](int d, int s) {
-        wb[d][0] = w0[(int64_t)s * KW * 64];
-        wb[d][1] = w1[(int64_t)s * KW * 64];
-        const int col = O::KU * (part + KW * s) + O::EPL * g;
-        const bool inside = col < K;  // the last k-step's columns past the width are zero
+        const unsigned ks = wv + 4 * s;
+        wb[d][0] = load16_once(w, 16 * lane, 1024 * ks);
+        wb[d][1] = load16_once(w, 16 * lane, 1024 * (KS + ks));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const u32x4 v = *reinterpret_cast<const u32x4*>(row[t] + (inside ? col : 0));
-          xb[d][t] = inside ? v : u32x4{0u, 0u, 0u, 0u};
-        }
+        for (int t = 0; t < NT; ++t)  // columns past the width are zero, as the weights' padding
+          xb[d][t] = load16(x, 64 * ks + 16 * g < width ? row[t] : kOutside, 64 * ks);
       };
       auto multiply = [&](int d) {
 #pragma unroll
@@ -332,60 +492,199 @@ __global__ __launch_bounds__(256) void expert_product(const T* __restrict__ in, 
         for (int d = 0; d < kDepth; ++d)
           if (s + d < steps) multiply(d);
       }
-      auto store = [&](int t, f32x4 a, f32x4 b) {
-        if (!live || first + 16 * t + j >= n) return;
-        if constexpr (PRODUCT == kGateUp) {
-          T* to = static_cast<T*>(out) + pair[t] * shape.Fp + 16 * block + 4 * g;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) to[i] = from_f32<T>(a[i] / (1.f + expf(-a[i])) * b[i]);
-        } else {
-          const int64_t p = pair[t];
-          const float gate = gates[p];
-          float* to = static_cast<float*>(out) + ((p % k) * rows + p / k) * shape.D + 32 * block + 4 * g;
-          const int left = shape.D - 32 * block - 4 * g;
-          if (left > 0) *reinterpret_cast<f32x4*>(to) = gate * a;
-          if (left > 16) *reinterpret_cast<f32x4*>(to + 16) = gate * b;
-        }
-      };
-      if constexpr (KW == 1) {
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) store(t, acc[t][0], acc[t][1]);
-      } else {
-        static_assert(KW == 1 || KW == 4, "a block pair's k-steps over the whole workgroup, or one wavefront");
+        for (int i = 0; i < 8; ++i) red[((wv * NT + t) * 8 + i) * 64 + lane] = acc[t][i >> 2][i & 3];
+      __syncthreads();
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
+        if (t % 4 == wv && first + 16 * t + j < n) {
+          float sum[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) red[((wv * NT + t) * 8 + i) * 64 + lane] = acc[t][i >> 2][i & 3];
-        __syncthreads();
+          for (int i = 0; i < 8; ++i) {
+            sum[i] = red[(t * 8 + i) * 64 + lane];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-          if (t % 4 == wv) {
-            float sum[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              sum[i] = red[(t * 8 + i) * 64 + lane];
-#pragma unroll
-              for (int u = 1; u < 4; ++u) sum[i] += red[((u * NT + t) * 8 + i) * 64 + lane];
-            }
-            store(t, f32x4{sum[0], sum[1], sum[2], sum[3]}, f32x4{sum[4], sum[5], sum[6], sum[7]});
+            for (int u = 1; u < 4; ++u) sum[i] += red[((u * NT + t) * 8 + i) * 64 + lane];
           }
-        __syncthreads();
+          store_block<T, PRODUCT>(f32x4{sum[0], sum[1], sum[2], sum[3]}, f32x4{sum[4], sum[5], sum[6], sum[7]}, pair[t],
+                                  block, g, shape, total, k, gates, out);
+        }
+      __syncthreads();
+    }
+    __syncthreads();  // the lists are written again
+  }
+}
+
+// grid (row-block pairs / 8, experts): a workgroup's eight wavefronts take a
+// row-block pair of one expert's matrix each, over tiles of up to 64 of the
+// expert's tokens.  The tokens' columns go through LDS, kChunk k-steps at a time in
+// two buffers, in the order the matrix instructions take them; the weights go
+// straight from memory into registers, kTileDepth k-steps ahead, across the chunks'
+// barriers, which wait for LDS alone.
+constexpr int kTileWaves = 8, kTileTokens = 4, kChunk = 8, kTileDepth = 4;
+
+// A tile of NT times 16 tokens, `first` the list's place of the first.
+template <typename T, int PRODUCT, int NT>
+__device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned width,
+                                          const PairList<kTileWaves>& list, u32x4 (*xs)[kTileTokens * kChunk * 64],
+                                          int r0, int first, int n, int block, bool live, const ExpertShape& shape,
+                                          int64_t total, int k, const float* __restrict__ gates,
+                                          void* __restrict__ out) {
+  using O = Operand<T>;
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
+  u32x4 wb[kTileDepth][2], xr[NT];
+  auto load = [&](int d, int s) {
+    const unsigned ks = min(s, KS - 1);
+    wb[d][0] = load16_once(w, 16 * lane, 1024 * ks);
+    wb[d][1] = load16_once(w, 16 * lane, 1024 * (KS + ks));
+  };
+#pragma unroll
+  for (int d = 0; d < kTileDepth; ++d) load(d, d);
+  // thread tid stages piece tid % 32 of a chunk's columns of tokens tid / 32 + 16 i
+  const int piece = tid & 31, token = tid >> 5;
+  unsigned row[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int p = r0 + list.at(min(first + 16 * i + token, n - 1));
+    row[i] = (PRODUCT == kGateUp ? p / k : p) * width + 16 * piece;
+  }
+  auto fetch = [&](int c) {
+    const unsigned at = 64 * kChunk * c;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)  // columns past the width are zero, as the weights' padding
+      xr[i] = load16(in, at + 16 * piece < width ? row[i] : kOutside, at);
+  };
+  u32x4* to = xs[0] + (piece >> 2) * 64 + (piece & 3) * 16 + token;
+  auto stage = [&](int buffer) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) to[buffer * (kTileTokens * kChunk * 64) + i * kChunk * 64] = xr[i];
+  };
+  f32x4 acc[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto step = [&](const u32x4* x, int q, int s) {
+    const int d = q % kTileDepth;
+    u32x4 xb[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) xb[t] = x[(t * kChunk + q) * 64];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      acc[t][0] = O::mfma(wb[d][0], xb[t], acc[t][0]);
+      acc[t][1] = O::mfma(wb[d][1], xb[t], acc[t][1]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load(d, s + kTileDepth);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // LDS alone: this chunk's reads and the next one's writes; the loads from memory go on
+  auto barrier = [] {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  const int whole = KS / kChunk, left = KS % kChunk;
+  fetch(0);
+  stage(0);
+  barrier();
+  for (int c = 0; c < whole; ++c) {
+    const bool more = c + 1 < whole || left;
+    if (more) fetch(c + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const u32x4* x = xs[c & 1] + lane;
+#pragma unroll
+    for (int q = 0; q < kChunk; ++q) step(x, q, c * kChunk + q);
+    if (more) stage((c + 1) & 1);
+    barrier();
+  }
+  const u32x4* x = xs[whole & 1] + lane;
+#pragma unroll
+  for (int q = 0; q < kChunk - 1; ++q)
+    if (q < left) step(x, q, whole * kChunk + q);
+  if (left) barrier();
+  if (live)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      if (first + 16 * t + j < n)
+        store_block<T, PRODUCT>(acc[t][0], acc[t][1], r0 + list.at(first + 16 * t + j), block, g, shape, total, k, gates,
+                                out);
+}
+
+template <typename T, int PRODUCT>
+__global__ __launch_bounds__(64 * kTileWaves, 4) void expert_tiles(const T* __restrict__ in,
+                                                                   const u32x4* __restrict__ weights,
+                                                                   const int* __restrict__ chosen,
+                                                                   const float* __restrict__ gates, ExpertShape shape,
+                                                                   int rows, int64_t total, int E, int k, int clears,
+                                                                   void* __restrict__ out) {
+  __shared__ PairList<kTileWaves> list;
+  __shared__ u32x4 xs[2][kTileTokens * kChunk * 64];
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pairs = rows * k;
+  const int e = (int)blockIdx.y < clears ? E : blockIdx.y - clears;
+  const int KS = PRODUCT == kGateUp ? shape.KSx : shape.KSf;
+  const unsigned width = (PRODUCT == kGateUp ? shape.D : shape.Fp) * sizeof(T);
+  const int blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
+  const int block = blockIdx.x * kTileWaves + wv;
+  const bool live = block < blocks;
+  // wavefronts past the last row blocks multiply it again and store nothing
+  const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + min(block, blocks - 1)) * 2 * KS * 64,
+                          2u * KS * 1024);
+  const Buffer x = buffer(in, (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width));
+
+  for (int r0 = 0; r0 < pairs; r0 += kRange) {
+    PairList<kTileWaves>::Choices choices;
+    list.load(choices, chosen, r0, pairs);
+    const int n = list.fill(choices, r0, pairs, e, E);
+    if (e == E) {
+      if (PRODUCT == kDown && clears > 0)
+        clear_rows(list, n, r0, blockIdx.y, clears, 32 * (int)blockIdx.x * kTileWaves, 32 * (int)(blockIdx.x + 1) * kTileWaves, shape.D,
+                   total, k, static_cast<float*>(out));
+    } else {
+      for (int first = 0; first < n; first += 16 * kTileTokens) {
+#define WPTV_TILE(NT) \
+  tile_pass<T, PRODUCT, NT>(x, w, KS, width, list, xs, r0, first, n, block, live, shape, total, k, gates, out)
+        switch ((n - first + 15) / 16) {
+          case 1: WPTV_TILE(1); break;
+          case 2: WPTV_TILE(2); break;
+          case 3: WPTV_TILE(3); break;
+          default: WPTV_TILE(4); break;
+        }
+#undef WPTV_TILE
       }
     }
     __syncthreads();  // the lists are written again
   }
 }
 
-// y[m] = the sum of a token's parts in the order of its choices, rounded once.
+// y[m] = the sum of a token's parts in the order of its choices, rounded once; the
+// parts of no expert hold nothing and are passed over.
 template <typename T>
-__global__ __launch_bounds__(256) void join_experts(const float* __restrict__ parts, int64_t rows, int D, int k,
-                                                    T* __restrict__ y) {
+__global__ __launch_bounds__(256) void join_experts(const float* __restrict__ parts, const int* __restrict__ chosen,
+                                                    int64_t rows, int D, int E, int k, T* __restrict__ y) {
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= rows * D) return;
-  f32x4 sum = *reinterpret_cast<const f32x4*>(parts + at);
-  for (int i = 1; i < k; ++i) sum += *reinterpret_cast<const f32x4*>(parts + i * rows * D + at);
+  const int* choice = chosen + at / D * k;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int first = 0; first < k; first += 8) {
+    bool some[8];
+    f32x4 part[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[at + i] = from_f32<T>(sum[i]);
+    for (int i = 0; i < 8; ++i) some[i] = first + i < k && (unsigned)choice[min(first + i, k - 1)] < (unsigned)E;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)  // all asked for at once
+      part[i] = *reinterpret_cast<const f32x4*>(parts + (some[i] ? (first + i) * rows * D : 0) + at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += some[i] ? part[i] : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  union {
+    T element[4];
+    unsigned int word[sizeof(T)];
+  } v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.element[i] = from_f32<T>(sum[i]);
+  typedef unsigned int words __attribute__((ext_vector_type(sizeof(T))));
+  *reinterpret_cast<words*>(y + at) = *reinterpret_cast<const words*>(v.word);
 }
 
 // ---- host side ---------------------------------------------------------------
@@ -413,43 +712,65 @@ int check_features(const char* what, int F) {
   return WPTV_OK;
 }
 
+size_t route_bytes(int64_t rows, int D, int E) { return (size_t)route_splits(rows, D, E) * rows * E * sizeof(double); }
+
 template <typename T>
 int run_route(const void* x, const float* router, const float* bias, const int64_t* counts, int rows, int per_row, int D,
-              int E, int k, int* chosen, float* gates, hipStream_t stream) {
+              int E, int k, int* chosen, float* gates, void* workspace, hipStream_t stream) {
   const T* xt = static_cast<const T*>(x);
-  if (rows <= 256)
-    route<T, 1><<<rows, kRouteThreads, 0, stream>>>(xt, router, bias, counts, rows, per_row, D, E, k, chosen, gates);
-  else
-    route<T, 4><<<(rows + 3) / 4, kRouteThreads, 0, stream>>>(xt, router, bias, counts, rows, per_row, D, E, k, chosen,
-                                                             gates);
-  return launched("route");
+  const int splits = route_splits(rows, D, E);
+  if (splits == 0) {
+    route_token<T><<<rows, 256, 0, stream>>>(xt, router, bias, counts, per_row, D, E, k, chosen, gates);
+    return launched("route");
+  }
+  double* sums = static_cast<double*>(workspace);
+  // 2^19 tokens a launch: the grid's second dimension ends at 65535 (more tokens than that have one part)
+  for (int m = 0; m < rows; m += 1 << 19) {
+    const int here = rows - m < (1 << 19) ? rows - m : 1 << 19;
+    route_logits<T><<<dim3((E + 15) / 16, (here + 15) / 16, splits), 256, 0, stream>>>(
+        xt + (int64_t)m * D, router, here, D, E, sums + (int64_t)m * E);
+  }
+  const int status = launched("route (logits)");
+  if (status != WPTV_OK) return status;
+  route_choose<<<(rows + 3) / 4, 256, 0, stream>>>(sums, bias, counts, rows, per_row, E, splits, k, chosen, gates);
+  return launched("route (choice)");
 }
 
 template <typename T, int PRODUCT>
 int run_product(const void* in, const void* weights, const int* chosen, const float* gates, const ExpertShape& shape,
-                int64_t rows, int E, int k, void* out, hipStream_t stream) {
-  const int64_t pairs = rows * k;
+                int rows, int64_t total, int E, int k, bool clear, void* out, hipStream_t stream) {
+  const int64_t pairs = (int64_t)rows * k;
   const int blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
   const bool by_pair = pairs < E;
-  // one workgroup more clears the rows of no expert
-  const int lists = by_pair ? (int)pairs : E + (PRODUCT == kDown ? 1 : 0);
-#define WPTV_PRODUCT(NT, KW, BY)                                                                               \
-  expert_product<T, PRODUCT, NT, KW, BY><<<dim3((blocks * KW + 3) / 4, lists), 256, 0, stream>>>(              \
-      static_cast<const T*>(in), static_cast<const u32x4*>(weights), chosen, gates, shape, rows, E, k, out)
+  const int clears = !clear ? 0 : by_pair || pairs < 1024 ? 1 : 16;
+  const int lists = by_pair ? (int)pairs : E + clears;
+  const T* from = static_cast<const T*>(in);
+  const u32x4* w = static_cast<const u32x4*>(weights);
+#define WPTV_COLUMNS(NT, BY)                                                                                         \
+  expert_columns<T, PRODUCT, NT, BY><<<dim3(blocks, lists), 256, 0, stream>>>(from, w, chosen, gates, shape, rows, total, \
+                                                                              E, k, clears, out)
   if (by_pair)
-    WPTV_PRODUCT(1, 4, true);
+    WPTV_COLUMNS(1, true);
   else if (rows <= 16)
-    WPTV_PRODUCT(1, 4, false);
-  else if (pairs <= 16 * (int64_t)E)
-    WPTV_PRODUCT(2, 1, false);
+    WPTV_COLUMNS(1, false);
+  else if ((int64_t)E * blocks < 2048)
+    WPTV_COLUMNS(2, false);
   else
-    WPTV_PRODUCT(4, 1, false);
-#undef WPTV_PRODUCT
+    expert_tiles<T, PRODUCT><<<dim3((blocks + kTileWaves - 1) / kTileWaves, lists), 64 * kTileWaves, 0, stream>>>(
+        from, w, chosen, gates, shape, rows, total, E, k, clears, out);
+#undef WPTV_COLUMNS
   return launched(PRODUCT == kGateUp ? "experts (gate, up)" : "experts (down)");
 }
 
+// The rows of one round of the two products: their operands stay within a buffer.
+int round_rows(int64_t rows, int k, const ExpertShape& shape, int dtype) {
+  const int64_t widest = (dtype == WPTV_BF16 ? 2 : 4) * (shape.D > (int64_t)k * shape.Fp ? shape.D : (int64_t)k * shape.Fp);
+  const int64_t fit = kBufferBytes / widest;
+  return (int)(rows < fit ? rows : fit);
+}
+
 size_t act_bytes(int64_t rows, int k, const ExpertShape& shape, int dtype) {
-  return align_up((size_t)rows * k * shape.Fp * (dtype == WPTV_BF16 ? 2 : 4), 256);
+  return align_up((size_t)round_rows(rows, k, shape, dtype) * k * shape.Fp * (dtype == WPTV_BF16 ? 2 : 4), 256);
 }
 
 template <typename T>
@@ -458,12 +779,20 @@ int run_experts(const void* x, const void* gate_up, const void* down, const int*
                 hipStream_t stream) {
   char* act = static_cast<char*>(workspace);
   float* sums = parts ? parts : reinterpret_cast<float*>(act + act_bytes(rows, k, shape, dtype));
-  int status = run_product<T, kGateUp>(x, gate_up, chosen, gates, shape, rows, E, k, act, stream);
-  if (status != WPTV_OK) return status;
-  status = run_product<T, kDown>(act, down, chosen, gates, shape, rows, E, k, sums, stream);
-  if (status != WPTV_OK || parts) return status;
+  const int round = round_rows(rows, k, shape, dtype);
+  for (int64_t m = 0; m < rows; m += round) {
+    const int here = rows - m < round ? (int)(rows - m) : round;
+    int status = run_product<T, kGateUp>(static_cast<const T*>(x) + m * shape.D, gate_up, chosen + m * k, gates + m * k,
+                                         shape, here, rows, E, k, false, act, stream);
+    if (status != WPTV_OK) return status;
+    status = run_product<T, kDown>(act, down, chosen + m * k, gates + m * k, shape, here, rows, E, k, parts != nullptr,
+                                   sums + m * shape.D, stream);
+    if (status != WPTV_OK) return status;
+  }
+  if (parts) return WPTV_OK;
   const int64_t threads = rows * shape.D / 4;
-  join_experts<T><<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(sums, rows, shape.D, k, static_cast<T*>(y));
+  join_experts<T><<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(sums, chosen, rows, shape.D, E, k,
+                                                                              static_cast<T*>(y));
   return launched("experts (join)");
 }
 
@@ -490,13 +819,18 @@ int check_experts(const char* what, const void* x, const void* gate_up, const vo
 }
 
 int check_route(const char* what, const void* x, const float* router, int B, int T, int D, int E, int k, int dtype,
-                const int* chosen, const float* gates) {
+                const int* chosen, const float* gates, const void* workspace, size_t workspace_bytes) {
   if (B < 0 || T < 0) return fail(WPTV_E_INVALID, "%s: bad shape B=%d T=%d", what, B, T);
   const int status = check_shape(what, (int64_t)B * T, D, E, k, dtype);
   if (status != WPTV_OK) return status;
   if ((int64_t)B * T == 0) return WPTV_OK;
   if (!x || !router || !chosen || !gates) return fail(WPTV_E_INVALID, "%s: a required pointer is NULL", what);
-  if (!aligned(x, 16) || !aligned(router, 16)) return fail(WPTV_E_INVALID, "%s: rows must be 16-byte aligned", what);
+  if (!aligned(x, 16) || !aligned(router, 16) || !aligned(workspace, 16))
+    return fail(WPTV_E_INVALID, "%s: rows must be 16-byte aligned", what);
+  const size_t need = route_bytes((int64_t)B * T, D, E);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(WPTV_E_INVALID, "%s: the workspace holds %zu bytes; %zu are needed", what, workspace ? workspace_bytes : 0,
+                need);
   return WPTV_OK;
 }
 
@@ -542,13 +876,23 @@ extern "C" int wptv_pack_experts(const void* gate_up, const void* down, int E, i
   return launched("pack_experts");
 }
 
+extern "C" int wptv_route_workspace(int rows, int D, int E, size_t* bytes) {
+  const int status = check_shape("route_workspace", rows, D, E, 1, WPTV_F32);
+  if (status != WPTV_OK) return status;
+  if (!bytes) return fail(WPTV_E_INVALID, "route_workspace: a required pointer is NULL");
+  *bytes = route_bytes(rows, D, E);
+  return WPTV_OK;
+}
+
 extern "C" int wptv_route(const void* x, int dtype, const float* router, const float* bias, const int64_t* counts, int B,
-                          int T, int D, int E, int k, int32_t* chosen, float* gates, hipStream_t stream) {
-  const int status = check_route("route", x, router, B, T, D, E, k, dtype, chosen, gates);
+                          int T, int D, int E, int k, int32_t* chosen, float* gates, void* workspace,
+                          size_t workspace_bytes, hipStream_t stream) {
+  const int status =
+      check_route("route", x, router, B, T, D, E, k, dtype, chosen, gates, workspace, workspace_bytes);
   if (status != WPTV_OK || (int64_t)B * T == 0) return status;
   return dtype == WPTV_BF16
-             ? run_route<unsigned short>(x, router, bias, counts, B * T, T, D, E, k, chosen, gates, stream)
-             : run_route<float>(x, router, bias, counts, B * T, T, D, E, k, chosen, gates, stream);
+             ? run_route<unsigned short>(x, router, bias, counts, B * T, T, D, E, k, chosen, gates, workspace, stream)
+             : run_route<float>(x, router, bias, counts, B * T, T, D, E, k, chosen, gates, workspace, stream);
 }
 
 extern "C" int wptv_experts_workspace(int rows, int D, int F, int k, int dtype, int parts_out, size_t* bytes) {
@@ -574,16 +918,27 @@ extern "C" int wptv_experts(const void* x, int dtype, const void* gate_up_packed
                                                  parts, y, workspace, stream);
 }
 
+extern "C" int wptv_mixture_workspace(int rows, int D, int E, int F, int k, int dtype, int parts_out, size_t* bytes) {
+  size_t products = 0, sums = 0;
+  int status = wptv_experts_workspace(rows, D, F, k, dtype, parts_out, &products);
+  if (status == WPTV_OK) status = wptv_route_workspace(rows, D, E, &sums);
+  if (status != WPTV_OK) return status;
+  if (!bytes) return fail(WPTV_E_INVALID, "mixture_workspace: a required pointer is NULL");
+  *bytes = products > sums ? products : sums;  // one after the other
+  return WPTV_OK;
+}
+
 extern "C" int wptv_mixture(const void* x, int dtype, const float* router, const float* bias, const int64_t* counts,
                             int B, int T, int D, int E, int k, int F, const void* gate_up_packed,
                             const void* down_packed, int32_t* chosen, float* gates, float* parts, void* y,
                             void* workspace, size_t workspace_bytes, hipStream_t stream) {
-  int status = check_route("mixture", x, router, B, T, D, E, k, dtype, chosen, gates);
+  int status = check_route("mixture", x, router, B, T, D, E, k, dtype, chosen, gates, workspace, workspace_bytes);
   if (status == WPTV_OK)
     status = check_experts("mixture", x, gate_up_packed, down_packed, chosen, gates, (int64_t)B * T, D, E, k, F, dtype,
                            parts, y, workspace, workspace_bytes);
   if (status != WPTV_OK) return status;
-  status = wptv_route(x, dtype, router, bias, counts, B, T, D, E, k, chosen, gates, stream);
+  // the router's sums are read before the products write
+  status = wptv_route(x, dtype, router, bias, counts, B, T, D, E, k, chosen, gates, workspace, workspace_bytes, stream);
   if (status != WPTV_OK) return status;
   return wptv_experts(x, dtype, gate_up_packed, down_packed, chosen, gates, B * T, D, E, k, F, parts, y, workspace,
                       workspace_bytes, stream);

@@ -103,8 +103,10 @@ def route(x, router, k, bias=None, counts=None):
     chosen = torch.empty(B, T, k, dtype=torch.int32, device=x.device)
     gates = torch.empty(B, T, k, dtype=torch.float32, device=x.device)
     with _lib.on(x.device):
+        _, size = _lib.plan("wptv_route_workspace", "route", B * T, D, E)
+        workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         check(_lib.lib().wptv_route(ptr(x_), dtype, ptr(router), ptr(bias), ptr(counts), B, T, D, E, int(k),
-                                    ptr(chosen), ptr(gates), _lib.stream(x.device)), "route")
+                                    ptr(chosen), ptr(gates), ptr(workspace), size, _lib.stream(x.device)), "route")
     return chosen, _forward_only(gates, x, router)
 
 
@@ -114,14 +116,13 @@ def _match(x, weights, what):
                          f"got {tuple(x.shape)} {x.dtype} on {x.device}")
 
 
-def _result(x, dtype, F, k, parts):
-    """(parts, y, workspace, its bytes) of a call on x."""
+def _result(x, size, k, parts):
+    """(parts, y, workspace) of a call on x."""
     B, T, D = x.shape
-    _, size = _lib.plan("wptv_experts_workspace", "experts", B * T, D, F, int(k), dtype, int(parts))
     workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     if parts:
-        return torch.empty(int(k), B * T, D, dtype=torch.float32, device=x.device), None, workspace, size
-    return None, torch.empty(B, T, D, dtype=x.dtype, device=x.device), workspace, size
+        return torch.empty(int(k), B * T, D, dtype=torch.float32, device=x.device), None, workspace
+    return None, torch.empty(B, T, D, dtype=x.dtype, device=x.device), workspace
 
 
 def _feed_forward(x, weights, chosen, gates, parts):
@@ -132,7 +133,8 @@ def _feed_forward(x, weights, chosen, gates, parts):
         if t.shape != (B, T, k) or t.dtype != kind or t.device != x.device or k == 0:
             raise ValueError(f"{name} must be {kind} (B={B}, T={T}, k) on {x.device}; got {t.dtype} {tuple(t.shape)}")
     with _lib.on(x.device):
-        out, y, workspace, size = _result(x_, dtype, weights.features, k, parts)
+        _, size = _lib.plan("wptv_experts_workspace", "feed_forward", B * T, D, weights.features, k, dtype, int(parts))
+        out, y, workspace = _result(x_, size, k, parts)
         check(_lib.lib().wptv_experts(ptr(x_), dtype, ptr(weights.gate_up), ptr(weights.down), ptr(chosen.contiguous()),
                                       ptr(gates.contiguous()), B * T, D, weights.experts, k, weights.features, ptr(out),
                                       ptr(y), ptr(workspace), size, _lib.stream(x.device)), "feed_forward")
@@ -163,7 +165,8 @@ def _mixture(x, router, weights, k, bias, counts, parts):
     chosen = torch.empty(B, T, k, dtype=torch.int32, device=device)
     gates = torch.empty(B, T, k, dtype=torch.float32, device=device)
     with _lib.on(device):
-        out, y, workspace, size = _result(x_, dtype, weights.features, k, parts)
+        _, size = _lib.plan("wptv_mixture_workspace", "mixture", B * T, D, E, weights.features, int(k), dtype, int(parts))
+        out, y, workspace = _result(x_, size, k, parts)
         check(_lib.lib().wptv_mixture(ptr(x_), dtype, ptr(router_), ptr(bias), ptr(counts), B, T, D, E, int(k),
                                       weights.features, ptr(weights.gate_up), ptr(weights.down), ptr(chosen), ptr(gates),
                                       ptr(out), ptr(y), ptr(workspace), size, _lib.stream(device)), "mixture")
