@@ -109,36 +109,41 @@ __device__ __forceinline__ uint64_t order_key64(double f) {
 constexpr int kMaxExperts = 512, kMaxChosen = 16;
 
 // The places of a token's experts (the count of those before each), by the
-// `threads` threads tid, tid + threads, ... of its own; place holds -1 before.
+// `threads` threads tid, tid + threads, ... of its own; place holds -1 before.  key
+// is filled up to a multiple of 8 with keys that are before none (0).
 __device__ __forceinline__ void place_experts(const uint64_t* key, int tid, int threads, int E, int k, int* place) {
   const uint64_t none = order_key64(-__builtin_inf());
   for (int e = tid; e < E; e += threads) {
     const uint64_t mine = key[e];
     int before = 0;
-    for (int i = 0; i < E; ++i) {
-      const uint64_t other = key[i];
-      before += other > mine || (other == mine && i < e) ? 1 : 0;
+    for (int i = 0; i < E; i += 8) {
+      uint64_t other[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) other[u] = key[i + u];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) before += other[u] > mine || (other[u] == mine && i + u < e) ? 1 : 0;
     }
     if (before < k && mine != none) place[before] = e;
   }
 }
 
-// Choice i of a token and its gate, the softmax of the chosen logits in 64 bits.
-__device__ __forceinline__ void store_choice(const double* logit, const int* place, int i, int k, int* chosen,
-                                             float* gates) {
-  double high = -__builtin_inf(), total = 0.;
-  bool nan = false;
-  for (int c = 0; c < k; ++c)
-    if (place[c] >= 0) {
-      const double l = logit[place[c]];
-      nan |= l != l;
-      high = fmax(high, l);
-    }
-  for (int c = 0; c < k; ++c)
-    if (place[c] >= 0) total += exp(logit[place[c]] - high);
-  const int e = place[i];
-  *chosen = e;
-  *gates = e < 0 ? 0.f : nan ? __builtin_nanf("") : (float)(exp(logit[e] - high) / total);
+// A token's choices and gates, the softmax of the chosen logits in 64 bits, by the
+// first 16 lanes of a wavefront (every lane calls).
+__device__ __forceinline__ void store_choices(const double* logit, const int* place, int lane, int k,
+                                              int* __restrict__ chosen, float* __restrict__ gates) {
+  const int e = lane < k ? place[lane] : -1;
+  const double l = e < 0 ? -__builtin_inf() : logit[e];
+  double high = l;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) high = fmax(high, __shfl_xor(high, o, 64));
+  const double share = e < 0 ? 0. : exp(l - high);  // a NaN among them, or +inf, makes the total one
+  double total = share;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+  if (lane < k) {
+    chosen[lane] = e;
+    gates[lane] = e < 0 ? 0.f : (float)(share / total);
+  }
 }
 
 template <typename T>
@@ -160,7 +165,7 @@ __global__ __launch_bounds__(256) void route_token(const T* __restrict__ x, cons
                                                    int per_row, int D, int E, int k, int* __restrict__ chosen,
                                                    float* __restrict__ gates) {
   __shared__ double logit[kMaxExperts];
-  __shared__ uint64_t key[kMaxExperts];
+  __shared__ uint64_t key[kMaxExperts + 8];
   __shared__ int place[kMaxChosen];
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t m = blockIdx.x;
@@ -184,10 +189,11 @@ __global__ __launch_bounds__(256) void route_token(const T* __restrict__ x, cons
     }
   }
   if (tid < k) place[tid] = -1;
+  if (tid < 8) key[E + tid] = 0;
   __syncthreads();
   if (!counts || m % per_row < counts[m / per_row]) place_experts(key, tid, 256, E, k, place);
   __syncthreads();
-  if (tid < k) store_choice(logit, place, tid, k, chosen + m * k + tid, gates + m * k + tid);
+  if (tid < 64) store_choices(logit, place, lane, k, chosen + m * k, gates + m * k);
 }
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -244,24 +250,30 @@ __global__ __launch_bounds__(256) void route_choose(const double* __restrict__ s
                                                     int splits, int k, int* __restrict__ chosen,
                                                     float* __restrict__ gates) {
   __shared__ double logits[4][kMaxExperts];
-  __shared__ uint64_t keys[4][kMaxExperts];
+  __shared__ uint64_t keys[4][kMaxExperts + 8];
   __shared__ int places[4][kMaxChosen];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, m = blockIdx.x * 4 + wv;
   double* logit = logits[wv];
   const bool read = m < rows && (!counts || m % per_row < counts[m / per_row]);
   if (lane < k) places[wv][lane] = -1;
+  if (lane < 8) keys[wv][E + lane] = 0;
   if (read)
     for (int e = lane; e < E; e += 64) {
       double sum = 0.;
-      for (int z = 0; z < splits; ++z) sum += sums[((int64_t)z * rows + m) * E + e];
+      for (int z = 0; z < splits; z += 8) {
+        double part[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) part[u] = sums[((int64_t)min(z + u, splits - 1) * rows + m) * E + e];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) sum += z + u < splits ? part[u] : 0.;
+      }
       logit[e] = sum;
       keys[wv][e] = order_key64(bias ? sum + (double)bias[e] : sum);
     }
   __syncthreads();
   if (read) place_experts(keys[wv], lane, 64, E, k, places[wv]);
   __syncthreads();
-  if (m < rows && lane < k)
-    store_choice(logit, places[wv], lane, k, chosen + (int64_t)m * k + lane, gates + (int64_t)m * k + lane);
+  if (m < rows) store_choices(logit, places[wv], lane, k, chosen + (int64_t)m * k, gates + (int64_t)m * k);
 }
 
 // The router's form: one launch where a token's workgroup reads little, else the
@@ -522,7 +534,7 @@ __global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, 
 // two buffers, in the order the matrix instructions take them; the weights go
 // straight from memory into registers, kTileDepth k-steps ahead, across the chunks'
 // barriers, which wait for LDS alone.
-constexpr int kTileWaves = 8, kTileTokens = 4, kChunk = 8, kTileDepth = 4;
+constexpr int kTileWaves = 4, kTileTokens = 4, kChunk = 4, kTileDepth = 4;
 
 // A tile of NT times 16 tokens, `first` the list's place of the first.
 template <typename T, int PRODUCT, int NT>
@@ -534,15 +546,17 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
   using O = Operand<T>;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
   u32x4 wb[kTileDepth][2], xr[NT];
+  const unsigned at = live ? 16 * lane : kOutside;  // wavefronts past the last row blocks load nothing
   auto load = [&](int d, int s) {
     const unsigned ks = min(s, KS - 1);
-    wb[d][0] = load16_once(w, 16 * lane, 1024 * ks);
-    wb[d][1] = load16_once(w, 16 * lane, 1024 * (KS + ks));
+    wb[d][0] = load16_once(w, at, 1024 * ks);
+    wb[d][1] = load16_once(w, at, 1024 * (KS + ks));
   };
 #pragma unroll
   for (int d = 0; d < kTileDepth; ++d) load(d, d);
-  // thread tid stages piece tid % 32 of a chunk's columns of tokens tid / 32 + 16 i
-  const int piece = tid & 31, token = tid >> 5;
+  // a thread stages one 16-byte piece of a chunk's columns of every 16th token
+  static_assert(kTileWaves == kChunk, "16 tokens a turn");
+  const int piece = tid % (4 * kChunk), token = tid / (4 * kChunk);
   unsigned row[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
@@ -550,10 +564,10 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
     row[i] = (PRODUCT == kGateUp ? p / k : p) * width + 16 * piece;
   }
   auto fetch = [&](int c) {
-    const unsigned at = 64 * kChunk * c;
+    const unsigned column = 64 * kChunk * c;
 #pragma unroll
     for (int i = 0; i < NT; ++i)  // columns past the width are zero, as the weights' padding
-      xr[i] = load16(in, at + 16 * piece < width ? row[i] : kOutside, at);
+      xr[i] = load16(in, column + 16 * piece < width ? row[i] : kOutside, column);
   };
   u32x4* to = xs[0] + (piece >> 2) * 64 + (piece & 3) * 16 + token;
   auto stage = [&](int buffer) {
@@ -611,7 +625,7 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
 }
 
 template <typename T, int PRODUCT>
-__global__ __launch_bounds__(64 * kTileWaves, 4) void expert_tiles(const T* __restrict__ in,
+__global__ __launch_bounds__(64 * kTileWaves, 3) void expert_tiles(const T* __restrict__ in,
                                                                    const u32x4* __restrict__ weights,
                                                                    const int* __restrict__ chosen,
                                                                    const float* __restrict__ gates, ExpertShape shape,
@@ -627,7 +641,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 4) void expert_tiles(const T* __re
   const int blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
   const int block = blockIdx.x * kTileWaves + wv;
   const bool live = block < blocks;
-  // wavefronts past the last row blocks multiply it again and store nothing
   const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + min(block, blocks - 1)) * 2 * KS * 64,
                           2u * KS * 1024);
   const Buffer x = buffer(in, (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width));
