@@ -44,12 +44,14 @@ once under autocast):
     layers.{i}.down (D, F)
     window layers also: layers.{i}.gate (H*c, D), layers.{i}.sink (H,)
     sparse layers: layers.{i}.q (H*c, D) in place of qkv, no k_norm; gate, sink
+    blocks of experts: layers.{i}.router (E, D), gate_up (E, 2F, D), down
+        (E, D, F), and router_bias (E,) where there is one
 """
 
 import torch
 import torch.nn.functional as F
 
-from . import attention, cache
+from . import attention, cache, experts
 
 EPS = 1e-6
 
@@ -77,10 +79,10 @@ def bf16_dense_attention(q, k, v, sink, visible, scale):
 
 class Decoder:
     def __init__(self, weights, layers, heads, head_dim, kinds=(), window=128, rope_dims=64, rope_base=10000.0,
-                 top_k=1024, autocast=False):
-        self.autocast = autocast
+                 top_k=1024, autocast=False, experts_per_token=0):
+        self.autocast, self.experts_per_token = autocast, experts_per_token
         if autocast:  # matrices rounded to bf16 once (held as FP32 values); norm weights and sinks FP32
-            self.w = {name: value.float() if name.endswith("norm") or name.endswith("sink")
+            self.w = {name: value.float() if name.endswith(("norm", "sink", "router", "router_bias"))
                       else value.to(torch.bfloat16).float() for name, value in weights.items()}
         else:
             self.w = {name: value.float() for name, value in weights.items()}
@@ -95,6 +97,9 @@ class Decoder:
         # against the layer's own choice kept in choices[i] = (chosen, q,
         # keys, positions) of the last reading
         self.given, self.choices = {}, {}
+        # likewise the experts each layer's tokens take (given_routes[i], (B, T, k) with -1 for none), and what the
+        # layer's router gave: routed[i] = (chosen, x) of the last reading
+        self.given_routes, self.routed = {}, {}
 
     def new_cache(self, rows):
         return cache.Rows(rows)
@@ -152,8 +157,24 @@ class Decoder:
         B, T, H, c = o.shape
         h = h + self._linear(o.reshape(B, T, H * c), w("out"))
         x = self._norm(h, w("ffn_norm"))
+        if f"layers.{i}.router" in self.w:
+            return h + self._experts(i, x)
         gate, up = self._linear(x, w("gate_up")).chunk(2, -1)
         return h + self._linear(F.silu(gate) * up, w("down"))
+
+    def _experts(self, i, x):
+        """The gated sum of each token's experts, in 64 bits but for x."""
+        w = lambda name: self.w[f"layers.{i}.{name}"]  # noqa: E731
+        bias = self.w.get(f"layers.{i}.router_bias")
+        chosen, gates = experts.route(x, w("router"), self.experts_per_token, bias)
+        self.routed[i] = (chosen, x)
+        if i in self.given_routes:
+            chosen = self.given_routes[i]
+            logits = x.double() @ w("router").double().T
+            taken = torch.where(chosen >= 0, logits.gather(-1, chosen.clamp(min=0).long()), -torch.inf)
+            gates = torch.nan_to_num(torch.softmax(taken, -1))
+        y, _ = experts.feed_forward(x, w("gate_up"), w("down"), chosen, gates)
+        return y.to(x.dtype)
 
     def extend(self, ids, rows, counts=None, undoable=False, features=()):
         """(scores (B, n, V) FP32, hidden (B, n, D)) of ids (B, n), row b's

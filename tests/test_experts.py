@@ -2,6 +2,7 @@
 hand, and what the entry points refuse before anything runs."""
 
 import ctypes
+import json
 import math
 
 import pytest
@@ -9,7 +10,8 @@ import torch
 
 from oracle import experts as oracle
 from oracle import log_probs as oracle_log_probs
-from wpt_amd import _lib, experts, sampling
+from wpt_amd import _lib, experts, folder, sampling
+from wpt_amd.decoder import DecoderConfig, random_weights
 
 INF, NAN = math.inf, math.nan
 
@@ -148,3 +150,25 @@ def test_tensors_off_the_gpu_and_mismatched_ones_are_refused():
         sampling.log_probs(torch.zeros(1, 2, 8), torch.zeros(1, 2, dtype=torch.long))
     with pytest.raises(ValueError):
         sampling.log_probs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.long))
+
+
+@pytest.mark.parametrize("experts_, per_token", [(-1, 0), (4, 0), (0, 2), (4, 5), (20, 9)])
+def test_a_decoder_s_experts_are_whole(experts_, per_token):
+    with pytest.raises(ValueError):
+        DecoderConfig(layers=1, d_model=64, heads=1, head_dim=64, ffn=32, vocab=64, experts=experts_,
+                      experts_per_token=per_token)
+
+
+def test_a_folder_keeps_a_decoder_s_experts(tmp_path):
+    config = DecoderConfig(layers=2, d_model=64, heads=1, head_dim=64, ffn=24, vocab=64, experts=5, experts_per_token=2)
+    weights = random_weights(config, dtype=torch.bfloat16)
+    assert weights["layers.1.gate_up"].shape == (5, 48, 64) and weights["layers.0.router"].dtype == torch.float32
+    folder.save_folder(config, weights, tmp_path, b"{}", "test version 1")
+    folder.save_drafter_record(tmp_path)
+    loaded_config, loaded = folder.load_weights(tmp_path)
+    assert loaded_config == config and all(torch.equal(weights[k], loaded[k]) for k in weights)
+    # a folder written before there were experts
+    fields = json.loads((tmp_path / folder.CONFIG_NAME).read_text())
+    del fields["experts"], fields["experts_per_token"]
+    (tmp_path / folder.CONFIG_NAME).write_text(json.dumps(fields))
+    assert folder.load_weights(tmp_path)[0].experts == 0

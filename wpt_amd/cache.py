@@ -33,6 +33,10 @@ in place: from then on token p is no longer at row p of the exact layers' tables
 entries taken out, so that the window layers' rings still place token
 lengths + evicted.
 
+A cache that records routes also keeps, beside each token's entries, the experts
+each layer's router chose for it (`routes`, int32 (layers, B, capacity, k), -1 where
+none was read), written by each reading at its rows' places and cut back with them.
+
 The lengths stay on the device; `bound` is a host-side upper bound of every
 row's length (raised by each reading's width, never lowered by undo) so that
 growing the tables needs no host synchronization.  The tables grow to
@@ -61,10 +65,13 @@ class Cache:
     layers); bare: the layers with no table (sparse layers); every other
     layer's table grows with the text.  weighted: the growing tables' rows
     carry the attention weight they have received, and may be evicted, but for
-    the last `recent` (what the sparse layers read of them by position)."""
+    the last `recent` (what the sparse layers read of them by position).  routes:
+    the experts a token that are recorded (0: none)."""
 
     def __init__(self, rows, layers, width, dtype, device, capacity=256, rings=(), ring_rows=256, bare=(),
-                 weighted=False, recent=0):
+                 weighted=False, recent=0, routes=0):
+        if weighted and routes:
+            raise ValueError("a weighted cache moves its rows: it records no routes, which stay at their tokens' places")
         if ring_rows <= 0 or ring_rows & (ring_rows - 1):
             raise ValueError(f"a ring holds a power of 2 of rows, not {ring_rows}")
         self.lengths = torch.zeros(rows, dtype=torch.long, device=device)
@@ -75,7 +82,7 @@ class Cache:
                        for i in range(layers)]
         self.pending = False
         self.bound = 0
-        self.routes = None
+        self.routes = torch.full((layers, rows, capacity, routes), -1, dtype=torch.int32, device=device) if routes else None
         self.weights = self.evicted = None
         self.recent = recent
         self._read = []  # a weighted cache's undoable reading: (weights' row, layer, q, positions, lse, scale, counts)
@@ -109,18 +116,22 @@ class Cache:
     def reserve(self, need):
         """Growing tables of at least `need` rows (grown to max(need, 2 x
         capacity)); the rings keep their size."""
-        if self.capacity is None or need <= self.capacity:
+        held = self.capacity if self.routes is None else self.routes.shape[2]
+        if held is None or need <= held:
             return
         if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError(f"the cache needs {need} rows but holds {self.capacity}: reserve them before "
+            raise RuntimeError(f"the cache needs {need} rows but holds {held}: reserve them before "
                                "capturing a step")
-        grown = max(need, 2 * self.capacity)
+        grown = max(need, 2 * held)
         self.tables = [t if t is None or i in self.rings else torch.cat([t, t.new_zeros(t.shape[0], grown - t.shape[1],
                                                                            t.shape[2])], 1)
                        for i, t in enumerate(self.tables)]
         if self.weights is not None:
             self.weights = torch.cat([self.weights, self.weights.new_zeros(*self.weights.shape[:2],
                                                                            grown - self.weights.shape[2])], 2)
+        if self.routes is not None:
+            L, B, _, k = self.routes.shape
+            self.routes = torch.cat([self.routes, self.routes.new_full((L, B, grown - held, k), -1)], 2)
 
     def starts(self):
         """The position of each row's next token in its text: its length, and
@@ -174,6 +185,12 @@ class Cache:
         self.pending = False
         return self.lengths, self.before
 
+    def record(self, layer, chosen, counts):
+        """Writes a reading's choices of experts (B, T, k) int32 at its tokens'
+        places, the first counts[b] of row b; nothing where no routes are kept."""
+        if self.routes is not None:  # 4-byte values, moved as they are
+            kernels.kv_append(self.routes[layer].view(torch.float32), chosen.view(torch.float32), self.lengths, counts)
+
     def weigh(self, layer, q, positions, lse, scale, counts, undoable):
         """Adds the weights that a growing layer's rows got from a reading of
         counts tokens (q (B, T, H, c) at positions, lse the attention's); an
@@ -220,7 +237,8 @@ class Cache:
         copy.before = torch.zeros_like(copy.lengths)
         copy.tables = [None if t is None else t[index] for t in self.tables]
         copy.rings, copy.recent = self.rings, self.recent
-        copy.pending, copy.bound, copy.routes = False, self.bound, None
+        copy.pending, copy.bound = False, self.bound
+        copy.routes = None if self.routes is None else self.routes[:, index]
         copy.weights = None if self.weights is None else self.weights[:, index]
         copy.evicted = None if self.evicted is None else self.evicted[index]
         copy._read, copy._captured, copy._reading = [], False, []
@@ -237,6 +255,8 @@ class Cache:
         tables = [self.tables[i] for i in self.growing]
         if self.weights is not None:
             tables += [w[..., None] for w in self.weights]
+        if self.routes is not None:
+            tables += list(self.routes)
         if tables:  # not bounded by `bound`: replays of a captured reading do not raise it
             kernels.reorder_rows(tables, parents, self.lengths)
         if self.rings:

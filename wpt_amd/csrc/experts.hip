@@ -775,38 +775,46 @@ int run_product(const void* in, const void* weights, const int* chosen, const fl
   return launched(PRODUCT == kGateUp ? "experts (gate, up)" : "experts (down)");
 }
 
-// The rows of one round of the two products: their operands stay within a buffer.
-int round_rows(int64_t rows, int k, const ExpertShape& shape, int dtype) {
-  const int64_t widest = (dtype == WPTV_BF16 ? 2 : 4) * (shape.D > (int64_t)k * shape.Fp ? shape.D : (int64_t)k * shape.Fp);
-  const int64_t fit = kBufferBytes / widest;
+// The rows of one round of the two products: their operands stay within a buffer,
+// and the terms that a join reads within 512 MiB.
+int round_rows(int64_t rows, int k, const ExpertShape& shape, int dtype, bool join) {
+  const int64_t act = (int64_t)k * shape.Fp, widest = (dtype == WPTV_BF16 ? 2 : 4) * (shape.D > act ? shape.D : act);
+  int64_t fit = kBufferBytes / widest;
+  const int64_t terms = (int64_t)k * shape.D * 4, most = terms < (1 << 20) ? (1 << 29) / terms : 512;
+  if (join && most < fit) fit = most;
   return (int)(rows < fit ? rows : fit);
 }
 
-size_t act_bytes(int64_t rows, int k, const ExpertShape& shape, int dtype) {
-  return align_up((size_t)round_rows(rows, k, shape, dtype) * k * shape.Fp * (dtype == WPTV_BF16 ? 2 : 4), 256);
+size_t act_bytes(int round, int k, const ExpertShape& shape, int dtype) {
+  return align_up((size_t)round * k * shape.Fp * (dtype == WPTV_BF16 ? 2 : 4), 256);
 }
 
 template <typename T>
 int run_experts(const void* x, const void* gate_up, const void* down, const int* chosen, const float* gates,
-                const ExpertShape& shape, int64_t rows, int E, int k, int dtype, float* parts, void* y, void* workspace,
+                const ExpertShape& shape, int rows, int E, int k, int dtype, float* parts, void* y, void* workspace,
                 hipStream_t stream) {
+  const int round = round_rows(rows, k, shape, dtype, y != nullptr);
   char* act = static_cast<char*>(workspace);
-  float* sums = parts ? parts : reinterpret_cast<float*>(act + act_bytes(rows, k, shape, dtype));
-  const int round = round_rows(rows, k, shape, dtype);
+  float* terms = reinterpret_cast<float*>(act + act_bytes(round, k, shape, dtype));
   for (int64_t m = 0; m < rows; m += round) {
     const int here = rows - m < round ? (int)(rows - m) : round;
-    int status = run_product<T, kGateUp>(static_cast<const T*>(x) + m * shape.D, gate_up, chosen + m * k, gates + m * k,
-                                         shape, here, rows, E, k, false, act, stream);
+    const int* choice = chosen + m * k;
+    int status = run_product<T, kGateUp>(static_cast<const T*>(x) + m * shape.D, gate_up, choice, gates + m * k, shape,
+                                         here, here, E, k, false, act, stream);
+    if (status == WPTV_OK)
+      status = y ? run_product<T, kDown>(act, down, choice, gates + m * k, shape, here, here, E, k, false, terms, stream)
+                 : run_product<T, kDown>(act, down, choice, gates + m * k, shape, here, rows, E, k, true,
+                                         parts + m * shape.D, stream);
     if (status != WPTV_OK) return status;
-    status = run_product<T, kDown>(act, down, chosen + m * k, gates + m * k, shape, here, rows, E, k, parts != nullptr,
-                                   sums + m * shape.D, stream);
-    if (status != WPTV_OK) return status;
+    if (y) {
+      const int64_t threads = (int64_t)here * shape.D / 4;
+      join_experts<T><<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(terms, choice, here, shape.D, E, k,
+                                                                            static_cast<T*>(y) + m * shape.D);
+      status = launched("experts (join)");
+      if (status != WPTV_OK) return status;
+    }
   }
-  if (parts) return WPTV_OK;
-  const int64_t threads = rows * shape.D / 4;
-  join_experts<T><<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(sums, chosen, rows, shape.D, E, k,
-                                                                              static_cast<T*>(y));
-  return launched("experts (join)");
+  return WPTV_OK;
 }
 
 int check_experts(const char* what, const void* x, const void* gate_up, const void* down, const int* chosen,
@@ -914,7 +922,8 @@ extern "C" int wptv_experts_workspace(int rows, int D, int F, int k, int dtype, 
   if (status != WPTV_OK) return status;
   if (!bytes) return fail(WPTV_E_INVALID, "experts_workspace: a required pointer is NULL");
   const ExpertShape s = expert_shape(D, F, dtype);
-  *bytes = act_bytes(rows, k, s, dtype) + (parts_out ? 0 : (size_t)k * rows * D * 4);
+  const int round = round_rows(rows, k, s, dtype, !parts_out);
+  *bytes = act_bytes(round, k, s, dtype) + (parts_out ? 0 : (size_t)k * round * D * 4);
   return WPTV_OK;
 }
 

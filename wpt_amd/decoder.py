@@ -18,7 +18,10 @@ query (its top_k rows outside the last `window`, by the largest
 max_h log-softmax weight) and to the last `window` rows of that layer's table,
 with a sink per head and the same output gate.  An exact layer followed by a
 sparse layer makes that choice (model.py:134-135); layer_kinds gives the
-reference's layout of the three kinds (config.py:17-23).
+reference's layout of the three kinds (config.py:17-23).  With experts, every
+feed-forward block is a mixture of them: a linear router chooses
+experts_per_token for each token, each a SwiGLU block of ffn features
+(wpt_amd.experts); new_cache(routes=True) records the choices beside the entries.
 
 On the GPU:
     the input       wptv_embed_rms_norm: the embedding rows, the first norm
@@ -54,6 +57,9 @@ On the GPU:
                     (wptv_exact_choice), wptv_heads_rms_norm for the queries,
                     wptv_sparse_attention over the exact layer's table with
                     the sink and the output gate fused
+    experts         wptv_mixture: the router's choice and the chosen experts'
+                    products, whose gated terms the residual add + norm sums
+                    (wptv_add_rms_norm_parts) at up to SPLIT_K_ROWS rows
     sampling        wpt_amd.sampling (wptv_accept), called by the Writer
 The decoder keeps no state between calls but the cache; a step of fixed
 shape can be captured in a HIP graph (wpt_amd.step).
@@ -64,7 +70,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from . import kernels, layers
+from . import experts, kernels, layers
 from .cache import Cache
 
 EPS = 1e-6
@@ -98,8 +104,14 @@ class DecoderConfig:
     rope_dims: int = 64        # ROPE_DIMS, attention.py:55
     rope_base: float = 10000.0  # ROPE_BASE, attention.py:56
     top_k: int = 1024          # TOP_K, attention.py:54: rows an exact layer chooses for the sparse layers
+    experts: int = 0           # experts of every feed-forward block, ffn features each; 0 = one dense block
+    experts_per_token: int = 0
 
     def __post_init__(self):
+        if self.experts < 0 or bool(self.experts) != bool(self.experts_per_token):
+            raise ValueError(f"experts = {self.experts} and experts_per_token = {self.experts_per_token}: both or neither")
+        if not 0 <= self.experts_per_token <= min(self.experts, 8):
+            raise ValueError(f"a token takes 1 .. 8 of the {self.experts} experts, not {self.experts_per_token}")
         if self.kinds:
             if len(self.kinds) != self.layers or set(self.kinds) - {WINDOW, EXACT, SPARSE}:
                 raise ValueError(f"kinds must name one of {WINDOW!r}, {EXACT!r}, {SPARSE!r} for each of the "
@@ -160,8 +172,13 @@ def random_weights(config, seed=0, std=0.02, dtype=torch.float32, device="cpu"):
             weights[f"layers.{i}.k_norm"] = ones(c)
         weights[f"layers.{i}.out"] = normal(D, H * c)
         weights[f"layers.{i}.ffn_norm"] = ones(D)
-        weights[f"layers.{i}.gate_up"] = normal(2 * Fw, D)
-        weights[f"layers.{i}.down"] = normal(D, Fw)
+        if config.experts:  # a router in FP32, as the norms; layers.{i}.router_bias (E,) may join it
+            weights[f"layers.{i}.router"] = torch.randn(config.experts, D, generator=generator, device=device) * std
+            weights[f"layers.{i}.gate_up"] = normal(config.experts, 2 * Fw, D)
+            weights[f"layers.{i}.down"] = normal(config.experts, D, Fw)
+        else:
+            weights[f"layers.{i}.gate_up"] = normal(2 * Fw, D)
+            weights[f"layers.{i}.down"] = normal(D, Fw)
         if config.kind(i) in (WINDOW, SPARSE):
             weights[f"layers.{i}.gate"] = normal(H * c, D)
             # the reference starts its sinks at 0; drawn here so that they matter
@@ -173,7 +190,8 @@ def random_weights(config, seed=0, std=0.02, dtype=torch.float32, device="cpu"):
 
 class MQADecoder:
     """config: DecoderConfig; weights: random_weights' names; dtype: the
-    compute dtype (float32 or bfloat16), on a GPU."""
+    compute dtype (float32 or bfloat16), on a GPU.  The experts' matrices are
+    kept in the layout their products read alone, not among the parameters()."""
 
     def __init__(self, config, weights, dtype=torch.bfloat16, device="cuda"):
         self.config, self.dtype = config, dtype
@@ -183,20 +201,26 @@ class MQADecoder:
             raise kernels.KernelUnavailable(f"the decoder's verify step runs on a GPU, not {self.device}")
         self.w = {}
         for name, value in weights.items():
-            keep_fp32 = name.endswith("norm") or name.endswith("sink")
+            keep_fp32 = name.endswith(("norm", "sink", "router", "router_bias"))
             self.w[name] = value.to(device=self.device, dtype=torch.float32 if keep_fp32 else dtype).contiguous()
         for i in config.windows:  # one projection for q, k, v and the gate
             self.w[f"layers.{i}.qkvg"] = torch.cat([self.w[f"layers.{i}.qkv"], self.w[f"layers.{i}.gate"]]).contiguous()
         for i in config.sparse:  # one projection for q and the gate
             self.w[f"layers.{i}.qg"] = torch.cat([self.w[f"layers.{i}.q"], self.w[f"layers.{i}.gate"]]).contiguous()
-        if dtype == torch.bfloat16:  # the gate/up rows in the order the fused SwiGLU product reads, kept instead
+        self.experts = []
+        if config.experts:
+            for i in range(config.layers):
+                self.experts.append(experts.ExpertWeights(self.w.pop(f"layers.{i}.gate_up"),
+                                                          self.w.pop(f"layers.{i}.down")))
+        elif dtype == torch.bfloat16:  # the gate/up rows in the order the fused SwiGLU product reads, kept instead
             for i in range(config.layers):
                 self.w[f"layers.{i}.gate_up_tiles"] = layers.interleave_gate_up(self.w.pop(f"layers.{i}.gate_up"))
         # the fm products' weights, packed once (beside the row-major ones that wider readings use)
         self.fm = {}
         if dtype == torch.bfloat16:
             for i in range(config.layers):
-                names = ["gate_up_tiles", "down"] + (["qkv", "out"] if config.kind(i) == EXACT else [])
+                names = ["gate_up_tiles", "down"] if not config.experts else []
+                names += ["qkv", "out"] if config.kind(i) == EXACT else []
                 for name in names:
                     key = f"layers.{i}.{name}"
                     self.fm[key] = layers.FmWeight(self.w[key])
@@ -210,13 +234,15 @@ class MQADecoder:
         window layers' rings hold readings of up to `widest` tokens (wider
         ones are read in pieces).  weighted: it keeps the attention weight that
         the exact layers' rows receive (from those layers' own queries), so
-        that evict can bound it."""
-        if routes:
+        that evict can bound it.  routes: it records the experts each token is
+        routed to (Cache.routes)."""
+        if routes and not self.config.experts:
             raise NotImplementedError("this decoder has no routed experts to record")
         c = self.config.head_dim
         ring = 1 << max(0, (self.config.window - 1 + widest - 1).bit_length())
         return Cache(rows, self.config.layers, 2 * c, self.dtype, self.device, capacity, self.config.windows, ring,
-                     self.config.sparse, weighted, self.config.window if self.config.sparse else 0)
+                     self.config.sparse, weighted, self.config.window if self.config.sparse else 0,
+                     self.config.experts_per_token if routes else 0)
 
     def widest(self, cache):
         """The most tokens one reading of the cache takes (its rings' size)."""
@@ -264,7 +290,10 @@ class MQADecoder:
         elif kind == SPARSE:
             self._sparse_attention(i, h, x_in, positions, handoff, xf)
         else:
-            handoff = self._exact_attention(i, h, x_in, cache, positions, counts, xf, undoable)
+            handoff = self._exact_attention(i, h, x_in, cache, positions, counts, xf, undoable, x)
+        if self.experts:
+            self._mixture(i, h, x, cache, counts, next_norm, xf)
+            return handoff
         if fm:
             act = layers.linear_fm_swiglu(xf, B * T, self.fm[f"layers.{i}.gate_up_tiles"], any_rows=True)
             nxt = self._attn_input_fm(i + 1, fm)
@@ -287,6 +316,21 @@ class MQADecoder:
             layers.add_rms_norm(h, F.linear(act, down), next_norm, x)
         return handoff
 
+    def _mixture(self, i, h, x, cache, counts, next_norm, xf=None):
+        """A feed-forward block of experts on x: h += the gated sum, x =
+        RMSNorm(h) with next_norm.  The padding past counts chooses no expert."""
+        rows, D = x.shape[0] * x.shape[1], x.shape[2]
+        arguments = (x, self.w[f"layers.{i}.router"], self.experts[i], self.config.experts_per_token,
+                     self.w.get(f"layers.{i}.router_bias"), counts)
+        if rows <= SPLIT_K_ROWS or D > 4096:  # the norm after it sums the terms
+            parts, chosen, _ = experts.mixture_parts(*arguments)
+            nxt = self._attn_input_fm(i + 1, xf is not None)
+            layers.add_rms_norm_parts(h, parts, next_norm, xf if nxt else x, fm=nxt)
+        else:
+            y, chosen, _ = experts.mixture(*arguments)
+            layers.add_rms_norm(h, y, next_norm, x)
+        cache.record(i, chosen, counts)
+
     @staticmethod
     def _linear(x, w):
         """x . w^T in x's dtype: the build's product for bf16 at up to
@@ -297,8 +341,8 @@ class MQADecoder:
 
     def _attention_out(self, i, h, x, o, xf=None):
         """h += out(o), x = RMSNorm(h) with the feed-forward norm (into xf,
-        the fm operand, when given).  o (B, T, H, c), or a flat fm operand of
-        the B T rows."""
+        the fm operand, when given and the block's products read it).  o
+        (B, T, H, c), or a flat fm operand of the B T rows."""
         if xf is not None:
             B, T, D = h.shape
             rows = B * T
@@ -306,7 +350,8 @@ class MQADecoder:
                 parts = layers.linear_fm_parts(o, rows, self.fm[f"layers.{i}.out"], any_rows=True)
             else:
                 parts = layers.linear_parts(o.reshape(rows, -1), self.w[f"layers.{i}.out"])
-            layers.add_rms_norm_parts(h, parts, self.w[f"layers.{i}.ffn_norm"], xf, fm=True)
+            dense = not self.experts
+            layers.add_rms_norm_parts(h, parts, self.w[f"layers.{i}.ffn_norm"], xf if dense else x, fm=dense)
             return
         B, T, H, c = o.shape
         out = self.w[f"layers.{i}.out"]
@@ -344,12 +389,12 @@ class MQADecoder:
                                      gate=proj[..., H * c:])
         self._attention_out(i, h, x, o, xf)
 
-    def _exact_attention(self, i, h, x, cache, positions, counts, xf=None, undoable=False):
+    def _exact_attention(self, i, h, x, cache, positions, counts, xf=None, undoable=False, rows=None):
         """An exact layer's attention block: h += out(o), x = RMSNorm(h) with
         the feed-forward norm.  Returns (keys, values, chosen), the sparse
         layers' handoff (chosen None when no sparse layer follows).  xf
         given: x is that fm operand, and the output goes through the fm
-        products."""
+        products; rows: the row-major x that a block of experts reads."""
         w, cfg = self.w, self.config
         B, T, _ = h.shape
         H, c = cfg.heads, cfg.head_dim
@@ -383,7 +428,7 @@ class MQADecoder:
         else:
             o = kernels.verify_attention(q, keys, values, positions, c ** -0.5, from_positions=True, out_fm=fm,
                                          captured=True)  # a decoder's steady steps are graphs
-        self._attention_out(i, h, x, o, xf)
+        self._attention_out(i, h, x if rows is None else rows, o, xf)
         return keys, values, chosen
 
     @torch.no_grad()
