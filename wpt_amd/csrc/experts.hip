@@ -146,6 +146,8 @@ __device__ __forceinline__ void store_choices(const double* logit, const int* pl
   }
 }
 
+constexpr int kAhead = 4;  // steps whose loads a wavefront waits for together
+
 template <typename T>
 __device__ __forceinline__ void load_four(const T* p, float* to) {
   typedef T four __attribute__((ext_vector_type(4)));
@@ -172,14 +174,20 @@ __global__ __launch_bounds__(256) void route_token(const T* __restrict__ x, cons
   const T* row = x + m * D;
   for (int e = tid >> 6; e < E; e += 4) {
     double sum = 0.;
-    for (int d = 4 * lane; d < D; d += 256) {
-      const float4 w = *reinterpret_cast<const float4*>(router + (int64_t)e * D + d);
-      float b[4];
-      load_four<T>(row + d, b);
-      sum = fma((double)w.x, (double)b[0], sum);
-      sum = fma((double)w.y, (double)b[1], sum);
-      sum = fma((double)w.z, (double)b[2], sum);
-      sum = fma((double)w.w, (double)b[3], sum);
+    const float* w = router + (int64_t)e * D;
+    for (int first = 4 * lane; first - 4 * lane < D; first += kAhead * 256) {
+      float a[kAhead][4], b[kAhead][4];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {  // all asked for at once; past the width nothing is added
+        const int d = first + 256 * u < D ? first + 256 * u : 0;
+        load_four<float>(w + d, a[u]);
+        load_four<T>(row + d, b[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (first + 256 * u < D)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum = fma((double)a[u][i], (double)b[u][i], sum);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -197,8 +205,6 @@ __global__ __launch_bounds__(256) void route_token(const T* __restrict__ x, cons
 }
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
-constexpr int kAhead = 4;  // steps whose loads a wavefront waits for together
-
 // The logits of a wider one on the 64-bit matrix instruction (16 experts by 16
 // tokens by 4 columns; the product of two FP32 values is exact): grid (E / 16,
 // rows / 16, splits), workgroup z's four wavefronts taking the 16-column steps
@@ -281,7 +287,7 @@ __global__ __launch_bounds__(256) void route_choose(const double* __restrict__ s
 int route_splits(int64_t rows, int D, int E) {
   if ((int64_t)E * D <= 16384) return 0;
   const int64_t tiles = (rows + 15) / 16 * ((E + 15) / 16);
-  const int64_t want = 512 / tiles, most = (D + 63) / 64;
+  const int64_t want = 512 / tiles, most = (D + 255) / 256;  // a wavefront's steps at once
   const int64_t splits = want < 1 ? 1 : want < most ? want : most;
   return (int)(splits < 32 ? splits : 32);
 }
@@ -373,16 +379,15 @@ struct PairList {
   __device__ __forceinline__ int at(int i) const { return list[i]; }
 };
 
-// The parts' rows that no expert of the range writes, cleared by workgroups of
-// their own, the grid's first `groups` (at least one) of each column.
-template <int WAVES>
-__device__ __forceinline__ void clear_rows(const PairList<WAVES>& pairs, int n, int r0, int group, int groups, int first, int last, int D,
-                                           int64_t total, int k, float* __restrict__ parts) {
-  const int lane = threadIdx.x & 63;
-  for (int i = group * WAVES + (threadIdx.x >> 6); i < n; i += groups * WAVES) {  // a wavefront a row
-    const int p = r0 + pairs.at(i);
+// The parts' rows that no expert of the range writes, cleared by `waves` (at least
+// one) wavefronts of their own, one after the other a row each.
+__device__ __forceinline__ void clear_rows(const uint16_t* pairs, int n, int r0, int wave, int waves, int first,
+                                           int last, int D, int64_t total, int k, float* __restrict__ parts) {
+  for (int i = wave; i < n; i += waves) {
+    const int p = r0 + pairs[i];
     float* to = parts + ((p % k) * total + p / k) * D;
-    for (int d = first + 4 * lane; d < min(D, last); d += 256) *reinterpret_cast<f32x4*>(to + d) = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = first + 4 * (threadIdx.x & 63); d < min(D, last); d += 256)
+      *reinterpret_cast<f32x4*>(to + d) = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 }
 
@@ -433,29 +438,54 @@ __global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, 
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pairs = rows * k;
-  int e = BY_PAIR ? blockIdx.y : (int)blockIdx.y < clears ? E : blockIdx.y - clears;
-  if constexpr (BY_PAIR) {
-    const int at = e;
-    e = chosen[at];
-    for (int p = lane; p - lane < at; p += 64)
-      if (__builtin_amdgcn_ballot_w64(p < at && chosen[p] == e)) return;
-    e = __builtin_amdgcn_readfirstlane(e);
-    if ((unsigned)e >= (unsigned)E) e = E;  // no expert: several of them clear the same rows
-  }
+  int e = BY_PAIR ? chosen[blockIdx.y] : (int)blockIdx.y < clears ? E : blockIdx.y - clears;
+  if constexpr (BY_PAIR) e = (unsigned)__builtin_amdgcn_readfirstlane(e) < (unsigned)E ? __builtin_amdgcn_readfirstlane(e) : E;
   const int KS = PRODUCT == kGateUp ? shape.KSx : shape.KSf;
   const unsigned width = (PRODUCT == kGateUp ? shape.D : shape.Fp) * sizeof(T);
   const int block = blockIdx.x, blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
   const int steps = (KS - wv + 3) / 4;
   const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + block) * 2 * KS * 64, 2u * KS * 1024);
   const Buffer x = buffer(in, (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width));
+  u32x4 wb[kDepth][2], xb[kDepth][NT];
+  auto load_weights = [&](int d, int s) {
+    const unsigned ks = wv + 4 * s;
+    wb[d][0] = load16_once(w, 16 * lane, 1024 * ks);
+    wb[d][1] = load16_once(w, 16 * lane, 1024 * (KS + ks));
+  };
+  // a few pairs: the first weights are asked for before the expert's tokens are known (one token's layer 32.0 -> 30.1
+  // us; with more of them the registers cost more than it gives, 16 tokens over wide experts 101 -> 103)
+  if constexpr (BY_PAIR) {
+    if (e < E && steps > 0) {
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) load_weights(d, min(d, steps - 1));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
 
   for (int r0 = 0; r0 < pairs; r0 += kRange) {
-    PairList<4>::Choices choices;
-    list.load(choices, chosen, r0, pairs);
-    const int n = list.fill(choices, r0, pairs, e, E);
+    const uint16_t* mine = list.list;
+    int n = 0;
+    if constexpr (BY_PAIR) {  // fewer pairs than 512: every wavefront lists them for itself
+      uint16_t* own = list.list + wv * kMaxExperts;
+      for (int p = lane; p - lane < pairs; p += 64) {
+        const int c = chosen[min(p, pairs - 1)];
+        const bool same = p < pairs && (c == e || (e == E && (unsigned)c >= (unsigned)E));
+        const uint64_t found = __builtin_amdgcn_ballot_w64(same);
+        if (__builtin_amdgcn_ballot_w64(same && p < (int)blockIdx.y)) return;  // an earlier pair's workgroup serves it
+        if (same) own[n + __builtin_popcountll(found & ((1ull << lane) - 1ull))] = (uint16_t)p;
+        n += __builtin_popcountll(found);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      mine = own;
+    } else {
+      PairList<4>::Choices choices;
+      list.load(choices, chosen, r0, pairs);
+      n = list.fill(choices, r0, pairs, e, E);
+    }
     if (e == E) {
       if (PRODUCT == kDown && clears > 0)
-        clear_rows(list, n, r0, BY_PAIR ? 0 : blockIdx.y, BY_PAIR ? 1 : clears, 32 * block, 32 * block + 32, shape.D, total, k, static_cast<float*>(out));
+        clear_rows(mine, n, r0, BY_PAIR ? wv : blockIdx.y * 4 + wv, BY_PAIR ? 4 : clears * 4, 32 * block, 32 * block + 32,
+                   shape.D, total, k, static_cast<float*>(out));
       __syncthreads();
       continue;
     }
@@ -465,17 +495,14 @@ __global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, 
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         // columns past the last token repeat it; nothing of them is stored
-        pair[t] = r0 + list.at(min(first + 16 * t + j, n - 1));
+        pair[t] = r0 + mine[min(first + 16 * t + j, n - 1)];
         row[t] = (PRODUCT == kGateUp ? pair[t] / k : pair[t]) * width + 16 * g;
       }
       f32x4 acc[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-      u32x4 wb[kDepth][2], xb[kDepth][NT];
-      auto load = [&](int d, int s) {
+      auto load_tokens = [&](int d, int s) {
         const unsigned ks = wv + 4 * s;
-        wb[d][0] = load16_once(w, 16 * lane, 1024 * ks);
-        wb[d][1] = load16_once(w, 16 * lane, 1024 * (KS + ks));
 #pragma unroll
         for (int t = 0; t < NT; ++t)  // columns past the width are zero, as the weights' padding
           xb[d][t] = load16(x, 64 * ks + 16 * g < width ? row[t] : kOutside, 64 * ks);
@@ -488,15 +515,20 @@ __global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, 
         }
       };
       if (steps > 0) {
+        if (!BY_PAIR || first > 0) {
 #pragma unroll
-        for (int d = 0; d < kDepth; ++d) load(d, min(d, steps - 1));
+          for (int d = 0; d < kDepth; ++d) load_weights(d, min(d, steps - 1));
+        }
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) load_tokens(d, min(d, steps - 1));
         int s = 0;
         for (; s + kDepth <= steps; s += kDepth) {
 #pragma unroll
           for (int d = 0; d < kDepth; ++d) {
             multiply(d);
             __builtin_amdgcn_sched_barrier(0);
-            load(d, min(s + kDepth + d, steps - 1));
+            load_weights(d, min(s + kDepth + d, steps - 1));
+            load_tokens(d, min(s + kDepth + d, steps - 1));
             __builtin_amdgcn_sched_barrier(0);
           }
         }
@@ -651,7 +683,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 3) void expert_tiles(const T* __re
     const int n = list.fill(choices, r0, pairs, e, E);
     if (e == E) {
       if (PRODUCT == kDown && clears > 0)
-        clear_rows(list, n, r0, blockIdx.y, clears, 32 * (int)blockIdx.x * kTileWaves, 32 * (int)(blockIdx.x + 1) * kTileWaves, shape.D,
+        clear_rows(list.list, n, r0, blockIdx.y * kTileWaves + wv, clears * kTileWaves,
+                   32 * (int)blockIdx.x * kTileWaves, 32 * (int)(blockIdx.x + 1) * kTileWaves, shape.D,
                    total, k, static_cast<float*>(out));
     } else {
       for (int first = 0; first < n; first += 16 * kTileTokens) {
@@ -667,6 +700,97 @@ __global__ __launch_bounds__(64 * kTileWaves, 3) void expert_tiles(const T* __re
       }
     }
     __syncthreads();  // the lists are written again
+  }
+}
+
+// y of at most 16 tokens in one launch after the gate/up product: grid (D / 16), a
+// workgroup's eight wavefronts share out the k-steps of 16 output rows over every
+// expert that some token takes, one after the other, the tokens' columns in their
+// own places, so that the matrix instructions add up the experts' terms as well.
+// Pairs of one expert make a group, and one that a token names twice makes another;
+// prow[group][token] is the pair, or kNone.
+constexpr int kFewTokens = 16, kFewPairs = 128, kFewWaves = 8, kNone = 0xffff;
+
+template <typename T>
+__global__ __launch_bounds__(64 * kFewWaves) void expert_rows(const T* __restrict__ act,
+                                                              const u32x4* __restrict__ weights,
+                                                              const int* __restrict__ chosen, ExpertShape shape,
+                                                              int rows, int E, int k, T* __restrict__ y) {
+  using O = Operand<T>;
+  constexpr int kDepth = 8;
+  __shared__ int key[kFewPairs], expert[kFewPairs];
+  __shared__ uint64_t leaders[kFewPairs / 64];
+  static_assert(kFewPairs == 128, "two wavefronts of pairs");
+  __shared__ uint16_t prow[kFewPairs][kFewTokens];
+  __shared__ float red[kFewWaves][4 * 64];
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int pairs = rows * k;  // at most kFewPairs
+  int e = -1, times = 0;
+  if (tid < pairs) {
+    e = chosen[tid];
+    for (int i = tid / k * k; i < tid; ++i) times += chosen[i] == e ? 1 : 0;
+    if ((unsigned)e >= (unsigned)E) e = -1;
+    key[tid] = e < 0 ? -1 - tid : e * kMaxChosen + times;
+  }
+  for (int i = tid; i < kFewPairs * kFewTokens / 2; i += 64 * kFewWaves) reinterpret_cast<uint32_t*>(prow)[i] = ~0u;
+  __syncthreads();
+  // the first pair of a group is its leader; the groups in their leaders' order
+  int leader = tid;
+  if (e >= 0)
+    for (int i = tid - 1; i >= 0; --i) leader = key[i] == key[tid] ? i : leader;
+  const uint64_t first = __builtin_amdgcn_ballot_w64(e >= 0 && leader == tid);
+  if (lane == 0 && wv < kFewPairs / 64) leaders[wv] = first;
+  __syncthreads();
+  if (e >= 0) {
+    int group = __builtin_popcountll(leaders[leader >> 6] & ((1ull << (leader & 63)) - 1ull));
+    if (leader >= 64) group += __builtin_popcountll(leaders[0]);
+    prow[group][tid / k] = (uint16_t)tid;
+    if (leader == tid) expert[group] = e;
+  }
+  const int groups = __builtin_popcountll(leaders[0]) + __builtin_popcountll(leaders[1]);
+  __syncthreads();
+  const int KS = shape.KSf, total = groups * KS;
+  const unsigned width = shape.Fp * sizeof(T);
+  const Buffer x = buffer(act, pairs * width);
+  const int64_t matrix = (int64_t)shape.DB * 2 * KS * 64;
+  const u32x4* w0 = weights + (int64_t)blockIdx.x * KS * 64;
+  const int steps = (total - wv + kFewWaves - 1) / kFewWaves;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  u32x4 wb[kDepth], xb[kDepth];
+  auto load = [&](int d, int s) {
+    const int step = wv + kFewWaves * s, which = step / KS, ks = step - which * KS;
+    const u32x4* w = w0 + __builtin_amdgcn_readfirstlane(expert[which]) * matrix;
+    wb[d] = load16_once(buffer(w, 1024u * KS), 16 * lane, 1024 * ks);
+    const unsigned p = prow[which][j];
+    xb[d] = load16(x, p == kNone ? kOutside : p * width + 16 * g, 64 * ks);
+  };
+  if (steps > 0) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) load(d, min(d, steps - 1));
+    int s = 0;
+    for (; s + kDepth <= steps; s += kDepth) {
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        acc = O::mfma(wb[d], xb[d], acc);
+        __builtin_amdgcn_sched_barrier(0);
+        load(d, min(s + kDepth + d, steps - 1));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d)
+      if (s + d < steps) acc = O::mfma(wb[d], xb[d], acc);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) red[wv][i * 64 + lane] = acc[i];
+  __syncthreads();
+  if (tid < 256) {  // output row 4 g + i of token j
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < kFewWaves; ++u) sum += red[u][tid];
+    const int n = 16 * blockIdx.x + 4 * g + wv;
+    if (j < rows && n < shape.D) y[(int64_t)j * shape.D + n] = from_f32<T>(sum);
   }
 }
 
@@ -789,6 +913,17 @@ size_t act_bytes(int round, int k, const ExpertShape& shape, int dtype) {
   return align_up((size_t)round * k * shape.Fp * (dtype == WPTV_BF16 ? 2 : 4), 256);
 }
 
+// Whether 16 output rows a workgroup, over all experts, are the faster down product
+// of a few tokens: where a workgroup reads little, which saves the join, or where
+// they cover the compute units.  Whole layers in a graph, us, this and the other
+// form: one token, D 256, 2 of 8 experts of 704 12.6, 13.8; D 4096, 4 of 64 of 1408
+// 42.0, 45.3, 4 tokens 105, 112; D 2048, 8 of 64 of 704 30.7, 29.9, 4 tokens, 2 of 8
+// of 5632 89, 80; FP32, 3 tokens, D 1024, 4 of 64 of 300 29.9, 25.8.
+bool few_rows(int rows, int k, const ExpertShape& shape) {
+  if (rows > kFewTokens || rows * k > kFewPairs) return false;
+  return (int64_t)rows * k * shape.KSf <= 64 || shape.D >= 4096;
+}
+
 template <typename T>
 int run_experts(const void* x, const void* gate_up, const void* down, const int* chosen, const float* gates,
                 const ExpertShape& shape, int rows, int E, int k, int dtype, float* parts, void* y, void* workspace,
@@ -801,6 +936,11 @@ int run_experts(const void* x, const void* gate_up, const void* down, const int*
     const int* choice = chosen + m * k;
     int status = run_product<T, kGateUp>(static_cast<const T*>(x) + m * shape.D, gate_up, choice, gates + m * k, shape,
                                          here, here, E, k, false, act, stream);
+    if (status == WPTV_OK && y && few_rows(rows, k, shape)) {
+      expert_rows<T><<<(shape.D + 15) / 16, 64 * kFewWaves, 0, stream>>>(
+          reinterpret_cast<const T*>(act), static_cast<const u32x4*>(down), chosen, shape, rows, E, k, static_cast<T*>(y));
+      return launched("experts (rows)");
+    }
     if (status == WPTV_OK)
       status = y ? run_product<T, kDown>(act, down, choice, gates + m * k, shape, here, here, E, k, false, terms, stream)
                  : run_product<T, kDown>(act, down, choice, gates + m * k, shape, here, rows, E, k, true,
