@@ -76,7 +76,7 @@ __host__ __device__ __forceinline__ ExpertShape expert_shape(int D, int F, int d
 // N gate rows, then the N up rows).
 template <typename T, bool PAIRED>
 __global__ __launch_bounds__(256) void pack_experts(const T* __restrict__ w, int N, int K, int blocks, int KS,
-                                                    u32x4* __restrict__ out) {
+                                                    bool whole, u32x4* __restrict__ out) {
   using O = Operand<T>;
   const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (item >= (int64_t)blocks * KS * 64) return;
@@ -87,12 +87,16 @@ __global__ __launch_bounds__(256) void pack_experts(const T* __restrict__ w, int
     u32x4 all;
   } v;
   v.all = u32x4{0u, 0u, 0u, 0u};
-  if (row < N) {
+  if (row < N && col < K) {
     const int64_t rows = PAIRED ? 2 * (int64_t)N : N;
-    const T* from = w + ((int64_t)blockIdx.y * rows + row + (PAIRED && (rb & 1) ? N : 0)) * K;
+    const T* from = w + ((int64_t)blockIdx.y * rows + row + (PAIRED && (rb & 1) ? N : 0)) * K + col;
+    if (whole) {  // rows of whole, aligned 16 bytes
+      v.all = *reinterpret_cast<const u32x4*>(from);
+    } else {
 #pragma unroll
-    for (int i = 0; i < O::EPL; ++i)
-      if (col + i < K) v.element[i] = from[col + i];
+      for (int i = 0; i < O::EPL; ++i)
+        if (col + i < K) v.element[i] = from[i];
+    }
   }
   out[(int64_t)blockIdx.y * blocks * KS * 64 + item] = v.all;
 }
@@ -314,16 +318,14 @@ __device__ __forceinline__ u32x4 load16_once(Buffer from, unsigned lane_offset, 
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset, offset, 2));
 }
 
-constexpr int kRange = 4096;  // pairs whose expert is looked up at a time
-
 enum Product { kGateUp = 0, kDown = 1 };
 
-// The pairs of a range [r0, r0 + kRange) that one expert takes, in their order,
+// The pairs of a range [r0, r0 + RANGE) that one expert takes, in their order,
 // listed by a workgroup of WAVES wavefronts, a stretch of the range each.
-template <int WAVES>
+template <int WAVES, int RANGE>
 struct PairList {
-  static constexpr int kTurns = kRange / WAVES / 64;
-  uint16_t list[kRange];
+  static constexpr int kTurns = RANGE / WAVES / 64;
+  uint16_t list[RANGE];
   int listed[WAVES];
 
   // A thread's choices of a range (loaded ahead of other loads, whose arrival the
@@ -336,7 +338,7 @@ struct PairList {
 
   static __device__ __forceinline__ void load(Choices& choices, const int* __restrict__ chosen, int r0, int pairs) {
     // the stretches follow the pairs' count, in whole wavefronts, so that a few pairs are listed by all at once
-    const int here = min(pairs - r0, kRange), many = turns(here);
+    const int here = min(pairs - r0, RANGE), many = turns(here);
     const int at = (threadIdx.x >> 6) * many * 64 + (threadIdx.x & 63);
 #pragma unroll
     for (int i = 0; i < kTurns; ++i)
@@ -348,7 +350,7 @@ struct PairList {
   __device__ __forceinline__ int fill(const Choices& choices, int r0, int pairs, int e, int E) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const uint64_t below = (1ull << lane) - 1ull;
-    const int here = min(pairs - r0, kRange), many = turns(here), begin = wv * many * 64;
+    const int here = min(pairs - r0, RANGE), many = turns(here), begin = wv * many * 64;
     auto mine = [&](int i) {
       const int c = choices.c[i];
       return begin + 64 * i + lane < here && (c == e || (e == E && (unsigned)c >= (unsigned)E));
@@ -376,7 +378,6 @@ struct PairList {
     return total;
   }
 
-  __device__ __forceinline__ int at(int i) const { return list[i]; }
 };
 
 // The parts' rows that no expert of the range writes, cleared by `waves` (at least
@@ -426,15 +427,16 @@ __device__ __forceinline__ void store_block(f32x4 a, f32x4 b, int p, int block, 
 //   kDown     act -> parts [k, rows, D] FP32
 // BY_PAIR (fewer pairs than experts): workgroup y serves the expert of pair y,
 // if that is the expert's first.
-template <typename T, int PRODUCT, int NT, bool BY_PAIR>
-__global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, const u32x4* __restrict__ weights,
+template <typename T, int PRODUCT, int NT, int WAVES, bool BY_PAIR>
+__global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict__ in, const u32x4* __restrict__ weights,
                                                       const int* __restrict__ chosen, const float* __restrict__ gates,
                                                       ExpertShape shape, int rows, int64_t total, int E, int k,
                                                       int clears, void* __restrict__ out) {
   using O = Operand<T>;
-  constexpr int kDepth = NT == 1 ? 8 : 4;
-  __shared__ PairList<4> list;
-  __shared__ float red[4 * NT * 2 * 4 * 64];
+  constexpr int kDepth = 3, kRange = NT == 1 ? 1024 : 4096;
+  typedef PairList<WAVES, kRange> List;
+  __shared__ List list;
+  __shared__ float red[WAVES * NT * 2 * 4 * 64];
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pairs = rows * k;
@@ -443,12 +445,12 @@ __global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, 
   const int KS = PRODUCT == kGateUp ? shape.KSx : shape.KSf;
   const unsigned width = (PRODUCT == kGateUp ? shape.D : shape.Fp) * sizeof(T);
   const int block = blockIdx.x, blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
-  const int steps = (KS - wv + 3) / 4;
+  const int steps = (KS - wv + WAVES - 1) / WAVES;
   const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + block) * 2 * KS * 64, 2u * KS * 1024);
   const Buffer x = buffer(in, (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width));
   u32x4 wb[kDepth][2], xb[kDepth][NT];
   auto load_weights = [&](int d, int s) {
-    const unsigned ks = wv + 4 * s;
+    const unsigned ks = wv + WAVES * s;
     wb[d][0] = load16_once(w, 16 * lane, 1024 * ks);
     wb[d][1] = load16_once(w, 16 * lane, 1024 * (KS + ks));
   };
@@ -478,13 +480,13 @@ __global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, 
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       mine = own;
     } else {
-      PairList<4>::Choices choices;
+      typename List::Choices choices;
       list.load(choices, chosen, r0, pairs);
       n = list.fill(choices, r0, pairs, e, E);
     }
     if (e == E) {
       if (PRODUCT == kDown && clears > 0)
-        clear_rows(mine, n, r0, BY_PAIR ? wv : blockIdx.y * 4 + wv, BY_PAIR ? 4 : clears * 4, 32 * block, 32 * block + 32,
+        clear_rows(mine, n, r0, BY_PAIR ? wv : blockIdx.y * WAVES + wv, BY_PAIR ? WAVES : clears * WAVES, 32 * block, 32 * block + 32,
                    shape.D, total, k, static_cast<float*>(out));
       __syncthreads();
       continue;
@@ -502,7 +504,7 @@ __global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, 
 #pragma unroll
       for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
       auto load_tokens = [&](int d, int s) {
-        const unsigned ks = wv + 4 * s;
+        const unsigned ks = wv + WAVES * s;
 #pragma unroll
         for (int t = 0; t < NT; ++t)  // columns past the width are zero, as the weights' padding
           xb[d][t] = load16(x, 64 * ks + 16 * g < width ? row[t] : kOutside, 64 * ks);
@@ -543,13 +545,13 @@ __global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, 
       __syncthreads();
 #pragma unroll
       for (int t = 0; t < NT; ++t)
-        if (t % 4 == wv && first + 16 * t + j < n) {
+        if (t % WAVES == wv && first + 16 * t + j < n) {
           float sum[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             sum[i] = red[(t * 8 + i) * 64 + lane];
 #pragma unroll
-            for (int u = 1; u < 4; ++u) sum[i] += red[((u * NT + t) * 8 + i) * 64 + lane];
+            for (int u = 1; u < WAVES; ++u) sum[i] += red[((u * NT + t) * 8 + i) * 64 + lane];
           }
           store_block<T, PRODUCT>(f32x4{sum[0], sum[1], sum[2], sum[3]}, f32x4{sum[4], sum[5], sum[6], sum[7]}, pair[t],
                                   block, g, shape, total, k, gates, out);
@@ -564,20 +566,20 @@ __global__ __launch_bounds__(256) void expert_columns(const T* __restrict__ in, 
 // row-block pair of one expert's matrix each, over tiles of up to 64 of the
 // expert's tokens.  The tokens' columns go through LDS, kChunk k-steps at a time in
 // two buffers, in the order the matrix instructions take them; the weights go
-// straight from memory into registers, kTileDepth k-steps ahead, across the chunks'
+// straight from memory into registers, DEPTH k-steps ahead, across the chunks'
 // barriers, which wait for LDS alone.
-constexpr int kTileWaves = 4, kTileTokens = 4, kChunk = 4, kTileDepth = 4;
+constexpr int kTileWaves = 4, kTileTokens = 4, kChunk = 4;
 
 // A tile of NT times 16 tokens, `first` the list's place of the first.
-template <typename T, int PRODUCT, int NT>
+template <typename T, int PRODUCT, int NT, int DEPTH>
 __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned width,
-                                          const PairList<kTileWaves>& list, u32x4 (*xs)[kTileTokens * kChunk * 64],
+                                          const uint16_t* list, u32x4 (*xs)[kTileTokens * kChunk * 64],
                                           int r0, int first, int n, int block, bool live, const ExpertShape& shape,
                                           int64_t total, int k, const float* __restrict__ gates,
                                           void* __restrict__ out) {
   using O = Operand<T>;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
-  u32x4 wb[kTileDepth][2], xr[NT];
+  u32x4 wb[DEPTH][2], xr[NT];
   const unsigned at = live ? 16 * lane : kOutside;  // wavefronts past the last row blocks load nothing
   auto load = [&](int d, int s) {
     const unsigned ks = min(s, KS - 1);
@@ -585,14 +587,14 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
     wb[d][1] = load16_once(w, at, 1024 * (KS + ks));
   };
 #pragma unroll
-  for (int d = 0; d < kTileDepth; ++d) load(d, d);
+  for (int d = 0; d < DEPTH; ++d) load(d, d);
   // a thread stages one 16-byte piece of a chunk's columns of every 16th token
   static_assert(kTileWaves == kChunk, "16 tokens a turn");
   const int piece = tid % (4 * kChunk), token = tid / (4 * kChunk);
   unsigned row[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    const int p = r0 + list.at(min(first + 16 * i + token, n - 1));
+    const int p = r0 + list[min(first + 16 * i + token, n - 1)];
     row[i] = (PRODUCT == kGateUp ? p / k : p) * width + 16 * piece;
   }
   auto fetch = [&](int c) {
@@ -610,7 +612,7 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto step = [&](const u32x4* x, int q, int s) {
-    const int d = q % kTileDepth;
+    const int d = q % DEPTH;
     u32x4 xb[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) xb[t] = x[(t * kChunk + q) * 64];
@@ -620,7 +622,7 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
       acc[t][1] = O::mfma(wb[d][1], xb[t], acc[t][1]);
     }
     __builtin_amdgcn_sched_barrier(0);
-    load(d, s + kTileDepth);
+    load(d, s + DEPTH);
     __builtin_amdgcn_sched_barrier(0);
   };
   // LDS alone: this chunk's reads and the next one's writes; the loads from memory go on
@@ -652,18 +654,19 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
 #pragma unroll
     for (int t = 0; t < NT; ++t)
       if (first + 16 * t + j < n)
-        store_block<T, PRODUCT>(acc[t][0], acc[t][1], r0 + list.at(first + 16 * t + j), block, g, shape, total, k, gates,
+        store_block<T, PRODUCT>(acc[t][0], acc[t][1], r0 + list[first + 16 * t + j], block, g, shape, total, k, gates,
                                 out);
 }
 
-template <typename T, int PRODUCT>
-__global__ __launch_bounds__(64 * kTileWaves, 3) void expert_tiles(const T* __restrict__ in,
+template <typename T, int PRODUCT, int RANGE, int DEPTH>
+__global__ __launch_bounds__(64 * kTileWaves, DEPTH == 2 ? 4 : 3) void expert_tiles(const T* __restrict__ in,
                                                                    const u32x4* __restrict__ weights,
                                                                    const int* __restrict__ chosen,
                                                                    const float* __restrict__ gates, ExpertShape shape,
                                                                    int rows, int64_t total, int E, int k, int clears,
                                                                    void* __restrict__ out) {
-  __shared__ PairList<kTileWaves> list;
+  typedef PairList<kTileWaves, RANGE> List;
+  __shared__ List list;
   __shared__ u32x4 xs[2][kTileTokens * kChunk * 64];
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pairs = rows * k;
@@ -677,8 +680,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 3) void expert_tiles(const T* __re
                           2u * KS * 1024);
   const Buffer x = buffer(in, (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width));
 
-  for (int r0 = 0; r0 < pairs; r0 += kRange) {
-    PairList<kTileWaves>::Choices choices;
+  for (int r0 = 0; r0 < pairs; r0 += RANGE) {
+    typename List::Choices choices;
     list.load(choices, chosen, r0, pairs);
     const int n = list.fill(choices, r0, pairs, e, E);
     if (e == E) {
@@ -689,7 +692,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 3) void expert_tiles(const T* __re
     } else {
       for (int first = 0; first < n; first += 16 * kTileTokens) {
 #define WPTV_TILE(NT) \
-  tile_pass<T, PRODUCT, NT>(x, w, KS, width, list, xs, r0, first, n, block, live, shape, total, k, gates, out)
+  tile_pass<T, PRODUCT, NT, DEPTH>(x, w, KS, width, list.list, xs, r0, first, n, block, live, shape, total, k, gates, out)
         switch ((n - first + 15) / 16) {
           case 1: WPTV_TILE(1); break;
           case 2: WPTV_TILE(2); break;
@@ -883,18 +886,24 @@ int run_product(const void* in, const void* weights, const int* chosen, const fl
   const int lists = by_pair ? (int)pairs : E + clears;
   const T* from = static_cast<const T*>(in);
   const u32x4* w = static_cast<const u32x4*>(weights);
-#define WPTV_COLUMNS(NT, BY)                                                                                         \
-  expert_columns<T, PRODUCT, NT, BY><<<dim3(blocks, lists), 256, 0, stream>>>(from, w, chosen, gates, shape, rows, total, \
-                                                                              E, k, clears, out)
+#define WPTV_COLUMNS(NT, WAVES, BY)                                                                         \
+  expert_columns<T, PRODUCT, NT, WAVES, BY><<<dim3(blocks, lists), 64 * WAVES, 0, stream>>>(                \
+      from, w, chosen, gates, shape, rows, total, E, k, clears, out)
+#define WPTV_TILES(RANGE, DEPTH)                                                                            \
+  expert_tiles<T, PRODUCT, RANGE, DEPTH>                                                                    \
+      <<<dim3((blocks + kTileWaves - 1) / kTileWaves, lists), 64 * kTileWaves, 0, stream>>>(                \
+          from, w, chosen, gates, shape, rows, total, E, k, clears, out)
   if (by_pair)
-    WPTV_COLUMNS(1, true);
+    WPTV_COLUMNS(1, 4, true);
   else if (rows <= 16)
-    WPTV_COLUMNS(1, false);
+    WPTV_COLUMNS(1, 4, false);
   else if ((int64_t)E * blocks < 2048)
-    WPTV_COLUMNS(2, false);
+    WPTV_COLUMNS(2, 4, false);
+  else if (pairs <= 2048)
+    WPTV_TILES(2048, 2);
   else
-    expert_tiles<T, PRODUCT><<<dim3((blocks + kTileWaves - 1) / kTileWaves, lists), 64 * kTileWaves, 0, stream>>>(
-        from, w, chosen, gates, shape, rows, total, E, k, clears, out);
+    WPTV_TILES(4096, 4);
+#undef WPTV_TILES
 #undef WPTV_COLUMNS
   return launched(PRODUCT == kGateUp ? "experts (gate, up)" : "experts (down)");
 }
@@ -1025,8 +1034,9 @@ extern "C" int wptv_pack_experts(const void* gate_up, const void* down, int E, i
   const dim3 gu_grid((unsigned)((gu + 255) / 256), E), dn_grid((unsigned)((dn + 255) / 256), E);
 #define WPTV_PACK(TT)                                                                                             \
   pack_experts<TT, true><<<gu_grid, 256, 0, stream>>>(static_cast<const TT*>(gate_up), F, D, s.FB * 2, s.KSx,     \
-                                                      static_cast<u32x4*>(gate_up_packed));                       \
+                                                      aligned(gate_up, 16), static_cast<u32x4*>(gate_up_packed)); \
   pack_experts<TT, false><<<dn_grid, 256, 0, stream>>>(static_cast<const TT*>(down), D, F, s.DB * 2, s.KSf,       \
+                                                       aligned(down, 16) && F % Operand<TT>::EPL == 0,            \
                                                        static_cast<u32x4*>(down_packed))
   if (dtype == WPTV_BF16) {
     WPTV_PACK(unsigned short);
