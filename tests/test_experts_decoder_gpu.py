@@ -153,6 +153,21 @@ def test_beams_carry_their_routes_and_a_weighted_cache_has_none(device):
     assert len(found[0]) == 3
 
 
+def test_window_layers_alone_read_a_long_prompt(device):
+    config = DecoderConfig(layers=2, d_model=128, heads=2, head_dim=64, ffn=32, vocab=128, kinds=(WINDOW, WINDOW), window=8,
+                           rope_dims=32, experts=4, experts_per_token=2)
+    model, _ = models(config, BF16)
+    ids = torch.randint(0, config.vocab, (3, 250), generator=torch.Generator().manual_seed(1))
+    whole = model.new_cache(3, widest=250, routes=True, capacity=8)
+    scores = model.extend(ids, whole)[0]
+    pieces = model.new_cache(3, widest=250, routes=True)
+    parts = torch.cat([model.extend(ids[:, a:a + 50], pieces)[0] for a in range(0, 250, 50)], 1)
+    assert whole.routes.shape[2] >= 250 and int((whole.routes[:, :, :250] < 0).sum()) == 0
+    same = (whole.routes[:, :, :250] == pieces.routes[:, :, :250]).all(-1).all(0)  # (3, 250): no near tie fell the other way
+    assert float(same.float().mean()) > 0.9
+    assert float((scores - parts).abs()[same].max()) <= 2e-2 * float(parts.abs().max())
+
+
 def test_a_dense_decoder_records_no_routes(device):
     config = DecoderConfig(layers=1, d_model=64, heads=1, head_dim=64, ffn=32, vocab=64)
     with pytest.raises(NotImplementedError):

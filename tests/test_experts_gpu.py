@@ -71,6 +71,18 @@ def test_the_choice_is_the_sorted_logits(device, B, T, D, E, k, dtype):
     check_route(device, x, router, k, torch.randn(E, generator=g), torch.randint(0, T + 1, (B,), generator=g))
 
 
+def test_more_tokens_than_a_grid_s_dimension(device):
+    rows, D, E = (1 << 19) + 1000, 40, 512
+    g = torch.Generator(device=device).manual_seed(0)
+    x = torch.randn(1, rows, D, generator=g, device=device).to(BF16)
+    router = torch.randn(E, D, generator=g, device=device)
+    chosen, gates = experts.route(x, router, 2)
+    for part in (slice(0, 500), slice((1 << 19) - 500, None)):
+        expected = torch.topk(x[0, part].double() @ router.double().T, 2, -1)
+        assert torch.equal(chosen[0, part].long(), expected.indices)
+        gates_close(gates[0, part], torch.softmax(expected.values, -1).cpu())
+
+
 def test_equal_logits_and_experts_taken_out(device):
     x, router, _, _ = layer(1, 4, 64, 12, 8, FP32)
     router[3] = router[7] = router[1]  # equal whatever the token
@@ -129,10 +141,44 @@ def test_a_layer_is_the_gated_sum_of_its_experts(device, B, T, D, E, k, F, dtype
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_many_pairs_are_taken_range_by_range(device, dtype):
-    # 2100 tokens of 4 choices: three ranges of pairs, several tiles an expert, one expert far ahead
+    # 2100 tokens of 4 choices: three ranges of pairs, several tiles an expert, one expert far ahead; few row blocks
+    # and (E times 512 features) many
     x, router, gate_up, down = layer(3, 700, 32, 6, 16, dtype)
     router[2] += 0.5 * x.float().mean((0, 1))
     check_mixture(device, x, router, gate_up, down, 4, torch.tensor([0.0, 0.0, 5.0, 0.0, 0.0, 0.0]))
+
+
+@pytest.mark.parametrize("rows, k", [(150, 2), (256, 8), (600, 8)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_tiles_of_tokens_of_many_row_blocks(device, rows, k, dtype):
+    # 64 x 512 features, 64 x 1040 outputs: the products over tiles, in one range of pairs and in two, against torch in
+    # 64 bits on the GPU within the oracle's bound of one token, taken as the largest
+    E, D, F = 64, 1040, 512
+    g = torch.Generator(device=device).manual_seed(rows)
+    x = torch.randn(1, rows, D, generator=g, device=device).to(dtype)
+    router = torch.randn(E, D, generator=g, device=device) * D ** -0.5
+    gate_up = (torch.randn(E, 2 * F, D, generator=g, device=device) * D ** -0.5).to(dtype)
+    down = (torch.randn(E, D, F, generator=g, device=device) * F ** -0.5).to(dtype)
+    bias = torch.zeros(E, device=device)
+    bias[3] = 2.0  # one expert with several tiles
+    weights = experts.ExpertWeights(gate_up, down)
+    y, chosen, gates = experts.mixture(x, router, weights, k, bias)
+    expected = torch.zeros(rows, D, dtype=torch.float64, device=device)
+    for e in range(E):
+        token, slot = (chosen[0] == e).nonzero(as_tuple=True)
+        h = x[0, token].double() @ gate_up[e].double().T
+        act = torch.nn.functional.silu(h[:, :F]) * h[:, F:]
+        expected[token] += gates[0, token, slot, None].double() * (act @ down[e].double().T)
+    assert int((chosen == 3).sum()) > 64  # more than a tile
+    worst = 0.0
+    for m in (0, rows // 2, rows - 1):
+        _, bound = oracle.feed_forward(x[:, m:m + 1].cpu(), gate_up.cpu(), down.cpu(), chosen[:, m:m + 1].cpu(),
+                                       gates[:, m:m + 1].cpu())
+        worst = max(worst, float(bound.max()))
+    assert float((y[0].double() - expected).abs().max()) <= 2 * worst
+    parts, again, _ = experts.mixture_parts(x, router, weights, k, bias)
+    assert torch.equal(again, chosen)
+    assert float((parts.double().sum(0) - expected).abs().max()) <= 2 * worst
 
 
 def test_one_expert_may_take_every_row_and_another_none(device):

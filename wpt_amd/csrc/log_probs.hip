@@ -259,9 +259,28 @@ __global__ __launch_bounds__(THREADS) void log_probs_held(const T* __restrict__ 
                         __builtin_popcountll(__builtin_amdgcn_ballot_w64(two >= trial));
       if (reach >= top) border = trial;
     }
-    if (nan || score_key(own) >= border) each([&](int at, uint32_t x) {
-        if (x >= border) note(at, x);
-      });
+    if (nan || score_key(own) >= border) {
+      // as a comparison of scores: one below every score's key gives a NaN, which nothing is less than, as a NaN
+      // is less than nothing
+      const float least = key_value(border);
+      constexpr int kHeld = CHUNKS * C::N, kWord = kHeld < 32 ? kHeld : 32;
+#pragma unroll
+      for (int word = 0; word < kHeld / kWord; ++word) {
+        uint32_t reach = 0u;
+#pragma unroll
+        for (int c = word * kWord / C::N; c < (word + 1) * kWord / C::N; ++c) {
+          const u32x4 chunk = held(v[c]);
+#pragma unroll
+          for (int i = 0; i < C::N; ++i)
+            reach |= C::at(chunk, i) < least ? 0u : 1u << (c * C::N + i) % kWord;
+        }
+        for (; reach; reach &= reach - 1u) {  // few: read again
+          const int b = word * kWord + __builtin_ctz(reach), c = b / C::N;
+          const int first = c * kStep + tid * C::N, at = min(first, count - C::N) + b % C::N;
+          if (at >= first) note(at, score_key(load_f32<T>(s + from + at)));
+        }
+      }
+    }
   }
   __syncthreads();
   Part part = {high, 0.f, 0.f, 0.f};
@@ -489,22 +508,28 @@ __global__ __launch_bounds__(THREADS) void log_probs_row(const T* __restrict__ s
   }
 }
 
-// How a row is read: the threads and 16-byte chunks of a workgroup, and the parts
-// the row is cut into (0: from memory, rows shorter than a chunk and rows longer
+// How rows are read: the threads and 16-byte chunks of a workgroup, and the parts
+// a row is cut into (0: from memory, rows shorter than a chunk and rows longer
 // than kMaxParts of the largest workgroup).
 struct Form {
   int threads, chunks, parts, stretch;
 };
 
-Form row_form(int V, int dtype) {
+Form row_form(int64_t rows, int V, int dtype) {
   const int per = dtype == WPTV_BF16 ? 8 : 4;
+  const int64_t units = compute_units();
   if (V < per) return Form{0, 0, 0, 0};
-  static const int sizes[5][2] = {{256, 2}, {512, 4}, {512, 8}, {1024, 8}, {1024, 16}};
-  for (const auto& size : sizes)
-    if (V <= size[0] * size[1] * per) return Form{size[0], size[1], 1, V};
-  const int held = 1024 * 16 * per, parts = (V + held - 1) / held;
+  if (V <= 256 * 2 * per) return Form{256, 2, 1, V};
+  if (V <= 512 * 4 * per) return Form{512, 4, 1, V};
+  // few rows: as many threads as there are; more rows hide each other's steps, and smaller workgroups do it better
+  if (V <= 512 * 8 * per) return rows <= units ? Form{1024, 4, 1, V} : Form{512, 8, 1, V};
+  const int few = 1024 * 4 * per, many = 1024 * 16 * per;
+  int parts = (V + few - 1) / few;
+  if (parts <= kMaxParts && rows * parts <= units) return Form{1024, 4, parts, ((V + parts - 1) / parts + 7) / 8 * 8};
+  if (V <= 1024 * 8 * per) return Form{1024, 8, 1, V};
+  parts = (V + many - 1) / many;
   if (parts > kMaxParts) return Form{0, 0, 0, 0};
-  return Form{1024, 16, parts, ((V + parts - 1) / parts + 7) / 8 * 8};
+  return Form{1024, 16, parts, parts == 1 ? V : ((V + parts - 1) / parts + 7) / 8 * 8};
 }
 
 size_t part_bytes(int64_t rows, const Form& form, int top) {
@@ -531,6 +556,8 @@ int run_log_probs(const T* scores, int64_t ssb, int64_t sst, const int64_t* toke
     WPTV_HELD(512, 4);
   else if (form.threads == 512)
     WPTV_HELD(512, 8);
+  else if (form.chunks == 4)
+    WPTV_HELD(1024, 4);
   else if (form.chunks == 8)
     WPTV_HELD(1024, 8);
   else
@@ -555,8 +582,8 @@ extern "C" int wptv_log_probs_workspace(int B, int T, int V, int top, size_t* by
   if (top > kMaxTop) return fail(WPTV_E_UNSUPPORTED, "log_probs: %d alternatives above %d", top, kMaxTop);
   if (V > (1 << 24) || (int64_t)B * T > INT32_MAX)
     return fail(WPTV_E_UNSUPPORTED, "log_probs: B=%d T=%d V=%d is too large", B, T, V);
-  const size_t bf16 = part_bytes((int64_t)B * T, row_form(V, WPTV_BF16), top);
-  const size_t fp32 = part_bytes((int64_t)B * T, row_form(V, WPTV_F32), top);
+  const size_t bf16 = part_bytes((int64_t)B * T, row_form((int64_t)B * T, V, WPTV_BF16), top);
+  const size_t fp32 = part_bytes((int64_t)B * T, row_form((int64_t)B * T, V, WPTV_F32), top);
   *bytes = bf16 > fp32 ? bf16 : fp32;
   return WPTV_OK;
 }
@@ -568,7 +595,7 @@ extern "C" int wptv_log_probs(const void* scores, int64_t scores_stride_b, int64
   size_t need = 0;
   const int status = wptv_log_probs_workspace(B, T, V, top, &need);
   if (status != WPTV_OK) return status;
-  if (!(temperature > 0.f) || std::isinf(temperature))
+  if (!(temperature > 0.f) || std::isinf(temperature) || std::isinf(1.f / temperature))
     return fail(WPTV_E_INVALID, "log_probs: the temperature must be positive and finite; got %g", temperature);
   if (scores_dtype != WPTV_F32 && scores_dtype != WPTV_BF16)
     return fail(WPTV_E_UNSUPPORTED, "log_probs: dtype %d is neither fp32 nor bf16", scores_dtype);
@@ -580,7 +607,7 @@ extern "C" int wptv_log_probs(const void* scores, int64_t scores_stride_b, int64
                 need);
   const float inverse = 1.f / temperature;
   const Outputs out{logprobs, entropy, ids, best};
-  const Form form = row_form(V, scores_dtype);
+  const Form form = row_form((int64_t)B * T, V, scores_dtype);
   return scores_dtype == WPTV_BF16
              ? run_log_probs(static_cast<const unsigned short*>(scores), scores_stride_b, scores_stride_t, tokens, inverse,
                              B * T, T, V, top, form, out, workspace, stream)

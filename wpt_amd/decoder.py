@@ -257,7 +257,7 @@ class MQADecoder:
         readings)."""
         ok = self._fm_rows.get((rows, any_rows))
         if ok is None:
-            ok = self.dtype == torch.bfloat16 and self.config.head_dim in (64, 128) and all(
+            ok = self.dtype == torch.bfloat16 and self.config.head_dim in (64, 128) and bool(self.fm) and all(
                 layers.fm_plan(rows, w.shape[0], w.shape[1], swiglu=name.endswith("gate_up_tiles"),
                                any_rows=any_rows) is not None
                 for name, w in self.fm.items())

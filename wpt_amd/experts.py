@@ -41,7 +41,7 @@ def _router(router, bias, counts, x, k):
     if router.dim() != 2 or router.shape[1] != D or router.dtype != torch.float32 or router.device != x.device:
         raise ValueError(f"router must be FP32 (E, D={D}) on {x.device}; got {router.dtype} {tuple(router.shape)}")
     E = router.shape[0]
-    if not 1 <= int(k) <= E:
+    if not 1 <= k <= E:
         raise ValueError(f"k = {k} of {E} experts")
     router = router.contiguous()
     if router.data_ptr() % 16:
@@ -98,6 +98,7 @@ def route(x, router, k, bias=None, counts=None):
     experts' l, without the bias.  counts (B,): the tokens read of each row, the
     others padding (None: all).  Where no expert is chosen (padding, or fewer
     than k above -inf) chosen is -1 and the gate 0."""
+    k = int(k)
     x_, dtype, (B, T, D) = _input(x, "route")
     router, bias, counts, E = _router(router, bias, counts, x_, k)
     chosen = torch.empty(B, T, k, dtype=torch.int32, device=x.device)
@@ -105,7 +106,7 @@ def route(x, router, k, bias=None, counts=None):
     with _lib.on(x.device):
         _, size = _lib.plan("wptv_route_workspace", "route", B * T, D, E)
         workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        check(_lib.lib().wptv_route(ptr(x_), dtype, ptr(router), ptr(bias), ptr(counts), B, T, D, E, int(k),
+        check(_lib.lib().wptv_route(ptr(x_), dtype, ptr(router), ptr(bias), ptr(counts), B, T, D, E, k,
                                     ptr(chosen), ptr(gates), ptr(workspace), size, _lib.stream(x.device)), "route")
     return chosen, _forward_only(gates, x, router)
 
@@ -121,7 +122,7 @@ def _result(x, size, k, parts):
     B, T, D = x.shape
     workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     if parts:
-        return torch.empty(int(k), B * T, D, dtype=torch.float32, device=x.device), None, workspace
+        return torch.empty(k, B * T, D, dtype=torch.float32, device=x.device), None, workspace
     return None, torch.empty(B, T, D, dtype=x.dtype, device=x.device), workspace
 
 
@@ -156,6 +157,7 @@ def feed_forward_parts(x, weights, chosen, gates):
 
 
 def _mixture(x, router, weights, k, bias, counts, parts):
+    k = int(k)
     x_, dtype, (B, T, D) = _input(x, "mixture")
     _match(x_, weights, "mixture")
     router_, bias, counts, E = _router(router, bias, counts, x_, k)
@@ -165,9 +167,9 @@ def _mixture(x, router, weights, k, bias, counts, parts):
     chosen = torch.empty(B, T, k, dtype=torch.int32, device=device)
     gates = torch.empty(B, T, k, dtype=torch.float32, device=device)
     with _lib.on(device):
-        _, size = _lib.plan("wptv_mixture_workspace", "mixture", B * T, D, E, weights.features, int(k), dtype, int(parts))
+        _, size = _lib.plan("wptv_mixture_workspace", "mixture", B * T, D, E, weights.features, k, dtype, int(parts))
         out, y, workspace = _result(x_, size, k, parts)
-        check(_lib.lib().wptv_mixture(ptr(x_), dtype, ptr(router_), ptr(bias), ptr(counts), B, T, D, E, int(k),
+        check(_lib.lib().wptv_mixture(ptr(x_), dtype, ptr(router_), ptr(bias), ptr(counts), B, T, D, E, k,
                                       weights.features, ptr(weights.gate_up), ptr(weights.down), ptr(chosen), ptr(gates),
                                       ptr(out), ptr(y), ptr(workspace), size, _lib.stream(device)), "mixture")
     return (out, chosen, gates) if parts else (_forward_only(y, x, router), chosen, _forward_only(gates, x, router))
