@@ -313,9 +313,10 @@ __device__ __forceinline__ u32x4 load16(Buffer from, unsigned lane_offset, unsig
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset, offset, 0));
 }
 
-// Weights: read once, no cache line kept for them.
-__device__ __forceinline__ u32x4 load16_once(Buffer from, unsigned lane_offset, unsigned offset) {
-  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset, offset, 2));
+// Weights that one workgroup reads (ONCE): no cache line is kept for them.
+template <bool ONCE>
+__device__ __forceinline__ u32x4 load16_weights(Buffer from, unsigned lane_offset, unsigned offset) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset, offset, ONCE ? 2 : 0));
 }
 
 enum Product { kGateUp = 0, kDown = 1 };
@@ -380,6 +381,23 @@ struct PairList {
 
 };
 
+// A workgroup's column of row blocks, list of pairs and tile of that list's tokens,
+// of a grid in one dimension (product_grid): the tiles of one expert's rows follow
+// each other on one XCD (workgroup i runs on XCD i mod 8), whose cache then gives
+// the weights to all of them.
+struct Place {
+  int column, list, tile;
+};
+
+__device__ __forceinline__ Place product_place(int columns, int tiles) {
+  const int id = blockIdx.x, t = id >> 3, at = t / tiles * 8 + (id & 7);
+  return Place{at % columns, at / columns, t % tiles};
+}
+
+inline unsigned product_grid(int columns, int lists, int tiles) {
+  return (unsigned)(((int64_t)columns * lists + 7) / 8 * 8 * tiles);
+}
+
 // The parts' rows that no expert of the range writes, cleared by `waves` (at least
 // one) wavefronts of their own, one after the other a row each.
 __device__ __forceinline__ void clear_rows(const uint16_t* pairs, int n, int r0, int wave, int waves, int first,
@@ -427,11 +445,11 @@ __device__ __forceinline__ void store_block(f32x4 a, f32x4 b, int p, int block, 
 //   kDown     act -> parts [k, rows, D] FP32
 // BY_PAIR (fewer pairs than experts): workgroup y serves the expert of pair y,
 // if that is the expert's first.
-template <typename T, int PRODUCT, int NT, int WAVES, bool BY_PAIR>
+template <typename T, int PRODUCT, int NT, int WAVES, bool BY_PAIR, bool ONCE>
 __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict__ in, const u32x4* __restrict__ weights,
                                                       const int* __restrict__ chosen, const float* __restrict__ gates,
                                                       ExpertShape shape, int rows, int64_t total, int E, int k,
-                                                      int clears, void* __restrict__ out) {
+                                                      int clears, int lists, int tiles, void* __restrict__ out) {
   using O = Operand<T>;
   constexpr int kDepth = 3, kRange = NT == 1 ? 1024 : 4096;
   typedef PairList<WAVES, kRange> List;
@@ -440,19 +458,21 @@ __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pairs = rows * k;
-  int e = BY_PAIR ? chosen[blockIdx.y] : (int)blockIdx.y < clears ? E : blockIdx.y - clears;
+  const Place place = product_place(PRODUCT == kGateUp ? shape.FB : shape.DB, tiles);
+  if (place.list >= lists) return;
+  int e = BY_PAIR ? chosen[place.list] : place.list < clears ? E : place.list - clears;
   if constexpr (BY_PAIR) e = (unsigned)__builtin_amdgcn_readfirstlane(e) < (unsigned)E ? __builtin_amdgcn_readfirstlane(e) : E;
   const int KS = PRODUCT == kGateUp ? shape.KSx : shape.KSf;
   const unsigned width = (PRODUCT == kGateUp ? shape.D : shape.Fp) * sizeof(T);
-  const int block = blockIdx.x, blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
+  const int block = place.column, blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
   const int steps = (KS - wv + WAVES - 1) / WAVES;
   const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + block) * 2 * KS * 64, 2u * KS * 1024);
   const Buffer x = buffer(in, (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width));
   u32x4 wb[kDepth][2], xb[kDepth][NT];
   auto load_weights = [&](int d, int s) {
     const unsigned ks = wv + WAVES * s;
-    wb[d][0] = load16_once(w, 16 * lane, 1024 * ks);
-    wb[d][1] = load16_once(w, 16 * lane, 1024 * (KS + ks));
+    wb[d][0] = load16_weights<ONCE>(w, 16 * lane, 1024 * ks);
+    wb[d][1] = load16_weights<ONCE>(w, 16 * lane, 1024 * (KS + ks));
   };
   // a few pairs: the first weights are asked for before the expert's tokens are known (one token's layer 32.0 -> 30.1
   // us; with more of them the registers cost more than it gives, 16 tokens over wide experts 101 -> 103)
@@ -473,7 +493,7 @@ __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict
         const int c = chosen[min(p, pairs - 1)];
         const bool same = p < pairs && (c == e || (e == E && (unsigned)c >= (unsigned)E));
         const uint64_t found = __builtin_amdgcn_ballot_w64(same);
-        if (__builtin_amdgcn_ballot_w64(same && p < (int)blockIdx.y)) return;  // an earlier pair's workgroup serves it
+        if (__builtin_amdgcn_ballot_w64(same && p < place.list)) return;  // an earlier pair's workgroup serves it
         if (same) own[n + __builtin_popcountll(found & ((1ull << lane) - 1ull))] = (uint16_t)p;
         n += __builtin_popcountll(found);
       }
@@ -485,13 +505,13 @@ __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict
       n = list.fill(choices, r0, pairs, e, E);
     }
     if (e == E) {
-      if (PRODUCT == kDown && clears > 0)
-        clear_rows(mine, n, r0, BY_PAIR ? wv : blockIdx.y * WAVES + wv, BY_PAIR ? WAVES : clears * WAVES, 32 * block, 32 * block + 32,
+      if (PRODUCT == kDown && clears > 0 && place.tile == 0)
+        clear_rows(mine, n, r0, BY_PAIR ? wv : place.list * WAVES + wv, BY_PAIR ? WAVES : clears * WAVES, 32 * block, 32 * block + 32,
                    shape.D, total, k, static_cast<float*>(out));
       __syncthreads();
       continue;
     }
-    for (int first = 0; first < n; first += 16 * NT) {
+    for (int first = 16 * NT * place.tile; first < n; first += 16 * NT * tiles) {
       int pair[NT];
       unsigned row[NT];
 #pragma unroll
@@ -571,7 +591,7 @@ __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict
 constexpr int kTileWaves = 4, kTileTokens = 4, kChunk = 4;
 
 // A tile of NT times 16 tokens, `first` the list's place of the first.
-template <typename T, int PRODUCT, int NT, int DEPTH>
+template <typename T, int PRODUCT, int NT, int DEPTH, bool ONCE>
 __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned width,
                                           const uint16_t* list, u32x4 (*xs)[kTileTokens * kChunk * 64],
                                           int r0, int first, int n, int block, bool live, const ExpertShape& shape,
@@ -583,8 +603,8 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
   const unsigned at = live ? 16 * lane : kOutside;  // wavefronts past the last row blocks load nothing
   auto load = [&](int d, int s) {
     const unsigned ks = min(s, KS - 1);
-    wb[d][0] = load16_once(w, at, 1024 * ks);
-    wb[d][1] = load16_once(w, at, 1024 * (KS + ks));
+    wb[d][0] = load16_weights<ONCE>(w, at, 1024 * ks);
+    wb[d][1] = load16_weights<ONCE>(w, at, 1024 * (KS + ks));
   };
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) load(d, d);
@@ -658,23 +678,27 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
                                 out);
 }
 
-template <typename T, int PRODUCT, int RANGE, int DEPTH>
+template <typename T, int PRODUCT, int RANGE, int DEPTH, bool ONCE>
 __global__ __launch_bounds__(64 * kTileWaves, DEPTH == 2 ? 4 : 3) void expert_tiles(const T* __restrict__ in,
                                                                    const u32x4* __restrict__ weights,
                                                                    const int* __restrict__ chosen,
                                                                    const float* __restrict__ gates, ExpertShape shape,
                                                                    int rows, int64_t total, int E, int k, int clears,
+                                                                   int lists, int tiles,
                                                                    void* __restrict__ out) {
   typedef PairList<kTileWaves, RANGE> List;
   __shared__ List list;
   __shared__ u32x4 xs[2][kTileTokens * kChunk * 64];
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pairs = rows * k;
-  const int e = (int)blockIdx.y < clears ? E : blockIdx.y - clears;
+  const Place place =
+      product_place(((PRODUCT == kGateUp ? shape.FB : shape.DB) + kTileWaves - 1) / kTileWaves, tiles);
+  if (place.list >= lists) return;
+  const int e = place.list < clears ? E : place.list - clears;
   const int KS = PRODUCT == kGateUp ? shape.KSx : shape.KSf;
   const unsigned width = (PRODUCT == kGateUp ? shape.D : shape.Fp) * sizeof(T);
   const int blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
-  const int block = blockIdx.x * kTileWaves + wv;
+  const int block = place.column * kTileWaves + wv;
   const bool live = block < blocks;
   const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + min(block, blocks - 1)) * 2 * KS * 64,
                           2u * KS * 1024);
@@ -685,14 +709,14 @@ __global__ __launch_bounds__(64 * kTileWaves, DEPTH == 2 ? 4 : 3) void expert_ti
     list.load(choices, chosen, r0, pairs);
     const int n = list.fill(choices, r0, pairs, e, E);
     if (e == E) {
-      if (PRODUCT == kDown && clears > 0)
-        clear_rows(list.list, n, r0, blockIdx.y * kTileWaves + wv, clears * kTileWaves,
-                   32 * (int)blockIdx.x * kTileWaves, 32 * (int)(blockIdx.x + 1) * kTileWaves, shape.D,
+      if (PRODUCT == kDown && clears > 0 && place.tile == 0)
+        clear_rows(list.list, n, r0, place.list * kTileWaves + wv, clears * kTileWaves, 32 * place.column * kTileWaves,
+                   32 * (place.column + 1) * kTileWaves, shape.D,
                    total, k, static_cast<float*>(out));
     } else {
-      for (int first = 0; first < n; first += 16 * kTileTokens) {
+      for (int first = 16 * kTileTokens * place.tile; first < n; first += 16 * kTileTokens * tiles) {
 #define WPTV_TILE(NT) \
-  tile_pass<T, PRODUCT, NT, DEPTH>(x, w, KS, width, list.list, xs, r0, first, n, block, live, shape, total, k, gates, out)
+  tile_pass<T, PRODUCT, NT, DEPTH, ONCE>(x, w, KS, width, list.list, xs, r0, first, n, block, live, shape, total, k, gates, out)
         switch ((n - first + 15) / 16) {
           case 1: WPTV_TILE(1); break;
           case 2: WPTV_TILE(2); break;
@@ -764,7 +788,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void expert_rows(const T* __restric
   auto load = [&](int d, int s) {
     const int step = wv + kFewWaves * s, which = step / KS, ks = step - which * KS;
     const u32x4* w = w0 + __builtin_amdgcn_readfirstlane(expert[which]) * matrix;
-    wb[d] = load16_once(buffer(w, 1024u * KS), 16 * lane, 1024 * ks);
+    wb[d] = load16_weights<true>(buffer(w, 1024u * KS), 16 * lane, 1024 * ks);
     const unsigned p = prow[which][j];
     xb[d] = load16(x, p == kNone ? kOutside : p * width + 16 * g, 64 * ks);
   };
@@ -886,23 +910,35 @@ int run_product(const void* in, const void* weights, const int* chosen, const fl
   const int lists = by_pair ? (int)pairs : E + clears;
   const T* from = static_cast<const T*>(in);
   const u32x4* w = static_cast<const u32x4*>(weights);
-#define WPTV_COLUMNS(NT, WAVES, BY)                                                                         \
-  expert_columns<T, PRODUCT, NT, WAVES, BY><<<dim3(blocks, lists), 64 * WAVES, 0, stream>>>(                \
-      from, w, chosen, gates, shape, rows, total, E, k, clears, out)
-#define WPTV_TILES(RANGE, DEPTH)                                                                            \
-  expert_tiles<T, PRODUCT, RANGE, DEPTH>                                                                    \
-      <<<dim3((blocks + kTileWaves - 1) / kTileWaves, lists), 64 * kTileWaves, 0, stream>>>(                \
-          from, w, chosen, gates, shape, rows, total, E, k, clears, out)
+  // tiles of one expert's tokens side by side, as many as its mean count in a range of pairs fills
+  const int64_t mean = (pairs < 8192 ? pairs : 8192) / E;
+  const int tiles = (int)((mean + 63) / 64), few = (int)((mean + 31) / 32);
+#define WPTV_COLUMNS(NT, TILES, BY, ONCE)                                                                   \
+  expert_columns<T, PRODUCT, NT, 4, BY, ONCE><<<product_grid(blocks, lists, TILES), 256, 0, stream>>>(      \
+      from, w, chosen, gates, shape, rows, total, E, k, clears, lists, TILES, out)
+#define WPTV_TILES(RANGE, DEPTH, ONCE)                                                                      \
+  expert_tiles<T, PRODUCT, RANGE, DEPTH, ONCE>                                                              \
+      <<<product_grid((blocks + kTileWaves - 1) / kTileWaves, lists, tiles), 64 * kTileWaves, 0, stream>>>( \
+          from, w, chosen, gates, shape, rows, total, E, k, clears, lists, tiles, out)
+  // The k-steps of a block pair over a workgroup, or tiles of 64 tokens a wavefront.  Whole layers, us, columns and
+  // tiles: bf16, E blocks 352 (8 experts of 704, 300 tokens of 1000) 40.8, 39.1; 528 (6 of 1408, 100 tokens of 4096)
+  // 99, 83; 1408 (16 of 1408, 256 tokens) 130, 115; FP32, whose instructions take four times as long, 512 (16 of 512,
+  // 200 tokens of 1024) 61, 103.
+  const int64_t least = sizeof(T) == 2 ? 512 : 1024;
   if (by_pair)
-    WPTV_COLUMNS(1, 4, true);
+    WPTV_COLUMNS(1, 1, true, true);
   else if (rows <= 16)
-    WPTV_COLUMNS(1, 4, false);
-  else if ((int64_t)E * blocks < 2048)
-    WPTV_COLUMNS(2, 4, false);
+    WPTV_COLUMNS(1, 1, false, true);
+  else if ((int64_t)E * blocks * tiles < least && few == 1)
+    WPTV_COLUMNS(2, 1, false, true);
+  else if ((int64_t)E * blocks * tiles < least)
+    WPTV_COLUMNS(2, few, false, false);
+  else if (tiles > 1 || pairs > 4096)
+    WPTV_TILES(8192, 4, false);
   else if (pairs <= 2048)
-    WPTV_TILES(2048, 2);
+    WPTV_TILES(2048, 2, true);
   else
-    WPTV_TILES(4096, 4);
+    WPTV_TILES(4096, 4, true);
 #undef WPTV_TILES
 #undef WPTV_COLUMNS
   return launched(PRODUCT == kGateUp ? "experts (gate, up)" : "experts (down)");
