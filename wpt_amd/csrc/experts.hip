@@ -112,41 +112,55 @@ __device__ __forceinline__ uint64_t order_key64(double f) {
 
 constexpr int kMaxExperts = 512, kMaxChosen = 16;
 
-// The places of a token's experts (the count of those before each), by the
-// `threads` threads tid, tid + threads, ... of its own; place holds -1 before.  key
-// is filled up to a multiple of 8 with keys that are before none (0).
-__device__ __forceinline__ void place_experts(const uint64_t* key, int tid, int threads, int E, int k, int* place) {
+// A token's choices and gates by one wavefront (every lane calls): lane l holds the
+// logits of experts l, l + 64, ... and their keys (0, below every key, past the
+// last).  k times the largest key left, the lowest expert of equal ones; the softmax
+// of the chosen logits in 64 bits.
+template <int SLOTS>
+__device__ __forceinline__ void choose_experts(const double (&logit)[SLOTS], uint64_t (&key)[SLOTS], int k,
+                                               int* __restrict__ chosen, float* __restrict__ gates) {
+  const int lane = threadIdx.x & 63;
   const uint64_t none = order_key64(-__builtin_inf());
-  for (int e = tid; e < E; e += threads) {
-    const uint64_t mine = key[e];
-    int before = 0;
-    for (int i = 0; i < E; i += 8) {
-      uint64_t other[8];
+  int mine = -1;  // lane i keeps choice i
+  double l = -__builtin_inf();
+  for (int i = 0; i < k; ++i) {
+    uint64_t best = key[0];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) other[u] = key[i + u];
+    for (int s = 1; s < SLOTS; ++s) best = key[s] > best ? key[s] : best;
+    const int flip = INT_MIN;  // signed maxima of unsigned halves
+    const int high = wave_max_i32((int)(best >> 32) ^ flip);
+    const int low = wave_max_i32((int)(best >> 32 ^ (unsigned)flip) == high ? (int)(uint32_t)best ^ flip : INT_MIN);
+    const uint64_t top = (uint64_t)(unsigned)(high ^ flip) << 32 | (unsigned)(low ^ flip);
+    if (top <= none) break;
+    int e = -1;
+    double its = 0.;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) before += other[u] > mine || (other[u] == mine && i + u < e) ? 1 : 0;
+    for (int s = SLOTS - 1; s >= 0; --s) {
+      const uint64_t same = __builtin_amdgcn_ballot_w64(key[s] == top);
+      if (same) {
+        const int at = __builtin_ctzll(same);
+        e = 64 * s + at;
+        its = __shfl(logit[s], at, 64);
+      }
     }
-    if (before < k && mine != none) place[before] = e;
-  }
-}
-
-// A token's choices and gates, the softmax of the chosen logits in 64 bits, by the
-// first 16 lanes of a wavefront (every lane calls).
-__device__ __forceinline__ void store_choices(const double* logit, const int* place, int lane, int k,
-                                              int* __restrict__ chosen, float* __restrict__ gates) {
-  const int e = lane < k ? place[lane] : -1;
-  const double l = e < 0 ? -__builtin_inf() : logit[e];
-  double high = l;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) high = fmax(high, __shfl_xor(high, o, 64));
-  const double share = e < 0 ? 0. : exp(l - high);  // a NaN among them, or +inf, makes the total one
+    for (int s = 0; s < SLOTS; ++s)
+      if (e == 64 * s + lane) key[s] = 0;
+    if (lane == i) {
+      mine = e;
+      l = its;
+    }
+  }
+  double most = l;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) most = fmax(most, __shfl_xor(most, o, 64));
+  const double share = mine < 0 ? 0. : exp(l - most);  // a NaN among them, or +inf, makes the total one
   double total = share;
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
   if (lane < k) {
-    chosen[lane] = e;
-    gates[lane] = e < 0 ? 0.f : (float)(share / total);
+    chosen[lane] = mine;
+    gates[lane] = mine < 0 ? 0.f : (float)(share / total);
   }
 }
 
@@ -165,14 +179,12 @@ __device__ __forceinline__ void load_four(const T* p, float* to) {
 
 // A narrow router in one launch: a workgroup a token, its wavefronts share out the
 // experts, the lanes the width.
-template <typename T>
+template <typename T, int SLOTS>
 __global__ __launch_bounds__(256) void route_token(const T* __restrict__ x, const float* __restrict__ router,
                                                    const float* __restrict__ bias, const int64_t* __restrict__ counts,
                                                    int per_row, int D, int E, int k, int* __restrict__ chosen,
                                                    float* __restrict__ gates) {
-  __shared__ double logit[kMaxExperts];
-  __shared__ uint64_t key[kMaxExperts + 8];
-  __shared__ int place[kMaxChosen];
+  __shared__ double logit[64 * SLOTS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t m = blockIdx.x;
   const T* row = x + m * D;
@@ -195,17 +207,20 @@ __global__ __launch_bounds__(256) void route_token(const T* __restrict__ x, cons
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) {
-      logit[e] = sum;
-      key[e] = order_key64(bias ? sum + (double)bias[e] : sum);
-    }
+    if (lane == 0) logit[e] = sum;
   }
-  if (tid < k) place[tid] = -1;
-  if (tid < 8) key[E + tid] = 0;
   __syncthreads();
-  if (!counts || m % per_row < counts[m / per_row]) place_experts(key, tid, 256, E, k, place);
-  __syncthreads();
-  if (tid < 64) store_choices(logit, place, lane, k, chosen + m * k, gates + m * k);
+  if (tid >= 64) return;
+  const bool read = !counts || m % per_row < counts[m / per_row];
+  double own[SLOTS];
+  uint64_t key[SLOTS];
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s) {
+    const int e = lane + 64 * s;
+    own[s] = e < E ? logit[e] : 0.;
+    key[s] = read && e < E ? order_key64(bias ? own[s] + (double)bias[e] : own[s]) : 0;
+  }
+  choose_experts<SLOTS>(own, key, k, chosen + m * k, gates + m * k);
 }
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -255,35 +270,36 @@ __global__ __launch_bounds__(256) void route_logits(const T* __restrict__ x, con
 }
 
 // A wavefront a token.
+template <int SLOTS>
 __global__ __launch_bounds__(256) void route_choose(const double* __restrict__ sums, const float* __restrict__ bias,
                                                     const int64_t* __restrict__ counts, int rows, int per_row, int E,
                                                     int splits, int k, int* __restrict__ chosen,
                                                     float* __restrict__ gates) {
-  __shared__ double logits[4][kMaxExperts];
-  __shared__ uint64_t keys[4][kMaxExperts + 8];
-  __shared__ int places[4][kMaxChosen];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, m = blockIdx.x * 4 + wv;
-  double* logit = logits[wv];
-  const bool read = m < rows && (!counts || m % per_row < counts[m / per_row]);
-  if (lane < k) places[wv][lane] = -1;
-  if (lane < 8) keys[wv][E + lane] = 0;
-  if (read)
-    for (int e = lane; e < E; e += 64) {
-      double sum = 0.;
-      for (int z = 0; z < splits; z += 8) {
-        double part[8];
+  const int lane = threadIdx.x & 63, m = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (m >= rows) return;
+  const bool read = !counts || m % per_row < counts[m / per_row];
+  double own[SLOTS];
+  uint64_t key[SLOTS];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) part[u] = sums[((int64_t)min(z + u, splits - 1) * rows + m) * E + e];
+  for (int s = 0; s < SLOTS; ++s) own[s] = 0.;
+  for (int z = 0; z < splits; z += 4) {
+    double part[4][SLOTS];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) sum += z + u < splits ? part[u] : 0.;
-      }
-      logit[e] = sum;
-      keys[wv][e] = order_key64(bias ? sum + (double)bias[e] : sum);
-    }
-  __syncthreads();
-  if (read) place_experts(keys[wv], lane, 64, E, k, places[wv]);
-  __syncthreads();
-  if (m < rows) store_choices(logit, places[wv], lane, k, chosen + (int64_t)m * k, gates + (int64_t)m * k);
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s)
+        part[u][s] = sums[((int64_t)min(z + u, splits - 1) * rows + m) * E + min(lane + 64 * s, E - 1)];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) own[s] += z + u < splits ? part[u][s] : 0.;
+  }
+#pragma unroll
+  for (int s = 0; s < SLOTS; ++s) {
+    const int e = lane + 64 * s;
+    key[s] = read && e < E ? order_key64(bias ? own[s] + (double)bias[e] : own[s]) : 0;
+  }
+  choose_experts<SLOTS>(own, key, k, chosen + (int64_t)m * k, gates + (int64_t)m * k);
 }
 
 // The router's form: one launch where a token's workgroup reads little, else the
@@ -878,13 +894,27 @@ int check_features(const char* what, int F) {
 
 size_t route_bytes(int64_t rows, int D, int E) { return (size_t)route_splits(rows, D, E) * rows * E * sizeof(double); }
 
+// The experts a lane of a token's wavefront holds.
+#define WPTV_SLOTS(FORM) \
+  if (E <= 64)           \
+    FORM(1);             \
+  else if (E <= 128)     \
+    FORM(2);             \
+  else if (E <= 256)     \
+    FORM(4);             \
+  else                   \
+    FORM(8)
+
 template <typename T>
 int run_route(const void* x, const float* router, const float* bias, const int64_t* counts, int rows, int per_row, int D,
               int E, int k, int* chosen, float* gates, void* workspace, hipStream_t stream) {
   const T* xt = static_cast<const T*>(x);
   const int splits = route_splits(rows, D, E);
   if (splits == 0) {
-    route_token<T><<<rows, 256, 0, stream>>>(xt, router, bias, counts, per_row, D, E, k, chosen, gates);
+#define WPTV_TOKEN(SLOTS) \
+  route_token<T, SLOTS><<<rows, 256, 0, stream>>>(xt, router, bias, counts, per_row, D, E, k, chosen, gates)
+    WPTV_SLOTS(WPTV_TOKEN);
+#undef WPTV_TOKEN
     return launched("route");
   }
   double* sums = static_cast<double*>(workspace);
@@ -896,7 +926,11 @@ int run_route(const void* x, const float* router, const float* bias, const int64
   }
   const int status = launched("route (logits)");
   if (status != WPTV_OK) return status;
-  route_choose<<<(rows + 3) / 4, 256, 0, stream>>>(sums, bias, counts, rows, per_row, E, splits, k, chosen, gates);
+#define WPTV_CHOOSE(SLOTS) \
+  route_choose<SLOTS>      \
+      <<<(rows + 3) / 4, 256, 0, stream>>>(sums, bias, counts, rows, per_row, E, splits, k, chosen, gates)
+  WPTV_SLOTS(WPTV_CHOOSE);
+#undef WPTV_CHOOSE
   return launched("route (choice)");
 }
 
