@@ -29,6 +29,22 @@ struct Outputs {
   float* best;
 };
 
+// The workgroup's row (b, t) of scores.
+template <typename T>
+__device__ __forceinline__ const T* row_of(const T* scores, int64_t ssb, int64_t sst, int per_row) {
+  const unsigned b = blockIdx.x / (unsigned)per_row, t = blockIdx.x - b * (unsigned)per_row;
+  return scores + b * ssb + t * sst;
+}
+
+// The maximum over a wavefront without LDS; every lane must be active.
+__device__ __forceinline__ float wave_max_dpp(float x) {
+  x = row16_max(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // What a stretch of a row's scores comes to: their maximum, how many hold it, the
 // others' sums of exp d and d exp d with d = (x - high) / temperature.
 struct Part {
@@ -151,7 +167,7 @@ __global__ __launch_bounds__(THREADS) void log_probs_held(const T* __restrict__ 
   __shared__ TopShared<TOP ? THREADS : 0> shared;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t m = blockIdx.x;
-  const T* s = scores + m / per_row * ssb + m % per_row * sst;
+  const T* s = row_of(scores, ssb, sst, per_row);
   const int from = blockIdx.y * stretch, count = min(stretch, V - from);  // at least 8, and `top`
   // chunk c of a thread starts at its place in the stretch, or 16 bytes before the stretch's end if that comes
   // first: what it then holds of the chunk before it, `skip` scores, counts as -inf
@@ -174,7 +190,7 @@ __global__ __launch_bounds__(THREADS) void log_probs_held(const T* __restrict__ 
 #pragma unroll
     for (int i = 0; i < C::N; ++i) own = fmaxf(own, C::at(chunk, i));
   }
-  float high = wave_max(own);
+  float high = wave_max_dpp(own);
   if (lane == 0) sums[0][w] = high;
   if constexpr (TOP) {
     float group = own;  // of THREADS / kGroups lanes
@@ -364,7 +380,7 @@ __global__ __launch_bounds__(256) void log_probs_join(const T* __restrict__ scor
   __shared__ uint64_t all[kMaxParts * kMaxTop];
   const int tid = threadIdx.x, total = count * top;
   const int64_t m = blockIdx.x;
-  const T* s = scores + m / per_row * ssb + m % per_row * sst;
+  const T* s = row_of(scores, ssb, sst, per_row);
   const int64_t token = tokens[m];
   const bool written = token >= 0 && token < V;
   const float given = load_f32<T>(s + (written ? token : 0));
@@ -411,7 +427,7 @@ __global__ __launch_bounds__(THREADS) void log_probs_row(const T* __restrict__ s
   __shared__ int at[kMaxTop];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t m = blockIdx.x;
-  const T* s = scores + m / per_row * ssb + m % per_row * sst;
+  const T* s = row_of(scores, ssb, sst, per_row);
   float high = -__builtin_inff();
   for (int i = tid; i < V; i += THREADS) high = fmaxf(high, load_f32<T>(s + i));
   high = wave_max(high);
