@@ -604,8 +604,8 @@ int wptv_route(const void* x, int dtype, const float* router, const float* bias,
  *   buffers of E times the bytes wptv_experts_packed gives an expert.
  * wptv_experts: y[m] = the sum over j of gates[m, j] down_e (silu(gate_e x[m])
  *   * (up_e x[m])), e = chosen[m, j]; a choice outside 0 .. E - 1 adds nothing.
- *   FP32 sums; silu(g) u is rounded once to dtype between the products.  x
- *   [rows, D]; the result in one of two forms, the other pointer NULL:
+ *   FP32 sums; gates[m, j] silu(g) u is rounded once to dtype between the
+ *   products.  x [rows, D]; the result in one of two forms, the other pointer NULL:
  *   parts    [k, rows, D] fp32: choice j's gated term in parts[j], for a
  *            consumer that sums them (wptv_add_rms_norm_parts, k <= 8)
  *   y        [rows, D] in dtype, their sum in order, rounded once

@@ -32,8 +32,8 @@ def feed_forward(x, gate_up, down, chosen, gates):
     """(y, bound): the gated sum of the chosen experts' SwiGLU blocks, (B, T, D)
     in 64 bits, and a bound on the error of a computation that sums in FP32 in
     any order (n terms: n 2^-24 of the sum of their magnitudes), rounds
-    silu(g) u once to x's dtype and the result once; the exponential and the
-    quotient take 8 steps of 2^-24 of silu."""
+    silu(g) u, gated or not, once to x's dtype and the result once; the
+    exponential and the quotient take 8 steps of 2^-24 of silu."""
     B, T, D = x.shape
     E, F2, _ = gate_up.shape
     F, step, unit = F2 // 2, HALF_STEP[x.dtype], 2.0 ** -24

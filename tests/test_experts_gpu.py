@@ -190,6 +190,23 @@ def test_one_expert_may_take_every_row_and_another_none(device):
         assert chosen[..., 0].unique().tolist() == [5] and chosen[..., 1].unique().tolist() == [-1]
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_fewer_pairs_than_experts_all_of_one(device, dtype):
+    # several tiles of an expert that is served by its first pair's workgroups
+    for rows, k, E in ((60, 1, 64), (100, 2, 300), (511, 1, 512)):
+        x, router, gate_up, down = layer(rows, 1, 72, E, 24, dtype, seed=rows)
+        weights = experts.ExpertWeights(gate_up.to(device), down.to(device))
+        chosen = torch.full((rows, 1, k), E // 2, dtype=torch.int32)
+        chosen[rows // 3, 0, 0], chosen[rows // 2, 0, k - 1] = 5, -1
+        gates = torch.rand(rows, 1, k, generator=torch.Generator().manual_seed(1))
+        expected = oracle.feed_forward(x, gate_up, down, chosen, gates)
+        on = [t.to(device) for t in (x, chosen, gates)]
+        for _ in range(3):
+            y_close(experts.feed_forward(on[0], weights, on[1], on[2]), expected, dtype)
+            parts = experts.feed_forward_parts(on[0], weights, on[1], on[2])
+            assert bool(((parts.double().sum(0).cpu() - expected[0].view(rows, -1)).abs() <= expected[1].view(rows, -1)).all())
+
+
 @pytest.mark.parametrize("rows", [1, 6, 40])
 def test_given_choices_may_repeat_an_expert_or_name_none(device, rows):
     x, _, gate_up, down = layer(1, rows, 64, 7, 24, BF16)

@@ -8,6 +8,16 @@
 // Every (token, choice) is a "pair" p = m k + j.  What bounds the products is
 // the stream of the experts' weights, read once each: a pair adds a column to a
 // matrix instruction that its expert's weights feed anyway.
+//
+// Each product is one launch over all experts, in a form by the counts:
+//   expert_columns  few tokens, or few row blocks: a workgroup a pair of 16-row
+//                   blocks, its wavefronts sharing out the width
+//   expert_tiles    more: a pair of blocks a wavefront, the tokens through LDS
+//   expert_rows     the down product of a few tokens, joined in the same launch
+// then join_experts, or the residual norm, adds a token's terms.  Kernels, us: 160
+// rows (120 of them read), 8 of 64 experts of 704 features, width 2048 (0.55 GB):
+// products 66 and 37 (5.5 and 4.9 TB/s), router 5 and 4, join 5; one row 12 and 7;
+// 512 rows (384 read) over 128 experts (1.1 GB) 138 and 84.
 #include "wptv_common.h"
 
 #include <climits>
@@ -33,8 +43,8 @@ template <>
 struct Operand<unsigned short> {
   static constexpr int KU = 32, EPL = 8;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                   0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
   }
 };
 
@@ -224,6 +234,7 @@ __global__ __launch_bounds__(256) void route_token(const T* __restrict__ x, cons
 }
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
+
 // The logits of a wider one on the 64-bit matrix instruction (16 experts by 16
 // tokens by 4 columns; the product of two FP32 values is exact): grid (E / 16,
 // rows / 16, splits), workgroup z's four wavefronts taking the 16-column steps
@@ -394,7 +405,6 @@ struct PairList {
     __syncthreads();
     return total;
   }
-
 };
 
 // A workgroup's column of row blocks, list of pairs and tile of that list's tokens,
@@ -451,23 +461,27 @@ __device__ __forceinline__ void store_block(f32x4 a, f32x4 b, int p, int block, 
   }
 }
 
-// grid (row-block pairs, experts or pairs): a workgroup's four wavefronts share
-// out the k-steps of one row-block pair of one expert's matrix (their sums joined
-// in LDS, in order), over tiles of 16 NT of the expert's tokens.  The weights are
-// the A operand, the tokens the B operand, both straight from memory into
-// registers, kDepth k-steps ahead.
+// A workgroup's four wavefronts share out the k-steps of one row-block pair of one
+// expert's matrix (their sums joined in LDS, in order), over tiles of 16 NT of the
+// expert's tokens.  The weights are the A operand, the tokens the B operand, both
+// straight from memory into registers, kDepth k-steps ahead: three keep the stream
+// going and leave room for four workgroups a compute unit (6 tokens, 8 of 64 experts
+// of 704, whole layers: 8 ahead 81 us, 6 73, 4 71, 3 69).
 //   kGateUp   x [rows, D] -> act [pairs, Fp]: gates[p] silu(g) u of the FP32 sums,
 //             rounded once to T, which the down product takes
 //   kDown     act -> parts [k, rows, D] FP32
-// BY_PAIR (fewer pairs than experts): workgroup y serves the expert of pair y,
-// if that is the expert's first.
+// BY_PAIR (fewer pairs than experts): a workgroup serves the expert of one pair, if
+// that is the expert's first.
 template <typename T, int PRODUCT, int NT, int WAVES, bool BY_PAIR, bool ONCE>
-__global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict__ in, const u32x4* __restrict__ weights,
-                                                      const int* __restrict__ chosen, const float* __restrict__ gates,
-                                                      ExpertShape shape, int rows, int64_t total, int E, int k,
-                                                      int clears, int lists, int tiles, void* __restrict__ out) {
+__global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict__ in,
+                                                             const u32x4* __restrict__ weights,
+                                                             const int* __restrict__ chosen,
+                                                             const float* __restrict__ gates, ExpertShape shape,
+                                                             int rows, int64_t total, int E, int k, int clears,
+                                                             int lists, int tiles, void* __restrict__ out) {
   using O = Operand<T>;
-  constexpr int kDepth = 3, kRange = NT == 1 ? 1024 : 4096;
+  // a list of its own a wavefront, for fewer than kMaxExperts pairs; 16 tokens have up to 256 pairs
+  constexpr int kDepth = 3, kRange = BY_PAIR ? WAVES * kMaxExperts : NT == 1 ? 1024 : 4096;
   typedef PairList<WAVES, kRange> List;
   __shared__ List list;
   __shared__ float red[WAVES * NT * 2 * 4 * 64];
@@ -477,7 +491,8 @@ __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict
   const Place place = product_place(PRODUCT == kGateUp ? shape.FB : shape.DB, tiles);
   if (place.list >= lists) return;
   int e = BY_PAIR ? chosen[place.list] : place.list < clears ? E : place.list - clears;
-  if constexpr (BY_PAIR) e = (unsigned)__builtin_amdgcn_readfirstlane(e) < (unsigned)E ? __builtin_amdgcn_readfirstlane(e) : E;
+  e = __builtin_amdgcn_readfirstlane(e);
+  if ((unsigned)e >= (unsigned)E) e = E;  // no expert
   const int KS = PRODUCT == kGateUp ? shape.KSx : shape.KSf;
   const unsigned width = (PRODUCT == kGateUp ? shape.D : shape.Fp) * sizeof(T);
   const int block = place.column, blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
@@ -522,8 +537,8 @@ __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict
     }
     if (e == E) {
       if (PRODUCT == kDown && clears > 0 && place.tile == 0)
-        clear_rows(mine, n, r0, BY_PAIR ? wv : place.list * WAVES + wv, BY_PAIR ? WAVES : clears * WAVES, 32 * block, 32 * block + 32,
-                   shape.D, total, k, static_cast<float*>(out));
+        clear_rows(mine, n, r0, BY_PAIR ? wv : place.list * WAVES + wv, BY_PAIR ? WAVES : clears * WAVES, 32 * block,
+                   32 * block + 32, shape.D, total, k, static_cast<float*>(out));
       __syncthreads();
       continue;
     }
@@ -598,21 +613,23 @@ __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict
   }
 }
 
-// grid (row-block pairs / 8, experts): a workgroup's eight wavefronts take a
-// row-block pair of one expert's matrix each, over tiles of up to 64 of the
-// expert's tokens.  The tokens' columns go through LDS, kChunk k-steps at a time in
-// two buffers, in the order the matrix instructions take them; the weights go
-// straight from memory into registers, DEPTH k-steps ahead, across the chunks'
-// barriers, which wait for LDS alone.
+// A workgroup's four wavefronts take a row-block pair of one expert's matrix each,
+// over tiles of up to 64 of the expert's tokens.  The tokens' columns go through LDS,
+// kChunk k-steps at a time in two buffers, in the order the matrix instructions take
+// them; the weights go straight from memory into registers, DEPTH k-steps ahead,
+// across the chunks' barriers, which wait for LDS alone.  Whole layers, us, of 160
+// and of 512 rows (above): eight wavefronts a workgroup 135, 291, four 125, 254; tiles
+// of 32 tokens 138, 314, of 48 132, 270, of 64 125, 255; weights kept in the caches
+// 131, 263.  Up to 2048 pairs, shorter lists and two k-steps ahead let four workgroups
+// share a compute unit in place of three: 160 rows 124 -> 119.
 constexpr int kTileWaves = 4, kTileTokens = 4, kChunk = 4;
 
 // A tile of NT times 16 tokens, `first` the list's place of the first.
 template <typename T, int PRODUCT, int NT, int DEPTH, bool ONCE>
-__device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned width,
-                                          const uint16_t* list, u32x4 (*xs)[kTileTokens * kChunk * 64],
-                                          int r0, int first, int n, int block, bool live, const ExpertShape& shape,
-                                          int64_t total, int k, const float* __restrict__ gates,
-                                          void* __restrict__ out) {
+__device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned width, const uint16_t* list,
+                                          u32x4 (*xs)[kTileTokens * kChunk * 64], int r0, int first, int n, int block,
+                                          bool live, const ExpertShape& shape, int64_t total, int k,
+                                          const float* __restrict__ gates, void* __restrict__ out) {
   using O = Operand<T>;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
   u32x4 wb[DEPTH][2], xr[NT];
@@ -695,13 +712,10 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
 }
 
 template <typename T, int PRODUCT, int RANGE, int DEPTH, bool ONCE>
-__global__ __launch_bounds__(64 * kTileWaves, DEPTH == 2 ? 4 : 3) void expert_tiles(const T* __restrict__ in,
-                                                                   const u32x4* __restrict__ weights,
-                                                                   const int* __restrict__ chosen,
-                                                                   const float* __restrict__ gates, ExpertShape shape,
-                                                                   int rows, int64_t total, int E, int k, int clears,
-                                                                   int lists, int tiles,
-                                                                   void* __restrict__ out) {
+__global__ __launch_bounds__(64 * kTileWaves, DEPTH == 2 ? 4 : 3) void expert_tiles(
+    const T* __restrict__ in, const u32x4* __restrict__ weights, const int* __restrict__ chosen,
+    const float* __restrict__ gates, ExpertShape shape, int rows, int64_t total, int E, int k, int clears, int lists,
+    int tiles, void* __restrict__ out) {
   typedef PairList<kTileWaves, RANGE> List;
   __shared__ List list;
   __shared__ u32x4 xs[2][kTileTokens * kChunk * 64];
@@ -727,12 +741,12 @@ __global__ __launch_bounds__(64 * kTileWaves, DEPTH == 2 ? 4 : 3) void expert_ti
     if (e == E) {
       if (PRODUCT == kDown && clears > 0 && place.tile == 0)
         clear_rows(list.list, n, r0, place.list * kTileWaves + wv, clears * kTileWaves, 32 * place.column * kTileWaves,
-                   32 * (place.column + 1) * kTileWaves, shape.D,
-                   total, k, static_cast<float*>(out));
+                   32 * (place.column + 1) * kTileWaves, shape.D, total, k, static_cast<float*>(out));
     } else {
       for (int first = 16 * kTileTokens * place.tile; first < n; first += 16 * kTileTokens * tiles) {
-#define WPTV_TILE(NT) \
-  tile_pass<T, PRODUCT, NT, DEPTH, ONCE>(x, w, KS, width, list.list, xs, r0, first, n, block, live, shape, total, k, gates, out)
+#define WPTV_TILE(NT)                                                                                                 \
+  tile_pass<T, PRODUCT, NT, DEPTH, ONCE>(x, w, KS, width, list.list, xs, r0, first, n, block, live, shape, total, k, \
+                                         gates, out)
         switch ((n - first + 15) / 16) {
           case 1: WPTV_TILE(1); break;
           case 2: WPTV_TILE(2); break;
@@ -879,7 +893,8 @@ int check_shape(const char* what, int64_t rows, int D, int E, int k, int dtype) 
     return fail(WPTV_E_INVALID, "%s: bad shape rows=%lld D=%d E=%d k=%d", what, (long long)rows, D, E, k);
   }
   if (k > E) return fail(WPTV_E_INVALID, "%s: k=%d of %d experts", what, k, E);
-  if (D % 8 != 0 || D > (1 << 20)) return fail(WPTV_E_UNSUPPORTED, "%s: width %d is not a multiple of 8 up to 2^20", what, D);
+  if (D % 8 != 0 || D > (1 << 20))
+    return fail(WPTV_E_UNSUPPORTED, "%s: width %d is not a multiple of 8 up to 2^20", what, D);
   if (E > kMaxExperts || k > kMaxChosen)
     return fail(WPTV_E_UNSUPPORTED, "%s: k=%d of E=%d experts is above %d of %d", what, k, E, kMaxChosen, kMaxExperts);
   if (rows > (1 << 24)) return fail(WPTV_E_UNSUPPORTED, "%s: %lld rows above 2^24", what, (long long)rows);
@@ -906,8 +921,8 @@ size_t route_bytes(int64_t rows, int D, int E) { return (size_t)route_splits(row
     FORM(8)
 
 template <typename T>
-int run_route(const void* x, const float* router, const float* bias, const int64_t* counts, int rows, int per_row, int D,
-              int E, int k, int* chosen, float* gates, void* workspace, hipStream_t stream) {
+int run_route(const void* x, const float* router, const float* bias, const int64_t* counts, int rows, int per_row,
+              int D, int E, int k, int* chosen, float* gates, void* workspace, hipStream_t stream) {
   const T* xt = static_cast<const T*>(x);
   const int splits = route_splits(rows, D, E);
   if (splits == 0) {
@@ -946,7 +961,7 @@ int run_product(const void* in, const void* weights, const int* chosen, const fl
   const u32x4* w = static_cast<const u32x4*>(weights);
   // tiles of one expert's tokens side by side, as many as its mean count in a range of pairs fills
   const int64_t mean = (pairs < 8192 ? pairs : 8192) / E;
-  const int tiles = (int)((mean + 63) / 64), few = (int)((mean + 31) / 32);
+  const int tiles = mean > 1024 ? 16 : (int)((mean + 63) / 64), few = mean > 512 ? 16 : (int)((mean + 31) / 32);
 #define WPTV_COLUMNS(NT, TILES, BY, ONCE)                                                                   \
   expert_columns<T, PRODUCT, NT, 4, BY, ONCE><<<product_grid(blocks, lists, TILES), 256, 0, stream>>>(      \
       from, w, chosen, gates, shape, rows, total, E, k, clears, lists, TILES, out)
@@ -981,7 +996,8 @@ int run_product(const void* in, const void* weights, const int* chosen, const fl
 // The rows of one round of the two products: their operands stay within a buffer,
 // and the terms that a join reads within 512 MiB.
 int round_rows(int64_t rows, int k, const ExpertShape& shape, int dtype, bool join) {
-  const int64_t act = (int64_t)k * shape.Fp, widest = (dtype == WPTV_BF16 ? 2 : 4) * (shape.D > act ? shape.D : act);
+  const int64_t act = (int64_t)k * shape.Fp;
+  const int64_t widest = (dtype == WPTV_BF16 ? 2 : 4) * (shape.D > act ? shape.D : act);
   int64_t fit = kBufferBytes / widest;
   const int64_t terms = (int64_t)k * shape.D * 4, most = terms < (1 << 20) ? (1 << 29) / terms : 512;
   if (join && most < fit) fit = most;
@@ -1017,12 +1033,13 @@ int run_experts(const void* x, const void* gate_up, const void* down, const int*
                                          here, here, E, k, false, act, stream);
     if (status == WPTV_OK && y && few_rows(rows, k, shape)) {
       expert_rows<T><<<(shape.D + 15) / 16, 64 * kFewWaves, 0, stream>>>(
-          reinterpret_cast<const T*>(act), static_cast<const u32x4*>(down), chosen, shape, rows, E, k, static_cast<T*>(y));
+          reinterpret_cast<const T*>(act), static_cast<const u32x4*>(down), chosen, shape, rows, E, k,
+          static_cast<T*>(y));
       return launched("experts (rows)");
     }
     if (status == WPTV_OK)
-      status = y ? run_product<T, kDown>(act, down, choice, gates + m * k, shape, here, here, E, k, false, terms, stream)
-                 : run_product<T, kDown>(act, down, choice, gates + m * k, shape, here, rows, E, k, true,
+      status = y ? run_product<T, kDown>(act, down, choice, nullptr, shape, here, here, E, k, false, terms, stream)
+                 : run_product<T, kDown>(act, down, choice, nullptr, shape, here, rows, E, k, true,
                                          parts + m * shape.D, stream);
     if (status != WPTV_OK) return status;
     if (y) {
@@ -1053,8 +1070,8 @@ int check_experts(const char* what, const void* x, const void* gate_up, const vo
   status = wptv_experts_workspace((int)rows, D, F, k, dtype, parts ? 1 : 0, &need);
   if (status != WPTV_OK) return status;
   if (!workspace || workspace_bytes < need)
-    return fail(WPTV_E_INVALID, "%s: the workspace holds %zu bytes; %zu are needed", what, workspace ? workspace_bytes : 0,
-                need);
+    return fail(WPTV_E_INVALID, "%s: the workspace holds %zu bytes; %zu are needed", what,
+                workspace ? workspace_bytes : 0, need);
   return WPTV_OK;
 }
 
@@ -1069,8 +1086,8 @@ int check_route(const char* what, const void* x, const float* router, int B, int
     return fail(WPTV_E_INVALID, "%s: rows must be 16-byte aligned", what);
   const size_t need = route_bytes((int64_t)B * T, D, E);
   if (need && (!workspace || workspace_bytes < need))
-    return fail(WPTV_E_INVALID, "%s: the workspace holds %zu bytes; %zu are needed", what, workspace ? workspace_bytes : 0,
-                need);
+    return fail(WPTV_E_INVALID, "%s: the workspace holds %zu bytes; %zu are needed", what,
+                workspace ? workspace_bytes : 0, need);
   return WPTV_OK;
 }
 
@@ -1125,8 +1142,8 @@ extern "C" int wptv_route_workspace(int rows, int D, int E, size_t* bytes) {
   return WPTV_OK;
 }
 
-extern "C" int wptv_route(const void* x, int dtype, const float* router, const float* bias, const int64_t* counts, int B,
-                          int T, int D, int E, int k, int32_t* chosen, float* gates, void* workspace,
+extern "C" int wptv_route(const void* x, int dtype, const float* router, const float* bias, const int64_t* counts,
+                          int B, int T, int D, int E, int k, int32_t* chosen, float* gates, void* workspace,
                           size_t workspace_bytes, hipStream_t stream) {
   const int status =
       check_route("route", x, router, B, T, D, E, k, dtype, chosen, gates, workspace, workspace_bytes);

@@ -113,8 +113,8 @@ def route(x, router, k, bias=None, counts=None):
 
 def _match(x, weights, what):
     if weights.dtype != x.dtype or weights.device != x.device or weights.width != x.shape[2]:
-        raise ValueError(f"{what}: x must be (B, T, {weights.width}) {weights.dtype} on {weights.device} as the experts; "
-                         f"got {tuple(x.shape)} {x.dtype} on {x.device}")
+        raise ValueError(f"{what}: x must be (B, T, {weights.width}) {weights.dtype} on {weights.device} as the experts "
+                         f"are; got {tuple(x.shape)} {x.dtype} on {x.device}")
 
 
 def _result(x, size, k, parts):
@@ -146,7 +146,7 @@ def feed_forward(x, weights, chosen, gates):
     """The gated sum of each token's experts: y (B, T, D) in x's dtype, the sum
     over j of gates[..., j] down_e (silu(gate_e x) * (up_e x)), e = chosen[..., j]
     (route's; a choice outside 0 .. E - 1 adds nothing).  weights: ExpertWeights.
-    FP32 sums, silu(g) u rounded once to the dtype between the products."""
+    FP32 sums; gates silu(g) u is rounded once to the dtype between the products."""
     return _feed_forward(x, weights, chosen, gates, False)
 
 
