@@ -302,24 +302,9 @@ __global__ __launch_bounds__(THREADS) void log_probs_held(const T* __restrict__ 
     }
   }
   __syncthreads();
-  Part part = {high, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    part.rest += sums[1][i];
-    part.weighted += sums[2][i];
-    part.many += sums[3][i];
-  }
-  part.weighted *= kLn2;
-  const Level level(part, inverse);
-  const int64_t place = m * gridDim.y + blockIdx.y;
-  if (tid == 0) {
-    if (gridDim.y == 1)
-      store_row(part, level, written, given, m, out);
-    else
-      parts[place] = part;
-  }
+  int found = 0;
   if constexpr (TOP) {
-    int found = shared.count;
+    found = shared.count;
     if (found > kCandidates) {
       const uint32_t tau = kth_largest<THREADS, true>(each, top, shared.select);
       int above = 0, equal = 0;
@@ -357,7 +342,26 @@ __global__ __launch_bounds__(THREADS) void log_probs_held(const T* __restrict__ 
       __syncthreads();
       found = shared.count;  // top of them
     }
-    if (tid < min(found, kCandidates)) {
+  }
+  if (64 * w >= (found > 0 ? found : 1)) return;  // the first wavefronts rank and store
+  Part part = {high, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    part.rest += sums[1][i];
+    part.weighted += sums[2][i];
+    part.many += sums[3][i];
+  }
+  part.weighted *= kLn2;
+  const Level level(part, inverse);
+  const int64_t place = m * gridDim.y + blockIdx.y;
+  if (tid == 0) {
+    if (gridDim.y == 1)
+      store_row(part, level, written, given, m, out);
+    else
+      parts[place] = part;
+  }
+  if constexpr (TOP) {
+    if (tid < found) {
       const uint64_t mine = shared.best[tid];
       const int before = larger(shared.best, found, mine);
       if (before < top) {
