@@ -21,8 +21,12 @@ Modules, each citing the reference lines it follows:
                reordering of rows (no counterpart in the reference)
     eviction   the attention weight that cached rows receive, the rows a
                bounded cache keeps and their move (no counterpart)
+    experts    a mixture of experts token by token, and how far FP32 sums may
+               be from it
+    log_probs  log-probabilities, entropies and alternatives of written
+               tokens, and their FP32 bounds (no counterpart)
     decoder    the build's generic MQA decoder (random-init weights, exact
-               and window layers) behind the reference's model protocol
+               and window layers, dense blocks or experts) behind the reference's model protocol
                new_cache / extend / undo
 
 What pins each function (the checks live in tests/test_oracle_*.py and
@@ -45,6 +49,7 @@ tests/test_scheduling.py):
                rows); the scheduler's known answers (test_sampling.py:230-238)
                and a brute force over widths
     beam, eviction  cases done by hand (tests/test_beam_eviction.py)
+    experts, log_probs  cases done by hand (tests/test_experts.py)
 The exact token stream the reference's Writer draws from a seed through its
 lazy generator order (its own tests assert only "same seed, same tokens") is
 pinned by golden streams of the reference's Writer itself
