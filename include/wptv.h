@@ -590,7 +590,7 @@ int wptv_greedy_tree_best(const int32_t* best, const int64_t* node_tokens, const
  *   chosen (padding, fewer than k above -inf) chosen is -1 and the gate 0.  A
  *   NaN or +inf among a row's chosen l makes its gates NaN.
  *   D a multiple of 8, E <= 512, k <= 16; rows contiguous and 16-byte aligned.
- *   workspace  wptv_route_workspace(B T, D, E) bytes
+ *   workspace  wptv_route_workspace(B T, D, E) bytes (never less for more rows)
  * ------------------------------------------------------------------------- */
 int wptv_route_workspace(int rows, int D, int E, size_t* bytes);
 
@@ -610,7 +610,7 @@ int wptv_route(const void* x, int dtype, const float* router, const float* bias,
  *            consumer that sums them (wptv_add_rms_norm_parts, k <= 8)
  *   y        [rows, D] in dtype, their sum in order, rounded once
  *   workspace  wptv_experts_workspace bytes (parts_out: the parts are the
- *            output)
+ *            output; never less for more rows)
  * wptv_mixture: wptv_route, then wptv_experts on its choice (chosen and gates
  *   are outputs); workspace wptv_mixture_workspace bytes. */
 int wptv_experts_packed(int D, int F, int dtype, size_t* gate_up_bytes, size_t* down_bytes);

@@ -90,6 +90,20 @@ def test_routes_of_shapes_without_a_kernel_are_refused(B, T, D, E, k, dtype, sta
                                 None) == status
 
 
+@pytest.mark.parametrize("D, E, k, F", [(448, 37, 4, 2395), (64, 8, 2, 4000), (2048, 64, 8, 704), (9000, 16, 1, 40)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_a_workspace_is_enough_for_fewer_rows(D, E, k, F, dtype):
+    library, size = _lib.lib(), ctypes.c_size_t()
+    last = [0, 0]
+    for rows in [*range(0, 700), *range(700, 40000, 997)]:
+        assert library.wptv_experts_workspace(rows, D, F, k, dtype, 0, ctypes.byref(size)) == 0
+        assert size.value >= last[0]
+        last[0] = size.value
+        assert library.wptv_route_workspace(rows, D, E, ctypes.byref(size)) == 0
+        assert size.value >= last[1]
+        last[1] = size.value
+
+
 def test_null_and_misaligned_pointers_and_small_workspaces_are_refused():
     library = _lib.lib()
     assert library.wptv_route(None, 1, 16, None, None, 1, 1, 64, 4, 2, 16, 16, 16, 0, None) == -1

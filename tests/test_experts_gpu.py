@@ -125,6 +125,31 @@ def test_nan_and_infinite_logits(device):
     assert torch.equal(y[0, keep], whole[0, keep])
 
 
+@pytest.mark.parametrize("B, T, D, E, k", [
+    (160, 1, 256, 128, 8), (9, 1, 2048, 16, 2), (3, 1, 64, 500, 4), (3, 2, 64, 130, 3), (1025, 1, 16, 5, 2),
+    (1024, 1, 8, 5, 2), (2, 300, 512, 64, 4)])
+def test_the_router_s_forms_meet(device, B, T, D, E, k):
+    print(f"route B={B} T={T} D={D} E={E} k={k}", flush=True)
+    x, router, _, _ = layer(B, T, D, E, 8, BF16, seed=D + E)
+    check_route(device, x, router, k, torch.linspace(-1, 1, E))
+
+
+# long features over few rows of outputs: the down product's columns are cut
+@pytest.mark.parametrize("B, T, D, E, k, F, dtype", [
+    (1, 1, 40, 16, 2, 1200, BF16), (1, 1, 40, 16, 2, 1200, FP32),  # fewer pairs than experts
+    (4, 4, 136, 3, 2, 2100, BF16), (1, 1, 280, 2, 2, 1111, FP32),  # up to 16 rows
+    (6, 5, 96, 4, 1, 2500, BF16), (20, 4, 72, 4, 2, 1111, FP32),   # few rows an expert, more of them
+    (3, 40, 256, 64, 2, 1050, BF16), (64, 16, 512, 4, 2, 1041, BF16), (64, 16, 1024, 4, 2, 530, FP32)])
+def test_long_features_are_cut_and_joined(device, B, T, D, E, k, F, dtype):
+    print(f"mixture B={B} T={T} D={D} E={E} k={k} F={F} {dtype}", flush=True)
+    x, router, gate_up, down = layer(B, T, D, E, F, dtype, seed=D + F)
+    counts = torch.arange(B) % (T + 1)
+    counts[0] = T
+    weights, on, (y, _, _) = check_mixture(device, x, router, gate_up, down, k, None, counts)
+    again, _, _ = experts.mixture(on[0], on[1], weights, k, None, on[3])
+    assert torch.equal(again, y)
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("B, T, D, E, k, F", [
     (1, 1, 8, 1, 1, 1), (1, 1, 64, 8, 2, 32), (1, 1, 40, 8, 8, 33), (3, 1, 256, 16, 2, 100),   # fewer pairs than experts

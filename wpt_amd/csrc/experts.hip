@@ -187,38 +187,44 @@ __device__ __forceinline__ void load_four(const T* p, float* to) {
   }
 }
 
-// A narrow router in one launch: a workgroup a token, its wavefronts share out the
-// experts, the lanes the width.
+// A small router in one launch: a workgroup a token, `lanes` of its threads (a power
+// of two up to 64, as many as kTokenThreads gives each expert) an expert.  Few lanes an
+// expert keep the sums between them short: by whole wavefronts, one CU's LDS moves
+// every expert's six 64-bit exchanges (in a graph, us: 16 tokens, 72 experts of 104
+// 14.9 -> 5.8; 160 tokens, 64 of 256 8.2 -> 6.2; 512 of 32 30.7 -> 8.3; 256 threads and
+// 1024 4.8, 5.3 at 8 of 256, 512 4.9).
+constexpr int kTokenThreads = 512;
+
 template <typename T, int SLOTS>
-__global__ __launch_bounds__(256) void route_token(const T* __restrict__ x, const float* __restrict__ router,
-                                                   const float* __restrict__ bias, const int64_t* __restrict__ counts,
-                                                   int per_row, int D, int E, int k, int* __restrict__ chosen,
-                                                   float* __restrict__ gates) {
+__global__ __launch_bounds__(kTokenThreads) void route_token(const T* __restrict__ x,
+                                                             const float* __restrict__ router,
+                                                             const float* __restrict__ bias,
+                                                             const int64_t* __restrict__ counts, int per_row, int D,
+                                                             int E, int lanes, int k, int* __restrict__ chosen,
+                                                             float* __restrict__ gates) {
   __shared__ double logit[64 * SLOTS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t m = blockIdx.x;
   const T* row = x + m * D;
-  for (int e = tid >> 6; e < E; e += 4) {
-    double sum = 0.;
-    const float* w = router + (int64_t)e * D;
-    for (int first = 4 * lane; first - 4 * lane < D; first += kAhead * 256) {
-      float a[kAhead][4], b[kAhead][4];
+  const int e = tid / lanes, piece = tid % lanes;
+  const float* w = router + (int64_t)min(e, E - 1) * D;
+  double sum = 0.;
+  for (int first = 4 * piece; first - 4 * piece < D; first += kAhead * 4 * lanes) {
+    float a[kAhead][4], b[kAhead][4];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {  // all asked for at once; past the width nothing is added
-        const int d = first + 256 * u < D ? first + 256 * u : 0;
-        load_four<float>(w + d, a[u]);
-        load_four<T>(row + d, b[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (first + 256 * u < D)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum = fma((double)a[u][i], (double)b[u][i], sum);
+    for (int u = 0; u < kAhead; ++u) {  // all asked for at once; past the width nothing is added
+      const int d = first + 4 * lanes * u < D ? first + 4 * lanes * u : 0;
+      load_four<float>(w + d, a[u]);
+      load_four<T>(row + d, b[u]);
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) logit[e] = sum;
+    for (int u = 0; u < kAhead; ++u)
+      if (first + 4 * lanes * u < D)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum = fma((double)a[u][i], (double)b[u][i], sum);
   }
+  for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (piece == 0 && e < E) logit[e] = sum;
   __syncthreads();
   if (tid >= 64) return;
   const bool read = !counts || m % per_row < counts[m / per_row];
@@ -313,14 +319,21 @@ __global__ __launch_bounds__(256) void route_choose(const double* __restrict__ s
   choose_experts<SLOTS>(own, key, k, chosen + (int64_t)m * k, gates + (int64_t)m * k);
 }
 
-// The router's form: one launch where a token's workgroup reads little, else the
-// parts the width is cut into (the tiles of 16 by 16 cover the compute units twice).
+// The most parts the width is cut into: a wavefront's steps at once each.
+int64_t route_parts(int D) { return D > 32 * 256 ? 32 : (D + 255) / 256; }
+
+// The router's form: 0, one launch, where a token's workgroup and all of them together
+// read little, else the parts the width is cut into (the tiles of 16 by 16 cover the
+// compute units twice).  One launch and two, us: 160 tokens, 128 experts of 256 7.6, 9.4,
+// 16 of 2048 6.4, 8.0; 256 of 256 12.7, 11.1; 1 token, 500 of 64 9.4, 7.9; 512 tokens, 64
+// of 256 6.9, 7.9, 128 of 256 10.6, 9.6; 2000 tokens, 8 of 256 8.6, 7.7, 8 of 2048 13.5,
+// 10.9.
 int route_splits(int64_t rows, int D, int E) {
-  if ((int64_t)E * D <= 16384) return 0;
+  const int64_t size = (int64_t)E * D;
+  if (rows <= 1024 && size <= (E <= 128 ? 32768 : 16384) && rows * size <= (1 << 23)) return 0;
   const int64_t tiles = (rows + 15) / 16 * ((E + 15) / 16);
-  const int64_t want = 512 / tiles, most = (D + 255) / 256;  // a wavefront's steps at once
-  const int64_t splits = want < 1 ? 1 : want < most ? want : most;
-  return (int)(splits < 32 ? splits : 32);
+  const int64_t want = 512 / tiles, most = route_parts(D);
+  return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
 // ---- the experts' products ---------------------------------------------------
@@ -424,6 +437,19 @@ inline unsigned product_grid(int columns, int lists, int tiles) {
   return (unsigned)(((int64_t)columns * lists + 7) / 8 * 8 * tiles);
 }
 
+// The k-steps of one of the `cuts` that the down product's columns are cut into
+// (product_cuts), whose sums the join adds in order; the gate/up product's are whole.
+struct Cut {
+  int first, steps;
+};
+
+template <int PRODUCT>
+__device__ __forceinline__ Cut product_cut(int KS, int cut, int cuts) {
+  if constexpr (PRODUCT == kGateUp) return Cut{0, KS};
+  const int most = (KS + cuts - 1) / cuts;
+  return Cut{cut * most, min(most, KS - cut * most)};
+}
+
 // The parts' rows that no expert of the range writes, cleared by `waves` (at least
 // one) wavefronts of their own, one after the other a row each.
 __device__ __forceinline__ void clear_rows(const uint16_t* pairs, int n, int r0, int wave, int waves, int first,
@@ -478,7 +504,7 @@ __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict
                                                              const int* __restrict__ chosen,
                                                              const float* __restrict__ gates, ExpertShape shape,
                                                              int rows, int64_t total, int E, int k, int clears,
-                                                             int lists, int tiles, void* __restrict__ out) {
+                                                             int lists, int tiles, int cuts, void* __restrict__ out) {
   using O = Operand<T>;
   // a list of its own a wavefront, for fewer than kMaxExperts pairs; 16 tokens have up to 256 pairs
   constexpr int kDepth = 3, kRange = BY_PAIR ? WAVES * kMaxExperts : NT == 1 ? 1024 : 4096;
@@ -488,17 +514,22 @@ __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pairs = rows * k;
-  const Place place = product_place(PRODUCT == kGateUp ? shape.FB : shape.DB, tiles);
+  const Place place = product_place((PRODUCT == kGateUp ? shape.FB : shape.DB) * cuts, tiles);
   if (place.list >= lists) return;
   int e = BY_PAIR ? chosen[place.list] : place.list < clears ? E : place.list - clears;
   e = __builtin_amdgcn_readfirstlane(e);
   if ((unsigned)e >= (unsigned)E) e = E;  // no expert
   const int KS = PRODUCT == kGateUp ? shape.KSx : shape.KSf;
   const unsigned width = (PRODUCT == kGateUp ? shape.D : shape.Fp) * sizeof(T);
-  const int block = place.column, blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
-  const int steps = (KS - wv + WAVES - 1) / WAVES;
-  const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + block) * 2 * KS * 64, 2u * KS * 1024);
-  const Buffer x = buffer(in, (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width));
+  const int block = place.column / cuts, blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
+  const Cut cut = product_cut<PRODUCT>(KS, place.column % cuts, cuts);
+  const unsigned limit = width - 64 * cut.first;
+  const int steps = (cut.steps - wv + WAVES - 1) / WAVES;
+  const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + block) * 2 * KS * 64 + cut.first * 64,
+                          (2u * KS - cut.first) * 1024);
+  const Buffer x = buffer(reinterpret_cast<const char*>(in) + 64 * cut.first,
+                          (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width - 64 * cut.first));
+  if constexpr (PRODUCT == kDown) out = static_cast<float*>(out) + (place.column % cuts) * k * total * shape.D;
   u32x4 wb[kDepth][2], xb[kDepth][NT];
   auto load_weights = [&](int d, int s) {
     const unsigned ks = wv + WAVES * s;
@@ -558,7 +589,7 @@ __global__ __launch_bounds__(64 * WAVES) void expert_columns(const T* __restrict
         const unsigned ks = wv + WAVES * s;
 #pragma unroll
         for (int t = 0; t < NT; ++t)  // columns past the width are zero, as the weights' padding
-          xb[d][t] = load16(x, 64 * ks + 16 * g < width ? row[t] : kOutside, 64 * ks);
+          xb[d][t] = load16(x, 64 * ks + 16 * g < limit ? row[t] : kOutside, 64 * ks);
       };
       auto multiply = [&](int d) {
 #pragma unroll
@@ -626,7 +657,8 @@ constexpr int kTileWaves = 4, kTileTokens = 4, kChunk = 4;
 
 // A tile of NT times 16 tokens, `first` the list's place of the first.
 template <typename T, int PRODUCT, int NT, int DEPTH, bool ONCE>
-__device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned width, const uint16_t* list,
+__device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, int steps, unsigned width, unsigned limit,
+                                          const uint16_t* list,
                                           u32x4 (*xs)[kTileTokens * kChunk * 64], int r0, int first, int n, int block,
                                           bool live, const ExpertShape& shape, int64_t total, int k,
                                           const float* __restrict__ gates, void* __restrict__ out) {
@@ -635,7 +667,7 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
   u32x4 wb[DEPTH][2], xr[NT];
   const unsigned at = live ? 16 * lane : kOutside;  // wavefronts past the last row blocks load nothing
   auto load = [&](int d, int s) {
-    const unsigned ks = min(s, KS - 1);
+    const unsigned ks = min(s, steps - 1);
     wb[d][0] = load16_weights<ONCE>(w, at, 1024 * ks);
     wb[d][1] = load16_weights<ONCE>(w, at, 1024 * (KS + ks));
   };
@@ -654,7 +686,7 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
     const unsigned column = 64 * kChunk * c;
 #pragma unroll
     for (int i = 0; i < NT; ++i)  // columns past the width are zero, as the weights' padding
-      xr[i] = load16(in, column + 16 * piece < width ? row[i] : kOutside, column);
+      xr[i] = load16(in, column + 16 * piece < limit ? row[i] : kOutside, column);
   };
   u32x4* to = xs[0] + (piece >> 2) * 64 + (piece & 3) * 16 + token;
   auto stage = [&](int buffer) {
@@ -684,7 +716,7 @@ __device__ __forceinline__ void tile_pass(Buffer in, Buffer w, int KS, unsigned 
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  const int whole = KS / kChunk, left = KS % kChunk;
+  const int whole = steps / kChunk, left = steps % kChunk;
   fetch(0);
   stage(0);
   barrier();
@@ -715,24 +747,29 @@ template <typename T, int PRODUCT, int RANGE, int DEPTH, bool ONCE>
 __global__ __launch_bounds__(64 * kTileWaves, DEPTH == 2 ? 4 : 3) void expert_tiles(
     const T* __restrict__ in, const u32x4* __restrict__ weights, const int* __restrict__ chosen,
     const float* __restrict__ gates, ExpertShape shape, int rows, int64_t total, int E, int k, int clears, int lists,
-    int tiles, void* __restrict__ out) {
+    int tiles, int cuts, void* __restrict__ out) {
   typedef PairList<kTileWaves, RANGE> List;
   __shared__ List list;
   __shared__ u32x4 xs[2][kTileTokens * kChunk * 64];
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pairs = rows * k;
   const Place place =
-      product_place(((PRODUCT == kGateUp ? shape.FB : shape.DB) + kTileWaves - 1) / kTileWaves, tiles);
+      product_place(((PRODUCT == kGateUp ? shape.FB : shape.DB) + kTileWaves - 1) / kTileWaves * cuts, tiles);
   if (place.list >= lists) return;
   const int e = place.list < clears ? E : place.list - clears;
   const int KS = PRODUCT == kGateUp ? shape.KSx : shape.KSf;
   const unsigned width = (PRODUCT == kGateUp ? shape.D : shape.Fp) * sizeof(T);
   const int blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
-  const int block = place.column * kTileWaves + wv;
+  const int column = place.column / cuts, block = column * kTileWaves + wv;
   const bool live = block < blocks;
-  const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + min(block, blocks - 1)) * 2 * KS * 64,
-                          2u * KS * 1024);
-  const Buffer x = buffer(in, (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width));
+  const Cut cut = product_cut<PRODUCT>(KS, place.column % cuts, cuts);
+  const unsigned limit = width - 64 * cut.first;
+  const Buffer w = buffer(weights + ((int64_t)min(e, E - 1) * blocks + min(block, blocks - 1)) * 2 * KS * 64 +
+                              cut.first * 64,
+                          (2u * KS - cut.first) * 1024);
+  const Buffer x = buffer(reinterpret_cast<const char*>(in) + 64 * cut.first,
+                          (unsigned)((PRODUCT == kGateUp ? rows : pairs) * width - 64 * cut.first));
+  if constexpr (PRODUCT == kDown) out = static_cast<float*>(out) + (place.column % cuts) * k * total * shape.D;
 
   for (int r0 = 0; r0 < pairs; r0 += RANGE) {
     typename List::Choices choices;
@@ -740,13 +777,13 @@ __global__ __launch_bounds__(64 * kTileWaves, DEPTH == 2 ? 4 : 3) void expert_ti
     const int n = list.fill(choices, r0, pairs, e, E);
     if (e == E) {
       if (PRODUCT == kDown && clears > 0 && place.tile == 0)
-        clear_rows(list.list, n, r0, place.list * kTileWaves + wv, clears * kTileWaves, 32 * place.column * kTileWaves,
-                   32 * (place.column + 1) * kTileWaves, shape.D, total, k, static_cast<float*>(out));
+        clear_rows(list.list, n, r0, place.list * kTileWaves + wv, clears * kTileWaves, 32 * column * kTileWaves,
+                   32 * (column + 1) * kTileWaves, shape.D, total, k, static_cast<float*>(out));
     } else {
       for (int first = 16 * kTileTokens * place.tile; first < n; first += 16 * kTileTokens * tiles) {
 #define WPTV_TILE(NT)                                                                                                 \
-  tile_pass<T, PRODUCT, NT, DEPTH, ONCE>(x, w, KS, width, list.list, xs, r0, first, n, block, live, shape, total, k, \
-                                         gates, out)
+  tile_pass<T, PRODUCT, NT, DEPTH, ONCE>(x, w, KS, cut.steps, width, limit, list.list, xs, r0, first, n, block, live, \
+                                         shape, total, k, gates, out)
         switch ((n - first + 15) / 16) {
           case 1: WPTV_TILE(1); break;
           case 2: WPTV_TILE(2); break;
@@ -853,18 +890,23 @@ __global__ __launch_bounds__(64 * kFewWaves) void expert_rows(const T* __restric
 
 // y[m] = the sum of a token's parts in the order of its choices, rounded once; the
 // parts of no expert hold nothing and are passed over.
-template <typename T>
+template <typename T, bool CUT>
 __global__ __launch_bounds__(256) void join_experts(const float* __restrict__ parts, const int* __restrict__ chosen,
-                                                    int64_t rows, int D, int E, int k, T* __restrict__ y) {
+                                                    int64_t rows, int D, int E, int k, int cuts,
+                                                    T* __restrict__ y) {
   const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= rows * D) return;
   const int* choice = chosen + at / D * k;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int first = 0; first < k; first += 8) {
+  const int all = CUT ? k * cuts : k;
+  for (int first = 0; first < all; first += 8) {
     bool some[8];
     f32x4 part[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) some[i] = first + i < k && (unsigned)choice[min(first + i, k - 1)] < (unsigned)E;
+    for (int i = 0; i < 8; ++i) {
+      const int part = min(first + i, all - 1);
+      some[i] = first + i < all && (unsigned)choice[CUT ? part % k : part] < (unsigned)E;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)  // all asked for at once
       part[i] = *reinterpret_cast<const f32x4*>(parts + (some[i] ? (first + i) * rows * D : 0) + at);
@@ -907,7 +949,13 @@ int check_features(const char* what, int F) {
   return WPTV_OK;
 }
 
-size_t route_bytes(int64_t rows, int D, int E) { return (size_t)route_splits(rows, D, E) * rows * E * sizeof(double); }
+// The bytes of the parts' logits, no less for more rows: with more than one part they
+// have 512 tiles at most.
+size_t route_bytes(int64_t rows, int D, int E) {
+  if (rows == 0 || route_splits(rows, D, E) == 0) return 0;
+  const int64_t most = route_parts(D) * rows, tiles = 512 / ((E + 15) / 16) * 16, some = most < tiles ? most : tiles;
+  return (size_t)(rows > some ? rows : some) * E * sizeof(double);
+}
 
 // The experts a lane of a token's wavefront holds.
 #define WPTV_SLOTS(FORM) \
@@ -926,8 +974,11 @@ int run_route(const void* x, const float* router, const float* bias, const int64
   const T* xt = static_cast<const T*>(x);
   const int splits = route_splits(rows, D, E);
   if (splits == 0) {
-#define WPTV_TOKEN(SLOTS) \
-  route_token<T, SLOTS><<<rows, 256, 0, stream>>>(xt, router, bias, counts, per_row, D, E, k, chosen, gates)
+    int lanes = 64;
+    while (lanes * E > kTokenThreads) lanes /= 2;
+#define WPTV_TOKEN(SLOTS)                                                                                          \
+  route_token<T, SLOTS><<<rows, kTokenThreads, 0, stream>>>(xt, router, bias, counts, per_row, D, E, lanes, k, \
+                                                            chosen, gates)
     WPTV_SLOTS(WPTV_TOKEN);
 #undef WPTV_TOKEN
     return launched("route");
@@ -949,9 +1000,40 @@ int run_route(const void* x, const float* router, const float* bias, const int64
   return launched("route (choice)");
 }
 
+// The down product's columns are cut where the row blocks and the experts leave compute
+// units idle: into as many cuts as make 512 workgroups, of at least 16 k-steps each.
+// Whole layers in a graph, us, whole and cut: 496 tokens of 448, 4 of 37 experts of 2395
+// 132, 100; 160 of 1024, 2 of 16 of 4096 108, 89; 512 of 1024, 2 of 8 of 2816 86, 69; one
+// of 2048, 2 of 8 of 5632 38.8, 34.6; FP32, one of 280, 2 of 2 of 4715 39.0, 23.9.  More
+// do not give more: towards 768 tiles' workgroups 100, 92, 72 of the first three; towards
+// 1024 160 tokens of 512, 4 of 16 of 1408 38.8 -> 41.4, cuts of 8 k-steps among those
+// 238 of 1704, 6 of 16 of 509 56.8 -> 63.7.
+constexpr int kCutGroups = 512, kCutSteps = 16, kMostCuts = 16;
+constexpr int64_t kCutBytes = 32 << 20;  // the most that the terms of all cuts may take
+
+int product_cuts(int KS, int64_t want) {
+  int64_t cuts = want < kMostCuts ? want : kMostCuts;
+  if (cuts > KS / kCutSteps) cuts = KS / kCutSteps;
+  if (cuts <= 1) return 1;
+  const int steps = (int)((KS + cuts - 1) / cuts);
+  return (KS + steps - 1) / steps;  // none is empty
+}
+
+int64_t term_bytes(int64_t rows, int k, const ExpertShape& shape) { return rows * k * shape.D * 4; }
+
+// The bytes of a round's terms, no less for more rows: of as many cuts as k experts'
+// row blocks, the fewest there are, could be cut into.
+size_t terms_bytes(int round, int k, const ExpertShape& shape) {
+  const int64_t one = term_bytes(round, k, shape);
+  const int64_t all = one * product_cuts(shape.KSf, kTileWaves * kCutGroups / ((int64_t)k * shape.DB));
+  const int64_t some = all < kCutBytes ? all : kCutBytes;
+  return (size_t)(one > some ? one : some);
+}
+
 template <typename T, int PRODUCT>
 int run_product(const void* in, const void* weights, const int* chosen, const float* gates, const ExpertShape& shape,
-                int rows, int64_t total, int E, int k, bool clear, void* out, hipStream_t stream) {
+                int rows, int64_t total, int E, int k, bool clear, int* cut, void* out,
+                hipStream_t stream) {
   const int64_t pairs = (int64_t)rows * k;
   const int blocks = PRODUCT == kGateUp ? shape.FB : shape.DB;
   const bool by_pair = pairs < E;
@@ -963,24 +1045,31 @@ int run_product(const void* in, const void* weights, const int* chosen, const fl
   const int64_t mean = (pairs < 8192 ? pairs : 8192) / E;
   const int tiles = mean > 1024 ? 16 : (int)((mean + 63) / 64), few = mean > 512 ? 16 : (int)((mean + 31) / 32);
 #define WPTV_COLUMNS(NT, TILES, BY, ONCE)                                                                   \
-  expert_columns<T, PRODUCT, NT, 4, BY, ONCE><<<product_grid(blocks, lists, TILES), 256, 0, stream>>>(      \
-      from, w, chosen, gates, shape, rows, total, E, k, clears, lists, TILES, out)
+  expert_columns<T, PRODUCT, NT, 4, BY, ONCE><<<product_grid(blocks * cuts, lists, TILES), 256, 0, stream>>>( \
+      from, w, chosen, gates, shape, rows, total, E, k, clears, lists, TILES, cuts, out)
 #define WPTV_TILES(RANGE, DEPTH, ONCE)                                                                      \
   expert_tiles<T, PRODUCT, RANGE, DEPTH, ONCE>                                                              \
-      <<<product_grid((blocks + kTileWaves - 1) / kTileWaves, lists, tiles), 64 * kTileWaves, 0, stream>>>( \
-          from, w, chosen, gates, shape, rows, total, E, k, clears, lists, tiles, out)
+      <<<product_grid((blocks + kTileWaves - 1) / kTileWaves * cuts, lists, tiles), 64 * kTileWaves, 0, stream>>>( \
+          from, w, chosen, gates, shape, rows, total, E, k, clears, lists, tiles, cuts, out)
   // The k-steps of a block pair over a workgroup, or tiles of 64 tokens a wavefront.  Whole layers, us, columns and
   // tiles: bf16, E blocks 352 (8 experts of 704, 300 tokens of 1000) 40.8, 39.1; 528 (6 of 1408, 100 tokens of 4096)
   // 99, 83; 1408 (16 of 1408, 256 tokens) 130, 115; FP32, whose instructions take four times as long, 512 (16 of 512,
   // 200 tokens of 1024) 61, 103.
   const int64_t least = sizeof(T) == 2 ? 512 : 1024;
+  const bool columns = by_pair || rows <= 16 || (int64_t)E * blocks * tiles < least;
+  const int spread = by_pair || rows <= 16 ? 1 : columns ? few : tiles;
+  const int64_t groups =
+      (int64_t)(by_pair ? pairs : E) * (columns ? blocks : (blocks + kTileWaves - 1) / kTileWaves) * spread;
+  const int64_t fit = cut ? kCutBytes / term_bytes(rows, k, shape) : 1, want = kCutGroups / groups;
+  const int cuts = PRODUCT == kGateUp ? 1 : product_cuts(shape.KSf, want < fit ? want : fit);
+  if (cut) *cut = cuts;
   if (by_pair)
     WPTV_COLUMNS(1, 1, true, true);
   else if (rows <= 16)
     WPTV_COLUMNS(1, 1, false, true);
-  else if ((int64_t)E * blocks * tiles < least && few == 1)
+  else if (columns && few == 1)
     WPTV_COLUMNS(2, 1, false, true);
-  else if ((int64_t)E * blocks * tiles < least)
+  else if (columns)
     WPTV_COLUMNS(2, few, false, false);
   else if (tiles > 1 || pairs > 4096)
     WPTV_TILES(8192, 4, false);
@@ -1030,22 +1119,30 @@ int run_experts(const void* x, const void* gate_up, const void* down, const int*
     const int here = rows - m < round ? (int)(rows - m) : round;
     const int* choice = chosen + m * k;
     int status = run_product<T, kGateUp>(static_cast<const T*>(x) + m * shape.D, gate_up, choice, gates + m * k, shape,
-                                         here, here, E, k, false, act, stream);
+                                         here, here, E, k, false, nullptr, act, stream);
     if (status == WPTV_OK && y && few_rows(rows, k, shape)) {
       expert_rows<T><<<(shape.D + 15) / 16, 64 * kFewWaves, 0, stream>>>(
           reinterpret_cast<const T*>(act), static_cast<const u32x4*>(down), chosen, shape, rows, E, k,
           static_cast<T*>(y));
       return launched("experts (rows)");
     }
+    int cuts = 1;
     if (status == WPTV_OK)
-      status = y ? run_product<T, kDown>(act, down, choice, nullptr, shape, here, here, E, k, false, terms, stream)
-                 : run_product<T, kDown>(act, down, choice, nullptr, shape, here, rows, E, k, true,
+      status = y ? run_product<T, kDown>(act, down, choice, nullptr, shape, here, here, E, k, false, &cuts,
+                                         terms, stream)
+                 : run_product<T, kDown>(act, down, choice, nullptr, shape, here, rows, E, k, true, nullptr,
                                          parts + m * shape.D, stream);
     if (status != WPTV_OK) return status;
     if (y) {
       const int64_t threads = (int64_t)here * shape.D / 4;
-      join_experts<T><<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(terms, choice, here, shape.D, E, k,
-                                                                            static_cast<T*>(y) + m * shape.D);
+#define WPTV_JOIN(CUT)                                                                                         \
+  join_experts<T, CUT><<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(terms, choice, here, shape.D, E, \
+                                                                              k, cuts, static_cast<T*>(y) + m * shape.D)
+      if (cuts > 1)
+        WPTV_JOIN(true);
+      else
+        WPTV_JOIN(false);
+#undef WPTV_JOIN
       status = launched("experts (join)");
       if (status != WPTV_OK) return status;
     }
@@ -1160,7 +1257,7 @@ extern "C" int wptv_experts_workspace(int rows, int D, int F, int k, int dtype, 
   if (!bytes) return fail(WPTV_E_INVALID, "experts_workspace: a required pointer is NULL");
   const ExpertShape s = expert_shape(D, F, dtype);
   const int round = round_rows(rows, k, s, dtype, !parts_out);
-  *bytes = act_bytes(round, k, s, dtype) + (parts_out ? 0 : (size_t)k * round * D * 4);
+  *bytes = act_bytes(round, k, s, dtype) + (parts_out || rows == 0 ? 0 : terms_bytes(round, k, s));
   return WPTV_OK;
 }
 
