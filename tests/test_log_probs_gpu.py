@@ -56,6 +56,17 @@ def test_the_values_are_those_of_64_bits(device, B, T, V, top, dtype):
     check(device, scores, tokens, top, temperature=0.37)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, V, top", [(300, 16385, 40), (300, 20480, 6), (300, 20481, 0), (300, 24583, 3), (3, 8200, 9),
+                                          (300, 36864, 5), (300, 69633, 4)])
+def test_rows_that_fill_a_workgroup_in_part(device, rows, V, top, dtype):
+    print(f"log_probs rows={rows} V={V} top={top} {dtype}", flush=True)
+    scores, tokens = inputs(rows, 1, V, dtype, seed=V)
+    scores[1] = scores[1].round()  # many equal scores
+    scores[2] = 1.0
+    check(device, scores, tokens, top)
+
+
 @pytest.mark.parametrize("V", [7, 100, 5000, 30000, 40000, 140000, 600000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_equal_scores_fall_to_the_lowest_tokens(device, V, dtype):
