@@ -58,7 +58,8 @@ def test_the_values_are_those_of_64_bits(device, B, T, V, top, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows, V, top", [(300, 16385, 40), (300, 20480, 6), (300, 20481, 0), (300, 24583, 3), (3, 8200, 9),
-                                          (300, 36864, 5), (300, 69633, 4)])
+                                          (300, 36864, 5), (300, 69633, 4),
+                                          (300, 69633, 0), (260, 131073, 0)])
 def test_rows_that_fill_a_workgroup_in_part(device, rows, V, top, dtype):
     print(f"log_probs rows={rows} V={V} top={top} {dtype}", flush=True)
     scores, tokens = inputs(rows, 1, V, dtype, seed=V)

@@ -548,7 +548,7 @@ struct Form {
   int threads, chunks, parts, stretch;
 };
 
-Form row_form(int64_t rows, int V, int dtype) {
+Form row_form(int64_t rows, int V, int top, int dtype) {
   const int per = dtype == WPTV_BF16 ? 8 : 4;
   const int64_t units = compute_units();
   if (V < per) return Form{0, 0, 0, 0};
@@ -562,6 +562,12 @@ Form row_form(int64_t rows, int V, int dtype) {
   int parts = (V + few - 1) / few;
   if (parts <= kMaxParts && rows * parts <= units) return Form{1024, 4, parts, ((V + parts - 1) / parts + 7) / 8 * 8};
   if (V <= 1024 * 8 * per) return Form{1024, 8, 1, V};
+  // without alternatives in parts that three or four workgroups a compute unit take beside each other; with them each
+  // part's choice costs what that gives.  bf16, us, parts and one or two of the largest workgroup: 1024 rows of 128000
+  // 59, 81, of 152000 70, 103, 160 rows of 128000 19.2, 21.1; with 20 alternatives 102, 107, 160 rows 30.1, 27.6; 1024
+  // rows of 65536, in eight chunks, 34.8 both
+  parts = (V + 512 * 8 * per - 1) / (512 * 8 * per);
+  if (top == 0 && parts <= kMaxParts) return Form{512, 8, parts, ((V + parts - 1) / parts + 7) / 8 * 8};
   parts = (V + many - 1) / many;
   if (parts > kMaxParts) return Form{0, 0, 0, 0};
   return Form{1024, 16, parts, parts == 1 ? V : ((V + parts - 1) / parts + 7) / 8 * 8};
@@ -617,8 +623,8 @@ extern "C" int wptv_log_probs_workspace(int B, int T, int V, int top, size_t* by
   if (top > kMaxTop) return fail(WPTV_E_UNSUPPORTED, "log_probs: %d alternatives above %d", top, kMaxTop);
   if (V > (1 << 24) || (int64_t)B * T > INT32_MAX)
     return fail(WPTV_E_UNSUPPORTED, "log_probs: B=%d T=%d V=%d is too large", B, T, V);
-  const size_t bf16 = part_bytes((int64_t)B * T, row_form((int64_t)B * T, V, WPTV_BF16), top);
-  const size_t fp32 = part_bytes((int64_t)B * T, row_form((int64_t)B * T, V, WPTV_F32), top);
+  const size_t bf16 = part_bytes((int64_t)B * T, row_form((int64_t)B * T, V, top, WPTV_BF16), top);
+  const size_t fp32 = part_bytes((int64_t)B * T, row_form((int64_t)B * T, V, top, WPTV_F32), top);
   *bytes = bf16 > fp32 ? bf16 : fp32;
   return WPTV_OK;
 }
@@ -642,7 +648,7 @@ extern "C" int wptv_log_probs(const void* scores, int64_t scores_stride_b, int64
                 workspace ? workspace_bytes : 0, need);
   const float inverse = 1.f / temperature;
   const Outputs out{logprobs, entropy, ids, best};
-  const Form form = row_form((int64_t)B * T, V, scores_dtype);
+  const Form form = row_form((int64_t)B * T, V, top, scores_dtype);
   return scores_dtype == WPTV_BF16
              ? run_log_probs(static_cast<const unsigned short*>(scores), scores_stride_b, scores_stride_t, tokens,
                              inverse, B * T, T, V, top, form, out, workspace, stream)
