@@ -344,3 +344,19 @@ def test_a_captured_layer_replays_on_new_inputs_and_beside_another_stream(device
     torch.cuda.synchronize()
     for a, b in zip(first, second):
         assert torch.equal(a[0], eager[0][0]) and torch.equal(b[0], eager[1][0])
+
+
+def test_no_gradient_is_lost_in_silence(device):
+    x, router, gate_up, down = (t.to(device) for t in layer(1, 3, 64, 8, 32, FP32))
+    weights = experts.ExpertWeights(gate_up, down)
+    with torch.no_grad():
+        chosen, gates = experts.route(x, router, 2)
+    x.requires_grad_()
+    trained = experts.ExpertWeights(gate_up.requires_grad_(), down)
+    for out in (experts.mixture_parts(x, router, weights, 2)[0], experts.feed_forward_parts(x, weights, chosen, gates),
+                experts.mixture(x.detach(), router, trained, 2)[0],
+                experts.feed_forward(x.detach(), trained, chosen, gates)):
+        with pytest.raises(NotImplementedError):
+            out.sum().backward()
+    with torch.no_grad():
+        assert not experts.mixture(x, router, trained, 2)[0].requires_grad

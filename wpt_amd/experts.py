@@ -77,6 +77,8 @@ class ExpertWeights:
         if device.type != "cuda" or down.device != device:
             raise KernelUnavailable(f"the HIP experts run on one GPU; the weights are on {device} and {down.device}")
         self.experts, self.width, self.features, self.dtype, self.device = E, D, F, gate_up.dtype, device
+        # stands for matrices that ask for gradients, which no backward pass of these forms gives
+        self.trained = torch.empty(0, requires_grad=True) if gate_up.requires_grad or down.requires_grad else None
         gate_up, down = gate_up.detach().contiguous(), down.detach().contiguous()
         sizes = ctypes.c_size_t(0), ctypes.c_size_t(0)
         check(_lib.lib().wptv_experts_packed(D, F, dtype, ctypes.byref(sizes[0]), ctypes.byref(sizes[1])),
@@ -139,7 +141,7 @@ def _feed_forward(x, weights, chosen, gates, parts):
         check(_lib.lib().wptv_experts(ptr(x_), dtype, ptr(weights.gate_up), ptr(weights.down), ptr(chosen.contiguous()),
                                       ptr(gates.contiguous()), B * T, D, weights.experts, k, weights.features, ptr(out),
                                       ptr(y), ptr(workspace), size, _lib.stream(x.device)), "feed_forward")
-    return out if parts else _forward_only(y, x, gates)
+    return _forward_only(out if parts else y, x, gates, weights.trained)
 
 
 def feed_forward(x, weights, chosen, gates):
@@ -172,7 +174,7 @@ def _mixture(x, router, weights, k, bias, counts, parts):
         check(_lib.lib().wptv_mixture(ptr(x_), dtype, ptr(router_), ptr(bias), ptr(counts), B, T, D, E, k,
                                       weights.features, ptr(weights.gate_up), ptr(weights.down), ptr(chosen), ptr(gates),
                                       ptr(out), ptr(y), ptr(workspace), size, _lib.stream(device)), "mixture")
-    return (out, chosen, gates) if parts else (_forward_only(y, x, router), chosen, _forward_only(gates, x, router))
+    return _forward_only(out if parts else y, x, router, weights.trained), chosen, _forward_only(gates, x, router)
 
 
 def mixture(x, router, weights, k, bias=None, counts=None):
