@@ -135,12 +135,13 @@ def _feed_forward(x, weights, chosen, gates, parts):
     for name, t, kind in (("chosen", chosen, torch.int32), ("gates", gates, torch.float32)):
         if t.shape != (B, T, k) or t.dtype != kind or t.device != x.device or k == 0:
             raise ValueError(f"{name} must be {kind} (B={B}, T={T}, k) on {x.device}; got {t.dtype} {tuple(t.shape)}")
+    chosen_, gates_ = chosen.contiguous(), gates.contiguous()  # copies of views, held over the call
     with _lib.on(x.device):
         _, size = _lib.plan("wptv_experts_workspace", "feed_forward", B * T, D, weights.features, k, dtype, int(parts))
         out, y, workspace = _result(x_, size, k, parts)
-        check(_lib.lib().wptv_experts(ptr(x_), dtype, ptr(weights.gate_up), ptr(weights.down), ptr(chosen.contiguous()),
-                                      ptr(gates.contiguous()), B * T, D, weights.experts, k, weights.features, ptr(out),
-                                      ptr(y), ptr(workspace), size, _lib.stream(x.device)), "feed_forward")
+        check(_lib.lib().wptv_experts(ptr(x_), dtype, ptr(weights.gate_up), ptr(weights.down), ptr(chosen_),
+                                      ptr(gates_), B * T, D, weights.experts, k, weights.features, ptr(out), ptr(y),
+                                      ptr(workspace), size, _lib.stream(x.device)), "feed_forward")
     return _forward_only(out if parts else y, x, gates, weights.trained)
 
 
