@@ -202,9 +202,9 @@ def choose_rows(q, k, positions, lse, scale, top_k, window):
     _, size = _lib.plan("wptv_choice_workspace", "choose_rows", B, T, N)
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
     q_ = q.contiguous()
-    positions_ = _long(positions, device)
+    positions_, lse_ = _long(positions, device), lse.contiguous()
     check(library.wptv_exact_choice(ptr(q_), ptr(k), k.stride(0), k.stride(1), _lib.dtype_code(q.dtype),
-                                    ptr(positions_), ptr(lse.contiguous()), B, T, H, c, N, float(scale), int(top_k),
+                                    ptr(positions_), ptr(lse_), B, T, H, c, N, float(scale), int(top_k),
                                     int(window), ptr(chosen), ptr(workspace), size, _lib.stream(device)),
           "choose_rows")
     return chosen

@@ -270,7 +270,8 @@ def greedy_tree_from_argmax(best, node_tokens, parents):
     path = torch.empty(B, M + 1, dtype=torch.long, device=device)
     tokens = torch.empty(B, M + 1, dtype=torch.long, device=device)
     counts = torch.empty(B, dtype=torch.int32, device=device)
-    check(_lib.lib().wptv_greedy_tree_best(ptr(best.contiguous()), ptr(node_tokens), ptr(parents_), B, M, ptr(path),
+    best_ = best.contiguous()
+    check(_lib.lib().wptv_greedy_tree_best(ptr(best_), ptr(node_tokens), ptr(parents_), B, M, ptr(path),
                                            ptr(tokens), ptr(counts), _lib.stream(device)), "greedy_tree_best")
     return path, tokens, counts
 
