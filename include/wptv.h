@@ -584,8 +584,8 @@ int wptv_greedy_tree_best(const int32_t* best, const int64_t* node_tokens, const
  *   l_e + bias_e, l = x[m] . router[e] formed and ranked in 64 bits, largest
  *   first, equal values the lowest expert (a NaN counts as the largest); gates =
  *   the softmax of the chosen experts' l (without the bias), rounded to FP32.
- *   router [E, D] fp32; bias NULL or [E] fp32 (-inf takes an expert out: one at
- *   -inf is never chosen).  counts NULL or [B] int64: rows t >= counts[b] are
+ *   router [E, D] fp32; bias NULL or [E] fp32 (-inf takes an expert out, whatever
+ *   its l; one at -inf is never chosen).  counts NULL or [B] int64: rows t >= counts[b] are
  *   padding.  chosen [B, T, k] int32, gates [B, T, k] fp32; where no expert is
  *   chosen (padding, fewer than k above -inf) chosen is -1 and the gate 0.  A
  *   NaN or +inf among a row's chosen l makes its gates NaN.

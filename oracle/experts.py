@@ -11,12 +11,13 @@ HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}  # torch.finf
 def route(x, router, k, bias=None, counts=None):
     """(chosen (B, T, k), gates (B, T, k) in 64 bits): the k experts of the
     largest x . router^T + bias, equal ones the lowest, a NaN the largest, one at
-    -inf never; the softmax of their logits.  -1 and 0 where none is chosen."""
+    -inf or whose bias is -inf never; the softmax of their logits.  -1 and 0 where
+    none is chosen."""
     B, T, _ = x.shape
     chosen = torch.full((B, T, k), -1, dtype=torch.int32)
     gates = torch.zeros(B, T, k, dtype=torch.float64)
     logits = torch.einsum("btd,ed->bte", x.double(), router.double())
-    value = logits if bias is None else logits + bias.double()
+    value = logits if bias is None else torch.where(bias == -math.inf, -math.inf, logits + bias.double())
     for b in range(B):
         for t in range(T if counts is None else min(T, int(counts[b]))):
             row = value[b, t].tolist()

@@ -1,4 +1,7 @@
-"""Calls of the experts beside the plain ones: views of every argument."""
+"""Calls of the experts beside the plain ones: views of every argument, logits
+and biases that are not finite."""
+
+import math
 
 import pytest
 import torch
@@ -7,6 +10,7 @@ from oracle import experts as oracle
 from wpt_amd import experts
 
 pytestmark = pytest.mark.gpu
+INF, NAN = math.inf, math.nan
 BF16 = torch.bfloat16
 
 
@@ -40,3 +44,18 @@ def test_given_choices_and_gates_may_both_be_views(device, rows):
             same = torch.equal(experts.feed_forward(rows_, weights, c, g), expected)
             same_parts = torch.equal(experts.feed_forward_parts(rows_, weights, c, g), parts)
             assert same and same_parts
+
+
+@pytest.mark.parametrize("rows, D, E", [(1, 256, 8), (30, 64, 20), (3, 2048, 64), (200, 512, 100)])
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+def test_an_expert_taken_out_stays_out_whatever_its_logits(device, rows, D, E, value):
+    print(f"route rows={rows} D={D} E={E} {value}", flush=True)
+    x, router, _, _ = layer(1, rows, D, E, 8, BF16, seed=E)
+    bias = torch.randn(E, generator=torch.Generator().manual_seed(1))
+    router[2, 5], bias[2] = value, -INF
+    router[E - 1], bias[E - 1] = NAN, -INF
+    expected = oracle.route(x, router, 4, bias)
+    assert not bool(((expected[0] == 2) | (expected[0] == E - 1)).any()) and bool(expected[1].isfinite().all())
+    chosen, gates = experts.route(x.to(device), router.to(device), 4, bias.to(device))
+    assert torch.equal(chosen.cpu(), expected[0])
+    assert bool(((gates.cpu().double() - expected[1]).abs() <= expected[1] * (2.0 ** -24 + 1e-9)).all())

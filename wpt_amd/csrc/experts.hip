@@ -120,6 +120,14 @@ __device__ __forceinline__ uint64_t order_key64(double f) {
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
+// The key an expert is ranked by; 0, below every key, where its bias takes it out,
+// whatever its logit (NaN - inf and inf - inf would be the largest).
+__device__ __forceinline__ uint64_t expert_key(double logit, const float* __restrict__ bias, int e) {
+  if (!bias) return order_key64(logit);
+  const float b = bias[e];
+  return b == -__builtin_inff() ? 0 : order_key64(logit + (double)b);
+}
+
 constexpr int kMaxExperts = 512, kMaxChosen = 16;
 
 // A token's choices and gates by one wavefront (every lane calls): lane l holds the
@@ -234,7 +242,7 @@ __global__ __launch_bounds__(kTokenThreads) void route_token(const T* __restrict
   for (int s = 0; s < SLOTS; ++s) {
     const int e = lane + 64 * s;
     own[s] = e < E ? logit[e] : 0.;
-    key[s] = read && e < E ? order_key64(bias ? own[s] + (double)bias[e] : own[s]) : 0;
+    key[s] = read && e < E ? expert_key(own[s], bias, e) : 0;
   }
   choose_experts<SLOTS>(own, key, k, chosen + m * k, gates + m * k);
 }
@@ -309,7 +317,7 @@ __global__ __launch_bounds__(256) void route_choose(const double* __restrict__ s
 #pragma unroll
   for (int s = 0; s < SLOTS; ++s) {
     const int e = lane + 64 * s;
-    key[s] = read && e < E ? order_key64(bias ? own[s] + (double)bias[e] : own[s]) : 0;
+    key[s] = read && e < E ? expert_key(own[s], bias, e) : 0;
   }
   choose_experts<SLOTS>(own, key, k, chosen + (int64_t)m * k, gates + (int64_t)m * k);
 }

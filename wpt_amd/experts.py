@@ -95,8 +95,8 @@ def route(x, router, k, bias=None, counts=None):
 
     x (B, T, D) bf16 or FP32; router (E, D) FP32.  The logits l = x . router^T
     are formed and ranked in 64 bits: the k largest l + bias (bias (E,) FP32, a
-    load-balanced router's; -inf takes an expert out), largest first, equal
-    ones the lowest expert, a NaN the largest.  gates: the softmax of the chosen
+    load-balanced router's; -inf takes an expert out, whatever its l), largest
+    first, equal ones the lowest expert, a NaN the largest.  gates: the softmax of the chosen
     experts' l, without the bias.  counts (B,): the tokens read of each row, the
     others padding (None: all).  Where no expert is chosen (padding, or fewer
     than k above -inf) chosen is -1 and the gate 0."""
