@@ -1,5 +1,5 @@
-"""Calls of the experts beside the plain ones: views of every argument, logits
-and biases that are not finite."""
+"""Calls of the experts beside the plain ones: views of every argument, weights,
+logits and biases that are not finite."""
 
 import math
 
@@ -11,7 +11,7 @@ from wpt_amd import experts
 
 pytestmark = pytest.mark.gpu
 INF, NAN = math.inf, math.nan
-BF16 = torch.bfloat16
+BF16, FP32 = torch.bfloat16, torch.float32
 
 
 def layer(B, T, D, E, F, dtype, seed=0):
@@ -59,3 +59,35 @@ def test_an_expert_taken_out_stays_out_whatever_its_logits(device, rows, D, E, v
     chosen, gates = experts.route(x.to(device), router.to(device), 4, bias.to(device))
     assert torch.equal(chosen.cpu(), expected[0])
     assert bool(((gates.cpu().double() - expected[1]).abs() <= expected[1] * (2.0 ** -24 + 1e-9)).all())
+
+
+# the down product of a few tokens over all experts at once (few k-steps, or wide outputs), and the other forms beside it
+@pytest.mark.parametrize("rows, D, F", [(2, 256, 64), (3, 4096, 96), (16, 64, 32), (2, 256, 1200), (16, 512, 1200), (17, 256, 64),
+                                        (200, 64, 32)])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("value", [INF, NAN])
+def test_an_expert_that_is_not_finite_reaches_its_own_tokens_alone(device, rows, D, F, dtype, value):
+    print(f"rows={rows} D={D} F={F} {dtype} {value}", flush=True)
+    E, k = 9, 2
+    x, _, gate_up, down = layer(1, rows, D, E, F, dtype, seed=D + F)
+    chosen = torch.stack([torch.arange(rows) % 8, torch.full((rows,), 8)], -1).view(1, rows, k).to(torch.int32)
+    chosen[0, -1] = 3  # one expert twice
+    gates = torch.rand(1, rows, k, generator=torch.Generator().manual_seed(0)) + 0.5
+    on = [t.to(device) for t in (x, chosen, gates)]
+    finite = experts.ExpertWeights(gate_up.to(device), down.to(device))
+    y = experts.feed_forward(on[0], finite, on[1], on[2])
+    broken = down.clone()
+    broken[1, 5, F // 2] = value  # token 1's, 9's, ...; output 5
+    weights = experts.ExpertWeights(gate_up.to(device), broken.to(device))
+    got = experts.feed_forward(on[0], weights, on[1], on[2])
+    mine = (chosen[0] == 1).any(-1).to(device)
+    expected, _ = oracle.feed_forward(x, gate_up, broken, chosen, gates)
+    assert torch.equal(got.isnan().cpu(), expected.isnan())
+    assert not bool(got[0, mine, 5].isfinite().any())
+    got[0, mine, 5] = y[0, mine, 5]
+    assert torch.equal(got, y)
+    # a gate matrix that is not: every output of its tokens
+    broken = gate_up.clone()
+    broken[1, 3, 0] = NAN
+    got = experts.feed_forward(on[0], experts.ExpertWeights(broken.to(device), down.to(device)), on[1], on[2])
+    assert bool(got[0, mine].isnan().all()) and torch.equal(got[0, ~mine], y[0, ~mine])

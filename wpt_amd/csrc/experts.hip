@@ -855,12 +855,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void expert_rows(const T* __restric
   const int steps = (total - wv + kFewWaves - 1) / kFewWaves;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   u32x4 wb[kDepth], xb[kDepth];
+  bool taken[kDepth];  // by the lane's token
   auto load = [&](int d, int s) {
     const int step = wv + kFewWaves * s, which = step / KS, ks = step - which * KS;
     const u32x4* w = w0 + __builtin_amdgcn_readfirstlane(expert[which]) * matrix;
     wb[d] = load16_weights<true>(buffer(w, 1024u * KS), 16 * lane, 1024 * ks);
     const unsigned p = prow[which][j];
-    xb[d] = load16(x, p == kNone ? kOutside : p * width + 16 * g, 64 * ks);
+    taken[d] = p != kNone;
+    xb[d] = load16(x, taken[d] ? p * width + 16 * g : kOutside, 64 * ks);
+  };
+  auto multiply = [&](int d) {  // the other tokens' sums stay: 0 times a weight that is not finite is a NaN
+    const f32x4 sum = O::mfma(wb[d], xb[d], acc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = taken[d] ? sum[i] : acc[i];
   };
   if (steps > 0) {
 #pragma unroll
@@ -869,7 +876,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void expert_rows(const T* __restric
     for (; s + kDepth <= steps; s += kDepth) {
 #pragma unroll
       for (int d = 0; d < kDepth; ++d) {
-        acc = O::mfma(wb[d], xb[d], acc);
+        multiply(d);
         __builtin_amdgcn_sched_barrier(0);
         load(d, min(s + kDepth + d, steps - 1));
         __builtin_amdgcn_sched_barrier(0);
@@ -877,7 +884,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void expert_rows(const T* __restric
     }
 #pragma unroll
     for (int d = 0; d < kDepth; ++d)
-      if (s + d < steps) acc = O::mfma(wb[d], xb[d], acc);
+      if (s + d < steps) multiply(d);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) red[wv][i * 64 + lane] = acc[i];
