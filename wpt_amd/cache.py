@@ -109,6 +109,12 @@ class Cache:
         return grown[0] if grown else None
 
     @property
+    def room(self):
+        """The tokens a text may have before reserve() puts larger tables, or
+        routes, in the place of those held (None: none of them grows)."""
+        return self.capacity if self.routes is None else self.routes.shape[2]
+
+    @property
     def ring_rows(self):
         rings = [self.tables[i].shape[1] for i in sorted(self.rings)]
         return rings[0] if rings else None
@@ -116,7 +122,7 @@ class Cache:
     def reserve(self, need):
         """Growing tables of at least `need` rows (grown to max(need, 2 x
         capacity)); the rings keep their size."""
-        held = self.capacity if self.routes is None else self.routes.shape[2]
+        held = self.room
         if held is None or need <= held:
             return
         if torch.cuda.is_current_stream_capturing():

@@ -297,7 +297,7 @@ class Writer:
         tensors.  The generator hands its state over and takes it back."""
         cap = self._reads.get(L)
         width = L + 1
-        if cap is None or self.cache.bound + width > cap.limit:
+        if cap is None or (cap.limit is not None and self.cache.bound + width > cap.limit):
             cap = self._reads[L] = _CapturedRead(self, L)
         anchors = torch.tensor([row.unread[0] for row in self._rows], dtype=torch.long)
         cap.ids[:, 0].copy_(anchors, non_blocking=True)
@@ -317,7 +317,8 @@ class _CapturedRead:
     """A steady round's verify reading (every row: its anchor, then L drafts)
     and its acceptance, captured in a HIP graph over static inputs; the
     cache's tables are reserved for ROUNDS more such readings first (a
-    graph cannot grow them: past that a new one is captured)."""
+    graph cannot grow them: past that a new one is captured; a cache of rings
+    alone grows nothing)."""
 
     ROUNDS = 64
 
@@ -329,7 +330,7 @@ class _CapturedRead:
         self.drafts = torch.zeros(rows, L, dtype=torch.long, device=device)
         self.state = sampling.generator_state(writer.generator, device).clone()
         cache.reserve(cache.bound + width * self.ROUNDS)
-        self.limit = cache.capacity
+        self.limit = cache.room
         pending, bound = cache.pending, cache.bound
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):  # records the kernels; runs none
