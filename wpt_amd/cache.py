@@ -121,7 +121,9 @@ class Cache:
 
     def reserve(self, need):
         """Growing tables of at least `need` rows (grown to max(need, 2 x
-        capacity)); the rings keep their size."""
+        capacity)); the rings keep their size.  Whatever grows, `tables` becomes
+        another list: a graph captured over the one before reads and writes its
+        memory."""
         held = self.room
         if held is None or need <= held:
             return

@@ -297,7 +297,7 @@ class Writer:
         tensors.  The generator hands its state over and takes it back."""
         cap = self._reads.get(L)
         width = L + 1
-        if cap is None or (cap.limit is not None and self.cache.bound + width > cap.limit):
+        if cap is None or not cap.serves(self.cache):
             cap = self._reads[L] = _CapturedRead(self, L)
         anchors = torch.tensor([row.unread[0] for row in self._rows], dtype=torch.long)
         cap.ids[:, 0].copy_(anchors, non_blocking=True)
@@ -322,6 +322,12 @@ class _CapturedRead:
 
     ROUNDS = 64
 
+    def serves(self, cache):
+        """Whether one more replay stays within the memory that the graph was
+        captured over: a reading of another length, or the program, may have had
+        the cache put larger tables in its place (held here until then)."""
+        return cache.tables is self.tables and (self.limit is None or cache.bound + self.ids.shape[1] <= self.limit)
+
     def __init__(self, writer, L):
         model, cache, device = writer.model, writer.cache, writer.device
         rows, V, width = cache.rows, model.config.vocab, L + 1
@@ -330,7 +336,7 @@ class _CapturedRead:
         self.drafts = torch.zeros(rows, L, dtype=torch.long, device=device)
         self.state = sampling.generator_state(writer.generator, device).clone()
         cache.reserve(cache.bound + width * self.ROUNDS)
-        self.limit = cache.room
+        self.limit, self.tables = cache.room, cache.tables
         pending, bound = cache.pending, cache.bound
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):  # records the kernels; runs none
