@@ -1,13 +1,14 @@
 """Calls of the experts beside the plain ones: views of every argument, weights,
-logits and biases that are not finite."""
+logits and biases that are not finite, tangents."""
 
 import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from oracle import experts as oracle
-from wpt_amd import experts
+from wpt_amd import experts, kernels, sampling
 
 pytestmark = pytest.mark.gpu
 INF, NAN = math.inf, math.nan
@@ -91,3 +92,26 @@ def test_an_expert_that_is_not_finite_reaches_its_own_tokens_alone(device, rows,
     broken[1, 3, 0] = NAN
     got = experts.feed_forward(on[0], experts.ExpertWeights(broken.to(device), down.to(device)), on[1], on[2])
     assert bool(got[0, mine].isnan().all()) and torch.equal(got[0, ~mine], y[0, ~mine])
+
+
+def test_tangents_are_refused(device):
+    x, router, gate_up, down = (t.to(device) for t in layer(1, 3, 64, 8, 32, FP32))
+    weights = experts.ExpertWeights(gate_up, down)
+    chosen, gates = experts.route(x, router, 2)
+    scores, tokens = torch.randn(1, 3, 100, device=device), torch.zeros(1, 3, dtype=torch.long, device=device)
+    q, table = torch.randn(1, 3, 2, 64, device=device), torch.randn(1, 9, 128, device=device)
+    positions = torch.arange(3, device=device)[None]
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: experts.route(dual(x), router, 2), lambda: experts.route(x, dual(router), 2),
+                     lambda: experts.mixture(dual(x), router, weights, 2), lambda: experts.mixture(x, dual(router), weights, 2),
+                     lambda: experts.mixture_parts(dual(x), router, weights, 2),
+                     lambda: experts.feed_forward(x, weights, chosen, dual(gates)),
+                     lambda: experts.feed_forward_parts(dual(x), weights, chosen, gates),
+                     lambda: experts.ExpertWeights(gate_up, dual(down)), lambda: sampling.log_probs(dual(scores), tokens),
+                     lambda: kernels.verify_attention(dual(q), table[..., :64], table[..., 64:], positions, 0.125)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert experts.route(x, router, 2)[1].isfinite().all()

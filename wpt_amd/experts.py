@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._lib import KernelUnavailable, check, ptr
-from .kernels import _forward_only, _index
+from .kernels import _forward_only, _index, _no_tangents
 
 __all__ = ["ExpertWeights", "route", "feed_forward", "feed_forward_parts", "mixture", "mixture_parts"]
 
@@ -79,6 +79,7 @@ class ExpertWeights:
         self.experts, self.width, self.features, self.dtype, self.device = E, D, F, gate_up.dtype, device
         # stands for matrices that ask for gradients, which no backward pass of these forms gives
         self.trained = torch.empty(0, requires_grad=True) if gate_up.requires_grad or down.requires_grad else None
+        _no_tangents(gate_up, down)
         gate_up, down = gate_up.detach().contiguous(), down.detach().contiguous()
         sizes = ctypes.c_size_t(0), ctypes.c_size_t(0)
         check(_lib.lib().wptv_experts_packed(D, F, dtype, ctypes.byref(sizes[0]), ctypes.byref(sizes[1])),

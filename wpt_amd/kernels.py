@@ -14,7 +14,8 @@ scores and softmax in FP32.
 These forms are forward-only: the verify step runs under torch.no_grad
 (wpt_model.WPT.extend, model.py:456).  Their backward raises
 NotImplementedError, which the reference's kernel tests read as "not
-written yet" (test_kernels.py:149-154).
+written yet" (test_kernels.py:149-154); so does an input with a forward-mode
+tangent.
 A bad shape or dtype is ValueError; a device without the library is
 KernelUnavailable, never a fall back to another form.
 """
@@ -22,6 +23,7 @@ KernelUnavailable, never a fall back to another form.
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import KernelUnavailable, check, ptr
@@ -52,7 +54,18 @@ class _ForwardOnly(torch.autograd.Function):
         raise NotImplementedError("the HIP attention forms are forward-only (the verify step runs under no_grad)")
 
 
+def _no_tangents(*inputs):
+    """Refuses inputs with a forward-mode tangent, which the outputs would lose."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # outside of dual_level no tensor has one
+        for x in inputs:
+            if x is not None and forward_ad.unpack_dual(x).tangent is not None:
+                raise NotImplementedError("the HIP forms carry no forward-mode tangents")
+
+
 def _forward_only(out, *inputs):
+    """out, with a backward that says that there is none where an input asks for
+    gradients."""
+    _no_tangents(*inputs)
     if torch.is_grad_enabled():
         for x in inputs:
             if x is not None and x.requires_grad:
