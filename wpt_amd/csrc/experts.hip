@@ -1093,12 +1093,14 @@ int run_product(const void* in, const void* weights, const int* chosen, const fl
 }
 
 // The rows of one round of the two products: their operands stay within a buffer,
-// and the terms that a join reads within 512 MiB.
+// and the terms that a join reads within kRoundBytes (a row's are 64 MiB at most).
+constexpr int64_t kRoundBytes = 1 << 29;
+
 int round_rows(int64_t rows, int k, const ExpertShape& shape, int dtype, bool join) {
   const int64_t act = (int64_t)k * shape.Fp;
   const int64_t widest = (dtype == WPTV_BF16 ? 2 : 4) * (shape.D > act ? shape.D : act);
   int64_t fit = kBufferBytes / widest;
-  const int64_t terms = (int64_t)k * shape.D * 4, most = terms < (1 << 20) ? (1 << 29) / terms : 512;
+  const int64_t most = kRoundBytes / term_bytes(1, k, shape);
   if (join && most < fit) fit = most;
   return (int)(rows < fit ? rows : fit);
 }
@@ -1108,11 +1110,12 @@ size_t act_bytes(int round, int k, const ExpertShape& shape, int dtype) {
 }
 
 // Whether 16 output rows a workgroup, over all experts, are the faster down product
-// of a few tokens: where a workgroup reads little, which saves the join, or where
-// they cover the compute units.  Whole layers in a graph, us, this and the other
-// form: one token, D 256, 2 of 8 experts of 704 12.6, 13.8; D 4096, 4 of 64 of 1408
-// 42.0, 45.3, 4 tokens 105, 112; D 2048, 8 of 64 of 704 30.7, 29.9, 4 tokens, 2 of 8
-// of 5632 89, 80; FP32, 3 tokens, D 1024, 4 of 64 of 300 29.9, 25.8.
+// of a few tokens (of at most kFewPairs pairs, whose rows are one round): where a
+// workgroup reads little, which saves the join, or where they cover the compute units.
+// Whole layers in a graph, us, this and the other form: one token, D 256, 2 of 8 experts
+// of 704 12.6, 13.8; D 4096, 4 of 64 of 1408 42.0, 45.3, 4 tokens 105, 112; D 2048, 8 of
+// 64 of 704 30.7, 29.9, 4 tokens, 2 of 8 of 5632 89, 80; FP32, 3 tokens, D 1024, 4 of 64
+// of 300 29.9, 25.8.
 bool few_rows(int rows, int k, const ExpertShape& shape) {
   if (rows > kFewTokens || rows * k > kFewPairs) return false;
   return (int64_t)rows * k * shape.KSf <= 64 || shape.D >= 4096;
