@@ -643,8 +643,9 @@ int wptv_mixture(const void* x, int dtype, const float* router, const float* bia
  *   best     [B, T, top] fp32: their log-probabilities
  *   A row that holds a NaN or +inf, or nothing above -inf, has no distribution:
  *   its log-probabilities and its entropy are NaN.  -inf scores have
- *   log-probability -inf.  top <= 64, top <= V; V <= 2^24; temperature positive
- *   and finite.  The reference's Writer returns tokens alone.
+ *   log-probability -inf.  top <= 64, top <= V; V <= 2^24; fewer than 2^22
+ *   rows (more where a row takes fewer than 1024 threads); temperature positive and
+ *   finite.  The reference's Writer returns tokens alone.
  *   workspace  wptv_log_probs_workspace(B, T, V, top) bytes
  * ------------------------------------------------------------------------- */
 int wptv_log_probs_workspace(int B, int T, int V, int top, size_t* bytes);

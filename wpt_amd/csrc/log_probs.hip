@@ -548,6 +548,8 @@ struct Form {
   int threads, chunks, parts, stretch;
 };
 
+constexpr int kRowThreads = 512;  // of the form from memory
+
 Form row_form(int64_t rows, int V, int top, int dtype) {
   const int per = dtype == WPTV_BF16 ? 8 : 4;
   const int64_t units = compute_units();
@@ -581,7 +583,8 @@ template <typename T>
 int run_log_probs(const T* scores, int64_t ssb, int64_t sst, const int64_t* tokens, float inverse, int rows,
                   int per_row, int V, int top, const Form& form, const Outputs& out, void* workspace, hipStream_t stream) {
   if (form.parts == 0) {
-    log_probs_row<T, 512><<<rows, 512, 0, stream>>>(scores, ssb, sst, tokens, inverse, per_row, V, top, out);
+    log_probs_row<T, kRowThreads><<<rows, kRowThreads, 0, stream>>>(scores, ssb, sst, tokens, inverse, per_row, V, top,
+                                                                    out);
     return launched("log_probs");
   }
   Part* parts = static_cast<Part*>(workspace);
@@ -649,6 +652,10 @@ extern "C" int wptv_log_probs(const void* scores, int64_t scores_stride_b, int64
   const float inverse = 1.f / temperature;
   const Outputs out{logprobs, entropy, ids, best};
   const Form form = row_form((int64_t)B * T, V, top, scores_dtype);
+  const int64_t threads = (int64_t)B * T * (form.parts ? form.threads : kRowThreads);
+  if (threads > UINT32_MAX)  // a dimension of a grid
+    return fail(WPTV_E_UNSUPPORTED, "log_probs: %lld rows of %d scores are %lld threads, above 2^32 - 1",
+                (long long)B * T, V, (long long)threads);
   return scores_dtype == WPTV_BF16
              ? run_log_probs(static_cast<const unsigned short*>(scores), scores_stride_b, scores_stride_t, tokens,
                              inverse, B * T, T, V, top, form, out, workspace, stream)
