@@ -1,5 +1,5 @@
 """Calls of the experts beside the plain ones: views of every argument, weights,
-logits and biases that are not finite, tangents."""
+logits, biases and padding that are not finite, tangents."""
 
 import math
 
@@ -115,3 +115,29 @@ def test_tangents_are_refused(device):
             with pytest.raises(NotImplementedError):
                 call()
         assert experts.route(x, router, 2)[1].isfinite().all()
+
+
+@pytest.mark.parametrize("B, T, D, E, k, F", [
+    (1, 1, 256, 8, 2, 64), (2, 4, 64, 40, 2, 32),                   # fewer pairs than experts
+    (4, 4, 72, 6, 2, 1200), (10, 8, 72, 6, 2, 40),                  # the width shared out
+    (4, 2, 4096, 16, 2, 64), (30, 10, 1040, 64, 2, 512)])           # all experts at once; tiles
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_padding_may_hold_anything_and_be_all_there_is(device, B, T, D, E, k, F, dtype):
+    print(f"B={B} T={T} D={D} E={E} k={k} F={F} {dtype}", flush=True)
+    x, router, gate_up, down = (t.to(device) for t in layer(B, T, D, E, F, dtype, seed=F))
+    weights = experts.ExpertWeights(gate_up, down)
+    for counts in (torch.arange(B) % (T + 1), torch.zeros(B, dtype=torch.long)):
+        counts = counts.to(device)
+        padding = torch.arange(T, device=device) >= counts[:, None]
+        results = []
+        for value in (0.0, NAN, INF):
+            held = x.clone()
+            held[padding] = value
+            for shape, kind in (((B, T, D), dtype), ((k, B * T, D), FP32)):  # what is not written shows
+                torch.full(shape, NAN, dtype=kind, device=device)
+            y, chosen, gates = experts.mixture(held, router, weights, k, None, counts)
+            parts, _, _ = experts.mixture_parts(held, router, weights, k, None, counts)
+            assert bool((y[padding] == 0).all()) and bool((parts[:, padding.view(-1)] == 0).all())
+            assert bool((chosen[padding] == -1).all()) and bool((gates[padding] == 0).all())
+            results.append((y, chosen, gates, parts))
+        assert all(torch.equal(a, b) for other in results[1:] for a, b in zip(results[0], other))
