@@ -34,8 +34,10 @@ entries taken out, so that the window layers' rings still place token
 lengths + evicted.
 
 A cache that records routes also keeps, beside each token's entries, the experts
-each layer's router chose for it (`routes`, int32 (layers, B, capacity, k), -1 where
-none was read), written by each reading at its rows' places and cut back with them.
+each layer's router chose for it (`routes`, int32 (layers, B, capacity, k), -1 for a
+choice of none), written by each reading at its rows' places.  As with the entries,
+each row's first `lengths` are its text's: what an undo or a reorder leaves past them
+stays there until it is written over.
 
 The lengths stay on the device; `bound` is a host-side upper bound of every
 row's length (raised by each reading's width, never lowered by undo) so that

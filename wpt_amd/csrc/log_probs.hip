@@ -148,7 +148,7 @@ struct TopShared<0> {};
 
 // One workgroup a row, or a part of one (blockIdx.y of gridDim.y): its scores are
 // read once and stay in registers, CHUNKS times 16 bytes a thread.  What bounds it
-// is that stream and the arithmetic on it (2048 rows of 32768 bf16 scores 33 us, 4.1
+// is that stream and the arithmetic on it (2048 rows of 32768 bf16 scores 31 us, 4.3
 // TB/s, the exponentials and sums alone about 20), and for few rows the chain of its
 // steps: the maximum, a barrier, the sums and the candidates, a barrier, the ranks
 // (160 rows of them with 20 alternatives 10.5 us, without 7.5).

@@ -120,7 +120,9 @@ class Writer:
 
     @property
     def routes(self):
-        """Each row's recorded routes, from the model's cache (None without one)."""
+        """Each row's recorded routes, from the model's cache (None without one):
+        row r's are those of its first cache.lengths[r] tokens, past which drafts
+        that were taken back may have left theirs."""
         return self.cache.routes if self.cache is not None else None
 
     @property
