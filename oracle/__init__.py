@@ -49,7 +49,8 @@ tests/test_scheduling.py):
                rows); the scheduler's known answers (test_sampling.py:230-238)
                and a brute force over widths
     beam, eviction  cases done by hand (tests/test_beam_eviction.py)
-    experts, log_probs  cases done by hand (tests/test_experts.py)
+    experts, log_probs  cases done by hand (tests/test_experts.py,
+               tests/test_experts_calls.py)
 The exact token stream the reference's Writer draws from a seed through its
 lazy generator order (its own tests assert only "same seed, same tokens") is
 pinned by golden streams of the reference's Writer itself
