@@ -1,7 +1,9 @@
 """Whether a Writer's captured reading may be replayed, off the GPU: its graph is
 bound to the memory that it was captured over."""
 
+import gc
 import types
+import weakref
 
 import pytest
 import torch
@@ -66,7 +68,14 @@ def test_a_reading_captured_over_replaced_tables_is_not_replayed(monkeypatch, gr
         of.cache.reserve(5000)
     assert of.cache.room > 512
     before = Captured.made
+    of._reads[2] = stale = Captured(of, 2)  # of a length that does not come again, over tables that the next growth replaces
+    before += 1
+    of.cache.reserve(of.cache.room + 1)
+    held = weakref.ref(stale.tables[0])
+    del stale
     round_(4)  # 211 of 512 tokens, but of the tables before
     assert Captured.made == before + 1
+    gc.collect()
+    assert held() is None  # the tables that are gone are not kept
     round_(4)
     assert Captured.made == before + 1

@@ -301,6 +301,8 @@ class Writer:
         width = L + 1
         if cap is None or not cap.serves(self.cache):
             cap = self._reads[L] = _CapturedRead(self, L)
+            # graphs over tables that are gone would keep them in memory
+            self._reads = {n: read for n, read in self._reads.items() if read.tables is self.cache.tables}
         anchors = torch.tensor([row.unread[0] for row in self._rows], dtype=torch.long)
         cap.ids[:, 0].copy_(anchors, non_blocking=True)
         cap.ids[:, 1:].copy_(drafts)
